@@ -166,10 +166,11 @@ def prepare(case, seed):
 def _quantize(v, dim):
     """v in 8 bits with one scale along `dim` (zero below _TINY, NaN where a value is not finite)."""
     amax = v.abs().amax(dim, keepdim=True)
+    most = torch.full_like(amax, 127.0)  # (a tensor: by a number torch multiplies with the reciprocal)
     live = amax >= _TINY
     fine = torch.isfinite(amax)
-    scale = torch.where(fine, torch.where(live, amax / 127.0, torch.zeros_like(amax)), torch.full_like(amax, math.nan))
-    q = torch.round(v * torch.where(live & fine, 127.0 / amax, torch.zeros_like(amax)))
+    scale = torch.where(fine, torch.where(live, amax / most, torch.zeros_like(amax)), torch.full_like(amax, math.nan))
+    q = torch.round(v * torch.where(live & fine, most / amax, torch.zeros_like(amax)))
     return torch.where(live & fine, q, torch.zeros_like(q)), scale
 
 
