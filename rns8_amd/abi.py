@@ -389,6 +389,85 @@ def new_struct(cls):
     return s
 
 
+# operators of language models (include/rns8_mi355x.h)
+F32 = 0
+F16 = 1
+BF16 = 2
+B_CHANNELS = 0
+B_INNER = 1
+NORM_POST = 1
+NORM_PRE = 2
+
+
+class QuantizeArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("multiplier", C.c_void_p),
+                ("q", C.c_void_p), ("ldq", C.c_int64), ("scale", C.c_void_p), ("sums", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class GemmI8Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("m", C.c_int64),
+                ("n", C.c_int64), ("k", C.c_int64), ("a", C.c_void_p), ("lda", C.c_int64), ("b", C.c_void_p),
+                ("ldb", C.c_int64), ("b_layout", C.c_uint32), ("reserved", C.c_uint32), ("a_scale", C.c_void_p),
+                ("b_scale", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p), ("ldo", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class LinearI8Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("m", C.c_int64),
+                ("n", C.c_int64), ("k", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p),
+                ("ldw", C.c_int64), ("w_scale", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p),
+                ("ldo", C.c_int64), ("x_q", C.c_void_p), ("ldq", C.c_int64), ("x_scale", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class LinearI8BackwardArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("m", C.c_int64),
+                ("n", C.c_int64), ("k", C.c_int64), ("dy", C.c_void_p), ("lddy", C.c_int64), ("x_q", C.c_void_p),
+                ("ldq", C.c_int64), ("x_scale", C.c_void_p), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("w_scale", C.c_void_p), ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p),
+                ("lddw", C.c_int64), ("dbias", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("flags", C.c_uint32), ("eps", C.c_float), ("branch_scale", C.c_float),
+                ("residual_scale", C.c_float), ("x", C.c_void_p), ("ldx", C.c_int64), ("residual", C.c_void_p),
+                ("ldresidual", C.c_int64), ("gate", C.c_void_p), ("ldgate", C.c_int64), ("post_weight", C.c_void_p),
+                ("pre_weight", C.c_void_p), ("h", C.c_void_p), ("ldh", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("q", C.c_void_p), ("ldq", C.c_int64), ("q_scale", C.c_void_p),
+                ("rstd", C.c_void_p)]
+
+
+class BlockNormBackwardArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("flags", C.c_uint32), ("eps", C.c_float), ("branch_scale", C.c_float),
+                ("residual_scale", C.c_float), ("x", C.c_void_p), ("ldx", C.c_int64), ("residual", C.c_void_p),
+                ("ldresidual", C.c_int64), ("gate", C.c_void_p), ("ldgate", C.c_int64), ("post_weight", C.c_void_p),
+                ("pre_weight", C.c_void_p), ("rstd", C.c_void_p), ("dy", C.c_void_p), ("lddy", C.c_int64),
+                ("dh", C.c_void_p), ("lddh", C.c_int64), ("dx", C.c_void_p), ("lddx", C.c_int64),
+                ("dresidual", C.c_void_p), ("lddresidual", C.c_int64), ("dgate", C.c_void_p), ("lddgate", C.c_int64),
+                ("dpost_weight", C.c_void_p), ("dpre_weight", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class LogprobsArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("vocab", C.c_int64), ("logits", C.c_void_p), ("ldl", C.c_int64), ("targets", C.c_void_p),
+                ("scale", C.c_float), ("top", C.c_uint32), ("logp", C.c_void_p), ("entropy", C.c_void_p),
+                ("lse", C.c_void_p), ("top_ids", C.c_void_p), ("top_logp", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class LogprobsBackwardArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("vocab", C.c_int64), ("logits", C.c_void_p), ("ldl", C.c_int64), ("targets", C.c_void_p),
+                ("scale", C.c_float), ("reserved", C.c_uint32), ("lse", C.c_void_p), ("entropy", C.c_void_p),
+                ("dlogp", C.c_void_p), ("dentropy", C.c_void_p), ("dlogits", C.c_void_p), ("lddl", C.c_int64)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _U64 = C.c_uint64
@@ -455,6 +534,21 @@ PROTOTYPES = {
     "rns8_get_resident_lifetime_info": (_U32, [_P, _P, _P, _U32, C.POINTER(ResidentLifetimeInfo)]),
     "rns8_mi355x_get_matrix_planes": (_U32, [_P, C.POINTER(_P), C.POINTER(_I64), C.POINTER(_I64), C.POINTER(_U32)]),
     "rns8_mi355x_get_exact_proof": (_U32, [_P, _P, _P, C.POINTER(_U32), _P, _P]),
+    "rns8_mi355x_quantize_rows": (_U32, [_P, C.POINTER(QuantizeArgs), _P]),
+    "rns8_mi355x_quantize_columns": (_U32, [_P, C.POINTER(QuantizeArgs), _P]),
+    "rns8_mi355x_quantize_columns_workspace": (_U32, [C.POINTER(QuantizeArgs), C.POINTER(_U64)]),
+    "rns8_mi355x_gemm_i8_scaled": (_U32, [_P, C.POINTER(GemmI8Args), _P]),
+    "rns8_mi355x_gemm_i8_scaled_workspace": (_U32, [C.POINTER(GemmI8Args), C.POINTER(_U64)]),
+    "rns8_mi355x_linear_i8": (_U32, [_P, C.POINTER(LinearI8Args), _P]),
+    "rns8_mi355x_linear_i8_workspace": (_U32, [C.POINTER(LinearI8Args), C.POINTER(_U64)]),
+    "rns8_mi355x_linear_i8_backward": (_U32, [_P, C.POINTER(LinearI8BackwardArgs), _P]),
+    "rns8_mi355x_linear_i8_backward_workspace": (_U32, [C.POINTER(LinearI8BackwardArgs), C.POINTER(_U64)]),
+    "rns8_mi355x_block_norm": (_U32, [_P, C.POINTER(BlockNormArgs), _P]),
+    "rns8_mi355x_block_norm_backward": (_U32, [_P, C.POINTER(BlockNormBackwardArgs), _P]),
+    "rns8_mi355x_block_norm_backward_workspace": (_U32, [C.POINTER(BlockNormBackwardArgs), C.POINTER(_U64)]),
+    "rns8_mi355x_token_logprobs": (_U32, [_P, C.POINTER(LogprobsArgs), _P]),
+    "rns8_mi355x_token_logprobs_workspace": (_U32, [C.POINTER(LogprobsArgs), C.POINTER(_U64)]),
+    "rns8_mi355x_token_logprobs_backward": (_U32, [_P, C.POINTER(LogprobsBackwardArgs), _P]),
 }
 
 LIB_PATH = Path(__file__).resolve().parent / "librns8.so"

@@ -1,0 +1,38 @@
+// Host-side launchers of the language-model operators (defined in the .hip
+// files). The C entry points (api_operators.cpp) check the arguments; the
+// launchers check what their own grids and index arithmetic assume and return
+// hipErrorInvalidValue otherwise.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "rns8_mi355x.h"
+
+namespace rns8x {
+
+inline uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+// ---- quantization (quantize.hip) -------------------------------------------------
+hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& a, hipStream_t stream);
+uint64_t quantize_columns_bytes(int64_t rows, int64_t cols);
+hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& a, hipStream_t stream);
+
+// ---- scaled product (scaled_gemm.hip) ----------------------------------------------
+uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a);
+hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, hipStream_t stream);
+
+// ---- block norm (block_norm.hip) ------------------------------------------------------
+constexpr int64_t kMaxNormCols = 32768;
+hipError_t launch_block_norm(const rns8_mi355x_block_norm_args& a, hipStream_t stream);
+uint64_t block_norm_backward_bytes(const rns8_mi355x_block_norm_backward_args& a);
+hipError_t launch_block_norm_backward(const rns8_mi355x_block_norm_backward_args& a, hipStream_t stream);
+
+// ---- token log-probabilities (logprobs.hip) ----------------------------------------------
+constexpr uint32_t kMaxTop = 64;
+uint64_t logprobs_bytes(const rns8_mi355x_logprobs_args& a);
+hipError_t launch_logprobs(const rns8_mi355x_logprobs_args& a, hipStream_t stream);
+hipError_t launch_logprobs_backward(const rns8_mi355x_logprobs_backward_args& a, hipStream_t stream);
+
+}  // namespace rns8x

@@ -1,0 +1,67 @@
+// How a kernel that keeps a row in registers spreads it over threads.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+namespace rns8x {
+
+// Threads per row (64: a wave, four rows to a workgroup; 256 or 1024: the
+// workgroup) and 8-element vectors per thread (1, 2 or 4).
+struct RowShape {
+  int threads, vectors;
+};
+
+// The fewest threads that hold a row in four vectors each, so that one wave's
+// reductions need no barrier where rows are short; more where the rows are too
+// few to fill the chip and a row's own latency is what counts.
+inline RowShape choose_row_shape(int64_t rows, int64_t cols) {
+  const int64_t vectors = (cols + 7) / 8;
+  auto shape = [&](int threads) {
+    const int64_t v = (vectors + threads - 1) / threads;
+    return RowShape{threads, v <= 1 ? 1 : v <= 2 ? 2 : 4};
+  };
+  if (rows < 512) {
+    if (vectors <= 64) return shape(64);
+    return shape(vectors <= 256 ? 256 : 1024);
+  }
+  if (vectors <= 256) return shape(64);
+  return shape(vectors <= 1024 ? 256 : 1024);
+}
+
+// f(threads, vectors) with the shape as compile-time constants.
+template <typename F>
+hipError_t with_row_shape(RowShape s, F&& f) {
+  auto vectors = [&](auto threads) {
+    if (s.vectors == 1) return f(threads, std::integral_constant<int, 1>{});
+    if (s.vectors == 2) return f(threads, std::integral_constant<int, 2>{});
+    return f(threads, std::integral_constant<int, 4>{});
+  };
+  if (s.threads == 64) return vectors(std::integral_constant<int, 64>{});
+  if (s.threads == 256) return vectors(std::integral_constant<int, 256>{});
+  return vectors(std::integral_constant<int, 1024>{});
+}
+
+// A launch holds fewer than 2^32 threads; larger row counts are walked.
+constexpr int64_t kMaxBlocks = int64_t{1} << 21;
+
+inline dim3 row_grid(int threads, int64_t rows) {
+  const int64_t blocks = threads >= 256 ? rows : (rows + 3) / 4;
+  return dim3(static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks));
+}
+
+// body(row, thread of the row) for this workgroup's (kThreads >= 256) or this
+// wave's rows. Waves of a workgroup that own rows of their own may run
+// different counts: such a body has no barrier.
+template <int kThreads, typename F>
+__device__ __forceinline__ void for_rows(int64_t rows, F&& body) {
+  const bool shared = kThreads >= 256;
+  const int lane = shared ? threadIdx.x : threadIdx.x & 63;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (shared ? 1 : 4);
+  for (int64_t r = shared ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < rows; r += step)
+    body(r, lane);
+}
+
+}  // namespace rns8x

@@ -22,6 +22,7 @@ def runtime() -> C.CDLL:
         _lib.hipMemset.argtypes = [C.c_void_p, C.c_int, C.c_size_t]
         _lib.hipDeviceSynchronize.argtypes = []
         _lib.hipGetDeviceCount.argtypes = [C.POINTER(C.c_int)]
+        _lib.hipSetDevice.argtypes = [C.c_int]
     return _lib
 
 
@@ -35,6 +36,10 @@ def device_count() -> int:
     if runtime().hipGetDeviceCount(C.byref(n)) != 0:
         return 0
     return n.value
+
+
+def set_device(device: int) -> None:
+    _check(runtime().hipSetDevice(device), "hipSetDevice")
 
 
 def malloc(nbytes: int) -> int:
