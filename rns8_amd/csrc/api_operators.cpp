@@ -80,6 +80,7 @@ rns8_status check_gemm(const rns8_mi355x_gemm_i8_args& a) {
 struct LinearParts {
   rns8_mi355x_quantize_args quantize{};
   rns8_mi355x_gemm_i8_args gemm{};
+  bool zero_filled = false;  // the quantized rows end in the zeros that the product may read
   uint64_t bytes = 0;
 };
 
@@ -121,7 +122,8 @@ void linear_parts(const rns8_mi355x_linear_i8_args& a, LinearParts& p) {
   p.gemm.bias = a.bias;
   p.gemm.out = a.out;
   p.gemm.ldo = a.ldo;
-  const uint64_t bytes = gemm_i8_bytes(p.gemm);
+  p.zero_filled = p.quantize.ldq >= padded_row(a.k);
+  const uint64_t bytes = gemm_i8_bytes(p.gemm, p.zero_filled);
   p.gemm.workspace = take(bytes);
   p.gemm.workspace_bytes = bytes;
 }
@@ -180,7 +182,7 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.dx.a_scale = p.rows.scale;
     p.dx.out = a.dx;
     p.dx.ldo = a.lddx;
-    shared = gemm_i8_bytes(p.dx);
+    shared = gemm_i8_bytes(p.dx, true);
   }
   if (a.dw || a.dbias) {
     p.columns.dtype = a.dtype;
@@ -208,7 +210,7 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.dw.out = a.dw;
     p.dw.ldo = a.lddw;
     if (a.dw) {
-      const uint64_t bytes = gemm_i8_bytes(p.dw);
+      const uint64_t bytes = gemm_i8_bytes(p.dw, true);
       if (bytes > shared) shared = bytes;
     }
   }
@@ -396,13 +398,14 @@ rns8_status rns8_mi355x_gemm_i8_scaled(rns8_context* ctx, const rns8_mi355x_gemm
   return run_operator(
       ctx, args, stream, check_gemm,
       [](const rns8_mi355x_gemm_i8_args& a) {
-        return check_workspace(a.workspace, a.workspace_bytes, gemm_i8_bytes(a));
+        return check_workspace(a.workspace, a.workspace_bytes, gemm_i8_bytes(a, false));
       },
-      launch_gemm_i8);
+      [](const rns8_mi355x_gemm_i8_args& a, hipStream_t s) { return launch_gemm_i8(a, false, s); });
 }
 
 rns8_status rns8_mi355x_gemm_i8_scaled_workspace(const rns8_mi355x_gemm_i8_args* args, uint64_t* bytes) {
-  return workspace_query(args, bytes, check_gemm, gemm_i8_bytes);
+  return workspace_query(args, bytes, check_gemm,
+                         [](const rns8_mi355x_gemm_i8_args& a) { return gemm_i8_bytes(a, false); });
 }
 
 rns8_status rns8_mi355x_linear_i8(rns8_context* ctx, const rns8_mi355x_linear_i8_args* args, void* stream) {
@@ -415,7 +418,7 @@ rns8_status rns8_mi355x_linear_i8(rns8_context* ctx, const rns8_mi355x_linear_i8
         LinearParts p;
         linear_parts(a, p);
         const hipError_t e = launch_quantize_rows(p.quantize, s);
-        return e != hipSuccess ? e : launch_gemm_i8(p.gemm, s);
+        return e != hipSuccess ? e : launch_gemm_i8(p.gemm, p.zero_filled, s);
       });
 }
 
@@ -436,10 +439,10 @@ rns8_status rns8_mi355x_linear_i8_backward(rns8_context* ctx, const rns8_mi355x_
         hipError_t e = hipSuccess;
         if (a.dx) {
           e = launch_quantize_rows(p.rows, s);
-          if (e == hipSuccess) e = launch_gemm_i8(p.dx, s);
+          if (e == hipSuccess) e = launch_gemm_i8(p.dx, true, s);
         }
         if (e == hipSuccess && (a.dw || a.dbias)) e = launch_quantize_columns(p.columns, s);
-        if (e == hipSuccess && a.dw) e = launch_gemm_i8(p.dw, s);
+        if (e == hipSuccess && a.dw) e = launch_gemm_i8(p.dw, true, s);
         return e;
       });
 }

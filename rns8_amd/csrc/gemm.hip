@@ -746,8 +746,6 @@ hipError_t launch_zero_words(uint32_t* dst, uint64_t words, hipStream_t stream) 
   return hipGetLastError();
 }
 
-namespace {
-
 // Compute units of the current device (cached per device id; contexts on
 // several threads may launch at once, so the cache is atomic).
 int device_cu_count() {
@@ -761,6 +759,8 @@ int device_cu_count() {
   }
   return cus;
 }
+
+namespace {
 
 // K chunks of 128 that every unit of a launch runs.
 uint32_t k_pairs(int64_t k_slice) { return static_cast<uint32_t>((k_slice + 127) / 128); }

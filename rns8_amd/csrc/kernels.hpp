@@ -191,6 +191,7 @@ struct GemmShape {
   int64_t k_slice;    // K of one slice
   uint64_t ws_bytes;  // workspace: slices * nplanes * m * padded_ld(n) bytes when split, else 0
 };
+int device_cu_count();  // compute units of the current device (gemm.hip)
 // Workgroups of a persistent launch: one per unit, at most one per resident
 // slot (a multiple of 8), and from 8 units on a multiple of 8, one share per
 // XCD. Rounded up: the XCDs' shares differ by one unit at most, so no workgroup

@@ -20,8 +20,10 @@ uint64_t quantize_columns_bytes(int64_t rows, int64_t cols);
 hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& a, hipStream_t stream);
 
 // ---- scaled product (scaled_gemm.hip) ----------------------------------------------
-uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a);
-hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, hipStream_t stream);
+// a_zero_filled: a's rows hold zeros from k up to the next multiple of 16 (and
+// their stride reaches it), as quantized rows do: the product may read them.
+uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled);
+hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, hipStream_t stream);
 
 // ---- block norm (block_norm.hip) ------------------------------------------------------
 constexpr int64_t kMaxNormCols = 32768;

@@ -1,94 +1,111 @@
 // The product of 8-bit matrices with a scale for each row and each column
-// (gfx950):
-//   out[i][j] = a_scale[i] b_scale[j] sum_k a[i][k] b(k, j) + bias[j].
-//
-// 64 x 64 tiles, four waves; both operands are staged K-contiguous in LDS, 64
-// of K at a time, and multiplied by v_mfma_i32_16x16x64_i8. Sums run in int32
-// over blocks of 65536 K (|a b| <= 2^14: below 2^30) and are joined in 64 bits.
+// (gfx950): operands that the kernels cannot read in place are copied first,
+// then the kernel of the product's shape runs.
+#include <algorithm>
+
 #include "elements.hpp"
-#include "operators.hpp"
+#include "scaled_gemm.hpp"
 
 namespace rns8x {
 namespace {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
-
-struct GemmI8Args {
-  int64_t m, n, k;
-  const int8_t *a, *b;
-  int64_t lda, ldb;
-  const float *a_scale, *b_scale, *bias;
-  void* out;
-  int64_t ldo;
-  uint32_t tiles_n;
-  uint32_t inner;
+// Copies rows of `cols` bytes at any address and stride to rows at stride ldd
+// (cols rounded up to 16) and fills them up with zeros.
+struct CopyArgs {
+  const int8_t* src;
+  int64_t rows, cols, lds;
+  int8_t* dst;
+  int64_t ldd;
 };
 
-constexpr int kTile = 64, kStep = 64, kPitch = kStep + 16;
-
-template <typename T>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(GemmI8Args g) {
-  __shared__ __attribute__((aligned(16))) int8_t as[kTile * kPitch], bs[kTile * kPitch];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x / g.tiles_n) * kTile, n0 = static_cast<int64_t>(blockIdx.x % g.tiles_n) * kTile;
-  int64_t total[4][4] = {};
-  for (int64_t k0 = 0; k0 < g.k;) {
-    const int64_t stop = k0 + 65536 < g.k ? k0 + 65536 : g.k;
-    v4i acc[4] = {};
-    for (; k0 < stop; k0 += kStep) {
-      for (int e = threadIdx.x; e < kTile * kStep; e += 256) {
-        const int r = e / kStep, c = e % kStep;
-        const int64_t k = k0 + c;
-        as[r * kPitch + c] = m0 + r < g.m && k < stop ? g.a[(m0 + r) * g.lda + k] : 0;
-        if (!g.inner) bs[r * kPitch + c] = n0 + r < g.n && k < stop ? g.b[(n0 + r) * g.ldb + k] : 0;
-        else bs[c * kPitch + r] = n0 + c < g.n && k0 + r < stop ? g.b[(k0 + r) * g.ldb + n0 + c] : 0;
-      }
-      __syncthreads();
-      const v4i fa = *reinterpret_cast<const v4i*>(as + (16 * wave + (lane & 15)) * kPitch + 16 * (lane >> 4));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const v4i fb = *reinterpret_cast<const v4i*>(bs + (16 * j + (lane & 15)) * kPitch + 16 * (lane >> 4));
-        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb, fa, acc[j], 0, 0, 0);
-      }
-      __syncthreads();
+__global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
+  const int64_t chunks = a.ldd / 16, total = a.rows * chunks;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / chunks, c = 16 * (i - row * chunks);
+    const int8_t* const from = a.src + row * a.lds + c;
+    uint32_t w[4] = {};
+    if (c + 16 <= a.cols) {
+      __builtin_memcpy(w, from, 16);
+    } else {
+      for (int b = 0; c + b < a.cols; ++b) w[b >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(from[b])) << (8 * (b & 3));
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) total[j][e] += acc[j][e];
+    __builtin_memcpy(a.dst + row * a.ldd + c, w, 16);
   }
-  const int64_t row = m0 + 16 * wave + (lane & 15);
-  if (row >= g.m) return;
-  const float sa = g.a_scale ? g.a_scale[row] : 1.0f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t col = n0 + 16 * j + 4 * (lane >> 4) + e;
-      if (col >= g.n) continue;
-      const float v = static_cast<float>(total[j][e]) * sa * (g.b_scale ? g.b_scale[col] : 1.0f);
-      static_cast<T*>(g.out)[row * g.ldo + col] = static_cast<T>(v + (g.bias ? g.bias[col] : 0.0f));
-    }
+}
+
+hipError_t launch_copy_rows(const CopyArgs& a, hipStream_t stream) {
+  const int64_t blocks = (a.rows * (a.ldd / 16) + 255) / 256;
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL(copy_rows_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0,
+                     stream, a);
+  return hipGetLastError();
+}
+
+bool in_place(const int8_t* p, int64_t ld) { return ld % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// The workspace: copies of the operands that need one, then the partial sums.
+struct Plan {
+  bool copy_a, copy_b;
+  int64_t lda, ldb, b_rows, b_cols;
+  uint64_t a_at, b_at, sums_at, bytes;
+  TileShape tiles;
+};
+
+Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
+  Plan p{};
+  const bool inner = g.b_layout == RNS8_MI355X_B_INNER;
+  p.b_rows = inner ? g.k : g.n;
+  p.b_cols = inner ? g.n : g.k;
+  // where b is n x k, a's chunks are read whole: they have to end in zeros
+  p.copy_a = g.k > 0 && !(in_place(g.a, g.lda) && (inner || a_zero_filled || g.k % 16 == 0));
+  p.copy_b = g.k > 0 && !in_place(g.b, g.ldb);
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t got = at;
+    at += round_up(bytes, 256);
+    return got;
+  };
+  p.lda = p.copy_a ? static_cast<int64_t>(round_up(static_cast<uint64_t>(g.k), 16)) : g.lda;
+  p.ldb = p.copy_b ? static_cast<int64_t>(round_up(static_cast<uint64_t>(p.b_cols), 16)) : g.ldb;
+  if (p.copy_a) p.a_at = take(static_cast<uint64_t>(g.m) * static_cast<uint64_t>(p.lda));
+  if (p.copy_b) p.b_at = take(static_cast<uint64_t>(p.b_rows) * static_cast<uint64_t>(p.ldb));
+  p.tiles = choose_tile_shape(g.m, g.n, g.k, inner);
+  p.sums_at = take(p.tiles.bytes);
+  p.bytes = at;
+  return p;
 }
 
 }  // namespace
 
-uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args&) { return 0; }
+uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
+  return g.m == 0 || g.n == 0 ? 0u : make_plan(g, a_zero_filled).bytes;
+}
 
-hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, hipStream_t stream) {
+hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return hipSuccess;
-  const int64_t tiles_m = (g.m + kTile - 1) / kTile, tiles_n = (g.n + kTile - 1) / kTile;
-  if (tiles_m > (int64_t{1} << 23) / tiles_n) return hipErrorInvalidValue;
-  const GemmI8Args a{g.m, g.n, g.k, g.a, g.b, g.lda, g.ldb, g.a_scale, g.b_scale, g.bias, g.out, g.ldo,
-                     static_cast<uint32_t>(tiles_n), g.b_layout == RNS8_MI355X_B_INNER};
-  const dim3 grid(static_cast<unsigned>(tiles_m * tiles_n));
-  switch (g.dtype) {
-    case RNS8_MI355X_F32: hipLaunchKernelGGL(gemm_i8_kernel<float>, grid, dim3(256), 0, stream, a); break;
-    case RNS8_MI355X_F16: hipLaunchKernelGGL(gemm_i8_kernel<f16>, grid, dim3(256), 0, stream, a); break;
-    case RNS8_MI355X_BF16: hipLaunchKernelGGL(gemm_i8_kernel<bf16>, grid, dim3(256), 0, stream, a); break;
-    default: return hipErrorInvalidValue;
+  const Plan p = make_plan(g, a_zero_filled);
+  uint8_t* const ws = static_cast<uint8_t*>(g.workspace);
+  ScaledGemm s{g.m, g.n, g.k, g.a, g.b, p.lda, p.ldb, g.b_layout == RNS8_MI355X_B_INNER, g.a_scale, g.b_scale, g.bias,
+               g.out, g.ldo, g.dtype};
+  if (p.copy_a) {
+    int8_t* const to = reinterpret_cast<int8_t*>(ws + p.a_at);
+    const hipError_t e = launch_copy_rows({g.a, g.m, g.k, g.lda, to, p.lda}, stream);
+    if (e != hipSuccess) return e;
+    s.a = to;
   }
-  return hipGetLastError();
+  if (p.copy_b) {
+    int8_t* const to = reinterpret_cast<int8_t*>(ws + p.b_at);
+    const hipError_t e = launch_copy_rows({g.b, p.b_rows, p.b_cols, g.ldb, to, p.ldb}, stream);
+    if (e != hipSuccess) return e;
+    s.b = to;
+  }
+  if (g.k == 0) {  // no operand is read (their buffers are empty): any aligned address will do
+    s.a = s.b = static_cast<const int8_t*>(g.out) - reinterpret_cast<uintptr_t>(g.out) % 16;
+    s.lda = 0;
+    s.ldb = s.inner ? static_cast<int64_t>(round_up(static_cast<uint64_t>(g.n), 16)) : 0;
+  }
+  return launch_scaled_tiles(s, p.tiles, reinterpret_cast<int32_t*>(ws + p.sums_at), stream);
 }
 
 }  // namespace rns8x

@@ -1,0 +1,41 @@
+// Internal interface of the scaled 8-bit product's kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "operators.hpp"
+
+namespace rns8x {
+
+// Operands as the kernels read them: 16-byte aligned rows at strides that are
+// multiples of 16 below 2^23. `k` may end inside a 16-byte chunk: where b is n x
+// k, a's bytes from k to the chunk's end are zeros and b's may hold anything.
+struct ScaledGemm {
+  int64_t m, n, k;
+  const int8_t *a, *b;
+  int64_t lda, ldb;
+  bool inner;  // b is k x n
+  const float *a_scale, *b_scale, *bias;
+  void* out;
+  int64_t ldo;
+  uint32_t dtype;
+};
+
+// How the tile kernel splits a product: slices == 1 writes the output, more
+// leave int32 partial sums [slices][m][ldp] that launch_join_slices adds.
+struct TileShape {
+  uint32_t bm, bn;  // the tile
+  uint32_t slices;
+  int64_t k_slice;  // a multiple of 128 where slices > 1
+  int64_t ldp;
+  uint64_t bytes;
+};
+TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k, bool inner);
+hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int32_t* partials, hipStream_t stream);
+
+// Products of at most this many bytes in one int32 sum: |a b| <= 2^14.
+constexpr int64_t kExactK = 131071;
+
+}  // namespace rns8x
