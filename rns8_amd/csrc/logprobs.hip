@@ -1,12 +1,30 @@
 // Log-probabilities of given tokens, entropy and top alternatives, and their
 // gradient (gfx950).
 //
-// With z = scale * logit and a maximum m over the row:
-//   S = sum exp(z - m),  W = sum exp(z - m) (z - m)
-//   lse = m + log S,  logp = (z[target] - m) - log S,  entropy = log S - W / S
-// S and W are kept for a running maximum: when it rises by d, S becomes
-// S e^-d and W becomes (W - d S) e^-d, so one pass over the row is enough. The
-// kernels are bound by reading the logits.
+// With a maximum m over the row's logits, c = scale * log2(e) and d = (v - m) c
+// for each logit v:
+//   S = sum 2^d,  W = sum 2^d d
+//   lse = scale m + ln S,  logp = ln2 (d[target] - log2 S),  entropy = ln2 (log2 S - W / S)
+// S and W are kept for a running maximum: when it rises by t (in powers of two),
+// S becomes S 2^-t and W becomes (W - t S) 2^-t, so one pass over the row is
+// enough. The difference v - m comes first, so that a term's error goes with
+// its distance from the maximum and logits of any size (a mask of the type's
+// lowest value) are as good as others. 32 bits hold every sum. Both kernels are
+// bound by reading the logits (and writing their gradient): a logit costs about
+// eleven vector operations, the exponential counted as four, beside its bytes.
+//
+// Few rows are cut into parts of a few thousand logits, one workgroup each,
+// whose sums and alternatives a second kernel joins: 4 rows of 131072 would
+// occupy 4 of 256 CUs.
+//
+// Alternatives: a part keeps its logits in registers over both looks at them.
+// The n-th largest of any n different threads' maxima is a lower bound of the
+// part's n-th largest logit, so with 4 waves the least of the waves'
+// ceil(n/4)-th largest lane maxima is one: the few logits from there on are
+// gathered and ordered by counting. Where too many are equal (a part of one
+// value) the alternatives are taken one by one.
+#include <algorithm>
+
 #include "elements.hpp"
 #include "operators.hpp"
 #include "row_shape.hpp"
@@ -14,195 +32,483 @@
 namespace rns8x {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kVector = 8;                     // logits of one load
+constexpr int kStride = kThreads * kVector;    // logits of one round of a workgroup
+constexpr int kHeldRounds = 4;                 // rounds that stay in registers
+constexpr int64_t kMaxParts = 64;              // a wave joins a row
+constexpr uint32_t kMaxCandidates = 512;
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-// The sums of a part of a row. m = -infinity: nothing but ruled-out tokens yet.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The sums of a part of a row over its maximum m (a logit; -infinity: nothing
+// but ruled-out tokens so far, s = w = 0). A NaN logit makes s NaN.
 struct Sums {
   float m, s, w;
 };
 
-__device__ __forceinline__ Sums join(Sums a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return a.m != a.m || a.s != a.s ? a : b;
-  const float da = a.m == -INFINITY ? 0.0f : a.m - m, db = b.m == -INFINITY ? 0.0f : b.m - m;
-  const float ea = a.m == -INFINITY ? 0.0f : expf(da), eb = b.m == -INFINITY ? 0.0f : expf(db);
-  // (a part without tokens has s = w = 0; a NaN stays in s. A part that the
-  // maximum has left behind by more than floats hold adds nothing: its d s may
-  // be infinite, as beside a mask of the type's lowest value)
-  const float wa = ea > 0.0f ? (a.w + da * a.s) * ea : 0.0f, wb = eb > 0.0f ? (b.w + db * b.s) * eb : 0.0f;
-  return {m, a.s * ea + b.s * eb, wa + wb};
+__device__ __forceinline__ bool is_empty(Sums t) { return t.m == -INFINITY && t.s == 0.0f; }
+// What logits are compared with: m, or 0 while every logit is ruled out.
+__device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// `a` for a maximum m >= a.m.
+__device__ __forceinline__ Sums rescale(Sums a, float m, float c) {
+  if (a.m == m || a.m == -INFINITY) return {m, a.s, a.w};
+  const float t = (a.m - m) * c, e = exp2_fast(t);
+  // (sums that the maximum has left behind by more than floats hold: t s may be infinite)
+  return {m, a.s * e, e > 0.0f ? (a.w + t * a.s) * e : 0.0f};
+}
+
+struct MaxF {
+  __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const {
+    return as_uint(fmaxf(as_float(a), as_float(b)));
+  }
+};
+__device__ __forceinline__ float wave_max(float x) { return as_float(wave_reduce(as_uint(x), MaxF{})); }
+__device__ __forceinline__ float wave_sum(float x) { return as_float(wave_reduce(as_uint(x), AddF{})); }
+
+__device__ __forceinline__ Sums wave_join(Sums t, float c) {
+  t = rescale(t, wave_max(t.m), c);
+  t.s = wave_sum(t.s);
+  t.w = wave_sum(t.w);
+  return t;
+}
+
+// The workgroup's sums from its waves'.
+__device__ __forceinline__ Sums join_waves(const Sums* wave_sums, float c) {
+  float m = wave_sums[0].m;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, wave_sums[w].m);
+  Sums t = rescale(wave_sums[0], m, c);
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    const Sums u = rescale(wave_sums[w], m, c);
+    t.s += u.s;
+    t.w += u.w;
+  }
+  return t;
+}
+
+__device__ __forceinline__ void add_logits(Sums& t, const float (&v)[kVector], float c) {
+  float m = t.m;
+#pragma unroll
+  for (int i = 0; i < kVector; ++i) m = fmaxf(m, v[i]);
+  if (m > t.m) t = rescale(t, m, c);
+  const float from = origin(m);
+#pragma unroll
+  for (int i = 0; i < kVector; ++i) {
+    const float d = (v[i] - from) * c, e = exp2_fast(d);
+    t.s += e;
+    t.w = fmaf(e, fmaxf(d, -200.0f), t.w);  // (2^-200 is 0 in 32 bits, and so is its term)
+  }
+}
+
+// Order of the alternatives as one unsigned integer: the logit's order (NaNs
+// above infinity, 0 and -0 equal) above the complement of the index. Neither 0 nor all ones.
+__device__ __forceinline__ uint64_t rank_key(float v, uint32_t index) {
+  const uint32_t b = as_uint(v + 0.0f);
+  uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
+  if (v != v) order = 0xFFFFFFFEu;
+  return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~index);
+}
+
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
+  const uint32_t hi = wave_reduce(static_cast<uint32_t>(key >> 32), MaxU{});
+  const uint32_t lo = static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u;
+  return static_cast<uint64_t>(hi) << 32 | wave_reduce(lo, MaxU{});
 }
 
 struct Args {
   const void* logits;
   int64_t rows, vocab, ldl;
   const int64_t* targets;
-  float scale;
+  float scale, c;
   uint32_t top;
   float *logp, *entropy, *lse;
   int32_t* top_ids;
   float* top_logp;
+  int64_t parts, part_len;  // part_len: a multiple of kStride where parts > 1
+  float* part_sums;         // [rows][parts][4]
+  uint64_t* part_keys;      // [rows][parts][top]
 };
 
-// Order of the alternatives as one unsigned integer: the logit's order (NaNs
-// above infinity, 0 and -0 equal) above the complement of the index.
-__device__ __forceinline__ uint64_t rank_key(float z, uint32_t index) {
-  const uint32_t b = as_uint(z + 0.0f);
-  uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
-  if (z != z) order = 0xFFFFFFFFu;
-  return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~index);
+// The log-probability of a logit.
+__device__ __forceinline__ float logp_of(float v, Sums t, float c) {
+  return is_empty(t) ? -INFINITY : kLn2 * ((v - origin(t.m)) * c - log2f(t.s));
+}
+
+// A row's results from its sums (one thread).
+template <typename T>
+__device__ __forceinline__ void write_row(const Args& a, int64_t row, Sums t) {
+  const float log_s = log2f(t.s);
+  if (a.lse) a.lse[row] = is_empty(t) ? -INFINITY : origin(t.m) * a.scale + kLn2 * log_s;
+  if (a.entropy) a.entropy[row] = is_empty(t) ? 0.0f : kLn2 * (log_s - t.w / t.s);
+  if (a.logp) {
+    const int64_t target = a.targets[row];
+    const bool asked = target >= 0 && target < a.vocab;
+    a.logp[row] = asked ? logp_of(static_cast<float>(static_cast<const T*>(a.logits)[row * a.ldl + target]), t, a.c) : 0.0f;
+  }
 }
 
 template <typename T>
+__device__ __forceinline__ void write_alternative(const Args& a, int64_t row, uint32_t rank, uint64_t key, Sums t) {
+  const uint32_t id = ~static_cast<uint32_t>(key);
+  if (a.top_ids) a.top_ids[row * a.top + rank] = static_cast<int32_t>(id);
+  if (a.top_logp)
+    a.top_logp[row * a.top + rank] = logp_of(static_cast<float>(static_cast<const T*>(a.logits)[row * a.ldl + id]), t, a.c);
+}
+
+template <typename T>
+struct Held {
+  T v[kVector];
+};
+
+// kRounds: rounds of a part held in registers (0: every part is read again for
+// its alternatives, if any are asked for).
+template <typename T, int kRounds>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
-  __shared__ Sums parts[kThreads / 64];
-  __shared__ uint64_t keys[kThreads / 64];
+  __shared__ Sums wave_sums[kWaves];
+  __shared__ float wave_least[kWaves];
+  __shared__ uint64_t keys[kMaxCandidates];
+  __shared__ uint32_t count;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
+    const int64_t row = unit / a.parts, part = unit - row * a.parts;
     const T* const z = static_cast<const T*>(a.logits) + row * a.ldl;
+    const int64_t first = part * a.part_len, last = min(a.vocab, first + a.part_len);
     Sums t{-INFINITY, 0.0f, 0.0f};
-    for (int64_t c = 8 * threadIdx.x; c < a.vocab; c += 8 * kThreads) {
-      float v[8];
-      load_upto8(z + c, a.vocab - c, v, -INFINITY);
-      float m = t.m;
+    constexpr int kHold = kRounds > 0 ? kRounds : 1;
+    Held<T> held[kHold];
+    auto load = [&](int64_t at, Held<T>& h) {
+      if (at + kVector <= last) {
+        __builtin_memcpy(h.v, z + at, sizeof(h.v));
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] *= a.scale;
-        m = fmaxf(m, v[i]);
+        for (int i = 0; i < kVector; ++i) h.v[i] = at + i < last ? z[at + i] : static_cast<T>(-INFINITY);
       }
-      Sums u{m, 0.0f, 0.0f};
+    };
+    auto floats = [&](const Held<T>& h, float (&v)[kVector]) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool out = v[i] == -INFINITY;
-        const float d = out ? 0.0f : v[i] - m, e = out ? 0.0f : expf(d);
-        u.s += e;
-        u.w += e * d;
+      for (int i = 0; i < kVector; ++i) v[i] = static_cast<float>(h.v[i]);
+    };
+    float v[kVector];
+    if constexpr (kRounds > 0) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) load(first + r * kStride + kVector * threadIdx.x, held[r]);
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        floats(held[r], v);
+        add_logits(t, v, a.c);
       }
-      if (m != t.m) t = join({t.m, t.s, t.w}, {m, 0.0f, 0.0f});
-      t.s += u.s;
-      t.w += u.w;
+    } else {
+      int64_t at = first + kVector * threadIdx.x;
+      for (; at + kStride + kVector <= last; at += 2 * kStride) {
+        Held<T> next;
+        load(at, held[0]);
+        load(at + kStride, next);
+        floats(held[0], v);
+        add_logits(t, v, a.c);
+        floats(next, v);
+        add_logits(t, v, a.c);
+      }
+      for (; at < last; at += kStride) {
+        load(at, held[0]);
+        floats(held[0], v);
+        add_logits(t, v, a.c);
+      }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const Sums o{__shfl_xor(t.m, d), __shfl_xor(t.s, d), __shfl_xor(t.w, d)};
-      // (the same order of operands in both lanes: both get the same bits)
-      t = lane & d ? join(o, t) : join(t, o);
+    const float lane_max = t.m;
+    t = wave_join(t, a.c);
+    if (lane == 0) wave_sums[wave] = t;
+    if (a.top) {
+      // the wave's ceil(top / 4)-th largest lane maximum
+      float mine = lane_max, least = -INFINITY;
+      for (uint32_t k = 0; k < (a.top + kWaves - 1) / kWaves; ++k) {
+        least = wave_max(mine);
+        const uint64_t who = __ballot(mine == least);
+        if (lane == __ffsll(static_cast<unsigned long long>(who)) - 1) mine = -INFINITY;
+      }
+      if (lane == 0) wave_least[wave] = least;
+      if (threadIdx.x == 0) count = 0;
     }
-    if (lane == 0) parts[wave] = t;
     __syncthreads();
-    t = parts[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) t = join(t, parts[w]);
-    const float log_s = logf(t.s);
-    const bool empty = t.m == -INFINITY && t.s == 0.0f;
+    t = join_waves(wave_sums, a.c);
     if (threadIdx.x == 0) {
-      if (a.lse) a.lse[row] = empty ? -INFINITY : t.m + log_s;
-      if (a.entropy) a.entropy[row] = empty ? 0.0f : log_s - t.w / t.s;
-      if (a.logp) {
-        const int64_t target = a.targets[row];
-        const bool asked = target >= 0 && target < a.vocab;
-        a.logp[row] = !asked ? 0.0f : empty ? -INFINITY : (static_cast<float>(z[target]) * a.scale - t.m) - log_s;
+      if (a.parts == 1) {
+        write_row<T>(a, row, t);
+      } else {
+        const float w[4] = {t.m, t.s, t.w, 0.0f};
+        __builtin_memcpy(a.part_sums + 4 * unit, w, 16);
       }
     }
-    // the alternatives, one pass for each
-    uint64_t last = ~uint64_t{0};
-    for (uint32_t k = 0; k < a.top; ++k) {
-      uint64_t best = 0;
-      for (int64_t c = threadIdx.x; c < a.vocab; c += kThreads) {
-        const uint64_t key = rank_key(static_cast<float>(z[c]), static_cast<uint32_t>(c));
-        if ((k == 0 || key < last) && key > best) best = key;
-      }
+    if (a.top) {
+      float from = wave_least[0];
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(best), d));
-        best = best > o ? best : o;
-      }
-      if (lane == 0) keys[wave] = best;
-      __syncthreads();
+      for (int w = 1; w < kWaves; ++w) from = fminf(from, wave_least[w]);
+      auto gather = [&](int64_t at, const Held<T>& h) {
 #pragma unroll
-      for (int w = 0; w < kThreads / 64; ++w) best = best > keys[w] ? best : keys[w];
+        for (int i = 0; i < kVector; ++i) {
+          const float u = static_cast<float>(h.v[i]);
+          if (!(u < from) && at + i < last) {
+            const uint32_t slot = atomicAdd(&count, 1u);
+            if (slot < kMaxCandidates) keys[slot] = rank_key(u, static_cast<uint32_t>(at + i));
+          }
+        }
+      };
+      auto each = [&](auto&& f) {
+        if constexpr (kRounds > 0) {
+#pragma unroll
+          for (int r = 0; r < kRounds; ++r) f(first + r * kStride + kVector * threadIdx.x, held[r]);
+        } else {
+          for (int64_t at = first + kVector * threadIdx.x; at < last; at += kStride) {
+            load(at, held[0]);
+            f(at, held[0]);
+          }
+        }
+      };
+      each(gather);
       __syncthreads();
-      last = best;
-      if (threadIdx.x == 0) {
-        const uint32_t id = ~static_cast<uint32_t>(best);
-        if (a.top_ids) a.top_ids[row * a.top + k] = static_cast<int32_t>(id);
-        if (a.top_logp)
-          a.top_logp[row * a.top + k] = empty ? -INFINITY : (static_cast<float>(z[id]) * a.scale - t.m) - log_s;
+      auto put = [&](uint32_t rank, uint64_t key) {
+        if (a.parts == 1)
+          write_alternative<T>(a, row, rank, key, t);
+        else
+          a.part_keys[unit * a.top + rank] = key;
+      };
+      const uint32_t n = count;
+      if (n <= kMaxCandidates) {
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+          const uint64_t key = keys[i];
+          uint32_t rank = 0;
+          for (uint32_t j = 0; j < n; ++j) rank += keys[j] > key;
+          if (rank < a.top) put(rank, key);
+        }
+        // (a part shorter than `top`: its list ends in zeros, below every key)
+        for (uint32_t i = n + threadIdx.x; i < a.top; i += kThreads) put(i, 0);
+      } else {
+        uint64_t before = ~uint64_t{0};
+        for (uint32_t k = 0; k < a.top; ++k) {
+          uint64_t best = 0;
+          each([&](int64_t at, const Held<T>& h) {
+#pragma unroll
+            for (int i = 0; i < kVector; ++i) {
+              const uint64_t key = rank_key(static_cast<float>(h.v[i]), static_cast<uint32_t>(at + i));
+              if (at + i < last && key < before && key > best) best = key;
+            }
+          });
+          best = wave_max_key(best);
+          __syncthreads();  // (the last round's keys are read)
+          if (lane == 0) keys[wave] = best;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) best = best > keys[w] ? best : keys[w];
+          before = best;
+          if (threadIdx.x == 0) put(k, best);
+        }
       }
     }
-    __syncthreads();
+    __syncthreads();  // the next unit writes the shared words
   }
 }
+
+// One wave to a row: lane p holds part p.
+template <typename T>
+__global__ __launch_bounds__(64) void join_parts_kernel(Args a) {
+  extern __shared__ uint64_t lists[];  // [parts][top]
+  const int lane = threadIdx.x;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    Sums t{-INFINITY, 0.0f, 0.0f};
+    if (lane < a.parts) {
+      float w[4];
+      __builtin_memcpy(w, a.part_sums + 4 * (row * a.parts + lane), 16);
+      t = {w[0], w[1], w[2]};
+    }
+    const uint64_t* const from = a.part_keys + row * a.parts * a.top;
+    __syncthreads();
+    for (int64_t i = lane; i < a.parts * a.top; i += 64) lists[i] = from[i];
+    t = wave_join(t, a.c);
+    if (lane == 0) write_row<T>(a, row, t);
+    __syncthreads();
+    uint32_t at = 0;
+    uint64_t head = a.top && lane < a.parts ? lists[lane * a.top] : 0;
+    for (uint32_t k = 0; k < a.top; ++k) {
+      const uint64_t best = wave_max_key(head);
+      if (head == best) {  // (keys differ: one lane)
+        write_alternative<T>(a, row, k, best, t);
+        ++at;
+        head = at < a.top ? lists[lane * a.top + at] : 0;
+      }
+    }
+  }
+}
+
+// ---- gradient --------------------------------------------------------------------------
+// dlogit = -scale p (gl + ge (log p + entropy)), and scale gl more at the target,
+// log p = scale v - lse. Where lse is so large that its 32 bits have lost the
+// logarithm of the sum (a row of nothing but a mask's lowest value), the row's
+// maximum and sum are computed again.
+constexpr float kLargeLse = 4096.0f;  // a step of 2^-11
 
 struct BackArgs {
   const void* logits;
   int64_t rows, vocab, ldl;
   const int64_t* targets;
-  float scale;
+  float scale, c;
   const float *lse, *entropy, *dlogp, *dentropy;
   void* dlogits;
   int64_t lddl;
+  int64_t parts, part_len;
 };
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a) {
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  __shared__ Sums wave_sums[kWaves];
+  for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
+    const int64_t row = unit / a.parts, part = unit - row * a.parts;
+    const int64_t first = part * a.part_len, last = min(a.vocab, first + a.part_len);
     const T* const z = static_cast<const T*>(a.logits) + row * a.ldl;
     T* const out = static_cast<T*>(a.dlogits) + row * a.lddl;
-    const float lse = a.lse[row];
     const int64_t target = a.dlogp ? a.targets[row] : -1;
     const bool asked = target >= 0 && target < a.vocab;
     const float gl = asked ? a.dlogp[row] : 0.0f;
-    const float ge = a.dentropy ? a.dentropy[row] : 0.0f, entropy = a.dentropy ? a.entropy[row] : 0.0f;
-    for (int64_t c = 8 * threadIdx.x; c < a.vocab; c += 8 * kThreads) {
-      float v[8], d[8];
-      load_upto8(z + c, a.vocab - c, v, -INFINITY);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool out_of = v[i] == -INFINITY;
-        const float logp = out_of ? 0.0f : v[i] * a.scale - lse;
-        const float p = out_of ? 0.0f : expf(logp);
-        const float hit = asked && c + i == target ? 1.0f : 0.0f;
-        d[i] = out_of ? 0.0f : a.scale * (gl * (hit - p) - (p == 0.0f ? 0.0f : ge * p * (logp + entropy)));
+    const float ge = a.dentropy ? a.dentropy[row] : 0.0f;
+    const float rest = a.dentropy ? gl + ge * a.entropy[row] : gl;
+    float from = 0.0f, log_s = a.lse[row];  // log p = scale (v - from) - log_s
+    if (fabsf(log_s) > kLargeLse) {
+      Sums t{-INFINITY, 0.0f, 0.0f};
+      for (int64_t at = kVector * threadIdx.x; at < a.vocab; at += kStride) {
+        float v[kVector];
+        load_upto8(z + at, a.vocab - at, v, -INFINITY);
+        add_logits(t, v, a.c);
       }
-      store_upto8(out + c, a.vocab - c, d);
+      t = wave_join(t, a.c);
+      if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = t;
+      __syncthreads();
+      t = join_waves(wave_sums, a.c);
+      // (where dlogits is logits: nothing is written before the whole row is read)
+      __syncthreads();
+      from = origin(t.m);
+      log_s = is_empty(t) ? 0.0f : kLn2 * log2f(t.s);
+    }
+    auto grad = [&](int64_t at, float (&v)[kVector]) {
+      float d[kVector];
+#pragma unroll
+      for (int i = 0; i < kVector; ++i) {
+        const float logp = fmaf(v[i] - from, a.scale, -log_s), p = exp2_fast(logp * kLog2E);
+        // (p = 0 far below any logit that counts: its factor stays finite)
+        d[i] = -a.scale * p * fmaf(fmaxf(logp, -1e30f), ge, rest);
+      }
+      if (asked && static_cast<uint64_t>(target - at) < kVector) {
+#pragma unroll
+        for (int i = 0; i < kVector; ++i)
+          if (at + i == target && v[i] != -INFINITY) d[i] += a.scale * gl;
+      }
+      store_upto8(out + at, last - at, d);
+    };
+    int64_t at = first + kVector * threadIdx.x;
+    float v[kVector], w[kVector];
+    for (; at + kStride + kVector <= last; at += 2 * kStride) {
+      load8(z + at, v);
+      load8(z + at + kStride, w);
+      grad(at, v);
+      grad(at + kStride, w);
+    }
+    for (; at < last; at += kStride) {
+      load_upto8(z + at, last - at, v, -INFINITY);
+      grad(at, v);
     }
   }
 }
 
-dim3 grid_of(int64_t rows) { return dim3(static_cast<unsigned>(rows < kMaxBlocks ? rows : kMaxBlocks)); }
+// Parts of a row: as many as give about `units` workgroups, none shorter than
+// `least` rounds.
+void cut_rows(int64_t rows, int64_t vocab, int64_t units, int64_t least, int64_t& parts, int64_t& len) {
+  const int64_t rounds = (vocab + kStride - 1) / kStride;
+  parts = std::max<int64_t>(1, std::min({(units + rows - 1) / rows, (rounds + least - 1) / least, kMaxParts}));
+  const int64_t per = (rounds + parts - 1) / parts;
+  parts = (rounds + per - 1) / per;
+  len = per * kStride;
+}
+
+// With alternatives a part is at most kHeldRounds rounds while 64 parts are enough.
+void forward_parts(int64_t rows, int64_t vocab, uint32_t top, int64_t& parts, int64_t& len) {
+  cut_rows(rows, vocab, 1024, top ? 1 : 4, parts, len);
+  const int64_t rounds = (vocab + kStride - 1) / kStride, need = (rounds + kHeldRounds - 1) / kHeldRounds;
+  if (top && need > parts && need <= kMaxParts) {
+    const int64_t per = (rounds + need - 1) / need;
+    parts = (rounds + per - 1) / per;
+    len = per * kStride;
+  }
+}
+
+dim3 grid_of(int64_t units) { return dim3(static_cast<unsigned>(std::min(units, kMaxBlocks))); }
+
+template <typename T>
+hipError_t launch_forward(const Args& a, hipStream_t stream) {
+  const dim3 grid = grid_of(a.rows * a.parts), block(kThreads);
+  const int64_t rounds = a.part_len / kStride;
+  if (a.top == 0 || rounds > kHeldRounds)
+    hipLaunchKernelGGL((logprobs_kernel<T, 0>), grid, block, 0, stream, a);
+  else if (rounds <= 1)
+    hipLaunchKernelGGL((logprobs_kernel<T, 1>), grid, block, 0, stream, a);
+  else if (rounds <= 2)
+    hipLaunchKernelGGL((logprobs_kernel<T, 2>), grid, block, 0, stream, a);
+  else if (rounds <= 4)
+    hipLaunchKernelGGL((logprobs_kernel<T, 4>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((logprobs_kernel<T, kHeldRounds>), grid, block, 0, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == 1) return e;
+  hipLaunchKernelGGL((join_parts_kernel<T>), grid_of(a.rows), dim3(64),
+                     static_cast<unsigned>(a.parts * a.top * sizeof(uint64_t)), stream, a);
+  return hipGetLastError();
+}
+
+template <typename F>
+hipError_t of_dtype(uint32_t dtype, F&& f) {
+  switch (dtype) {
+    case RNS8_MI355X_F32: return f(float{});
+    case RNS8_MI355X_F16: return f(f16{});
+    case RNS8_MI355X_BF16: return f(bf16{});
+    default: return hipErrorInvalidValue;
+  }
+}
 
 }  // namespace
 
-uint64_t logprobs_bytes(const rns8_mi355x_logprobs_args&) { return 0; }
+uint64_t logprobs_bytes(const rns8_mi355x_logprobs_args& g) {
+  if (g.rows == 0) return 0;
+  int64_t parts, len;
+  forward_parts(g.rows, g.vocab, g.top, parts, len);
+  return parts == 1 ? 0u : static_cast<uint64_t>(g.rows) * static_cast<uint64_t>(parts) * (16u + 8u * g.top);
+}
 
 hipError_t launch_logprobs(const rns8_mi355x_logprobs_args& g, hipStream_t stream) {
   if (g.rows == 0) return hipSuccess;
   if (g.top > kMaxTop || g.vocab < 1 || g.vocab > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const bool wanted = g.top_ids || g.top_logp;
-  const Args a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, wanted ? g.top : 0u, g.logp, g.entropy, g.lse,
-               g.top_ids, g.top_logp};
-  switch (g.dtype) {
-    case RNS8_MI355X_F32: hipLaunchKernelGGL(logprobs_kernel<float>, grid_of(g.rows), dim3(kThreads), 0, stream, a); break;
-    case RNS8_MI355X_F16: hipLaunchKernelGGL(logprobs_kernel<f16>, grid_of(g.rows), dim3(kThreads), 0, stream, a); break;
-    case RNS8_MI355X_BF16: hipLaunchKernelGGL(logprobs_kernel<bf16>, grid_of(g.rows), dim3(kThreads), 0, stream, a); break;
-    default: return hipErrorInvalidValue;
-  }
-  return hipGetLastError();
+  Args a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.scale * kLog2E, g.top, g.logp, g.entropy, g.lse,
+         g.top_ids, g.top_logp, 1, 0, nullptr, nullptr};
+  forward_parts(g.rows, g.vocab, g.top, a.parts, a.part_len);
+  a.part_sums = static_cast<float*>(g.workspace);
+  a.part_keys = reinterpret_cast<uint64_t*>(a.part_sums + 4 * g.rows * a.parts);
+  return of_dtype(g.dtype, [&](auto t) { return launch_forward<decltype(t)>(a, stream); });
 }
 
 hipError_t launch_logprobs_backward(const rns8_mi355x_logprobs_backward_args& g, hipStream_t stream) {
   if (g.rows == 0) return hipSuccess;
-  const BackArgs a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.lse, g.entropy, g.dlogp, g.dentropy,
-                   g.dlogits, g.lddl};
-  const dim3 grid = grid_of(g.rows), block(kThreads);
-  switch (g.dtype) {
-    case RNS8_MI355X_F32: hipLaunchKernelGGL(logprobs_backward_kernel<float>, grid, block, 0, stream, a); break;
-    case RNS8_MI355X_F16: hipLaunchKernelGGL(logprobs_backward_kernel<f16>, grid, block, 0, stream, a); break;
-    case RNS8_MI355X_BF16: hipLaunchKernelGGL(logprobs_backward_kernel<bf16>, grid, block, 0, stream, a); break;
-    default: return hipErrorInvalidValue;
+  BackArgs a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.scale * kLog2E, g.lse, g.entropy, g.dlogp,
+             g.dentropy, g.dlogits, g.lddl, 1, 0};
+  cut_rows(g.rows, g.vocab, 1024, 2, a.parts, a.part_len);
+  if (g.dlogits == g.logits) {  // in place a row's logits may be read twice: by the workgroup that writes them
+    a.parts = 1;
+    a.part_len = (g.vocab + kStride - 1) / kStride * kStride;
   }
-  return hipGetLastError();
+  return of_dtype(g.dtype, [&](auto t) {
+    hipLaunchKernelGGL((logprobs_backward_kernel<decltype(t)>), grid_of(a.rows * a.parts), dim3(kThreads), 0, stream,
+                       a);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace rns8x

@@ -207,6 +207,28 @@ def test_gradient_against_differences(gpu_ctx):
         assert abs(slope - float((d.double() * step).sum())) <= 1e-4 * size + 1e-9
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_beside_masks_of_the_lowest_value(gpu_ctx, dtype, in_place):
+    """A row of nothing but the type's lowest value spreads evenly; one left beside such a mask takes it all."""
+    vocab, low = 20000, torch.finfo(dtype).min
+    v = torch.full((3, vocab), low, device="cuda").to(dtype)
+    v[1, 777], v[2, 5:9] = 2.0, -60.0
+    targets, gl, ge = torch.tensor([9, 777, 6], device="cuda"), torch.ones(3, device="cuda"), torch.ones(3, device="cuda")
+    fwd = run(gpu_ctx, v, targets)
+    d = v if in_place else torch.empty_like(v)
+    ops.TokenLogprobsBackward(gpu_ctx, logits=v, lse=fwd["lse"], entropy=fwd["entropy"], targets=targets, dlogp=gl,
+                              dentropy=ge, dlogits=d)()
+    ready()
+    want = torch.zeros(3, vocab, dtype=torch.float64, device="cuda")
+    want[0] = -1 / vocab
+    want[0, 9] += 1
+    want[2, 5:9] = -0.25
+    want[2, 6] += 1
+    # log p and entropy, both near 10 at most, each off by a few of their 32-bit steps, which p multiplies
+    assert_close(d, want, 128 * U32 * (want.abs() + 1.0 / vocab), "dlogits")
+
+
 def test_gradient_in_place(gpu_ctx):
     v = normal(1, 20, 3001).bfloat16()
     targets, gl = torch.arange(20, device="cuda"), normal(2, 20)
