@@ -13,6 +13,8 @@
 //
 // Both are bound by HBM: each row is read once into registers, crosses one
 // reduction for each norm, and is written once.
+#include <algorithm>
+
 #include "elements.hpp"
 #include "operators.hpp"
 #include "row_shape.hpp"
@@ -36,57 +38,53 @@ __device__ __forceinline__ float inverse_rms(float sum_sq, int64_t cols, float e
   return 1.0f / sqrtf(sum_sq / static_cast<float>(cols) + eps);
 }
 
-// Eight values of a row, or of a row that is the same everywhere.
-template <typename T>
-__device__ __forceinline__ void load_or(const void* base, int64_t at, int64_t n, float (&v)[8], float absent) {
+// The same value everywhere where there is no row to load.
+template <int kThreads, typename T, int kVectors>
+__device__ __forceinline__ void load_row_or(const void* base, int64_t at, int64_t cols, int lane, float absent,
+                                            RawRow<T, kVectors>& r) {
   if (base) {
-    load_upto8(static_cast<const T*>(base) + at, n, v, absent);
+    load_row<kThreads>(static_cast<const T*>(base) + at, cols, lane, r);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = absent;
+    for (int j = 0; j < kVectors; ++j) r.v[j].fill(static_cast<T>(absent));
   }
 }
 
 template <typename T, int kThreads, int kVectors>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_kernel(NormArgs a) {
   __shared__ uint32_t scratch[16];
+  using Raw = RawRow<T, kVectors>;
   for_rows<kThreads>(a.rows, [&](int64_t row, int lane) {
-    float v[kVectors][8];  // x, then h
+    Raw x, res, gate, post, pre;
+    load_row<kThreads>(static_cast<const T*>(a.x) + row * a.ldx, a.cols, lane, x);
+    load_row_or<kThreads>(a.residual, row * a.ldresidual, a.cols, lane, 0.0f, res);
+    load_row_or<kThreads>(a.gate, row * a.ldgate, a.cols, lane, 1.0f, gate);
+    load_row_or<kThreads>(a.has_post ? a.post : nullptr, 0, a.cols, lane, 1.0f, post);
     float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
-      if (c < a.cols) load_upto8(static_cast<const T*>(a.x) + row * a.ldx + c, a.cols - c, v[j], 0.0f);
-    }
     float r1 = 1.0f;
     if (a.has_post) {
 #pragma unroll
       for (int j = 0; j < kVectors; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += v[j][i] * v[j][i];
+        for (int i = 0; i < 8; ++i) {
+          const float v = x.v[j].at(i);
+          sum += v * v;
+        }
       r1 = inverse_rms(row_sum<kThreads>(sum, scratch), a.cols, a.eps);
     }
+    load_row_or<kThreads>(a.has_pre ? a.pre : nullptr, 0, a.cols, lane, 1.0f, pre);
+    float h[kVectors][8];
     sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
-      if (c >= a.cols) continue;
-      const int64_t n = a.cols - c;
-      float w[8], g[8], res[8];
-      load_or<T>(a.has_post ? a.post : nullptr, c, n, w, 1.0f);
-      load_or<T>(a.gate, row * a.ldgate + c, n, g, 1.0f);
-      load_or<T>(a.residual, row * a.ldresidual + c, n, res, 0.0f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        // (columns past the row keep 0: x is 0 there, and so is the residual)
-        const float f = v[j][i] * r1 * w[i];
-        const float kept = a.residual ? a.keep * res[i] : 0.0f;
-        v[j][i] = kept + a.branch * g[i] * f;
-        sum += v[j][i] * v[j][i];
+        // (columns past the row are 0: x and the residual are 0 there)
+        const float f = x.v[j].at(i) * r1 * post.v[j].at(i);
+        h[j][i] = a.keep * res.v[j].at(i) + a.branch * gate.v[j].at(i) * f;
+        sum += h[j][i] * h[j][i];
       }
-      if (a.h) store_upto8(static_cast<T*>(a.h) + row * a.ldh + c, n, v[j]);
+      if (a.h) store_vector<kThreads, T, kVectors>(static_cast<T*>(a.h) + row * a.ldh, a.cols, j, lane, h[j]);
     }
     if (!a.has_pre) {
       if (a.rstd && lane == 0) a.rstd[row] = r1;
@@ -100,26 +98,22 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ke
     uint32_t amax = 0;
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
-      if (c >= a.cols) continue;
-      float w[8];
-      load_or<T>(a.pre, c, a.cols - c, w, 1.0f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[j][i] = v[j][i] * r2 * w[i];
+        h[j][i] = h[j][i] * r2 * pre.v[j].at(i);
         // (a NaN row: columns past it hold 0 * NaN, in its scale already)
-        const uint32_t m = magnitude_bits(v[j][i]);
+        const uint32_t m = magnitude_bits(h[j][i]);
         amax = amax > m ? amax : m;
       }
-      if (a.y) store_upto8(static_cast<T*>(a.y) + row * a.ldy + c, a.cols - c, v[j]);
+      if (a.y) store_vector<kThreads, T, kVectors>(static_cast<T*>(a.y) + row * a.ldy, a.cols, j, lane, h[j]);
     }
     if (a.q) {
       const RowScale s = row_scale(row_reduce<kThreads>(amax, MaxU{}, scratch));
       if (lane == 0) a.q_scale[row] = s.scale;
 #pragma unroll
       for (int j = 0; j < kVectors; ++j) {
-        const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
-        if (c < a.stop) store_bytes8(a.q + row * a.ldq, c, a.stop, quantize8(v[j], s.inverse));
+        const int64_t c = column_of<kThreads>(j, lane);
+        if (c < a.stop) store_bytes8(a.q + row * a.ldq, c, a.stop, quantize8(h[j], s.inverse));
       }
     }
   });
@@ -143,91 +137,100 @@ struct NormBackArgs {
 template <typename T, int kThreads, int kVectors>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_backward_kernel(NormBackArgs a) {
   __shared__ uint32_t scratch[16];
+  using Raw = RawRow<T, kVectors>;
+  struct Rows {
+    Raw x, res, gate, dy, dh;
+  };
   float sum_post[kVectors][8] = {}, sum_pre[kVectors][8] = {}, sum_gate[kVectors][8] = {};
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
-  for_rows<kThreads>(a.rows, [&](int64_t row, int lane) {
+  auto load = [&](int64_t row, int lane, Rows& r) {
+    load_row<kThreads>(static_cast<const T*>(a.x) + row * a.ldx, a.cols, lane, r.x);
+    load_row_or<kThreads>(a.residual, row * a.ldresidual, a.cols, lane, 0.0f, r.res);
+    load_row_or<kThreads>(a.gate, row * a.ldgate, a.cols, lane, 1.0f, r.gate);
+    load_row_or<kThreads>(a.dy, row * a.lddy, a.cols, lane, 0.0f, r.dy);
+    load_row_or<kThreads>(a.dh, row * a.lddh, a.cols, lane, 0.0f, r.dh);
+  };
+  auto work = [&](int64_t row, int lane, const Rows& r) {
     const float r1 = a.has_post ? a.rstd[row] : 1.0f;
     const float r2 = a.has_pre ? a.rstd[a.rows + row] : 0.0f;
-    float x[kVectors][8], h[kVectors][8], wdy[kVectors][8];
+    Raw post, pre;
+    load_row_or<kThreads>(a.has_post ? a.post : nullptr, 0, a.cols, lane, 1.0f, post);
+    load_row_or<kThreads>(a.has_pre ? a.pre : nullptr, 0, a.cols, lane, 1.0f, pre);
+    float h[kVectors][8];
     float dot = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
+    for (int j = 0; j < kVectors; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = h[j][i] = wdy[j][i] = 0.0f;
-      if (c >= a.cols) continue;
-      const int64_t n = a.cols - c;
-      float g[8], w[8], res[8], dy[8];
-      load_upto8(static_cast<const T*>(a.x) + row * a.ldx + c, n, x[j], 0.0f);
-      load_or<T>(a.residual, row * a.ldresidual + c, n, res, 0.0f);
-      load_or<T>(a.gate, row * a.ldgate + c, n, g, 1.0f);
-      load_or<T>(a.has_post ? a.post : nullptr, c, n, w, 1.0f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        h[j][i] = (a.residual ? a.keep * res[i] : 0.0f) + a.branch * g[i] * (x[j][i] * r1 * w[i]);
-      if (a.has_pre) {
-        load_or<T>(a.dy, row * a.lddy + c, n, dy, 0.0f);
-        load_or<T>(a.pre, c, n, w, 1.0f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          wdy[j][i] = w[i] * dy[i];
-          dot += wdy[j][i] * h[j][i];
-          sum_pre[j][i] += dy[i] * (h[j][i] * r2);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float f = r.x.v[j].at(i) * r1 * post.v[j].at(i);
+        const float dy = r.dy.v[j].at(i);
+        h[j][i] = a.keep * r.res.v[j].at(i) + a.branch * r.gate.v[j].at(i) * f;
+        dot += pre.v[j].at(i) * dy * h[j][i];
+        sum_pre[j][i] += dy * (h[j][i] * r2);
       }
-    }
     float k2 = 0.0f;
     if (a.has_pre) k2 = r2 * r2 * r2 * (row_sum<kThreads>(dot, scratch) * inv_cols);
     dot = 0.0f;
-    // h becomes dH, wdy becomes w_post df
+    // h becomes w_post df
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
-      if (c >= a.cols) continue;
-      const int64_t n = a.cols - c;
-      float dh[8], g[8], w[8], out[8];
-      load_or<T>(a.dh, row * a.lddh + c, n, dh, 0.0f);
-      load_or<T>(a.gate, row * a.ldgate + c, n, g, 1.0f);
-      load_or<T>(a.has_post ? a.post : nullptr, c, n, w, 1.0f);
+      float out[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[j][i] = dh[i] + r2 * wdy[j][i] - h[j][i] * k2;
+      for (int i = 0; i < 8; ++i)
+        h[j][i] = r.dh.v[j].at(i) +
+                  r2 * (pre.v[j].at(i) * r.dy.v[j].at(i)) - h[j][i] * k2;
       if (a.dresidual) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[i] = a.keep * h[j][i];
-        store_upto8(static_cast<T*>(a.dresidual) + row * a.lddresidual + c, n, out);
-      }
-      if (a.dgate_rows || a.part_gate) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          out[i] = a.branch * (x[j][i] * r1 * w[i]) * h[j][i];
-          sum_gate[j][i] += out[i];
-        }
-        if (a.dgate_rows) store_upto8(static_cast<T*>(a.dgate_rows) + row * a.lddgate + c, n, out);
+        store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dresidual) + row * a.lddresidual, a.cols, j, lane, out);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float df = a.branch * g[i] * h[j][i];
-        sum_post[j][i] += df * (x[j][i] * r1);
-        wdy[j][i] = w[i] * df;
-        dot += wdy[j][i] * x[j][i];
+        const float xr = r.x.v[j].at(i) * r1, w = post.v[j].at(i);
+        const float dgate = a.branch * (xr * w) * h[j][i];
+        const float df = a.branch * r.gate.v[j].at(i) * h[j][i];
+        out[i] = dgate;
+        sum_gate[j][i] += dgate;
+        sum_post[j][i] += df * xr;
+        h[j][i] = w * df;
+        dot += h[j][i] * r.x.v[j].at(i);
       }
+      if (a.dgate_rows)
+        store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dgate_rows) + row * a.lddgate, a.cols, j, lane, out);
     }
     if (!a.dx) return;
     float k1 = 0.0f;
     if (a.has_post) k1 = r1 * r1 * r1 * (row_sum<kThreads>(dot, scratch) * inv_cols);
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
-      if (c >= a.cols) continue;
       float out[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = r1 * wdy[j][i] - x[j][i] * k1;
-      store_upto8(static_cast<T*>(a.dx) + row * a.lddx + c, a.cols - c, out);
+      for (int i = 0; i < 8; ++i) out[i] = r1 * h[j][i] - r.x.v[j].at(i) * k1;
+      store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dx) + row * a.lddx, a.cols, j, lane, out);
     }
-  });
+  };
   const bool shared = kThreads >= 256;
   const int lane = shared ? threadIdx.x : threadIdx.x & 63;
   const int64_t group = shared ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (shared ? 1 : 4);
+  // the next row's loads are in flight while a row is worked on (waves of a
+  // workgroup that own rows of their own may run different counts: no barrier
+  // is between them)
+  Rows now;
+  if constexpr (kThreads < 1024) {
+    Rows next;
+    if (group < a.rows) load(group, lane, now);
+    for (int64_t row = group; row < a.rows; row += step) {
+      load(row + step < a.rows ? row + step : row, lane, next);
+      work(row, lane, now);
+      now = next;
+    }
+  } else {  // (no registers for two rows)
+    for (int64_t row = group; row < a.rows; row += step) {
+      load(row, lane, now);
+      work(row, lane, now);
+    }
+  }
 #pragma unroll
   for (int j = 0; j < kVectors; ++j) {
     const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
@@ -245,35 +248,44 @@ struct SumArgs {
   int64_t groups, cols;
 };
 
-// 64 columns of one sum to a workgroup: 16 groups at a time, then across.
+// 32 columns of one sum to a workgroup: 32 threads of consecutive columns for
+// each of 32 groups at a time, four loads in flight, then across.
 __global__ __launch_bounds__(1024) void sum_groups_kernel(SumArgs a) {
-  __shared__ float part[16][64];
+  __shared__ float part[32][33];
   const float* const src = a.part[blockIdx.y];
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
-  const int sub = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float sum = 0.0f;
-  if (c < a.cols)
-    for (int64_t g = sub; g < a.groups; g += 16) sum += src[g * a.cols + c];
-  part[sub][threadIdx.x & 63] = sum;
-  __syncthreads();
-  if (sub == 0 && c < a.cols) {
+  if (c < a.cols) {
+    int64_t g = sub;
+    for (; g + 96 < a.groups; g += 128) {
+      float v[4];
 #pragma unroll
-    for (int s = 1; s < 16; ++s) sum += part[s][threadIdx.x];
-    a.out[blockIdx.y][c] = sum;
+      for (int i = 0; i < 4; ++i) v[i] = src[(g + 32 * i) * a.cols + c];
+      sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    for (; g < a.groups; g += 32) sum += src[g * a.cols + c];
   }
+  part[sub][lane] = sum;
+  __syncthreads();
+  // row `sub` of the transposed tile: column `sub`'s 32 sums, one to a lane
+  float v = part[lane][sub];
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) v += __shfl_xor(v, d, 32);
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + sub;
+  if (lane == 0 && col < a.cols) a.out[blockIdx.y][col] = v;
 }
+
+// One vector per thread as far as that goes: sums and two rows stay in registers.
+RowShape backward_shape(int64_t cols) { return row_shape(cols, cols <= 4096 ? 1 : 2); }
 
 // Row groups of a backward launch: enough to fill the chip, few enough that
 // their partial sums stay small beside the rows.
-int64_t backward_groups(int64_t rows, int threads) {
-  const int64_t most = threads == 64 ? 1024 : threads == 256 ? 512 : 256;
-  return rows < most ? rows : most;
-}
 dim3 backward_grid(int64_t rows, int threads) {
-  const int64_t groups = backward_groups(rows, threads);
-  return dim3(static_cast<unsigned>(threads == 64 ? (groups + 3) / 4 : groups));
+  const int64_t most = threads <= 256 ? 1024 : threads == 512 ? 512 : 256;
+  const int64_t groups = threads == 64 ? (rows + 3) / 4 : rows;
+  return dim3(static_cast<unsigned>(std::min(groups, threads == 64 ? most / 2 : most)));
 }
-// (whole workgroups: partial rows past the last group's are zero)
 int64_t partial_rows(int64_t rows, int threads) {
   const int64_t blocks = backward_grid(rows, threads).x;
   return threads == 64 ? 4 * blocks : blocks;
@@ -332,7 +344,7 @@ hipError_t launch_block_norm(const rns8_mi355x_block_norm_args& g, hipStream_t s
 uint64_t block_norm_backward_bytes(const rns8_mi355x_block_norm_backward_args& g) {
   if (g.rows == 0) return 0;
   const int sums = (g.dpost_weight ? 1 : 0) + (g.dpre_weight ? 1 : 0) + (g.dgate && g.ldgate == 0 ? 1 : 0);
-  const int threads = choose_row_shape(g.rows, g.cols).threads;
+  const int threads = backward_shape(g.cols).threads;
   return round_up(static_cast<uint64_t>(sums) * static_cast<uint64_t>(partial_rows(g.rows, threads)) *
                       static_cast<uint64_t>(g.cols) * sizeof(float),
                   256);
@@ -340,7 +352,7 @@ uint64_t block_norm_backward_bytes(const rns8_mi355x_block_norm_backward_args& g
 
 hipError_t launch_block_norm_backward(const rns8_mi355x_block_norm_backward_args& g, hipStream_t stream) {
   if (g.cols > kMaxNormCols) return hipErrorInvalidValue;
-  const RowShape shape = choose_row_shape(g.rows, g.cols);
+  const RowShape shape = backward_shape(g.cols);
   const int64_t groups = g.rows > 0 ? partial_rows(g.rows, shape.threads) : 0;
   SumArgs sums{};
   unsigned count = 0;
@@ -396,7 +408,7 @@ hipError_t launch_block_norm_backward(const rns8_mi355x_block_norm_backward_args
     if (e != hipSuccess) return e;
   }
   if (count == 0) return hipSuccess;
-  hipLaunchKernelGGL(sum_groups_kernel, dim3(static_cast<unsigned>((g.cols + 63) / 64), count), dim3(1024), 0, stream,
+  hipLaunchKernelGGL(sum_groups_kernel, dim3(static_cast<unsigned>((g.cols + 31) / 32), count), dim3(1024), 0, stream,
                      sums);
   return hipGetLastError();
 }

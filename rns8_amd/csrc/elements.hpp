@@ -12,6 +12,9 @@ namespace rns8x {
 using f16 = _Float16;
 using bf16 = __bf16;
 
+__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
+
 // Eight consecutive elements, as floats. Rows may start at any element: the
 // copy compiles to 16-byte loads that need no alignment (gfx9-family global
 // memory instructions take any address).
@@ -53,6 +56,104 @@ __device__ __forceinline__ void store_upto8(T* p, int64_t n, const float (&v)[8]
     if (i < n) p[i] = static_cast<T>(v[i]);
 }
 
+// ---- rows in registers -------------------------------------------------------------
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight consecutive elements as loaded.
+template <typename T>
+struct Packed8 {
+  static constexpr int kWords = 2 * sizeof(T);
+  u32x4 q[kWords / 4];
+  __device__ __forceinline__ uint32_t word(int i) const { return q[i >> 2][i & 3]; }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return as_float(word(i));
+    } else if constexpr (std::is_same_v<T, bf16>) {
+      return as_float(i & 1 ? word(i >> 1) & 0xFFFF0000u : word(i >> 1) << 16);
+    } else {
+      return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(word(i >> 1) >> (16 * (i & 1)))));
+    }
+  }
+  __device__ __forceinline__ void fill(T v) {
+    uint32_t w;
+    if constexpr (sizeof(T) == 4)
+      w = __builtin_bit_cast(uint32_t, v);
+    else
+      w = __builtin_bit_cast(uint16_t, v) * 0x10001u;
+#pragma unroll
+    for (auto& x : q) x = u32x4{w, w, w, w};
+  }
+  // Drops the first k (0 to 7) elements: the others move down, zeros follow.
+  __device__ __forceinline__ void drop(uint32_t k) {
+    uint32_t w[kWords + 4] = {};
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = word(i);
+#pragma unroll
+    for (int step = kWords / 2; step >= 1; step /= 2) {
+      const bool on = k & (step * 4 / sizeof(T));
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = on ? (i + step < kWords ? w[i + step] : 0u) : w[i];
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = k & 1 ? w[i] >> 16 | w[i + 1] << 16 : w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) q[i >> 2][i & 3] = w[i];
+  }
+};
+
+// kVectors vectors of 8 consecutive elements of a row for each of kThreads
+// threads, vector j of thread t at column 8 (j kThreads + t), as loaded: all
+// loads of a row (and of the rows beside it) are issued before the first
+// conversion waits for one.
+template <typename T, int kVectors>
+struct RawRow {
+  Packed8<T> v[kVectors];
+};
+
+template <int kThreads>
+__device__ __forceinline__ int64_t column_of(int vector, int lane) {
+  return 8 * (static_cast<int64_t>(vector) * kThreads + lane);
+}
+
+// Elements past the row are zeros. One load to a vector: lanes past the row
+// read its start, the lane that the row's end cuts reads the row's last eight
+// and drops those that are others'. Rows below eight are read by elements.
+template <int kThreads, typename T, int kVectors>
+__device__ __forceinline__ void load_row(const T* row, int64_t cols, int lane, RawRow<T, kVectors>& r) {
+  if (cols < 8) {
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) r.v[j].fill(static_cast<T>(0.0f));
+    if (lane == 0) {
+      T t[8] = {};
+      for (int i = 0; i < 8; ++i)
+        if (i < cols) t[i] = row[i];
+      __builtin_memcpy(r.v[0].q, t, sizeof(t));
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) {
+    const int64_t c = column_of<kThreads>(j, lane);
+    const int64_t at = c + 8 <= cols ? c : c < cols ? cols - 8 : 0;
+    __builtin_memcpy(r.v[j].q, row + at, sizeof(r.v[j].q));
+  }
+  if (cols == 8 * kThreads * kVectors) return;
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) {
+    const int64_t c = column_of<kThreads>(j, lane);
+    if (cols % 8 != 0) r.v[j].drop(c < cols && c + 8 > cols ? static_cast<uint32_t>(c + 8 - cols) : 0u);
+    if (c >= cols) r.v[j].fill(static_cast<T>(0.0f));
+  }
+}
+
+template <int kThreads, typename T, int kVectors>
+__device__ __forceinline__ void store_vector(T* row, int64_t cols, int vector, int lane, const float (&v)[8]) {
+  const int64_t c = column_of<kThreads>(vector, lane);
+  if (c < cols) store_upto8(row + c, cols - c, v);
+}
+
 // ---- reductions over a wave: every lane ends with the result --------------------
 // Within each 16-lane row by rotations, then across rows by lane swaps.
 template <int kCtrl>
@@ -73,9 +174,6 @@ __device__ __forceinline__ uint32_t wave_reduce(uint32_t x, Op op) {
   const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return op(b[0], b[1]);
 }
-
-__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
-__device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
 
 struct AddF {
   __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const {

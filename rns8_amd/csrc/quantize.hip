@@ -22,25 +22,12 @@ struct RowsArgs {
   float* scale;
 };
 
-template <typename T, bool kMul>
-__device__ __forceinline__ void load_scaled(const RowsArgs& a, const T* row, int64_t c, float (&v)[8]) {
-  load_upto8(row + c, a.cols - c, v, 0.0f);
-  if constexpr (kMul) {
-    float m[8];
-    load_upto8(a.multiplier + c, a.cols - c, m, 0.0f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= m[i];
-  }
-}
-
 // kThreads threads hold a row in kVectors vectors each (0: the row is read
 // again instead of held).
 template <typename T, int kThreads, int kVectors, bool kMul>
 __device__ __forceinline__ void quantize_row(const RowsArgs& a, int64_t row, int lane, uint32_t* scratch) {
   const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
   int8_t* const q = a.q + row * a.ldq;
-  constexpr int kHeld = kVectors > 0 ? kVectors : 1;
-  float v[kHeld][8];
   uint32_t amax = 0;
   auto take = [&](const float (&u)[8]) {
 #pragma unroll
@@ -50,35 +37,49 @@ __device__ __forceinline__ void quantize_row(const RowsArgs& a, int64_t row, int
     }
   };
   if constexpr (kVectors > 0) {
+    RawRow<T, kVectors> raw;
+    RawRow<float, kVectors> mul;
+    load_row<kThreads>(x, a.cols, lane, raw);
+    if constexpr (kMul) load_row<kThreads>(a.multiplier, a.cols, lane, mul);
+    float v[kVectors][8];
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
-      if (c < a.cols) load_scaled<T, kMul>(a, x, c, v[j]);
+      for (int i = 0; i < 8; ++i) {
+        v[j][i] = raw.v[j].at(i);
+        if constexpr (kMul) v[j][i] *= mul.v[j].at(i);
+      }
       take(v[j]);
     }
-  } else {
-    for (int64_t c = 8 * lane; c < a.cols; c += 8 * kThreads) {
-      load_scaled<T, kMul>(a, x, c, v[0]);
-      take(v[0]);
-    }
-  }
-  amax = row_reduce<kThreads>(amax, MaxU{}, scratch);
-  const RowScale s = row_scale(amax);
-  if (lane == 0) a.scale[row] = s.scale;
-  if constexpr (kVectors > 0) {
+    const RowScale s = row_scale(row_reduce<kThreads>(amax, MaxU{}, scratch));
+    if (lane == 0) a.scale[row] = s.scale;
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
+      const int64_t c = column_of<kThreads>(j, lane);
       if (c < a.stop) store_bytes8(q, c, a.stop, quantize8(v[j], s.inverse));
     }
   } else {
+    auto load = [&](int64_t c, float (&v)[8]) {
+      load_upto8(x + c, a.cols - c, v, 0.0f);
+      if constexpr (kMul) {
+        float m[8];
+        load_upto8(a.multiplier + c, a.cols - c, m, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= m[i];
+      }
+    };
+    float v[8];
+    for (int64_t c = 8 * lane; c < a.cols; c += 8 * kThreads) {
+      load(c, v);
+      take(v);
+    }
+    const RowScale s = row_scale(row_reduce<kThreads>(amax, MaxU{}, scratch));
+    if (lane == 0) a.scale[row] = s.scale;
     for (int64_t c = 8 * lane; c < a.stop; c += 8 * kThreads) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[0][i] = 0.0f;
-      if (c < a.cols) load_scaled<T, kMul>(a, x, c, v[0]);
-      store_bytes8(q, c, a.stop, quantize8(v[0], s.inverse));
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      if (c < a.cols) load(c, v);
+      store_bytes8(q, c, a.stop, quantize8(v, s.inverse));
     }
   }
 }

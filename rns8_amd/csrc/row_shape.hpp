@@ -8,39 +8,42 @@
 
 namespace rns8x {
 
-// Threads per row (64: a wave, four rows to a workgroup; 256 or 1024: the
+// Threads per row (64: a wave, four rows to a workgroup; 256, 512 or 1024: the
 // workgroup) and 8-element vectors per thread (1, 2 or 4).
 struct RowShape {
   int threads, vectors;
 };
 
-// The fewest threads that hold a row in four vectors each, so that one wave's
-// reductions need no barrier where rows are short; more where the rows are too
-// few to fill the chip and a row's own latency is what counts.
-inline RowShape choose_row_shape(int64_t rows, int64_t cols) {
+// The fewest threads that hold a row in `most` vectors each (more where 1024
+// threads are not enough).
+inline RowShape row_shape(int64_t cols, int most) {
   const int64_t vectors = (cols + 7) / 8;
-  auto shape = [&](int threads) {
+  for (const int threads : {64, 256, 512, 1024}) {
     const int64_t v = (vectors + threads - 1) / threads;
-    return RowShape{threads, v <= 1 ? 1 : v <= 2 ? 2 : 4};
-  };
-  if (rows < 512) {
-    if (vectors <= 64) return shape(64);
-    return shape(vectors <= 256 ? 256 : 1024);
+    if (v <= most || threads == 1024) return RowShape{threads, v <= 1 ? 1 : v <= 2 ? 2 : 4};
   }
-  if (vectors <= 256) return shape(64);
-  return shape(vectors <= 1024 ? 256 : 1024);
+  return RowShape{1024, 4};
 }
+
+// Two vectors each where there are rows enough to fill the chip; one where they
+// are few and a row's own latency is what counts.
+inline RowShape choose_row_shape(int64_t rows, int64_t cols) { return row_shape(cols, rows < 512 ? 1 : 2); }
 
 // f(threads, vectors) with the shape as compile-time constants.
 template <typename F>
 hipError_t with_row_shape(RowShape s, F&& f) {
   auto vectors = [&](auto threads) {
     if (s.vectors == 1) return f(threads, std::integral_constant<int, 1>{});
-    if (s.vectors == 2) return f(threads, std::integral_constant<int, 2>{});
-    return f(threads, std::integral_constant<int, 4>{});
+    if constexpr (decltype(threads)::value < 1024) {
+      return f(threads, std::integral_constant<int, 2>{});
+    } else {
+      if (s.vectors == 2) return f(threads, std::integral_constant<int, 2>{});
+      return f(threads, std::integral_constant<int, 4>{});
+    }
   };
   if (s.threads == 64) return vectors(std::integral_constant<int, 64>{});
   if (s.threads == 256) return vectors(std::integral_constant<int, 256>{});
+  if (s.threads == 512) return vectors(std::integral_constant<int, 512>{});
   return vectors(std::integral_constant<int, 1024>{});
 }
 
