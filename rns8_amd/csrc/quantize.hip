@@ -6,6 +6,8 @@
 // are read once and stay in registers between the maximum and the bytes;
 // columns are read twice (their maxima need every row), the second time mostly
 // from the Infinity Cache.
+#include <algorithm>
+
 #include "elements.hpp"
 #include "operators.hpp"
 #include "row_shape.hpp"
@@ -113,9 +115,9 @@ hipError_t launch_rows_of(const RowsArgs& a, hipStream_t stream) {
 // ---- columns ----------------------------------------------------------------------
 // A first kernel leaves every column's largest magnitude (and sum) over each
 // of `chunks` groups of rows; the second joins a column's chunks in their
-// order, quantizes 64 x 64 tiles and turns them over in LDS.
-constexpr int kTile = 64;
-constexpr int64_t kMaxChunks = 64;
+// order, quantizes 128 x 128 tiles and turns them over in LDS.
+constexpr int kTile = 128;
+constexpr int kPitch = kTile / 4 + 1;  // words of four rows' bytes to a column of the turned tile
 
 struct ColsArgs {
   const void* x;
@@ -131,14 +133,55 @@ struct ColsArgs {
   int64_t tiles_c;
 };
 
+// About 1024 workgroups of 256 columns, at least 16 rows each, and few enough
+// that joining them is a small part of the second kernel.
 int64_t column_chunks(int64_t rows, int64_t cols) {
   const int64_t col_blocks = (cols + 255) / 256;
-  int64_t chunks = (1024 + col_blocks - 1) / col_blocks;
-  if (chunks > (rows + 15) / 16) chunks = (rows + 15) / 16;
-  return chunks < 1 ? 1 : chunks > kMaxChunks ? kMaxChunks : chunks;
+  return std::max<int64_t>(1, std::min({(1024 + col_blocks - 1) / col_blocks, (rows + 15) / 16, int64_t{64}}));
 }
 
-// 256 threads: 32 vectors of 8 columns by 8 rows at a time.
+// Eight columns from column c on of four rows `step` apart and their factors,
+// all loads issued before any is looked at: rows past the last and columns past
+// the row read others in their place, which are then dropped.
+template <typename T>
+struct FourRows {
+  Packed8<T> p[4];
+  float m[4];
+  __device__ __forceinline__ void load(const ColsArgs& a, int64_t row, int64_t step, int64_t last, int64_t c) {
+    const T* const x = static_cast<const T*>(a.x);
+    const int64_t cols = a.cols;
+    if (cols >= 8) {
+      const int64_t at = c + 8 <= cols ? c : c < cols ? cols - 8 : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t r = min(row + k * step, last - 1);
+        __builtin_memcpy(p[k].q, x + r * a.ldx + at, sizeof(p[k].q));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t r = min(row + k * step, last - 1);
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = c + i < cols ? x[r * a.ldx + c + i] : static_cast<T>(0.0f);
+        __builtin_memcpy(p[k].q, t, sizeof(t));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = a.multiplier ? a.multiplier[min(row + k * step, last - 1)] : 1.0f;
+  }
+  __device__ __forceinline__ void settle(const ColsArgs& a, int64_t row, int64_t step, int64_t last, int64_t c) {
+    if (a.cols >= 8 && a.cols % 8 != 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[k].drop(c < a.cols && c + 8 > a.cols ? static_cast<uint32_t>(c + 8 - a.cols) : 0u);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (row + k * step >= last || c >= a.cols) p[k].fill(static_cast<T>(0.0f));
+  }
+};
+
+// 256 threads: 32 vectors of 8 columns by 8 rows, four rows in flight each.
 template <typename T>
 __global__ __launch_bounds__(256) void column_partials_kernel(ColsArgs a) {
   __shared__ uint32_t amax_lds[8][256];
@@ -149,18 +192,20 @@ __global__ __launch_bounds__(256) void column_partials_kernel(ColsArgs a) {
   const int64_t last = first + a.chunk_rows < a.rows ? first + a.chunk_rows : a.rows;
   uint32_t amax[8] = {};
   float sum[8] = {};
-  if (c < a.cols) {
-    for (int64_t r = first + sub; r < last; r += 8) {
-      float v[8];
-      load_upto8(static_cast<const T*>(a.x) + r * a.ldx + c, a.cols - c, v, 0.0f);
-      const float m = a.multiplier ? a.multiplier[r] : 1.0f;
+  for (int64_t r = first + sub; r < last; r += 32) {
+    FourRows<T> rows;
+    rows.load(a, r, 8, last, c);
+    rows.settle(a, r, 8, last, c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        sum[i] += v[i];
-        const uint32_t b = magnitude_bits(v[i] * m);
+        const float v = rows.p[k].at(i);
+        sum[i] += v;
+        // (a row that is not there: 0 times a factor that may be infinite counts as 0)
+        const uint32_t b = r + 8 * k < last ? magnitude_bits(v * rows.m[k]) : 0u;
         amax[i] = amax[i] > b ? amax[i] : b;
       }
-    }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -186,56 +231,91 @@ __global__ __launch_bounds__(256) void column_partials_kernel(ColsArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_columns_kernel(ColsArgs a) {
   __shared__ float inverse[kTile];
-  __shared__ __attribute__((aligned(16))) uint8_t tile[kTile][kTile + 8];  // [column][row]
+  __shared__ uint32_t tile[kTile * kPitch];  // [column][four rows]
+  __shared__ uint32_t amax_lds[kTile];
+  __shared__ float sum_lds[kTile];
   const int64_t tile_r = blockIdx.x / a.tiles_c;
   const int64_t c0 = (blockIdx.x - tile_r * a.tiles_c) * kTile, r0 = tile_r * kTile;
-  if (threadIdx.x < kTile) {
-    const int64_t c = c0 + threadIdx.x;
-    RowScale s{0.0f, 0.0f};
-    if (c < a.cols) {
-      uint32_t m = 0;
-      for (int64_t k = 0; k < a.chunks; ++k) {
-        const uint32_t b = a.amax_part[k * a.cols + c];
-        m = m > b ? m : b;
-      }
-      s = row_scale(m);
-      if (tile_r == 0) {
-        a.scale[c] = s.scale;
-        if (a.sums) {
-          float sum = 0.0f;
-          for (int64_t k = 0; k < a.chunks; ++k) sum += a.sum_part[k * a.cols + c];
-          a.sums[c] = sum;
-        }
+  const int vec = threadIdx.x & 15, quad = threadIdx.x >> 4;  // 16 vectors of 8 columns by 16 groups of four rows
+  const int64_t c = c0 + 8 * vec;
+  // the whole tile is on its way while the columns' scales are joined
+  FourRows<T> rows[2];
+  if (a.rows > 0) {
+    rows[0].load(a, r0 + 4 * quad, 1, a.rows, c);
+    rows[1].load(a, r0 + 64 + 4 * quad, 1, a.rows, c);
+  }
+  {
+    // two threads to a column, one for even and one for odd chunks, eight loads
+    // in flight (chunks past the last are read again: a maximum does not mind)
+    const int col = threadIdx.x & (kTile - 1), half = threadIdx.x / kTile;
+    const int64_t column = c0 + col, at = min(column, a.cols - 1);
+    uint32_t amax = 0;
+    for (int64_t k = half; k < a.chunks; k += 16) {
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = a.amax_part[min(k + 2 * i, a.chunks - 1) * a.cols + at];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = amax > v[i] ? amax : v[i];
+    }
+    float sum = 0.0f;
+    const bool summed = a.sums && tile_r == 0;
+    if (summed) {
+      for (int64_t k = half; k < a.chunks; k += 16) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = a.sum_part[min(k + 2 * i, a.chunks - 1) * a.cols + at];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += k + 2 * i < a.chunks ? v[i] : 0.0f;
       }
     }
-    inverse[threadIdx.x] = s.inverse;
-  }
-  __syncthreads();
-  // 8 vectors of 8 columns by 32 rows, twice
-  const int vec = threadIdx.x & 7;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = (threadIdx.x >> 3) + 32 * half;
-    const int64_t row = r0 + r, c = c0 + 8 * vec;
-    float v[8] = {};
-    if (row < a.rows && c < a.cols) {
-      load_upto8(static_cast<const T*>(a.x) + row * a.ldx + c, a.cols - c, v, 0.0f);
-      const float m = a.multiplier ? a.multiplier[row] : 1.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= m;
+    if (half) {
+      amax_lds[col] = amax;
+      sum_lds[col] = sum;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) tile[8 * vec + i][r] = static_cast<uint8_t>(quantize_byte(v[i], inverse[8 * vec + i]));
+    __syncthreads();
+    if (!half) {
+      const uint32_t b = amax_lds[col];
+      const RowScale s = row_scale(amax > b ? amax : b);
+      inverse[col] = s.inverse;
+      if (tile_r == 0 && column < a.cols) {
+        a.scale[column] = s.scale;
+        if (summed) a.sums[column] = sum + sum_lds[col];
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  const int vr = threadIdx.x & 7;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int c = (threadIdx.x >> 3) + 32 * half;
-    const int64_t col = c0 + c, r = r0 + 8 * vr;
-    uint64_t w;
-    __builtin_memcpy(&w, &tile[c][8 * vr], 8);
-    if (col < a.cols && r < a.stop) store_bytes8(a.q + col * a.ldq, r, a.stop, w);
+    const int64_t row = r0 + 64 * half + 4 * quad;
+    rows[half].settle(a, row, 1, a.rows, c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float inv = inverse[8 * vec + i];
+      uint32_t w = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w |= (row + k < a.rows ? quantize_byte(rows[half].p[k].at(i) * rows[half].m[k], inv) : 0u) << (8 * k);
+      tile[(8 * vec + i) * kPitch + 16 * half + quad] = w;
+    }
+  }
+  __syncthreads();
+  // 16 bytes of a column to a thread: 8 threads to a column, 32 columns at a time
+  const int part = threadIdx.x & 7;
+#pragma unroll
+  for (int group = 0; group < kTile / 32; ++group) {
+    const int col = (threadIdx.x >> 3) + 32 * group;
+    const int64_t column = c0 + col, r = r0 + 16 * part;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = tile[col * kPitch + 4 * part + k];
+    if (column < a.cols && r < a.stop) {
+      int8_t* const q = a.q + column * a.ldq;
+      if (r + 16 <= a.stop) {
+        __builtin_memcpy(q + r, w, 16);
+      } else {
+        for (int i = 0; r + i < a.stop; ++i) q[r + i] = static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)));
+      }
+    }
   }
 }
 

@@ -18,27 +18,69 @@ struct CopyArgs {
   int64_t ldd;
 };
 
+// Bytes [0, n) of four words, n at most 15; zeros from there on.
+__device__ __forceinline__ u32x4 first_bytes(u32x4 w, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int left = n - 4 * i;
+    w[i] = left >= 4 ? w[i] : left <= 0 ? 0u : w[i] & ((1u << (8 * left)) - 1u);
+  }
+  return w;
+}
+
+// Four rows to a wave, 16 bytes of each to a lane at a time, all four loads in
+// flight. The chunk that a row's end cuts comes from the row's last 16 bytes,
+// moved down by whole words and then by bytes.
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
-  const int64_t chunks = a.ldd / 16, total = a.rows * chunks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / chunks, c = 16 * (i - row * chunks);
-    const int8_t* const from = a.src + row * a.lds + c;
-    uint32_t w[4] = {};
-    if (c + 16 <= a.cols) {
-      __builtin_memcpy(w, from, 16);
-    } else {
-      for (int b = 0; c + b < a.cols; ++b) w[b >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(from[b])) << (8 * (b & 3));
+  const int lane = threadIdx.x & 63;
+  const uint32_t cols = static_cast<uint32_t>(a.cols), padded = static_cast<uint32_t>(a.ldd);
+  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * 4; row < a.rows;
+       row += static_cast<int64_t>(gridDim.x) * 16) {
+    const int64_t rows = a.rows - row;
+    for (uint32_t c = 16 * (64 * blockIdx.y + lane); c < padded; c += 16 * 64 * gridDim.y) {
+      u32x4 w[4];
+      const bool whole = c + 16 <= cols;
+      if (cols >= 16) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          __builtin_memcpy(&w[r], a.src + (row + (r < rows ? r : 0)) * a.lds + (whole ? c : cols - 16), 16);
+        if (!whole) {
+          const uint32_t drop = c + 16 - cols, words = drop / 4, bits = 8 * (drop % 4);  // 1 to 15 bytes
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            uint32_t x[5] = {w[r][0], w[r][1], w[r][2], w[r][3], 0u};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = words & 2 ? (i + 2 < 4 ? x[i + 2] : 0u) : x[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = words & 1 ? x[i + 1] : x[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_alignbit(x[i + 1], x[i], bits);
+            w[r] = first_bytes(u32x4{x[0], x[1], x[2], x[3]}, 16 - static_cast<int>(drop));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[r] = u32x4{0, 0, 0, 0};
+          const int8_t* const from = a.src + (row + (r < rows ? r : 0)) * a.lds;
+#pragma unroll
+          for (int i = 0; i < 15; ++i)
+            if (i < static_cast<int>(cols)) w[r][i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(from[i])) << (8 * (i & 3));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < rows) __builtin_memcpy(a.dst + (row + r) * a.ldd + c, &w[r], 16);
     }
-    __builtin_memcpy(a.dst + row * a.ldd + c, w, 16);
   }
 }
 
 hipError_t launch_copy_rows(const CopyArgs& a, hipStream_t stream) {
-  const int64_t blocks = (a.rows * (a.ldd / 16) + 255) / 256;
-  if (blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL(copy_rows_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16))), dim3(256), 0,
-                     stream, a);
+  if (a.rows == 0) return hipSuccess;
+  const int64_t blocks = (a.rows + 15) / 16;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16)),
+                  static_cast<unsigned>(std::min<int64_t>((a.ldd + 1023) / 1024, 64)));
+  hipLaunchKernelGGL(copy_rows_kernel, grid, dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
