@@ -18,19 +18,18 @@ struct CopyArgs {
   int64_t ldd;
 };
 
-// Bytes [0, n) of four words, n at most 15; zeros from there on.
-__device__ __forceinline__ u32x4 first_bytes(u32x4 w, int n) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int left = n - 4 * i;
-    w[i] = left >= 4 ? w[i] : left <= 0 ? 0u : w[i] & ((1u << (8 * left)) - 1u);
-  }
-  return w;
+// Sixteen bytes without the first n (0 to 15), zeros after them.
+__device__ __forceinline__ u32x4 drop_bytes(u32x4 w, uint32_t n) {
+  const uint64_t lo = static_cast<uint64_t>(w[1]) << 32 | w[0], hi = static_cast<uint64_t>(w[3]) << 32 | w[2];
+  const uint32_t bits = 8 * n & 63;
+  const uint64_t a = n & 8 ? hi : lo, b = n & 8 ? 0 : hi;
+  const uint64_t x = a >> bits | (b << 1) << (63 - bits), y = b >> bits;
+  return u32x4{static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(y),
+               static_cast<uint32_t>(y >> 32)};
 }
 
 // Four rows to a wave, 16 bytes of each to a lane at a time, all four loads in
-// flight. The chunk that a row's end cuts comes from the row's last 16 bytes,
-// moved down by whole words and then by bytes.
+// flight. The chunk that a row's end cuts comes from the row's last 16 bytes.
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
   const int lane = threadIdx.x & 63;
   const uint32_t cols = static_cast<uint32_t>(a.cols), padded = static_cast<uint32_t>(a.ldd);
@@ -40,34 +39,11 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
     for (uint32_t c = 16 * (64 * blockIdx.y + lane); c < padded; c += 16 * 64 * gridDim.y) {
       u32x4 w[4];
       const bool whole = c + 16 <= cols;
-      if (cols >= 16) {
+      const uint32_t at = whole ? c : cols - 16, drop = whole ? 0 : c + 16 - cols;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          __builtin_memcpy(&w[r], a.src + (row + (r < rows ? r : 0)) * a.lds + (whole ? c : cols - 16), 16);
-        if (!whole) {
-          const uint32_t drop = c + 16 - cols, words = drop / 4, bits = 8 * (drop % 4);  // 1 to 15 bytes
+      for (int r = 0; r < 4; ++r) __builtin_memcpy(&w[r], a.src + (row + min<int64_t>(r, rows - 1)) * a.lds + at, 16);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            uint32_t x[5] = {w[r][0], w[r][1], w[r][2], w[r][3], 0u};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = words & 2 ? (i + 2 < 4 ? x[i + 2] : 0u) : x[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = words & 1 ? x[i + 1] : x[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_alignbit(x[i + 1], x[i], bits);
-            w[r] = first_bytes(u32x4{x[0], x[1], x[2], x[3]}, 16 - static_cast<int>(drop));
-          }
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          w[r] = u32x4{0, 0, 0, 0};
-          const int8_t* const from = a.src + (row + (r < rows ? r : 0)) * a.lds;
-#pragma unroll
-          for (int i = 0; i < 15; ++i)
-            if (i < static_cast<int>(cols)) w[r][i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(from[i])) << (8 * (i & 3));
-        }
-      }
+      for (int r = 0; r < 4; ++r) w[r] = drop_bytes(w[r], drop);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (r < rows) __builtin_memcpy(a.dst + (row + r) * a.ldd + c, &w[r], 16);
@@ -75,8 +51,26 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
   }
 }
 
+// Rows below 16 bytes: one to a thread.
+__global__ __launch_bounds__(256) void copy_short_rows_kernel(CopyArgs a) {
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; row < a.rows;
+       row += static_cast<int64_t>(gridDim.x) * 256) {
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+      if (i < a.cols)
+        w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(a.src[row * a.lds + i])) << (8 * (i & 3));
+    __builtin_memcpy(a.dst + row * a.ldd, w, 16);
+  }
+}
+
 hipError_t launch_copy_rows(const CopyArgs& a, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;
+  if (a.cols < 16) {
+    const int64_t blocks = std::min<int64_t>((a.rows + 255) / 256, 1 << 16);
+    hipLaunchKernelGGL(copy_short_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
   const int64_t blocks = (a.rows + 15) / 16;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16)),
                   static_cast<unsigned>(std::min<int64_t>((a.ldd + 1023) / 1024, 64)));
