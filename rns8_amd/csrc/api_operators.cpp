@@ -353,6 +353,7 @@ rns8_status no_workspace(const A&) {
 }
 
 uint64_t linear_bytes(rns8_mi355x_linear_i8_args a) {
+  if (linear_rows_takes(a.m, a.n, a.k)) return 0;
   a.workspace = nullptr;
   LinearParts p;
   linear_parts(a, p);
@@ -415,6 +416,7 @@ rns8_status rns8_mi355x_linear_i8(rns8_context* ctx, const rns8_mi355x_linear_i8
         return check_workspace(a.workspace, a.workspace_bytes, linear_bytes(a));
       },
       [](const rns8_mi355x_linear_i8_args& a, hipStream_t s) {
+        if (a.m > 0 && a.n > 0 && linear_rows_takes(a.m, a.n, a.k)) return launch_linear_rows(a, s);
         LinearParts p;
         linear_parts(a, p);
         const hipError_t e = launch_quantize_rows(p.quantize, s);

@@ -103,6 +103,16 @@ struct Packed8 {
   }
 };
 
+// Sixteen bytes without the first n (0 to 15), zeros after them.
+__device__ __forceinline__ u32x4 drop_bytes(u32x4 w, uint32_t n) {
+  const uint64_t lo = static_cast<uint64_t>(w[1]) << 32 | w[0], hi = static_cast<uint64_t>(w[3]) << 32 | w[2];
+  const uint32_t bits = 8 * n & 63;
+  const uint64_t a = n & 8 ? hi : lo, b = n & 8 ? 0 : hi;
+  const uint64_t x = a >> bits | (b << 1) << (63 - bits), y = b >> bits;
+  return u32x4{static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(y),
+               static_cast<uint32_t>(y >> 32)};
+}
+
 // kVectors vectors of 8 consecutive elements of a row for each of kThreads
 // threads, vector j of thread t at column 8 (j kThreads + t), as loaded: all
 // loads of a row (and of the rows beside it) are issued before the first

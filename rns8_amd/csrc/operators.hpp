@@ -25,6 +25,10 @@ hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& a, hipStream
 uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled);
 hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, hipStream_t stream);
 
+// The linear layer for one or two tokens in one kernel (scaled_rows.hip).
+bool linear_rows_takes(int64_t m, int64_t n, int64_t k);
+hipError_t launch_linear_rows(const rns8_mi355x_linear_i8_args& a, hipStream_t stream);
+
 // ---- block norm (block_norm.hip) ------------------------------------------------------
 constexpr int64_t kMaxNormCols = 32768;
 hipError_t launch_block_norm(const rns8_mi355x_block_norm_args& a, hipStream_t stream);

@@ -18,16 +18,6 @@ struct CopyArgs {
   int64_t ldd;
 };
 
-// Sixteen bytes without the first n (0 to 15), zeros after them.
-__device__ __forceinline__ u32x4 drop_bytes(u32x4 w, uint32_t n) {
-  const uint64_t lo = static_cast<uint64_t>(w[1]) << 32 | w[0], hi = static_cast<uint64_t>(w[3]) << 32 | w[2];
-  const uint32_t bits = 8 * n & 63;
-  const uint64_t a = n & 8 ? hi : lo, b = n & 8 ? 0 : hi;
-  const uint64_t x = a >> bits | (b << 1) << (63 - bits), y = b >> bits;
-  return u32x4{static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(y),
-               static_cast<uint32_t>(y >> 32)};
-}
-
 // Four rows to a wave, 16 bytes of each to a lane at a time, all four loads in
 // flight. The chunk that a row's end cuts comes from the row's last 16 bytes.
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
@@ -82,6 +72,7 @@ bool in_place(const int8_t* p, int64_t ld) { return ld % 16 == 0 && reinterpret_
 
 // The workspace: copies of the operands that need one, then the partial sums.
 struct Plan {
+  bool few_rows;  // the kernel for few tokens, which reads any alignment and needs no workspace
   bool copy_a, copy_b;
   int64_t lda, ldb, b_rows, b_cols;
   uint64_t a_at, b_at, sums_at, bytes;
@@ -91,6 +82,10 @@ struct Plan {
 Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
   Plan p{};
   const bool inner = g.b_layout == RNS8_MI355X_B_INNER;
+  p.lda = g.lda;
+  p.ldb = g.ldb;
+  p.few_rows = scaled_rows_takes(g.m, g.n, g.k, inner);
+  if (p.few_rows) return p;
   p.b_rows = inner ? g.k : g.n;
   p.b_cols = inner ? g.n : g.k;
   // where b is n x k, a's chunks are read whole: they have to end in zeros
@@ -124,6 +119,7 @@ hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled,
   uint8_t* const ws = static_cast<uint8_t*>(g.workspace);
   ScaledGemm s{g.m, g.n, g.k, g.a, g.b, p.lda, p.ldb, g.b_layout == RNS8_MI355X_B_INNER, g.a_scale, g.b_scale, g.bias,
                g.out, g.ldo, g.dtype};
+  if (p.few_rows) return launch_scaled_rows(s, stream);
   if (p.copy_a) {
     int8_t* const to = reinterpret_cast<int8_t*>(ws + p.a_at);
     const hipError_t e = launch_copy_rows({g.a, g.m, g.k, g.lda, to, p.lda}, stream);

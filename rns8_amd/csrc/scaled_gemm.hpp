@@ -35,6 +35,10 @@ struct TileShape {
 TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k, bool inner);
 hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int32_t* partials, hipStream_t stream);
 
+// Few tokens (scaled_rows.hip): operands at any alignment, no workspace.
+bool scaled_rows_takes(int64_t m, int64_t n, int64_t k, bool inner);
+hipError_t launch_scaled_rows(const ScaledGemm& g, hipStream_t stream);
+
 // Products of at most this many bytes in one int32 sum: |a b| <= 2^14.
 constexpr int64_t kExactK = 131071;
 
