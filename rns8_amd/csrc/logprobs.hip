@@ -114,6 +114,12 @@ __device__ __forceinline__ uint64_t rank_key(float v, uint32_t index) {
   return static_cast<uint64_t>(order) << 32 | static_cast<uint32_t>(~index);
 }
 
+// The logit that a key stands for (0 for -0, a NaN for any).
+__device__ __forceinline__ float ranked_logit(uint64_t key) {
+  const uint32_t order = static_cast<uint32_t>(key >> 32);
+  return as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
+}
+
 __device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
   const uint32_t hi = wave_reduce(static_cast<uint32_t>(key >> 32), MaxU{});
   const uint32_t lo = static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u;
@@ -152,12 +158,9 @@ __device__ __forceinline__ void write_row(const Args& a, int64_t row, Sums t) {
   }
 }
 
-template <typename T>
 __device__ __forceinline__ void write_alternative(const Args& a, int64_t row, uint32_t rank, uint64_t key, Sums t) {
-  const uint32_t id = ~static_cast<uint32_t>(key);
-  if (a.top_ids) a.top_ids[row * a.top + rank] = static_cast<int32_t>(id);
-  if (a.top_logp)
-    a.top_logp[row * a.top + rank] = logp_of(static_cast<float>(static_cast<const T*>(a.logits)[row * a.ldl + id]), t, a.c);
+  if (a.top_ids) a.top_ids[row * a.top + rank] = static_cast<int32_t>(~static_cast<uint32_t>(key));
+  if (a.top_logp) a.top_logp[row * a.top + rank] = logp_of(ranked_logit(key), t, a.c);
 }
 
 template <typename T>
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
       __syncthreads();
       auto put = [&](uint32_t rank, uint64_t key) {
         if (a.parts == 1)
-          write_alternative<T>(a, row, rank, key, t);
+          write_alternative(a, row, rank, key, t);
         else
           a.part_keys[unit * a.top + rank] = key;
       };
@@ -312,34 +315,44 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   }
 }
 
-// One wave to a row: lane p holds part p.
+// A workgroup loads a row's lists, then lane p of its first wave holds part p:
+// the largest head goes out `top` times, and lane k keeps the k-th.
 template <typename T>
-__global__ __launch_bounds__(64) void join_parts_kernel(Args a) {
+__global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
   extern __shared__ uint64_t lists[];  // [parts][top]
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const uint32_t parts = static_cast<uint32_t>(a.parts), total = parts * a.top;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const uint64_t* const from = a.part_keys + row * total;
+    for (uint32_t i = threadIdx.x; i < total; i += 4 * kThreads) {
+      uint64_t key[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) key[j] = from[min(i + j * kThreads, total - 1)];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (i + j * kThreads < total) lists[i + j * kThreads] = key[j];
+    }
     Sums t{-INFINITY, 0.0f, 0.0f};
-    if (lane < a.parts) {
+    if (threadIdx.x < parts) {
       float w[4];
       __builtin_memcpy(w, a.part_sums + 4 * (row * a.parts + lane), 16);
       t = {w[0], w[1], w[2]};
     }
-    const uint64_t* const from = a.part_keys + row * a.parts * a.top;
     __syncthreads();
-    for (int64_t i = lane; i < a.parts * a.top; i += 64) lists[i] = from[i];
-    t = wave_join(t, a.c);
-    if (lane == 0) write_row<T>(a, row, t);
-    __syncthreads();
-    uint32_t at = 0;
-    uint64_t head = a.top && lane < a.parts ? lists[lane * a.top] : 0;
-    for (uint32_t k = 0; k < a.top; ++k) {
-      const uint64_t best = wave_max_key(head);
-      if (head == best) {  // (keys differ: one lane)
-        write_alternative<T>(a, row, k, best, t);
-        ++at;
-        head = at < a.top ? lists[lane * a.top + at] : 0;
+    if (threadIdx.x < 64) {
+      t = wave_join(t, a.c);
+      if (lane == 0) write_row<T>(a, row, t);
+      const uint32_t end = (lane + 1) * a.top;
+      uint32_t at = lane * a.top;
+      uint64_t head = a.top && threadIdx.x < parts ? lists[at] : 0, mine = 0;
+      for (uint32_t k = 0; k < a.top; ++k) {
+        const uint64_t best = wave_max_key(head);
+        if (k == threadIdx.x) mine = best;
+        if (head == best) head = ++at < end ? lists[at] : 0;  // (keys differ: one lane)
       }
+      if (threadIdx.x < a.top) write_alternative(a, row, threadIdx.x, mine, t);
     }
+    __syncthreads();  // the next row's lists
   }
 }
 
@@ -460,7 +473,7 @@ hipError_t launch_forward(const Args& a, hipStream_t stream) {
     hipLaunchKernelGGL((logprobs_kernel<T, kHeldRounds>), grid, block, 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
-  hipLaunchKernelGGL((join_parts_kernel<T>), grid_of(a.rows), dim3(64),
+  hipLaunchKernelGGL((join_parts_kernel<T>), grid_of(a.rows), dim3(kThreads),
                      static_cast<unsigned>(a.parts * a.top * sizeof(uint64_t)), stream, a);
   return hipGetLastError();
 }

@@ -72,7 +72,7 @@ bool in_place(const int8_t* p, int64_t ld) { return ld % 16 == 0 && reinterpret_
 
 // The workspace: copies of the operands that need one, then the partial sums.
 struct Plan {
-  bool few_rows;  // the kernel for few tokens, which reads any alignment and needs no workspace
+  bool few_rows;  // the kernel for few tokens (any alignment, no workspace) where it is predicted to be faster
   bool copy_a, copy_b;
   int64_t lda, ldb, b_rows, b_cols;
   uint64_t a_at, b_at, sums_at, bytes;
@@ -84,13 +84,22 @@ Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
   const bool inner = g.b_layout == RNS8_MI355X_B_INNER;
   p.lda = g.lda;
   p.ldb = g.ldb;
-  p.few_rows = scaled_rows_takes(g.m, g.n, g.k, inner);
-  if (p.few_rows) return p;
+  p.tiles = choose_tile_shape(g.m, g.n, g.k);
   p.b_rows = inner ? g.k : g.n;
   p.b_cols = inner ? g.n : g.k;
   // where b is n x k, a's chunks are read whole: they have to end in zeros
   p.copy_a = g.k > 0 && !(in_place(g.a, g.lda) && (inner || a_zero_filled || g.k % 16 == 0));
   p.copy_b = g.k > 0 && !in_place(g.b, g.ldb);
+  if (scaled_rows_takes(g.m, g.n, g.k, inner)) {
+    // a copy: a launch, and its bytes read and written
+    const double copies = (p.copy_a ? 2.0 + static_cast<double>(g.m) * static_cast<double>(g.k) / 2.5e6 : 0.0) +
+                          (p.copy_b ? 2.0 + static_cast<double>(g.n) * static_cast<double>(g.k) / 2.5e6 : 0.0);
+    p.few_rows = scaled_rows_cost(g.m, g.n, g.k) <= p.tiles.cost + copies;
+    if (p.few_rows) {
+      p.copy_a = p.copy_b = false;
+      return p;
+    }
+  }
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t got = at;
@@ -101,7 +110,6 @@ Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
   p.ldb = p.copy_b ? static_cast<int64_t>(round_up(static_cast<uint64_t>(p.b_cols), 16)) : g.ldb;
   if (p.copy_a) p.a_at = take(static_cast<uint64_t>(g.m) * static_cast<uint64_t>(p.lda));
   if (p.copy_b) p.b_at = take(static_cast<uint64_t>(p.b_rows) * static_cast<uint64_t>(p.ldb));
-  p.tiles = choose_tile_shape(g.m, g.n, g.k, inner);
   p.sums_at = take(p.tiles.bytes);
   p.bytes = at;
   return p;

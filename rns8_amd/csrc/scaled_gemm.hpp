@@ -31,13 +31,18 @@ struct TileShape {
   int64_t k_slice;  // a multiple of 128 where slices > 1
   int64_t ldp;
   uint64_t bytes;
+  double cost;  // predicted us
 };
-TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k, bool inner);
+TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k);
 hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int32_t* partials, hipStream_t stream);
 
 // Few tokens (scaled_rows.hip): operands at any alignment, no workspace.
 bool scaled_rows_takes(int64_t m, int64_t n, int64_t k, bool inner);
+double scaled_rows_cost(int64_t m, int64_t n, int64_t k);  // predicted us
 hipError_t launch_scaled_rows(const ScaledGemm& g, hipStream_t stream);
+
+// What operands read once arrive at, for the predicted times: bytes per us.
+constexpr double kBytesPerUs = 5.5e6;
 
 // Products of at most this many bytes in one int32 sum: |a b| <= 2^14.
 constexpr int64_t kExactK = 131071;

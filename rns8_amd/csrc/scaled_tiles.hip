@@ -481,11 +481,16 @@ __global__ __launch_bounds__(256) void join_slices_kernel(JoinArgs a) {
     const int64_t row = q / quads, c = 4 * (q - row * quads);
     if (c >= a.n) continue;
     int64_t sum[4] = {};
-    const int32_t* p = a.partials + row * a.ldp + c;
-    for (uint32_t s = 0; s < a.slices; ++s, p += a.m * a.ldp) {
-      const v4i v = *reinterpret_cast<const v4i*>(p);
+    const int32_t* const p = a.partials + row * a.ldp + c;
+    for (uint32_t s = 0; s < a.slices; s += 8) {  // eight loads in flight
+      v4i v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += v[e];
+      for (uint32_t i = 0; i < 8; ++i)
+        v[i] = *reinterpret_cast<const v4i*>(p + static_cast<int64_t>(min(s + i, a.slices - 1)) * a.m * a.ldp);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += s + i < a.slices ? v[i][e] : 0;
     }
     const float sa = a.a_scale ? a.a_scale[row] : 1.0f;
     float sb[4], bias[4], f[4];
@@ -527,22 +532,40 @@ hipError_t launch_tile(const TileArgs& a, const TileShape& s, hipStream_t stream
 
 }  // namespace
 
-TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k, bool) {
-  // The tile whose launch is predicted fastest, by the plane GEMM's costs (a
-  // start, then for the CU with the most units each unit's chunks and
-  // epilogue), over the K slices that the shape allows.
-  struct Cost {
-    uint32_t bm, bn;
-    int64_t start, chunk, unit;
-  };
-  constexpr Cost kCosts[] = {
-      {256, 256, 400, 150, 300}, {256, 128, 350, 84, 200}, {128, 256, 350, 84, 200}, {128, 128, 300, 45, 100},
-      {64, 64, 250, 25, 60}};
+namespace {
+
+// A tile's costs in us, fitted to launches of 19 shapes from 64 x 64 x 100000 to
+// 4096 x 8192 x 8192 in both layouts (bf16 outputs, every tile and 1 to 32
+// slices each): a start (launch, first loads, epilogue) and one chunk of 128 K
+// on a CU that holds one workgroup, where few CUs do (`alone`) and where all do
+// (`full`: clock and memory are shared), and per workgroup where it holds more
+// (`shared`).
+struct TileCost {
+  uint32_t bm, bn, resident;
+  double start, alone, full, shared;
+};
+constexpr TileCost kTileCosts[] = {{256, 256, 1, 10.8, 1.05, 1.60, 1.60},
+                                   {256, 128, 1, 6.6, 0.67, 1.10, 1.10},
+                                   {128, 256, 1, 6.6, 0.71, 1.15, 1.15},
+                                   {128, 128, 2, 5.8, 0.42, 0.50, 0.61},
+                                   {64, 64, 4, 3.6, 0.35, 0.35, 0.25}};
+
+double tile_cost(const TileCost& c, int64_t m, int64_t n, int64_t k, double units, int64_t k_slice) {
+  const double chunks = static_cast<double>(std::max<int64_t>(1, (k_slice + 127) / 128));
+  const double per_cu = std::ceil(units / 256);
+  double chunk = c.alone + (c.full - c.alone) * std::min(1.0, units / 256);
+  if (per_cu > 1) chunk = std::max(chunk, c.shared * per_cu);
+  const double operands = static_cast<double>(m + n) * static_cast<double>(k) / kBytesPerUs;
+  return c.start + std::max(chunks * chunk, operands);
+}
+
+}  // namespace
+
+TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k) {
   TileShape best{};
-  double best_cost = 0;
   const int64_t need = std::max<int64_t>(1, (k + kExactK - 1) / kExactK);
-  for (const Cost& c : kCosts) {
-    const int64_t tiles = ((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn);
+  for (const TileCost& c : kTileCosts) {
+    const double tiles = static_cast<double>((m + c.bm - 1) / c.bm) * static_cast<double>((n + c.bn - 1) / c.bn);
     for (const int64_t wanted : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
       int64_t s = std::max(wanted, need);
       if (s > 1 && k < 256 * s) continue;  // slices of two chunks at least
@@ -552,14 +575,15 @@ TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k, bool) {
         k_slice = std::min<int64_t>(k_slice, kExactK / 128 * 128);
         s = (k + k_slice - 1) / k_slice;
       }
-      const double units = static_cast<double>(tiles) * static_cast<double>(s);
+      const double units = tiles * static_cast<double>(s);
       if (units > 0x7FFFFFFF) continue;
-      const int64_t chunks = std::max<int64_t>(1, (k_slice + 127) / 128);
-      double cost = static_cast<double>(c.start) + std::ceil(units / 256) * static_cast<double>(chunks * c.chunk + c.unit);
-      // the join: a launch, and the partial sums written and read (about 5 TB/s)
-      if (s > 1) cost += 350 + static_cast<double>(s) * static_cast<double>(m) * static_cast<double>(n) * 8 / 5e4;
-      if (best_cost != 0 && cost >= best_cost) continue;
-      best_cost = cost;
+      double cost = tile_cost(c, m, n, k, units, k_slice);
+      // the join: a launch, and the partial sums written and read
+      if (s > 1)
+        cost += 2.2 + 0.03 * static_cast<double>(s) +
+                static_cast<double>(s) * static_cast<double>(m) * static_cast<double>(n) * 8 / 4e6;
+      if (best.cost != 0 && cost >= best.cost) continue;
+      best.cost = cost;
       best.bm = c.bm;
       best.bn = c.bn;
       best.slices = static_cast<uint32_t>(s);
