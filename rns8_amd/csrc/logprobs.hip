@@ -1,27 +1,29 @@
 // Log-probabilities of given tokens, entropy and top alternatives, and their
 // gradient (gfx950).
 //
-// With a maximum m over the row's logits, c = scale * log2(e) and d = (v - m) c
+// With a maximum m over the row's logits, c = scale * log2(e) and d = c v - c m
 // for each logit v:
 //   S = sum 2^d,  W = sum 2^d d
-//   lse = scale m + ln S,  logp = ln2 (d[target] - log2 S),  entropy = ln2 (log2 S - W / S)
-// S and W are kept for a running maximum: when it rises by t (in powers of two),
-// S becomes S 2^-t and W becomes (W - t S) 2^-t, so one pass over the row is
-// enough. The difference v - m comes first, so that a term's error goes with
-// its distance from the maximum and logits of any size (a mask of the type's
-// lowest value) are as good as others. 32 bits hold every sum. Both kernels are
-// bound by reading the logits (and writing their gradient): a logit costs about
-// eleven vector operations, the exponential counted as four, beside its bytes.
+//   lse = ln2 (c m + log2 S),  logp = ln2 (d[target] - log2 S),  entropy = ln2 (log2 S - W / S)
+// S and W are kept for a running maximum: when c m rises by t, S becomes S 2^-t
+// and W becomes (W - t S) 2^-t, so one pass over the row is enough. d is one
+// fused multiply-add against the rounded c m, which is what lse starts from, so
+// its error goes with its own size; rows of nothing but values near the type's
+// lowest (masks) take v - m first instead, where c m would overflow. 32 bits
+// hold every sum. Both kernels are bound by reading the logits (and writing
+// their gradient): a logit costs about ten vector operations, the exponential
+// counted as four, and the next loads are in flight beside them.
 //
 // Few rows are cut into parts of a few thousand logits, one workgroup each,
 // whose sums and alternatives a second kernel joins: 4 rows of 131072 would
 // occupy 4 of 256 CUs.
 //
-// Alternatives: a part keeps its logits in registers over both looks at them.
-// The n-th largest of any n different threads' maxima is a lower bound of the
-// part's n-th largest logit, so with 4 waves the least of the waves'
-// ceil(n/4)-th largest lane maxima is one: the few logits from there on are
-// gathered and ordered by counting. Where too many are equal (a part of one
+// Alternatives: the n-th largest of any n different threads' maxima is a lower
+// bound of the part's n-th largest logit, so with 4 waves the least of the waves'
+// ceil(n/4)-th largest lane maxima is one. Only threads whose maximum reaches it
+// hold candidates: short parts keep their logits in registers for that look,
+// longer ones read those threads' logits again (some tens of 256 threads). The
+// candidates are ordered by counting; where too many are equal (a part of one
 // value) the alternatives are taken one by one.
 #include <algorithm>
 
@@ -36,7 +38,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kVector = 8;                     // logits of one load
 constexpr int kStride = kThreads * kVector;    // logits of one round of a workgroup
-constexpr int kHeldRounds = 4;                 // rounds that stay in registers
+constexpr int kHeldRounds = 4;                 // rounds that may stay in registers
 constexpr int64_t kMaxParts = 64;              // a wave joins a row
 constexpr uint32_t kMaxCandidates = 512;
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
@@ -50,13 +52,20 @@ struct Sums {
 };
 
 __device__ __forceinline__ bool is_empty(Sums t) { return t.m == -INFINITY && t.s == 0.0f; }
-// What logits are compared with: m, or 0 while every logit is ruled out.
-__device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// d for a logit against the maximum m: c v - c m. Below kLow c m may overflow:
+// the difference comes first there (m = -infinity: nothing but ruled-out tokens,
+// d = -infinity).
+constexpr float kLow = -1e37f;
+__device__ __forceinline__ float exponent(float v, float m, float c) {
+  if (m > kLow) return fmaf(v, c, -(m * c));
+  return m == -INFINITY ? v : (v - m) * c;
+}
 
 // `a` for a maximum m >= a.m.
 __device__ __forceinline__ Sums rescale(Sums a, float m, float c) {
   if (a.m == m || a.m == -INFINITY) return {m, a.s, a.w};
-  const float t = (a.m - m) * c, e = exp2_fast(t);
+  const float t = a.m > kLow ? a.m * c - m * c : (a.m - m) * c, e = exp2_fast(t);
   // (sums that the maximum has left behind by more than floats hold: t s may be infinite)
   return {m, a.s * e, e > 0.0f ? (a.w + t * a.s) * e : 0.0f};
 }
@@ -96,13 +105,25 @@ __device__ __forceinline__ void add_logits(Sums& t, const float (&v)[kVector], f
 #pragma unroll
   for (int i = 0; i < kVector; ++i) m = fmaxf(m, v[i]);
   if (m > t.m) t = rescale(t, m, c);
-  const float from = origin(m);
+  auto add = [&](float d, float& s, float& w) {
+    const float e = exp2_fast(d);
+    s += e;
+    w = fmaf(e, fmaxf(d, -200.0f), w);  // (2^-200 is 0 in 32 bits, and so is its term)
+  };
+  float s = 0.0f, w = 0.0f;  // (a second pair of sums: two chains of additions)
+  if (m > kLow) {
+    const float base = -(m * c);
 #pragma unroll
-  for (int i = 0; i < kVector; ++i) {
-    const float d = (v[i] - from) * c, e = exp2_fast(d);
-    t.s += e;
-    t.w = fmaf(e, fmaxf(d, -200.0f), t.w);  // (2^-200 is 0 in 32 bits, and so is its term)
+    for (int i = 0; i < kVector; i += 2) {
+      add(fmaf(v[i], c, base), t.s, t.w);
+      add(fmaf(v[i + 1], c, base), s, w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVector; ++i) add(exponent(v[i], m, c), t.s, t.w);
   }
+  t.s += s;
+  t.w += w;
 }
 
 // Order of the alternatives as one unsigned integer: the logit's order (NaNs
@@ -140,16 +161,20 @@ struct Args {
   uint64_t* part_keys;      // [rows][parts][top]
 };
 
+__device__ __forceinline__ float lse_of(Sums t, float scale, float c, float log_s) {
+  return t.m > kLow ? kLn2 * (t.m * c + log_s) : t.m == -INFINITY ? kLn2 * log_s : t.m * scale + kLn2 * log_s;
+}
+
 // The log-probability of a logit.
 __device__ __forceinline__ float logp_of(float v, Sums t, float c) {
-  return is_empty(t) ? -INFINITY : kLn2 * ((v - origin(t.m)) * c - log2f(t.s));
+  return is_empty(t) ? -INFINITY : kLn2 * (exponent(v, t.m, c) - log2f(t.s));
 }
 
 // A row's results from its sums (one thread).
 template <typename T>
 __device__ __forceinline__ void write_row(const Args& a, int64_t row, Sums t) {
   const float log_s = log2f(t.s);
-  if (a.lse) a.lse[row] = is_empty(t) ? -INFINITY : origin(t.m) * a.scale + kLn2 * log_s;
+  if (a.lse) a.lse[row] = is_empty(t) ? -INFINITY : lse_of(t, a.scale, a.c, log_s);
   if (a.entropy) a.entropy[row] = is_empty(t) ? 0.0f : kLn2 * (log_s - t.w / t.s);
   if (a.logp) {
     const int64_t target = a.targets[row];
@@ -175,7 +200,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   __shared__ Sums wave_sums[kWaves];
   __shared__ float wave_least[kWaves];
   __shared__ uint64_t keys[kMaxCandidates];
-  __shared__ uint32_t count;
+  __shared__ uint32_t count, lane_count;
+  __shared__ uint8_t lanes[kThreads];  // threads with candidates
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int64_t unit = blockIdx.x; unit < a.rows * a.parts; unit += gridDim.x) {
     const int64_t row = unit / a.parts, part = unit - row * a.parts;
@@ -206,23 +232,42 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
         add_logits(t, v, a.c);
       }
     } else {
-      int64_t at = first + kVector * threadIdx.x;
-      for (; at + kStride + kVector <= last; at += 2 * kStride) {
-        Held<T> next;
-        load(at, held[0]);
-        load(at + kStride, next);
-        floats(held[0], v);
+      // two vectors at a time, the next two in flight (the last are loaded twice)
+      const int64_t at = first + kVector * threadIdx.x;
+      const int64_t whole = last - at >= kVector ? (last - at - kVector) / kStride + 1 : 0;
+      Held<T> x[2], y[2];
+      auto load_pair = [&](int64_t i, Held<T> (&h)[2]) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          __builtin_memcpy(h[k].v, z + at + min(i + k, whole - 1) * kStride, sizeof(h[k].v));
+      };
+      auto add_pair = [&](int64_t i, const Held<T> (&h)[2]) {
+        floats(h[0], v);
         add_logits(t, v, a.c);
-        floats(next, v);
-        add_logits(t, v, a.c);
+        if (i + 1 < whole) {
+          floats(h[1], v);
+          add_logits(t, v, a.c);
+        }
+      };
+      if (whole > 0) {
+        load_pair(0, x);
+        for (int64_t i = 0; i < whole; i += 4) {
+          load_pair(i + 2, y);
+          add_pair(i, x);
+          if (i + 2 >= whole) break;
+          load_pair(i + 4, x);
+          add_pair(i + 2, y);
+        }
       }
-      for (; at < last; at += kStride) {
-        load(at, held[0]);
+      const int64_t rest = at + whole * kStride;
+      if (rest < last) {  // the vector that the part's end cuts
+        load(rest, held[0]);
         floats(held[0], v);
         add_logits(t, v, a.c);
       }
     }
     const float lane_max = t.m;
+    const bool lane_nan = t.s != t.s;  // a NaN among the lane's logits, which comes first
     t = wave_join(t, a.c);
     if (lane == 0) wave_sums[wave] = t;
     if (a.top) {
@@ -234,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
         if (lane == __ffsll(static_cast<unsigned long long>(who)) - 1) mine = -INFINITY;
       }
       if (lane == 0) wave_least[wave] = least;
-      if (threadIdx.x == 0) count = 0;
+      if (threadIdx.x == 0) count = lane_count = 0;
     }
     __syncthreads();
     t = join_waves(wave_sums, a.c);
@@ -260,17 +305,30 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
           }
         }
       };
+      const bool mine = !(lane_max < from) || lane_nan;
+      const uint32_t rounds = static_cast<uint32_t>((last - first + kStride - 1) / kStride);
+      // f on every vector of the threads with candidates
       auto each = [&](auto&& f) {
         if constexpr (kRounds > 0) {
+          if (mine) {
 #pragma unroll
-          for (int r = 0; r < kRounds; ++r) f(first + r * kStride + kVector * threadIdx.x, held[r]);
+            for (int r = 0; r < kRounds; ++r) f(first + r * kStride + kVector * threadIdx.x, held[r]);
+          }
         } else {
-          for (int64_t at = first + kVector * threadIdx.x; at < last; at += kStride) {
-            load(at, held[0]);
-            f(at, held[0]);
+          for (uint32_t i = threadIdx.x; i < lane_count * rounds; i += kThreads) {
+            const uint32_t who = i / rounds;
+            const int64_t at = first + static_cast<int64_t>(i - who * rounds) * kStride + kVector * lanes[who];
+            if (at < last) {
+              load(at, held[0]);
+              f(at, held[0]);
+            }
           }
         }
       };
+      if constexpr (kRounds == 0) {
+        if (mine) lanes[atomicAdd(&lane_count, 1u)] = static_cast<uint8_t>(threadIdx.x);
+        __syncthreads();
+      }
       each(gather);
       __syncthreads();
       auto put = [&](uint32_t rank, uint64_t key) {
@@ -401,8 +459,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
       t = join_waves(wave_sums, a.c);
       // (where dlogits is logits: nothing is written before the whole row is read)
       __syncthreads();
-      from = origin(t.m);
-      log_s = is_empty(t) ? 0.0f : kLn2 * log2f(t.s);
+      from = t.m == -INFINITY ? 0.0f : t.m;
+      // (the sums' origin is the rounded c m; here it is m itself)
+      const float off = t.m > kLow ? fmaf(t.m, a.c, -(t.m * a.c)) : 0.0f;
+      log_s = is_empty(t) ? 0.0f : kLn2 * (log2f(t.s) - off);
     }
     auto grad = [&](int64_t at, float (&v)[kVector]) {
       float d[kVector];
@@ -444,15 +504,9 @@ void cut_rows(int64_t rows, int64_t vocab, int64_t units, int64_t least, int64_t
   len = per * kStride;
 }
 
-// With alternatives a part is at most kHeldRounds rounds while 64 parts are enough.
+// With alternatives a part may be one round, as it stays in registers.
 void forward_parts(int64_t rows, int64_t vocab, uint32_t top, int64_t& parts, int64_t& len) {
   cut_rows(rows, vocab, 1024, top ? 1 : 4, parts, len);
-  const int64_t rounds = (vocab + kStride - 1) / kStride, need = (rounds + kHeldRounds - 1) / kHeldRounds;
-  if (top && need > parts && need <= kMaxParts) {
-    const int64_t per = (rounds + need - 1) / need;
-    parts = (rounds + per - 1) / per;
-    len = per * kStride;
-  }
 }
 
 dim3 grid_of(int64_t units) { return dim3(static_cast<unsigned>(std::min(units, kMaxBlocks))); }
