@@ -11,6 +11,7 @@ namespace rns8x {
 
 using f16 = _Float16;
 using bf16 = __bf16;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
 __device__ __forceinline__ uint32_t as_uint(float x) { return __builtin_bit_cast(uint32_t, x); }
@@ -32,6 +33,18 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) t[i] = static_cast<T>(v[i]);  // to nearest even
   __builtin_memcpy(p, t, sizeof(t));
+}
+
+// Past the caches, to a 16-byte aligned address.
+template <typename T>
+__device__ __forceinline__ void stream8(T* p, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = static_cast<T>(v[i]);
+  u32x4 w[sizeof(t) / 16];
+  __builtin_memcpy(w, t, sizeof(t));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(t) / 16; ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4*>(p) + i);
 }
 
 // The first `n` (at most 8) of eight elements; the others read `other` and are not written.
@@ -57,8 +70,6 @@ __device__ __forceinline__ void store_upto8(T* p, int64_t n, const float (&v)[8]
 }
 
 // ---- rows in registers -------------------------------------------------------------
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // Eight consecutive elements as loaded.
 template <typename T>
 struct Packed8 {

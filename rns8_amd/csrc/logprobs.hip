@@ -100,30 +100,53 @@ __device__ __forceinline__ Sums join_waves(const Sums* wave_sums, float c) {
   return t;
 }
 
-__device__ __forceinline__ void add_logits(Sums& t, const float (&v)[kVector], float c) {
+// Adds kCount logits. The decisions are the wave's, so that none of them costs
+// more than a compare and a branch: a new maximum, a maximum below kLow, and
+// ruled-out tokens, whose 2^d d is 0 times infinity: the chunk's own W is then
+// NaN, its terms are taken again with d held above -200 (2^-200 is 0 in 32 bits,
+// and so is its term), and so are those of the wave's later chunks at once
+// (`held`: at first false).
+template <int kCount>
+__device__ __forceinline__ void add_logits(Sums& t, const float (&v)[kCount], float c, bool& held) {
   float m = t.m;
 #pragma unroll
-  for (int i = 0; i < kVector; ++i) m = fmaxf(m, v[i]);
-  if (m > t.m) t = rescale(t, m, c);
-  auto add = [&](float d, float& s, float& w) {
-    const float e = exp2_fast(d);
-    s += e;
-    w = fmaf(e, fmaxf(d, -200.0f), w);  // (2^-200 is 0 in 32 bits, and so is its term)
-  };
-  float s = 0.0f, w = 0.0f;  // (a second pair of sums: two chains of additions)
-  if (m > kLow) {
-    const float base = -(m * c);
+  for (int i = 0; i < kCount; ++i) m = fmaxf(m, v[i]);
+  if (__any(m > t.m)) t = rescale(t, m, c);
+  const float base = -(m * c);
+  float s[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};  // two chains of additions
+  if (__any(!(m > kLow))) {
 #pragma unroll
-    for (int i = 0; i < kVector; i += 2) {
-      add(fmaf(v[i], c, base), t.s, t.w);
-      add(fmaf(v[i + 1], c, base), s, w);
+    for (int i = 0; i < kCount; ++i) {
+      const float d = exponent(v[i], m, c), e = exp2_fast(d);
+      s[i & 1] += e;
+      w[i & 1] = fmaf(e, fmaxf(d, -200.0f), w[i & 1]);
     }
   } else {
+    if (!held) {
 #pragma unroll
-    for (int i = 0; i < kVector; ++i) add(exponent(v[i], m, c), t.s, t.w);
+      for (int i = 0; i < kCount; ++i) {
+        const float d = fmaf(v[i], c, base), e = exp2_fast(d);
+        s[i & 1] += e;
+        w[i & 1] = fmaf(e, d, w[i & 1]);
+      }
+      const float sum = w[0] + w[1];
+      held = __any(sum != sum);
+      if (held) s[0] = s[1] = w[0] = w[1] = 0.0f;
+      if (!held) {
+        t.s += s[0] + s[1];
+        t.w += sum;
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const float d = fmaf(v[i], c, base), e = exp2_fast(d);
+      s[i & 1] += e;
+      w[i & 1] = fmaf(e, fmaxf(d, -200.0f), w[i & 1]);
+    }
   }
-  t.s += s;
-  t.w += w;
+  t.s += s[0] + s[1];
+  t.w += w[0] + w[1];
 }
 
 // Order of the alternatives as one unsigned integer: the logit's order (NaNs
@@ -208,6 +231,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
     const T* const z = static_cast<const T*>(a.logits) + row * a.ldl;
     const int64_t first = part * a.part_len, last = min(a.vocab, first + a.part_len);
     Sums t{-INFINITY, 0.0f, 0.0f};
+    bool terms_held = false;
     constexpr int kHold = kRounds > 0 ? kRounds : 1;
     Held<T> held[kHold];
     auto load = [&](int64_t at, Held<T>& h) {
@@ -229,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
         floats(held[r], v);
-        add_logits(t, v, a.c);
+        add_logits(t, v, a.c, terms_held);
       }
     } else {
       // two vectors at a time, the next two in flight (the last are loaded twice)
@@ -242,12 +266,17 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
           __builtin_memcpy(h[k].v, z + at + min(i + k, whole - 1) * kStride, sizeof(h[k].v));
       };
       auto add_pair = [&](int64_t i, const Held<T> (&h)[2]) {
-        floats(h[0], v);
-        add_logits(t, v, a.c);
-        if (i + 1 < whole) {
-          floats(h[1], v);
-          add_logits(t, v, a.c);
+        float u[2 * kVector];
+#pragma unroll
+        for (int k = 0; k < kVector; ++k) {
+          u[k] = static_cast<float>(h[0].v[k]);
+          u[kVector + k] = static_cast<float>(h[1].v[k]);
         }
+        if (i + 1 >= whole) {  // the second was loaded twice
+#pragma unroll
+          for (int k = 0; k < kVector; ++k) u[kVector + k] = -INFINITY;
+        }
+        add_logits(t, u, a.c, terms_held);
       };
       if (whole > 0) {
         load_pair(0, x);
@@ -263,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
       if (rest < last) {  // the vector that the part's end cuts
         load(rest, held[0]);
         floats(held[0], v);
-        add_logits(t, v, a.c);
+        add_logits(t, v, a.c, terms_held);
       }
     }
     const float lane_max = t.m;
@@ -430,6 +459,7 @@ struct BackArgs {
   void* dlogits;
   int64_t lddl;
   int64_t parts, part_len;
+  uint32_t streamed;  // stores pass the caches by
 };
 
 template <typename T>
@@ -448,10 +478,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
     float from = 0.0f, log_s = a.lse[row];  // log p = scale (v - from) - log_s
     if (fabsf(log_s) > kLargeLse) {
       Sums t{-INFINITY, 0.0f, 0.0f};
+      bool terms_held = false;
       for (int64_t at = kVector * threadIdx.x; at < a.vocab; at += kStride) {
         float v[kVector];
         load_upto8(z + at, a.vocab - at, v, -INFINITY);
-        add_logits(t, v, a.c);
+        add_logits(t, v, a.c, terms_held);
       }
       t = wave_join(t, a.c);
       if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = t;
@@ -477,7 +508,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
         for (int i = 0; i < kVector; ++i)
           if (at + i == target && v[i] != -INFINITY) d[i] += a.scale * gl;
       }
-      store_upto8(out + at, last - at, d);
+      if (a.streamed && at + kVector <= last)
+        stream8(out + at, d);
+      else
+        store_upto8(out + at, last - at, d);
     };
     int64_t at = first + kVector * threadIdx.x;
     float v[kVector], w[kVector];
@@ -565,7 +599,8 @@ hipError_t launch_logprobs(const rns8_mi355x_logprobs_args& g, hipStream_t strea
 hipError_t launch_logprobs_backward(const rns8_mi355x_logprobs_backward_args& g, hipStream_t stream) {
   if (g.rows == 0) return hipSuccess;
   BackArgs a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.scale * kLog2E, g.lse, g.entropy, g.dlogp,
-             g.dentropy, g.dlogits, g.lddl, 1, 0};
+             g.dentropy, g.dlogits, g.lddl, 1, 0, 0};
+  a.streamed = streams(g.rows * g.vocab * (g.dtype == RNS8_MI355X_F32 ? 4 : 2), g.dlogits, g.lddl, g.dtype);
   cut_rows(g.rows, g.vocab, 1024, 2, a.parts, a.part_len);
   if (g.dlogits == g.logits) {  // in place a row's logits may be read twice: by the workgroup that writes them
     a.parts = 1;

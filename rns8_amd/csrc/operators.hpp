@@ -14,6 +14,14 @@ namespace rns8x {
 
 inline uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
+// Whether an output's stores pass the caches by: from 128 MB on they would fill
+// the Infinity Cache (256 MB) with dirty lines, whose way out competes with the
+// next kernel's reads. Rows of 16-byte aligned vectors only.
+inline bool streams(int64_t bytes, const void* p, int64_t ld, uint32_t dtype) {
+  return bytes >= (int64_t{128} << 20) && reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+         ld * (dtype == RNS8_MI355X_F32 ? 4 : 2) % 16 == 0;
+}
+
 // ---- quantization (quantize.hip) -------------------------------------------------
 hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& a, hipStream_t stream);
 uint64_t quantize_columns_bytes(int64_t rows, int64_t cols);
