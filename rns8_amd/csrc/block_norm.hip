@@ -24,6 +24,7 @@ struct NormArgs {
   int8_t* q;
   int64_t ldq, stop;
   float *q_scale, *rstd;
+  uint32_t stream_h, stream_y;  // stores pass the caches by
 };
 
 __device__ __forceinline__ float inverse_rms(float sum_sq, int64_t cols, float eps) {
@@ -32,14 +33,14 @@ __device__ __forceinline__ float inverse_rms(float sum_sq, int64_t cols, float e
 
 // kGates: a row of the gate for each token.
 template <typename T, int kThreads, int kVectors, bool kGates>
-__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_kernel(NormArgs a) {
+__global__ __launch_bounds__(row_block(kThreads)) void block_norm_kernel(NormArgs a) {
   __shared__ uint32_t scratch[16];
   using Raw = RawRow<T, kVectors>;
   struct Rows {
     Raw x, res;
     RawRow<T, kGates ? kVectors : 1> gate;
   };
-  const int lane = kThreads >= 256 ? threadIdx.x : threadIdx.x & 63;
+  const int lane = row_is_shared(kThreads) ? threadIdx.x : threadIdx.x & 63;
   Weights<T, kVectors> w;
   load_weights<kThreads>(a, lane, w);
   auto load = [&](int64_t row, Rows& r) {
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ke
     load_row_or<kThreads>(a.residual, row * a.ldresidual, a.cols, lane, 0.0f, r.res);
     if constexpr (kGates) load_row<kThreads>(static_cast<const T*>(a.gate) + row * a.ldgate, a.cols, lane, r.gate);
   };
-  walk_rows<kThreads, Rows>(a.rows, load, [&](int64_t row, const Rows& r) {
+  walk_rows<kThreads, (kThreads < 1024), Rows>(a.rows, load, [&](int64_t row, const Rows& r) {
     float sum = 0.0f;
     float r1 = 1.0f;
     if (a.has_post) {
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ke
         h[j][i] = a.keep * r.res.v[j].at(i) + a.branch * gate_at<kGates>(r, w, j, i) * f;
         sum += h[j][i] * h[j][i];
       }
-      if (a.h) store_vector<kThreads, T, kVectors>(static_cast<T*>(a.h) + row * a.ldh, a.cols, j, lane, h[j]);
+      if (a.h) store_vector<kThreads, T, kVectors>(static_cast<T*>(a.h) + row * a.ldh, a.cols, j, lane, h[j], a.stream_h);
     }
     if (!a.has_pre) {
       if (a.rstd && lane == 0) a.rstd[row] = r1;
@@ -89,24 +90,25 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ke
         const uint32_t m = magnitude_bits(h[j][i]);
         amax = amax > m ? amax : m;
       }
-      if (a.y) store_vector<kThreads, T, kVectors>(static_cast<T*>(a.y) + row * a.ldy, a.cols, j, lane, h[j]);
+      if (a.y) store_vector<kThreads, T, kVectors>(static_cast<T*>(a.y) + row * a.ldy, a.cols, j, lane, h[j], a.stream_y);
     }
     if (a.q) {
       const RowScale s = row_scale(row_reduce<kThreads>(amax, MaxU{}, scratch));
       if (lane == 0) a.q_scale[row] = s.scale;
 #pragma unroll
       for (int j = 0; j < kVectors; ++j) {
-        const int64_t c = column_of<kThreads>(j, lane);
+        const uint32_t c = column_of<kThreads>(j, lane);
         if (c < a.stop) store_bytes8(a.q + row * a.ldq, c, a.stop, quantize8(h[j], s.inverse));
       }
     }
   });
 }
 
-// As many workgroups as stay on the chip at once (1024 threads to a CU): each
-// walks its rows.
-dim3 forward_grid(int threads, int64_t rows) {
-  const int64_t groups = threads == 64 ? (rows + 3) / 4 : rows, per_cu = threads == 64 ? 4 : 1024 / threads;
+// As many workgroups as stay on the chip at once (by registers, 1536 threads to
+// a CU with one vector each, 1024 with two): each walks its rows.
+dim3 forward_grid(int threads, int vectors, int64_t rows) {
+  const int64_t groups = threads == 64 ? (rows + 3) / 4 : rows;
+  const int64_t per_cu = std::max(1, (vectors == 1 ? 1536 : 1024) / row_block(threads));
   return dim3(static_cast<unsigned>(std::min<int64_t>(groups, 256 * per_cu)));
 }
 
@@ -140,10 +142,14 @@ hipError_t launch_block_norm(const rns8_mi355x_block_norm_args& g, hipStream_t s
   a.stop = quantized_stop(g.cols, g.ldq);
   a.q_scale = g.q_scale;
   a.rstd = g.rstd;
+  const int64_t rows_moved = 1 + (g.residual ? 1 : 0) + (g.gate && g.ldgate != 0 ? 1 : 0) + (g.h ? 1 : 0) + (g.y ? 1 : 0);
+  const int64_t moved = rows_moved * g.rows * g.cols * (g.dtype == RNS8_MI355X_F32 ? 4 : 2);
+  a.stream_h = streams(moved, g.h, g.ldh, g.dtype);
+  a.stream_y = streams(moved, g.y, g.ldy, g.dtype);
   return of_dtype(g.dtype, [&](auto t) {
-    return with_row_shape(choose_row_shape(g.rows, g.cols), [&](auto threads, auto vectors) {
+    return with_row_shape(choose_row_shape(g.rows, g.cols, sizeof(t)), [&](auto threads, auto vectors) {
       constexpr int kThreads = decltype(threads)::value;
-      const dim3 grid = forward_grid(kThreads, a.rows), block(kThreads < 256 ? 256 : kThreads);
+      const dim3 grid = forward_grid(kThreads, decltype(vectors)::value, a.rows), block(row_block(kThreads));
       if (a.gate && a.ldgate != 0)
         hipLaunchKernelGGL((block_norm_kernel<decltype(t), kThreads, decltype(vectors)::value, true>), grid, block, 0,
                            stream, a);

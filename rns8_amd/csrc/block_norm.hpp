@@ -41,13 +41,13 @@ __device__ __forceinline__ float gate_at(const Rows& r, const W& w, int j, int i
 // flight beside each body where the registers hold two rows. (Waves of a
 // workgroup that own rows of their own may run different counts: no barrier is
 // between them.)
-template <int kThreads, typename Rows, typename Load, typename Body>
+template <int kThreads, bool kAhead, typename Rows, typename Load, typename Body>
 __device__ __forceinline__ void walk_rows(int64_t rows, Load&& load, Body&& body) {
-  const bool shared = kThreads >= 256;
+  constexpr bool shared = row_is_shared(kThreads);
   const int64_t group = shared ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t step = static_cast<int64_t>(gridDim.x) * (shared ? 1 : 4);
   Rows now;
-  if constexpr (kThreads < 1024) {
+  if constexpr (kAhead) {
     Rows next;
     if (group < rows) load(group, now);
     for (int64_t row = group; row < rows; row += step) {

@@ -6,7 +6,10 @@
 //   dw_pre = sum_rows dy h r2,  dw_post = sum_rows df x r1
 //
 // Bound by HBM: four rows are read into registers, cross one reduction for each
-// norm and leave as two, while the next row's four are on their way.
+// norm and leave as two. The sums over rows take half of the registers, so the
+// next row's loads are those of the CU's other workgroups (holding the next
+// row beside this one left room for one workgroup of 512 to a CU: 8192 x 4096
+// 114 us against 93).
 #include <algorithm>
 
 #include "block_norm.hpp"
@@ -26,11 +29,12 @@ struct NormBackArgs {
   const float* rstd;
   void *dx, *dresidual, *dgate_rows;
   int64_t lddx, lddresidual, lddgate;
+  uint32_t stream_dx, stream_dresidual;  // stores pass the caches by
   float *part_post, *part_pre, *part_gate;  // [groups][cols], or NULL
 };
 
 template <typename T, int kThreads, int kVectors, bool kGates>
-__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_backward_kernel(NormBackArgs a) {
+__global__ __launch_bounds__(row_block(kThreads)) void block_norm_backward_kernel(NormBackArgs a) {
   __shared__ uint32_t scratch[16];
   using Raw = RawRow<T, kVectors>;
   struct Rows {
@@ -39,7 +43,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ba
   };
   float sum_post[kVectors][8] = {}, sum_pre[kVectors][8] = {}, sum_gate[kVectors][8] = {};
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
-  const int lane = kThreads >= 256 ? threadIdx.x : threadIdx.x & 63;
+  const int lane = row_is_shared(kThreads) ? threadIdx.x : threadIdx.x & 63;
   Weights<T, kVectors> w;
   load_weights<kThreads>(a, lane, w);
   auto load = [&](int64_t row, Rows& r) {
@@ -49,7 +53,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ba
     load_row_or<kThreads>(a.dy, row * a.lddy, a.cols, lane, 0.0f, r.dy);
     load_row_or<kThreads>(a.dh, row * a.lddh, a.cols, lane, 0.0f, r.dh);
   };
-  walk_rows<kThreads, Rows>(a.rows, load, [&](int64_t row, const Rows& r) {
+  walk_rows<kThreads, false, Rows>(a.rows, load, [&](int64_t row, const Rows& r) {
     const float r1 = a.has_post ? a.rstd[row] : 1.0f;
     const float r2 = a.has_pre ? a.rstd[a.rows + row] : 0.0f;
     auto gate = [&](int j, int i) { return gate_at<kGates>(r, w, j, i); };
@@ -79,7 +83,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ba
       if (a.dresidual) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[i] = a.keep * h[j][i];
-        store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dresidual) + row * a.lddresidual, a.cols, j, lane, out);
+        store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dresidual) + row * a.lddresidual, a.cols, j, lane, out, a.stream_dresidual);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ba
         dot += h[j][i] * r.x.v[j].at(i);
       }
       if (a.dgate_rows)
-        store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dgate_rows) + row * a.lddgate, a.cols, j, lane, out);
+        store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dgate_rows) + row * a.lddgate, a.cols, j, lane, out, false);
     }
     if (!a.dx) return;
     float k1 = 0.0f;
@@ -103,10 +107,10 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void block_norm_ba
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) out[i] = r1 * h[j][i] - r.x.v[j].at(i) * k1;
-      store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dx) + row * a.lddx, a.cols, j, lane, out);
+      store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dx) + row * a.lddx, a.cols, j, lane, out, a.stream_dx);
     }
   });
-  const int64_t group = kThreads >= 256 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t group = row_is_shared(kThreads) ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
 #pragma unroll
   for (int j = 0; j < kVectors; ++j) {
     const int64_t c = 8 * (static_cast<int64_t>(j) * kThreads + lane);
@@ -158,9 +162,9 @@ RowShape backward_shape(int64_t cols) { return row_shape(cols, cols <= 4096 ? 1 
 // Row groups of a backward launch: enough to fill the chip, few enough that
 // their partial sums stay small beside the rows.
 dim3 backward_grid(int64_t rows, int threads) {
-  const int64_t most = threads <= 256 ? 1024 : threads == 512 ? 512 : 256;
+  const int64_t most = threads <= 128 ? 2048 : threads == 256 ? 1024 : threads == 512 ? 512 : 256;
   const int64_t groups = threads == 64 ? (rows + 3) / 4 : rows;
-  return dim3(static_cast<unsigned>(std::min(groups, threads == 64 ? most / 2 : most)));
+  return dim3(static_cast<unsigned>(std::min(groups, threads == 64 ? most / 4 : most)));
 }
 int64_t partial_rows(int64_t rows, int threads) {
   const int64_t blocks = backward_grid(rows, threads).x;
@@ -221,6 +225,11 @@ hipError_t launch_block_norm_backward(const rns8_mi355x_block_norm_backward_args
   a.lddresidual = g.lddresidual;
   a.dgate_rows = g.ldgate != 0 ? g.dgate : nullptr;
   a.lddgate = g.lddgate;
+  const int64_t rows_moved = 1 + (g.residual ? 1 : 0) + (g.gate && g.ldgate != 0 ? 1 : 0) + (g.dy ? 1 : 0) +
+                             (g.dh ? 1 : 0) + (g.dx ? 1 : 0) + (g.dresidual ? 1 : 0);
+  const int64_t moved = rows_moved * g.rows * g.cols * (g.dtype == RNS8_MI355X_F32 ? 4 : 2);
+  a.stream_dx = streams(moved, g.dx, g.lddx, g.dtype);
+  a.stream_dresidual = streams(moved, g.dresidual, g.lddresidual, g.dtype);
   a.part_post = part_of(g.dpost_weight);
   a.part_pre = part_of(g.dpre_weight);
   a.part_gate = part_of(g.ldgate == 0 ? static_cast<float*>(g.dgate) : nullptr);
@@ -228,7 +237,7 @@ hipError_t launch_block_norm_backward(const rns8_mi355x_block_norm_backward_args
     const hipError_t e = of_dtype(g.dtype, [&](auto t) {
       return with_row_shape(shape, [&](auto threads, auto vectors) {
         constexpr int kThreads = decltype(threads)::value;
-        const dim3 grid = backward_grid(g.rows, kThreads), block(kThreads < 256 ? 256 : kThreads);
+        const dim3 grid = backward_grid(g.rows, kThreads), block(row_block(kThreads));
         if (a.gate && a.ldgate != 0)
           hipLaunchKernelGGL((block_norm_backward_kernel<decltype(t), kThreads, decltype(vectors)::value, true>), grid,
                              block, 0, stream, a);

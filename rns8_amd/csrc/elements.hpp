@@ -134,21 +134,28 @@ struct RawRow {
 };
 
 template <int kThreads>
-__device__ __forceinline__ int64_t column_of(int vector, int lane) {
-  return 8 * (static_cast<int64_t>(vector) * kThreads + lane);
+__device__ __forceinline__ uint32_t column_of(int vector, int lane) {
+  return 8 * (static_cast<uint32_t>(vector) * kThreads + static_cast<uint32_t>(lane));
+}
+
+// Element `at` of a row below 2^32 bytes, as the row's (uniform) address and a 32-bit offset.
+template <typename T>
+__device__ __forceinline__ T* element(T* row, uint32_t at) {
+  using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(row) + static_cast<uint32_t>(at * sizeof(T)));
 }
 
 // Elements past the row are zeros. One load to a vector: lanes past the row
 // read its start, the lane that the row's end cuts reads the row's last eight
 // and drops those that are others'. Rows below eight are read by elements.
 template <int kThreads, typename T, int kVectors>
-__device__ __forceinline__ void load_row(const T* row, int64_t cols, int lane, RawRow<T, kVectors>& r) {
+__device__ __forceinline__ void load_row(const T* row, uint32_t cols, int lane, RawRow<T, kVectors>& r) {
   if (cols < 8) {
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) r.v[j].fill(static_cast<T>(0.0f));
     if (lane == 0) {
       T t[8] = {};
-      for (int i = 0; i < 8; ++i)
+      for (uint32_t i = 0; i < 8; ++i)
         if (i < cols) t[i] = row[i];
       __builtin_memcpy(r.v[0].q, t, sizeof(t));
     }
@@ -156,23 +163,27 @@ __device__ __forceinline__ void load_row(const T* row, int64_t cols, int lane, R
   }
 #pragma unroll
   for (int j = 0; j < kVectors; ++j) {
-    const int64_t c = column_of<kThreads>(j, lane);
-    const int64_t at = c + 8 <= cols ? c : c < cols ? cols - 8 : 0;
-    __builtin_memcpy(r.v[j].q, row + at, sizeof(r.v[j].q));
+    const uint32_t c = column_of<kThreads>(j, lane);
+    const uint32_t at = c + 8 <= cols ? c : c < cols ? cols - 8 : 0;
+    __builtin_memcpy(r.v[j].q, element(row, at), sizeof(r.v[j].q));
   }
   if (cols == 8 * kThreads * kVectors) return;
 #pragma unroll
   for (int j = 0; j < kVectors; ++j) {
-    const int64_t c = column_of<kThreads>(j, lane);
-    if (cols % 8 != 0) r.v[j].drop(c < cols && c + 8 > cols ? static_cast<uint32_t>(c + 8 - cols) : 0u);
+    const uint32_t c = column_of<kThreads>(j, lane);
+    if (cols % 8 != 0) r.v[j].drop(c < cols && c + 8 > cols ? c + 8 - cols : 0u);
     if (c >= cols) r.v[j].fill(static_cast<T>(0.0f));
   }
 }
 
 template <int kThreads, typename T, int kVectors>
-__device__ __forceinline__ void store_vector(T* row, int64_t cols, int vector, int lane, const float (&v)[8]) {
-  const int64_t c = column_of<kThreads>(vector, lane);
-  if (c < cols) store_upto8(row + c, cols - c, v);
+__device__ __forceinline__ void store_vector(T* row, uint32_t cols, int vector, int lane, const float (&v)[8],
+                                             bool streamed) {
+  const uint32_t c = column_of<kThreads>(vector, lane);
+  if (streamed && c + 8 <= cols)
+    stream8(element(row, c), v);
+  else if (c < cols)
+    store_upto8(element(row, c), static_cast<int64_t>(cols - c), v);
 }
 
 // ---- reductions over a wave: every lane ends with the result --------------------

@@ -600,7 +600,7 @@ hipError_t launch_logprobs_backward(const rns8_mi355x_logprobs_backward_args& g,
   if (g.rows == 0) return hipSuccess;
   BackArgs a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.scale * kLog2E, g.lse, g.entropy, g.dlogp,
              g.dentropy, g.dlogits, g.lddl, 1, 0, 0};
-  a.streamed = streams(g.rows * g.vocab * (g.dtype == RNS8_MI355X_F32 ? 4 : 2), g.dlogits, g.lddl, g.dtype);
+  a.streamed = streams(2 * g.rows * g.vocab * (g.dtype == RNS8_MI355X_F32 ? 4 : 2), g.dlogits, g.lddl, g.dtype);
   cut_rows(g.rows, g.vocab, 1024, 2, a.parts, a.part_len);
   if (g.dlogits == g.logits) {  // in place a row's logits may be read twice: by the workgroup that writes them
     a.parts = 1;

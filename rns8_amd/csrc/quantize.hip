@@ -57,7 +57,7 @@ __device__ __forceinline__ void quantize_row(const RowsArgs& a, int64_t row, int
     if (lane == 0) a.scale[row] = s.scale;
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      const int64_t c = column_of<kThreads>(j, lane);
+      const uint32_t c = column_of<kThreads>(j, lane);
       if (c < a.stop) store_bytes8(q, c, a.stop, quantize8(v[j], s.inverse));
     }
   } else {
@@ -87,7 +87,7 @@ __device__ __forceinline__ void quantize_row(const RowsArgs& a, int64_t row, int
 }
 
 template <typename T, int kThreads, int kVectors, bool kMul>
-__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void quantize_rows_kernel(RowsArgs a) {
+__global__ __launch_bounds__(row_block(kThreads)) void quantize_rows_kernel(RowsArgs a) {
   __shared__ uint32_t scratch[16];
   for_rows<kThreads>(a.rows, [&](int64_t row, int lane) {
     quantize_row<T, kThreads, kVectors, kMul>(a, row, lane, scratch);
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void quantize_rows
 
 template <typename T, int kThreads, int kVectors>
 hipError_t launch_rows(const RowsArgs& a, hipStream_t stream) {
-  const dim3 grid = row_grid(kThreads, a.rows), block(kThreads < 256 ? 256 : kThreads);
+  const dim3 grid = row_grid(kThreads, a.rows), block(row_block(kThreads));
   if (a.multiplier)
     hipLaunchKernelGGL((quantize_rows_kernel<T, kThreads, kVectors, true>), grid, block, 0, stream, a);
   else
@@ -107,7 +107,7 @@ hipError_t launch_rows(const RowsArgs& a, hipStream_t stream) {
 template <typename T>
 hipError_t launch_rows_of(const RowsArgs& a, hipStream_t stream) {
   if (a.cols > 32768) return launch_rows<T, 1024, 0>(a, stream);
-  return with_row_shape(choose_row_shape(a.rows, a.cols), [&](auto threads, auto vectors) {
+  return with_row_shape(choose_row_shape(a.rows, a.cols, sizeof(T)), [&](auto threads, auto vectors) {
     return launch_rows<T, decltype(threads)::value, decltype(vectors)::value>(a, stream);
   });
 }
