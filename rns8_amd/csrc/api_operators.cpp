@@ -128,6 +128,13 @@ void linear_parts(const rns8_mi355x_linear_i8_args& a, LinearParts& p) {
   p.gemm.workspace_bytes = bytes;
 }
 
+// The copies that can be made before the rows are quantized: the weights'. (Where
+// the rows, too, would be copied, the product makes both copies itself.)
+int weight_copies(const rns8_mi355x_gemm_i8_args& g, bool zero_filled, OperandCopy* copies) {
+  const int count = gemm_i8_copies(g, zero_filled, copies);
+  return count == 1 && copies[0].src == g.b ? 1 : 0;
+}
+
 rns8_status check_linear(const rns8_mi355x_linear_i8_args& a) {
   if (a.m < 0 || a.n < 0 || a.k < 1) return RNS8_INVALID_ARGUMENT;
   const uint64_t size = element_size(a.dtype);
@@ -144,8 +151,7 @@ rns8_status check_linear(const rns8_mi355x_linear_i8_args& a) {
 }
 
 // The backward pass's workspace: dy in 8 bits by rows and, transposed, by
-// columns, the column pass's partials and the products' own (one after the
-// other: they share it).
+// columns, the column pass's partials and the products' own.
 struct BackwardParts {
   rns8_mi355x_quantize_args rows{}, columns{};
   rns8_mi355x_gemm_i8_args dx{}, dw{};
@@ -159,7 +165,6 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.bytes += round_up(bytes, 256);
     return got;
   };
-  uint64_t shared = 0;
   if (a.dx) {
     p.rows.dtype = a.dtype;
     p.rows.rows = a.m;
@@ -182,7 +187,8 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.dx.a_scale = p.rows.scale;
     p.dx.out = a.dx;
     p.dx.ldo = a.lddx;
-    shared = gemm_i8_bytes(p.dx, true);
+    p.dx.workspace_bytes = gemm_i8_bytes(p.dx, true);
+    p.dx.workspace = take(p.dx.workspace_bytes);
   }
   if (a.dw || a.dbias) {
     p.columns.dtype = a.dtype;
@@ -196,7 +202,7 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.columns.scale = reinterpret_cast<float*>(take(static_cast<uint64_t>(a.n) * sizeof(float)));
     p.columns.sums = a.dbias;
     p.columns.workspace_bytes = quantize_columns_bytes(a.m, a.n);
-    if (p.columns.workspace_bytes > shared) shared = p.columns.workspace_bytes;
+    p.columns.workspace = take(p.columns.workspace_bytes);
     p.dw.dtype = RNS8_MI355X_F32;
     p.dw.m = a.n;
     p.dw.n = a.k;
@@ -210,12 +216,10 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.dw.out = a.dw;
     p.dw.ldo = a.lddw;
     if (a.dw) {
-      const uint64_t bytes = gemm_i8_bytes(p.dw, true);
-      if (bytes > shared) shared = bytes;
+      p.dw.workspace_bytes = gemm_i8_bytes(p.dw, true);
+      p.dw.workspace = take(p.dw.workspace_bytes);
     }
   }
-  p.dx.workspace = p.dw.workspace = p.columns.workspace = take(shared);
-  p.dx.workspace_bytes = p.dw.workspace_bytes = shared;
 }
 
 rns8_status check_linear_backward(const rns8_mi355x_linear_i8_backward_args& a) {
@@ -401,7 +405,7 @@ rns8_status rns8_mi355x_gemm_i8_scaled(rns8_context* ctx, const rns8_mi355x_gemm
       [](const rns8_mi355x_gemm_i8_args& a) {
         return check_workspace(a.workspace, a.workspace_bytes, gemm_i8_bytes(a, false));
       },
-      [](const rns8_mi355x_gemm_i8_args& a, hipStream_t s) { return launch_gemm_i8(a, false, s); });
+      [](const rns8_mi355x_gemm_i8_args& a, hipStream_t s) { return launch_gemm_i8(a, false, false, s); });
 }
 
 rns8_status rns8_mi355x_gemm_i8_scaled_workspace(const rns8_mi355x_gemm_i8_args* args, uint64_t* bytes) {
@@ -419,8 +423,11 @@ rns8_status rns8_mi355x_linear_i8(rns8_context* ctx, const rns8_mi355x_linear_i8
         if (a.m > 0 && a.n > 0 && linear_rows_takes(a.m, a.n, a.k)) return launch_linear_rows(a, s);
         LinearParts p;
         linear_parts(a, p);
-        const hipError_t e = launch_quantize_rows(p.quantize, s);
-        return e != hipSuccess ? e : launch_gemm_i8(p.gemm, p.zero_filled, s);
+        OperandCopy copies[2];
+        const int count = weight_copies(p.gemm, p.zero_filled, copies);
+        const hipError_t e = count ? launch_prepare(&p.quantize, nullptr, copies, count, s)
+                                   : launch_quantize_rows(p.quantize, s);
+        return e != hipSuccess ? e : launch_gemm_i8(p.gemm, p.zero_filled, count != 0, s);
       });
 }
 
@@ -438,13 +445,14 @@ rns8_status rns8_mi355x_linear_i8_backward(rns8_context* ctx, const rns8_mi355x_
       [](const rns8_mi355x_linear_i8_backward_args& a, hipStream_t s) {
         BackwardParts p;
         backward_parts(a, p);
-        hipError_t e = hipSuccess;
-        if (a.dx) {
-          e = launch_quantize_rows(p.rows, s);
-          if (e == hipSuccess) e = launch_gemm_i8(p.dx, true, s);
-        }
-        if (e == hipSuccess && (a.dw || a.dbias)) e = launch_quantize_columns(p.columns, s);
-        if (e == hipSuccess && a.dw) e = launch_gemm_i8(p.dw, true, s);
+        const bool columns = a.dw || a.dbias;
+        OperandCopy copies[4];
+        int count = a.dx ? gemm_i8_copies(p.dx, true, copies) : 0;
+        if (a.dw) count += gemm_i8_copies(p.dw, true, copies + count);
+        hipError_t e = launch_prepare(a.dx ? &p.rows : nullptr, columns ? &p.columns : nullptr, copies, count, s);
+        if (e == hipSuccess && columns) e = launch_quantize_columns_rest(p.columns, s);
+        if (e == hipSuccess && a.dx) e = launch_gemm_i8(p.dx, true, true, s);
+        if (e == hipSuccess && a.dw) e = launch_gemm_i8(p.dw, true, true, s);
         return e;
       });
 }

@@ -31,11 +31,34 @@ hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& a, hipStream_t 
 uint64_t quantize_columns_bytes(int64_t rows, int64_t cols);
 hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& a, hipStream_t stream);
 
+// A copy of rows of `cols` bytes at any address and stride to rows at stride
+// ldd (cols rounded up to 16), filled up with zeros (operand_copy.hpp).
+struct OperandCopy {
+  const int8_t* src;
+  int64_t rows, cols, lds;
+  int8_t* dst;
+  int64_t ldd;
+};
+inline uint32_t operand_copy_blocks(const OperandCopy& a) {
+  const int64_t units = a.cols < 16 ? (a.rows + 255) / 256 : (a.rows + 15) / 16 * ((a.ldd + 1023) / 1024);
+  return static_cast<uint32_t>(units < (1 << 16) ? units : 1 << 16);
+}
+
+// What a linear layer's products wait for, in one launch: rows to quantize,
+// columns' partial maxima and sums, and operand copies (any of them NULL or 0).
+// launch_quantize_columns_rest then finishes the columns.
+hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi355x_quantize_args* columns,
+                          const OperandCopy* copies, int copy_count, hipStream_t stream);
+hipError_t launch_quantize_columns_rest(const rns8_mi355x_quantize_args& a, hipStream_t stream);
+
 // ---- scaled product (scaled_gemm.hip) ----------------------------------------------
 // a_zero_filled: a's rows hold zeros from k up to the next multiple of 16 (and
 // their stride reaches it), as quantized rows do: the product may read them.
 uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled);
-hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, hipStream_t stream);
+// The copies (at most two) that the product needs of its operands, into its
+// workspace; launch_gemm_i8 makes them itself unless `copied`.
+int gemm_i8_copies(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, OperandCopy* copies);
+hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, bool copied, hipStream_t stream);
 
 // The linear layer for one or two tokens in one kernel (scaled_rows.hip).
 bool linear_rows_takes(int64_t m, int64_t n, int64_t k);

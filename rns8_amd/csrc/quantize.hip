@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "elements.hpp"
+#include "operand_copy.hpp"
 #include "operators.hpp"
 #include "row_shape.hpp"
 
@@ -183,12 +184,12 @@ struct FourRows {
 
 // 256 threads: 32 vectors of 8 columns by 8 rows, four rows in flight each.
 template <typename T>
-__global__ __launch_bounds__(256) void column_partials_kernel(ColsArgs a) {
+__device__ __forceinline__ void column_partials(const ColsArgs& a, int64_t strip, int64_t chunk) {
   __shared__ uint32_t amax_lds[8][256];
   __shared__ float sum_lds[8][256];
   const int vec = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + 8 * vec;
-  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.chunk_rows;
+  const int64_t c = strip * 256 + 8 * vec;
+  const int64_t first = chunk * a.chunk_rows;
   const int64_t last = first + a.chunk_rows < a.rows ? first + a.chunk_rows : a.rows;
   uint32_t amax[8] = {};
   float sum[8] = {};
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(256) void column_partials_kernel(ColsArgs a) {
     sum_lds[sub][8 * vec + i] = sum[i];
   }
   __syncthreads();
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t col = strip * 256 + threadIdx.x;
   if (col < a.cols) {
     uint32_t m = 0;
     float s = 0.0f;
@@ -223,8 +224,8 @@ __global__ __launch_bounds__(256) void column_partials_kernel(ColsArgs a) {
       m = m > b ? m : b;
       s += sum_lds[j][threadIdx.x];
     }
-    a.amax_part[blockIdx.y * a.cols + col] = m;
-    a.sum_part[blockIdx.y * a.cols + col] = s;
+    a.amax_part[chunk * a.cols + col] = m;
+    a.sum_part[chunk * a.cols + col] = s;
   }
 }
 
@@ -245,27 +246,29 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(ColsArgs a) {
     rows[1].load(a, r0 + 64 + 4 * quad, 1, a.rows, c);
   }
   {
-    // two threads to a column, one for even and one for odd chunks, eight loads
-    // in flight (chunks past the last are read again: a maximum does not mind)
+    // two threads to a column, one for even and one for odd chunks, 16 (and as
+    // many sums) in flight: chunks past the last are read again and not counted
     const int col = threadIdx.x & (kTile - 1), half = threadIdx.x / kTile;
-    const int64_t column = c0 + col, at = min(column, a.cols - 1);
-    uint32_t amax = 0;
-    for (int64_t k = half; k < a.chunks; k += 16) {
-      uint32_t v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = a.amax_part[min(k + 2 * i, a.chunks - 1) * a.cols + at];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = amax > v[i] ? amax : v[i];
-    }
-    float sum = 0.0f;
+    const int64_t column = c0 + col;
+    const uint32_t* const amax_at = a.amax_part + min(column, a.cols - 1);
+    const float* const sum_at = a.sum_part + min(column, a.cols - 1);
     const bool summed = a.sums && tile_r == 0;
-    if (summed) {
-      for (int64_t k = half; k < a.chunks; k += 16) {
-        float v[8];
+    uint32_t amax = 0;
+    float sum = 0.0f;
+    for (int64_t k = half; k < a.chunks; k += 32) {
+      uint32_t v[16];
+      float s[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = a.sum_part[min(k + 2 * i, a.chunks - 1) * a.cols + at];
+      for (int i = 0; i < 16; ++i) v[i] = amax_at[min(k + 2 * i, a.chunks - 1) * a.cols];
+      if (summed) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += k + 2 * i < a.chunks ? v[i] : 0.0f;
+        for (int i = 0; i < 16; ++i) s[i] = sum_at[min(k + 2 * i, a.chunks - 1) * a.cols];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) amax = amax > v[i] ? amax : v[i];
+      if (summed) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += k + 2 * i < a.chunks ? s[i] : 0.0f;
       }
     }
     if (half) {
@@ -320,37 +323,79 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(ColsArgs a) {
 }
 
 template <typename T>
-hipError_t launch_columns_of(const ColsArgs& a, hipStream_t stream) {
-  const int64_t col_blocks = (a.cols + 255) / 256;
+hipError_t launch_columns_rest(const ColsArgs& a, hipStream_t stream) {
   const int64_t tiles_r = a.stop > 0 ? (a.stop + kTile - 1) / kTile : 1;  // no rows: scales and sums alone
   if (tiles_r > kMaxBlocks / a.tiles_c) return hipErrorInvalidValue;
-  const dim3 part(static_cast<unsigned>(col_blocks), static_cast<unsigned>(a.chunks));
-  hipLaunchKernelGGL((column_partials_kernel<T>), part, dim3(256), 0, stream, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((quantize_columns_kernel<T>), dim3(static_cast<unsigned>(tiles_r * a.tiles_c)), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }
 
-}  // namespace
+// ---- rows, columns and copies in one launch -------------------------------------------
+// Workgroups of 256 threads in three ranges: rows to quantize, (256 columns,
+// rows of a chunk) for the columns' partials, copies. They share nothing: one
+// launch costs less than three, and small ones fill the chip together.
+struct PrepareArgs {
+  RowsArgs rows;
+  ColsArgs cols;
+  OperandCopy copies[4];
+  uint32_t row_blocks, col_blocks, col_strips;
+  uint32_t copy_blocks[4];
+};
 
-hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
-  if (g.rows == 0) return hipSuccess;
-  const RowsArgs a{g.x, g.rows, g.cols, g.ldx, g.multiplier, g.q, g.ldq, quantized_stop(g.cols, g.ldq), g.scale};
-  switch (g.dtype) {
-    case RNS8_MI355X_F32: return launch_rows_of<float>(a, stream);
-    case RNS8_MI355X_F16: return launch_rows_of<f16>(a, stream);
-    case RNS8_MI355X_BF16: return launch_rows_of<bf16>(a, stream);
-    default: return hipErrorInvalidValue;
+// kThreads (64 or 256) to a row, as quantize_row.
+template <typename T, int kThreads, int kVectors, bool kMul>
+__global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
+  __shared__ uint32_t scratch[4];
+  uint32_t block = blockIdx.x;
+  if (block < a.row_blocks) {
+    const int lane = kThreads == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t first = kThreads == 64 ? 4 * static_cast<int64_t>(block) + (threadIdx.x >> 6) : block;
+    for (int64_t row = first; row < a.rows.rows; row += static_cast<int64_t>(a.row_blocks) * (256 / kThreads))
+      quantize_row<T, kThreads, kVectors, kMul>(a.rows, row, lane, scratch);
+    return;
+  }
+  block -= a.row_blocks;
+  if (block < a.col_blocks) {
+    column_partials<T>(a.cols, block % a.col_strips, block / a.col_strips);
+    return;
+  }
+  block -= a.col_blocks;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    if (block < a.copy_blocks[i]) {
+      copy_rows(a.copies[i], block, a.copy_blocks[i]);
+      return;
+    }
+    block -= a.copy_blocks[i];
   }
 }
 
-uint64_t quantize_columns_bytes(int64_t rows, int64_t cols) {
-  return round_up(static_cast<uint64_t>(column_chunks(rows, cols)) * static_cast<uint64_t>(cols) * 8u, 256);
+template <typename T, int kThreads, int kVectors>
+hipError_t launch_prepare_as(const PrepareArgs& a, uint32_t blocks, hipStream_t stream) {
+  if (a.rows.multiplier)
+    hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, true>), dim3(blocks), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, false>), dim3(blocks), dim3(256), 0, stream, a);
+  return hipGetLastError();
 }
 
-hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
+template <typename T>
+hipError_t launch_prepare_of(const PrepareArgs& a, uint32_t blocks, hipStream_t stream) {
+  const int64_t cols = a.rows.cols;
+  if (cols <= 512) return launch_prepare_as<T, 64, 1>(a, blocks, stream);
+  if (cols <= 1024) return launch_prepare_as<T, 64, 2>(a, blocks, stream);
+  if (cols <= 2048) return launch_prepare_as<T, 256, 1>(a, blocks, stream);
+  if (cols <= 4096) return launch_prepare_as<T, 256, 2>(a, blocks, stream);
+  if (cols <= 8192) return launch_prepare_as<T, 256, 4>(a, blocks, stream);
+  return launch_prepare_as<T, 256, 0>(a, blocks, stream);
+}
+
+RowsArgs rows_args(const rns8_mi355x_quantize_args& g) {
+  return {g.x, g.rows, g.cols, g.ldx, g.multiplier, g.q, g.ldq, quantized_stop(g.cols, g.ldq), g.scale};
+}
+
+ColsArgs cols_args(const rns8_mi355x_quantize_args& g) {
   ColsArgs a{};
   a.x = g.x;
   a.rows = g.rows;
@@ -367,12 +412,70 @@ hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& g, hipStream
   a.amax_part = static_cast<uint32_t*>(g.workspace);
   a.sum_part = reinterpret_cast<float*>(a.amax_part + a.chunks * a.cols);
   a.tiles_c = (g.cols + kTile - 1) / kTile;
-  switch (g.dtype) {
-    case RNS8_MI355X_F32: return launch_columns_of<float>(a, stream);
-    case RNS8_MI355X_F16: return launch_columns_of<f16>(a, stream);
-    case RNS8_MI355X_BF16: return launch_columns_of<bf16>(a, stream);
+  return a;
+}
+
+template <typename F>
+hipError_t of_dtype(uint32_t dtype, F&& f) {
+  switch (dtype) {
+    case RNS8_MI355X_F32: return f(float{});
+    case RNS8_MI355X_F16: return f(f16{});
+    case RNS8_MI355X_BF16: return f(bf16{});
     default: return hipErrorInvalidValue;
   }
+}
+
+}  // namespace
+
+hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
+  if (g.rows == 0) return hipSuccess;
+  return of_dtype(g.dtype, [&](auto t) { return launch_rows_of<decltype(t)>(rows_args(g), stream); });
+}
+
+uint64_t quantize_columns_bytes(int64_t rows, int64_t cols) {
+  return round_up(static_cast<uint64_t>(column_chunks(rows, cols)) * static_cast<uint64_t>(cols) * 8u, 256);
+}
+
+hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi355x_quantize_args* columns,
+                          const OperandCopy* copies, int copy_count, hipStream_t stream) {
+  PrepareArgs a{};
+  uint32_t dtype = RNS8_MI355X_F32;
+  uint64_t blocks = 0;
+  if (rows && rows->rows > 0) {
+    dtype = rows->dtype;
+    a.rows = rows_args(*rows);
+    const int64_t wanted = rows->cols <= 1024 ? (rows->rows + 3) / 4 : rows->rows;
+    a.row_blocks = static_cast<uint32_t>(std::min(wanted, kMaxBlocks / 4));
+    blocks += a.row_blocks;
+  }
+  if (columns) {
+    dtype = columns->dtype;
+    a.cols = cols_args(*columns);
+    const int64_t strips = (columns->cols + 255) / 256;
+    if (strips > kMaxBlocks / 4 / a.cols.chunks) return hipErrorInvalidValue;
+    a.col_strips = static_cast<uint32_t>(strips);
+    a.col_blocks = static_cast<uint32_t>(strips * a.cols.chunks);
+    blocks += a.col_blocks;
+  }
+  if (copy_count > 4) return hipErrorInvalidValue;
+  for (int i = 0; i < copy_count; ++i) {
+    a.copies[i] = copies[i];
+    a.copy_blocks[i] = operand_copy_blocks(copies[i]);
+    blocks += a.copy_blocks[i];
+  }
+  if (blocks == 0) return hipSuccess;
+  return of_dtype(dtype, [&](auto t) {
+    return launch_prepare_of<decltype(t)>(a, static_cast<uint32_t>(blocks), stream);
+  });
+}
+
+hipError_t launch_quantize_columns_rest(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
+  return of_dtype(g.dtype, [&](auto t) { return launch_columns_rest<decltype(t)>(cols_args(g), stream); });
+}
+
+hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
+  const hipError_t e = launch_prepare(nullptr, &g, nullptr, 0, stream);
+  return e != hipSuccess ? e : launch_quantize_columns_rest(g, stream);
 }
 
 }  // namespace rns8x

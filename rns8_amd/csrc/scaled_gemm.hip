@@ -3,68 +3,17 @@
 // then the kernel of the product's shape runs.
 #include <algorithm>
 
-#include "elements.hpp"
+#include "operand_copy.hpp"
 #include "scaled_gemm.hpp"
 
 namespace rns8x {
 namespace {
 
-// Copies rows of `cols` bytes at any address and stride to rows at stride ldd
-// (cols rounded up to 16) and fills them up with zeros.
-struct CopyArgs {
-  const int8_t* src;
-  int64_t rows, cols, lds;
-  int8_t* dst;
-  int64_t ldd;
-};
+__global__ __launch_bounds__(256) void copy_rows_kernel(OperandCopy a) { copy_rows(a, blockIdx.x, gridDim.x); }
 
-// Four rows to a wave, 16 bytes of each to a lane at a time, all four loads in
-// flight. The chunk that a row's end cuts comes from the row's last 16 bytes.
-__global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs a) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t cols = static_cast<uint32_t>(a.cols), padded = static_cast<uint32_t>(a.ldd);
-  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * 4; row < a.rows;
-       row += static_cast<int64_t>(gridDim.x) * 16) {
-    const int64_t rows = a.rows - row;
-    for (uint32_t c = 16 * (64 * blockIdx.y + lane); c < padded; c += 16 * 64 * gridDim.y) {
-      u32x4 w[4];
-      const bool whole = c + 16 <= cols;
-      const uint32_t at = whole ? c : cols - 16, drop = whole ? 0 : c + 16 - cols;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) __builtin_memcpy(&w[r], a.src + (row + min<int64_t>(r, rows - 1)) * a.lds + at, 16);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) w[r] = drop_bytes(w[r], drop);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r < rows) __builtin_memcpy(a.dst + (row + r) * a.ldd + c, &w[r], 16);
-    }
-  }
-}
-
-// Rows below 16 bytes: one to a thread.
-__global__ __launch_bounds__(256) void copy_short_rows_kernel(CopyArgs a) {
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; row < a.rows;
-       row += static_cast<int64_t>(gridDim.x) * 256) {
-    uint32_t w[4] = {};
-#pragma unroll
-    for (int i = 0; i < 15; ++i)
-      if (i < a.cols)
-        w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(a.src[row * a.lds + i])) << (8 * (i & 3));
-    __builtin_memcpy(a.dst + row * a.ldd, w, 16);
-  }
-}
-
-hipError_t launch_copy_rows(const CopyArgs& a, hipStream_t stream) {
+hipError_t launch_copy_rows(const OperandCopy& a, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;
-  if (a.cols < 16) {
-    const int64_t blocks = std::min<int64_t>((a.rows + 255) / 256, 1 << 16);
-    hipLaunchKernelGGL(copy_short_rows_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
-    return hipGetLastError();
-  }
-  const int64_t blocks = (a.rows + 15) / 16;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16)),
-                  static_cast<unsigned>(std::min<int64_t>((a.ldd + 1023) / 1024, 64)));
-  hipLaunchKernelGGL(copy_rows_kernel, grid, dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(copy_rows_kernel, dim3(operand_copy_blocks(a)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -121,25 +70,33 @@ uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
   return g.m == 0 || g.n == 0 ? 0u : make_plan(g, a_zero_filled).bytes;
 }
 
-hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, hipStream_t stream) {
+int gemm_i8_copies(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, OperandCopy* copies) {
+  if (g.m == 0 || g.n == 0) return 0;
+  const Plan p = make_plan(g, a_zero_filled);
+  int8_t* const ws = static_cast<int8_t*>(g.workspace);
+  int count = 0;
+  if (p.copy_a) copies[count++] = {g.a, g.m, g.k, g.lda, ws + p.a_at, p.lda};
+  if (p.copy_b) copies[count++] = {g.b, p.b_rows, p.b_cols, g.ldb, ws + p.b_at, p.ldb};
+  return count;
+}
+
+hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool copied, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return hipSuccess;
   const Plan p = make_plan(g, a_zero_filled);
-  uint8_t* const ws = static_cast<uint8_t*>(g.workspace);
+  int8_t* const ws = static_cast<int8_t*>(g.workspace);
   ScaledGemm s{g.m, g.n, g.k, g.a, g.b, p.lda, p.ldb, g.b_layout == RNS8_MI355X_B_INNER, g.a_scale, g.b_scale, g.bias,
                g.out, g.ldo, g.dtype};
   if (p.few_rows) return launch_scaled_rows(s, stream);
-  if (p.copy_a) {
-    int8_t* const to = reinterpret_cast<int8_t*>(ws + p.a_at);
-    const hipError_t e = launch_copy_rows({g.a, g.m, g.k, g.lda, to, p.lda}, stream);
-    if (e != hipSuccess) return e;
-    s.a = to;
+  if (!copied) {
+    OperandCopy copies[2];
+    const int count = gemm_i8_copies(g, a_zero_filled, copies);
+    for (int i = 0; i < count; ++i) {
+      const hipError_t e = launch_copy_rows(copies[i], stream);
+      if (e != hipSuccess) return e;
+    }
   }
-  if (p.copy_b) {
-    int8_t* const to = reinterpret_cast<int8_t*>(ws + p.b_at);
-    const hipError_t e = launch_copy_rows({g.b, p.b_rows, p.b_cols, g.ldb, to, p.ldb}, stream);
-    if (e != hipSuccess) return e;
-    s.b = to;
-  }
+  if (p.copy_a) s.a = ws + p.a_at;
+  if (p.copy_b) s.b = ws + p.b_at;
   if (g.k == 0) {  // no operand is read (their buffers are empty): any aligned address will do
     s.a = s.b = static_cast<const int8_t*>(g.out) - reinterpret_cast<uintptr_t>(g.out) % 16;
     s.lda = 0;
