@@ -402,44 +402,67 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   }
 }
 
-// A workgroup loads a row's lists, then lane p of its first wave holds part p:
-// the largest head goes out `top` times, and lane k keeps the k-th.
+// A workgroup loads a row's lists; its first wave joins the sums, lane p part p.
+// The lists are in order, so the top-th largest of their heads bounds the row's
+// alternatives from below: the keys from there on are gathered and ordered by
+// counting, as within a part.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
-  extern __shared__ uint64_t lists[];  // [parts][top]
+  __shared__ uint64_t keys[kMaxTop * kMaxTop];
+  __shared__ uint64_t from;
+  __shared__ uint32_t count;
+  __shared__ Sums joined;
   const int lane = threadIdx.x & 63;
   const uint32_t parts = static_cast<uint32_t>(a.parts), total = parts * a.top;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const uint64_t* const from = a.part_keys + row * total;
-    for (uint32_t i = threadIdx.x; i < total; i += 4 * kThreads) {
-      uint64_t key[4];
+    const uint64_t* const lists = a.part_keys + row * total;
+    constexpr uint32_t kHeld = kMaxTop * kMaxTop / kThreads;  // 16: parts and top are at most 64
+    uint64_t key[kHeld];
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) key[j] = from[min(i + j * kThreads, total - 1)];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j)
-        if (i + j * kThreads < total) lists[i + j * kThreads] = key[j];
+    for (uint32_t j = 0; j < kHeld; ++j) {
+      key[j] = 0;
+      if (j * kThreads < total) key[j] = lists[min(threadIdx.x + j * kThreads, total - 1)];
     }
-    Sums t{-INFINITY, 0.0f, 0.0f};
-    if (threadIdx.x < parts) {
-      float w[4];
-      __builtin_memcpy(w, a.part_sums + 4 * (row * a.parts + lane), 16);
-      t = {w[0], w[1], w[2]};
+    if (threadIdx.x < 64) {
+      Sums t{-INFINITY, 0.0f, 0.0f};
+      uint64_t head = 0;
+      if (threadIdx.x < parts) {
+        float w[4];
+        __builtin_memcpy(w, a.part_sums + 4 * (row * a.parts + lane), 16);
+        t = {w[0], w[1], w[2]};
+        if (a.top) head = lists[lane * a.top];
+      }
+      t = wave_join(t, a.c);
+      if (lane == 0) {
+        write_row<T>(a, row, t);
+        joined = t;
+        count = 0;
+        from = 0;  // fewer parts than alternatives: every key
+      }
+      keys[lane] = head;
+      __builtin_amdgcn_wave_barrier();
+      uint32_t rank = 0;
+      for (uint32_t p = 0; p < parts; ++p) rank += keys[p] > head;
+      if (head && rank == a.top - 1) from = head;
     }
     __syncthreads();
-    if (threadIdx.x < 64) {
-      t = wave_join(t, a.c);
-      if (lane == 0) write_row<T>(a, row, t);
-      const uint32_t end = (lane + 1) * a.top;
-      uint32_t at = lane * a.top;
-      uint64_t head = a.top && threadIdx.x < parts ? lists[at] : 0, mine = 0;
-      for (uint32_t k = 0; k < a.top; ++k) {
-        const uint64_t best = wave_max_key(head);
-        if (k == threadIdx.x) mine = best;
-        if (head == best) head = ++at < end ? lists[at] : 0;  // (keys differ: one lane)
+    if (a.top) {
+      const uint64_t least = from;
+      const Sums t = joined;
+      __syncthreads();  // the heads are read
+#pragma unroll
+      for (uint32_t j = 0; j < kHeld; ++j)
+        if (threadIdx.x + j * kThreads < total && key[j] >= least && key[j]) keys[atomicAdd(&count, 1u)] = key[j];
+      __syncthreads();
+      const uint32_t n = count;
+      for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t mine = keys[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += keys[j] > mine;
+        if (rank < a.top) write_alternative(a, row, rank, mine, t);
       }
-      if (threadIdx.x < a.top) write_alternative(a, row, threadIdx.x, mine, t);
     }
-    __syncthreads();  // the next row's lists
+    __syncthreads();  // the next row's shared words
   }
 }
 
@@ -561,8 +584,7 @@ hipError_t launch_forward(const Args& a, hipStream_t stream) {
     hipLaunchKernelGGL((logprobs_kernel<T, kHeldRounds>), grid, block, 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
-  hipLaunchKernelGGL((join_parts_kernel<T>), grid_of(a.rows), dim3(kThreads),
-                     static_cast<unsigned>(a.parts * a.top * sizeof(uint64_t)), stream, a);
+  hipLaunchKernelGGL((join_parts_kernel<T>), grid_of(a.rows), dim3(kThreads), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -110,6 +110,18 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
   };
   Group now, next;
   if (first < last) load(first, now);
+  // this thread's four outputs in the end, whose scales and biases are on their
+  // way from here on: block (i, j), lane l of it
+  static_assert(MB * RB * 64 <= kThreads, "one quad of outputs to a thread");
+  const int e = threadIdx.x, l = e & 63, out_j = (e >> 6) % RB, out_i = (e >> 6) / RB;
+  const bool writes = e < MB * RB * 64 && 16 * out_i + (l & 15) < a.m && n0 + 16 * out_j + 4 * (l >> 4) < a.n;
+  const int64_t token = 16 * out_i + (l & 15), channel = n0 + 16 * out_j + 4 * (l >> 4);
+  float sb[4], bias[4], token_scale = 1.0f;
+  if (writes) {
+    load4_or(a.b_scale, channel, a.n, 1.0f, sb);
+    load4_or(a.bias, channel, a.n, 0.0f, bias);
+    if (!kFused && a.a_scale) token_scale = a.a_scale[token];
+  }
   float scale[2] = {1.0f, 1.0f};
   if constexpr (kFused) {
     // the tokens' maxima, then their bytes, zeros up to whole blocks
@@ -173,27 +185,21 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
 #pragma unroll
     for (int j = 0; j < RB; ++j) sums[((wave * MB + i) * RB + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  for (int e = threadIdx.x; e < MB * RB * 64; e += kThreads) {
-    const int l = e & 63, j = (e >> 6) % RB, i = (e >> 6) / RB;
-    v4i sum = sums[e];
+  if (!writes) return;
+  v4i sum = sums[e];
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) sum += sums[v * MB * RB * 64 + e];
-    const int64_t token = 16 * i + (l & 15), c = n0 + 16 * j + 4 * (l >> 4);
-    if (token >= a.m || c >= a.n) continue;
-    const float sa = kFused ? (token ? scale[1] : scale[0]) : a.a_scale ? a.a_scale[token] : 1.0f;
-    float sb[4], bias[4], f[4];
-    load4_or(a.b_scale, c, a.n, 1.0f, sb);
-    load4_or(a.bias, c, a.n, 0.0f, bias);
+  for (int v = 1; v < kWaves; ++v) sum += sums[v * MB * RB * 64 + e];
+  const float sa = kFused ? (token ? scale[1] : scale[0]) : token_scale;
+  float f[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) f[x] = static_cast<float>(sum[x]) * sa * sb[x] + bias[x];
-    const int64_t at = token * a.ldo + c;
-    if (a.dtype == RNS8_MI355X_BF16)
-      store4(static_cast<bf16*>(a.out) + at, a.n - c, f);
-    else if (a.dtype == RNS8_MI355X_F16)
-      store4(static_cast<f16*>(a.out) + at, a.n - c, f);
-    else
-      store4(static_cast<float*>(a.out) + at, a.n - c, f);
-  }
+  for (int x = 0; x < 4; ++x) f[x] = static_cast<float>(sum[x]) * sa * sb[x] + bias[x];
+  const int64_t at = token * a.ldo + channel;
+  if (a.dtype == RNS8_MI355X_BF16)
+    store4(static_cast<bf16*>(a.out) + at, a.n - channel, f);
+  else if (a.dtype == RNS8_MI355X_F16)
+    store4(static_cast<f16*>(a.out) + at, a.n - channel, f);
+  else
+    store4(static_cast<float*>(a.out) + at, a.n - channel, f);
 }
 
 template <int MB, int RB, int U, bool kFused, typename T>

@@ -199,6 +199,16 @@ __global__ __launch_bounds__(C::kThreads, kMinBlocks) void scaled_tiles_kernel(T
     return c;
   };
   Cursor cur = cursor_of(decode(u_first), true);
+  // One value to a thread of the first unit's scales and biases, so that its
+  // epilogue finds them in the L2. (Kept to the end: a use waits for the loads, and
+  // for the DMA behind them.)
+  float touched[3] = {0.0f, 0.0f, 0.0f};
+  if (!args.partials) {
+    const Unit U = decode(u_first);
+    if (args.a_scale) touched[0] = args.a_scale[min(U.m0 + static_cast<uint32_t>(tid) % BM, args.m - 1)];
+    if (args.b_scale) touched[1] = args.b_scale[min(U.n0 + static_cast<uint32_t>(tid) % BN, args.n - 1)];
+    if (args.bias) touched[2] = args.bias[min(U.n0 + static_cast<uint32_t>(tid) % BN, args.n - 1)];
+  }
   const uint64_t b_step = C::kInner ? static_cast<uint64_t>(BK) * ldb : BK;
   auto src_a = [&]() { return buffer_rsrc(cur.a, cur.a_n); };
   auto src_b = [&](int half) {
@@ -462,6 +472,7 @@ __global__ __launch_bounds__(C::kThreads, kMinBlocks) void scaled_tiles_kernel(T
     epilogue(U);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no DMA outlives the workgroup's LDS
+  asm volatile("" ::"v"(touched[0]), "v"(touched[1]), "v"(touched[2]));
 }
 
 // The slices' sums in 64 bits, then the epilogue: four columns to a thread.
