@@ -81,6 +81,7 @@ struct LinearParts {
   rns8_mi355x_quantize_args quantize{};
   rns8_mi355x_gemm_i8_args gemm{};
   bool zero_filled = false;  // the quantized rows end in the zeros that the product may read
+  bool fragments = false;    // the quantized rows, the caller wants none, are in fragment order
   uint64_t bytes = 0;
 };
 
@@ -94,6 +95,18 @@ void linear_parts(const rns8_mi355x_linear_i8_args& a, LinearParts& p) {
     p.bytes += round_up(bytes, 256);
     return got;
   };
+  p.gemm.dtype = a.dtype;
+  p.gemm.m = a.m;
+  p.gemm.n = a.n;
+  p.gemm.k = a.k;
+  p.gemm.b = a.w;
+  p.gemm.ldb = a.ldw;
+  p.gemm.b_layout = RNS8_MI355X_B_CHANNELS;
+  p.gemm.b_scale = a.w_scale;
+  p.gemm.bias = a.bias;
+  p.gemm.out = a.out;
+  p.gemm.ldo = a.ldo;
+  p.gemm.lda = padded_row(a.k);
   p.quantize.dtype = a.dtype;
   p.quantize.rows = a.m;
   p.quantize.cols = a.k;
@@ -104,24 +117,17 @@ void linear_parts(const rns8_mi355x_linear_i8_args& a, LinearParts& p) {
     p.quantize.ldq = a.ldq;
     p.quantize.scale = a.x_scale;
   } else {
+    p.fragments = gemm_i8_takes_fragments(p.gemm);
     p.quantize.ldq = padded_row(a.k);
-    p.quantize.q = reinterpret_cast<int8_t*>(take(static_cast<uint64_t>(a.m) * static_cast<uint64_t>(p.quantize.ldq)));
+    const uint64_t bytes = p.fragments ? fragment_bytes(a.m, a.k)
+                                       : static_cast<uint64_t>(a.m) * static_cast<uint64_t>(p.quantize.ldq);
+    p.quantize.q = reinterpret_cast<int8_t*>(take(bytes));
     p.quantize.scale = reinterpret_cast<float*>(take(static_cast<uint64_t>(a.m) * sizeof(float)));
   }
-  p.gemm.dtype = a.dtype;
-  p.gemm.m = a.m;
-  p.gemm.n = a.n;
-  p.gemm.k = a.k;
   p.gemm.a = p.quantize.q;
   p.gemm.lda = p.quantize.ldq;
-  p.gemm.b = a.w;
-  p.gemm.ldb = a.ldw;
-  p.gemm.b_layout = RNS8_MI355X_B_CHANNELS;
   p.gemm.a_scale = p.quantize.scale;
-  p.gemm.b_scale = a.w_scale;
-  p.gemm.bias = a.bias;
-  p.gemm.out = a.out;
-  p.gemm.ldo = a.ldo;
+  if (p.fragments) return;  // (the kernel for few tokens needs no more)
   p.zero_filled = p.quantize.ldq >= padded_row(a.k);
   const uint64_t bytes = gemm_i8_bytes(p.gemm, p.zero_filled);
   p.gemm.workspace = take(bytes);
@@ -423,6 +429,10 @@ rns8_status rns8_mi355x_linear_i8(rns8_context* ctx, const rns8_mi355x_linear_i8
         if (a.m > 0 && a.n > 0 && linear_rows_takes(a.m, a.n, a.k)) return launch_linear_rows(a, s);
         LinearParts p;
         linear_parts(a, p);
+        if (p.fragments) {
+          const hipError_t e = launch_quantize_fragments(p.quantize, s);
+          return e != hipSuccess ? e : launch_gemm_i8_fragments(p.gemm, s);
+        }
         OperandCopy copies[2];
         const int count = weight_copies(p.gemm, p.zero_filled, copies);
         const hipError_t e = count ? launch_prepare(&p.quantize, nullptr, copies, count, s)

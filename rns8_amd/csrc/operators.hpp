@@ -28,6 +28,17 @@ inline bool streams(int64_t bytes_moved, const void* p, int64_t ld, uint32_t dty
 
 // ---- quantization (quantize.hip) -------------------------------------------------
 hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& a, hipStream_t stream);
+// Rows in fragment order, as the matrix cores take them: blocks of 64 columns;
+// in each, tiles of 16 rows of 1024 bytes, chunk g (16 columns) of row r at 256 g
+// + 16 r. Zeros up to whole blocks. A product of few tokens then reads its rows
+// in whole cache lines.
+inline __host__ __device__ int64_t fragment_offset(int64_t row, int64_t col, uint32_t tiles) {
+  return ((col / 64) * tiles + row / 16) * 1024 + (col % 64) / 16 * 256 + row % 16 * 16 + col % 16;
+}
+inline uint64_t fragment_bytes(int64_t rows, int64_t cols) {
+  return static_cast<uint64_t>((rows + 15) / 16) * static_cast<uint64_t>((cols + 63) / 64) * 1024u;
+}
+hipError_t launch_quantize_fragments(const rns8_mi355x_quantize_args& a, hipStream_t stream);
 uint64_t quantize_columns_bytes(int64_t rows, int64_t cols);
 hipError_t launch_quantize_columns(const rns8_mi355x_quantize_args& a, hipStream_t stream);
 
@@ -59,6 +70,9 @@ uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled);
 // workspace; launch_gemm_i8 makes them itself unless `copied`.
 int gemm_i8_copies(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, OperandCopy* copies);
 hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, bool copied, hipStream_t stream);
+// Whether the product would rather have its rows in fragment order, and the product of such rows.
+bool gemm_i8_takes_fragments(const rns8_mi355x_gemm_i8_args& a);
+hipError_t launch_gemm_i8_fragments(const rns8_mi355x_gemm_i8_args& a, hipStream_t stream);
 
 // The linear layer for one or two tokens in one kernel (scaled_rows.hip).
 bool linear_rows_takes(int64_t m, int64_t n, int64_t k);

@@ -23,6 +23,7 @@ struct RowsArgs {
   int8_t* q;
   int64_t ldq, stop;
   float* scale;
+  uint32_t fragments;  // tiles of 16 rows: q in fragment order (operators.hpp); 0: in rows
 };
 
 // kThreads threads hold a row in kVectors vectors each (0: the row is read
@@ -59,7 +60,12 @@ __device__ __forceinline__ void quantize_row(const RowsArgs& a, int64_t row, int
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
       const uint32_t c = column_of<kThreads>(j, lane);
-      if (c < a.stop) store_bytes8(q, c, a.stop, quantize8(v[j], s.inverse));
+      if (c >= a.stop) continue;
+      const uint64_t w = quantize8(v[j], s.inverse);
+      if (a.fragments)
+        *reinterpret_cast<uint64_t*>(a.q + fragment_offset(row, c, a.fragments)) = w;
+      else
+        store_bytes8(q, c, a.stop, w);
     }
   } else {
     auto load = [&](int64_t c, float (&v)[8]) {
@@ -82,7 +88,11 @@ __device__ __forceinline__ void quantize_row(const RowsArgs& a, int64_t row, int
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = 0.0f;
       if (c < a.cols) load(c, v);
-      store_bytes8(q, c, a.stop, quantize8(v, s.inverse));
+      const uint64_t w = quantize8(v, s.inverse);
+      if (a.fragments)
+        *reinterpret_cast<uint64_t*>(a.q + fragment_offset(row, c, a.fragments)) = w;
+      else
+        store_bytes8(q, c, a.stop, w);
     }
   }
 }
@@ -322,6 +332,117 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(ColsArgs a) {
   }
 }
 
+// ---- columns that a workgroup holds whole ------------------------------------------------
+// At most kWholeRows rows: 32 columns to a workgroup, 4 vectors of 8 columns by
+// 64 groups of four rows, twice, all of them in registers between the maxima and
+// the bytes. One pass, no partials and no kernel of its own.
+constexpr int kWholeRows = 512, kWholeCols = 32;
+constexpr int kWholePitch = kWholeRows / 4 + 1;  // words of a column in LDS
+
+struct WholeLds {
+  uint32_t amax[64][kWholeCols + 1];
+  float sum[64][kWholeCols + 1];
+  float inverse[kWholeCols];
+};
+constexpr int kWholeBytes =
+    sizeof(WholeLds) > kWholeCols * kWholePitch * 4 ? sizeof(WholeLds) : kWholeCols * kWholePitch * 4;
+
+template <typename T>
+__device__ __forceinline__ void quantize_whole_columns(const ColsArgs& a, int64_t strip, uint8_t* lds) {
+  WholeLds& part = *reinterpret_cast<WholeLds*>(lds);
+  uint32_t* const bytes = reinterpret_cast<uint32_t*>(lds);  // [column][four rows], after the parts
+  const int vec = threadIdx.x & 3, sub = threadIdx.x >> 2;
+  const int64_t c0 = kWholeCols * strip, c = c0 + 8 * vec;
+  FourRows<T> rows[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+    if (256 * r < a.rows) rows[r].load(a, 256 * r + 4 * sub, 1, a.rows, c);
+  uint32_t amax[8] = {};
+  float sum[8] = {};
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int64_t row = 256 * r + 4 * sub;
+    rows[r].settle(a, row, 1, a.rows, c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = rows[r].p[k].at(i);
+        sum[i] += v;
+        const uint32_t b = row + k < a.rows ? magnitude_bits(v * rows[r].m[k]) : 0u;
+        amax[i] = amax[i] > b ? amax[i] : b;
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    part.amax[sub][8 * vec + i] = amax[i];
+    part.sum[sub][8 * vec + i] = sum[i];
+  }
+  __syncthreads();
+  // eight threads to a column, eight of its parts each
+  {
+    const int col = threadIdx.x >> 3, eighth = threadIdx.x & 7;
+    uint32_t top = 0;
+    float total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t b = part.amax[8 * k + eighth][col];
+      top = top > b ? top : b;
+      total += part.sum[8 * k + eighth][col];
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) {
+      const uint32_t b = __shfl_xor(top, d);
+      top = top > b ? top : b;
+      total += __shfl_xor(total, d);
+    }
+    const RowScale s = row_scale(top);
+    if (eighth == 0) {
+      part.inverse[col] = s.inverse;
+      if (c0 + col < a.cols) {
+        a.scale[c0 + col] = s.scale;
+        if (a.sums) a.sums[c0 + col] = total;
+      }
+    }
+  }
+  __syncthreads();
+  float inv[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) inv[i] = part.inverse[8 * vec + i];
+  __syncthreads();  // the bytes take the parts' place
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+    if (256 * r < a.rows) {
+      const int64_t row = 256 * r + 4 * sub;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w |= (row + k < a.rows ? quantize_byte(rows[r].p[k].at(i) * rows[r].m[k], inv[i]) : 0u) << (8 * k);
+        bytes[(8 * vec + i) * kWholePitch + 64 * r + sub] = w;
+      }
+    }
+  __syncthreads();
+  // 16 bytes of a column at a time
+  const uint32_t stop = static_cast<uint32_t>(a.stop), chunks = (stop + 15) / 16;
+  for (uint32_t e = threadIdx.x; e < chunks * kWholeCols; e += 256) {
+    const uint32_t col = e / chunks, r = 16 * (e - col * chunks);
+    if (c0 + col >= a.cols) break;  // (columns rise with e)
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = bytes[col * kWholePitch + r / 4 + k];
+    int8_t* const to = a.q + (c0 + col) * a.ldq + r;
+    if (r + 16 <= stop) {
+      __builtin_memcpy(to, w, 16);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i)
+        if (r + i < stop) to[i] = static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)));
+    }
+  }
+}
+
 template <typename T>
 hipError_t launch_columns_rest(const ColsArgs& a, hipStream_t stream) {
   const int64_t tiles_r = a.stop > 0 ? (a.stop + kTile - 1) / kTile : 1;  // no rows: scales and sums alone
@@ -332,9 +453,10 @@ hipError_t launch_columns_rest(const ColsArgs& a, hipStream_t stream) {
 }
 
 // ---- rows, columns and copies in one launch -------------------------------------------
-// Workgroups of 256 threads in three ranges: rows to quantize, (256 columns,
-// rows of a chunk) for the columns' partials, copies. They share nothing: one
-// launch costs less than three, and small ones fill the chip together.
+// Workgroups of 256 threads in three ranges: rows to quantize; columns, 64 of
+// them whole or (256 columns, rows of a chunk) for their partials; copies. They
+// share nothing: one launch costs less than three, and small ones fill the chip
+// together.
 struct PrepareArgs {
   RowsArgs rows;
   ColsArgs cols;
@@ -344,9 +466,10 @@ struct PrepareArgs {
 };
 
 // kThreads (64 or 256) to a row, as quantize_row.
-template <typename T, int kThreads, int kVectors, bool kMul>
+template <typename T, int kThreads, int kVectors, bool kMul, bool kWhole>
 __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
   __shared__ uint32_t scratch[4];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kWhole ? kWholeBytes : 16];
   uint32_t block = blockIdx.x;
   if (block < a.row_blocks) {
     const int lane = kThreads == 64 ? threadIdx.x & 63 : threadIdx.x;
@@ -357,7 +480,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
   }
   block -= a.row_blocks;
   if (block < a.col_blocks) {
-    column_partials<T>(a.cols, block % a.col_strips, block / a.col_strips);
+    if constexpr (kWhole)
+      quantize_whole_columns<T>(a.cols, block, lds);
+    else
+      column_partials<T>(a.cols, block % a.col_strips, block / a.col_strips);
     return;
   }
   block -= a.col_blocks;
@@ -371,28 +497,30 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs a) {
   }
 }
 
-template <typename T, int kThreads, int kVectors>
+bool whole_columns(int64_t rows) { return rows > 0 && rows <= kWholeRows; }
+
+template <typename T, int kThreads, int kVectors, bool kWhole>
 hipError_t launch_prepare_as(const PrepareArgs& a, uint32_t blocks, hipStream_t stream) {
   if (a.rows.multiplier)
-    hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, true>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, true, kWhole>), dim3(blocks), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, false>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, false, kWhole>), dim3(blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool kWhole>
 hipError_t launch_prepare_of(const PrepareArgs& a, uint32_t blocks, hipStream_t stream) {
   const int64_t cols = a.rows.cols;
-  if (cols <= 512) return launch_prepare_as<T, 64, 1>(a, blocks, stream);
-  if (cols <= 1024) return launch_prepare_as<T, 64, 2>(a, blocks, stream);
-  if (cols <= 2048) return launch_prepare_as<T, 256, 1>(a, blocks, stream);
-  if (cols <= 4096) return launch_prepare_as<T, 256, 2>(a, blocks, stream);
-  if (cols <= 8192) return launch_prepare_as<T, 256, 4>(a, blocks, stream);
-  return launch_prepare_as<T, 256, 0>(a, blocks, stream);
+  if (cols <= 512) return launch_prepare_as<T, 64, 1, kWhole>(a, blocks, stream);
+  if (cols <= 1024) return launch_prepare_as<T, 64, 2, kWhole>(a, blocks, stream);
+  if (cols <= 2048) return launch_prepare_as<T, 256, 1, kWhole>(a, blocks, stream);
+  if (cols <= 4096) return launch_prepare_as<T, 256, 2, kWhole>(a, blocks, stream);
+  if (cols <= 8192) return launch_prepare_as<T, 256, 4, kWhole>(a, blocks, stream);
+  return launch_prepare_as<T, 256, 0, kWhole>(a, blocks, stream);
 }
 
 RowsArgs rows_args(const rns8_mi355x_quantize_args& g) {
-  return {g.x, g.rows, g.cols, g.ldx, g.multiplier, g.q, g.ldq, quantized_stop(g.cols, g.ldq), g.scale};
+  return {g.x, g.rows, g.cols, g.ldx, g.multiplier, g.q, g.ldq, quantized_stop(g.cols, g.ldq), g.scale, 0};
 }
 
 ColsArgs cols_args(const rns8_mi355x_quantize_args& g) {
@@ -432,6 +560,14 @@ hipError_t launch_quantize_rows(const rns8_mi355x_quantize_args& g, hipStream_t 
   return of_dtype(g.dtype, [&](auto t) { return launch_rows_of<decltype(t)>(rows_args(g), stream); });
 }
 
+hipError_t launch_quantize_fragments(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
+  if (g.rows == 0) return hipSuccess;
+  RowsArgs a = rows_args(g);
+  a.fragments = static_cast<uint32_t>((g.rows + 15) / 16);
+  a.stop = (g.cols + 63) / 64 * 64;
+  return of_dtype(g.dtype, [&](auto t) { return launch_rows_of<decltype(t)>(a, stream); });
+}
+
 uint64_t quantize_columns_bytes(int64_t rows, int64_t cols) {
   return round_up(static_cast<uint64_t>(column_chunks(rows, cols)) * static_cast<uint64_t>(cols) * 8u, 256);
 }
@@ -451,10 +587,12 @@ hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi35
   if (columns) {
     dtype = columns->dtype;
     a.cols = cols_args(*columns);
-    const int64_t strips = (columns->cols + 255) / 256;
-    if (strips > kMaxBlocks / 4 / a.cols.chunks) return hipErrorInvalidValue;
+    const bool whole = whole_columns(columns->rows);
+    const int64_t width = whole ? kWholeCols : 256, chunks = whole ? 1 : a.cols.chunks;
+    const int64_t strips = (columns->cols + width - 1) / width;
+    if (strips > kMaxBlocks / 4 / chunks) return hipErrorInvalidValue;
     a.col_strips = static_cast<uint32_t>(strips);
-    a.col_blocks = static_cast<uint32_t>(strips * a.cols.chunks);
+    a.col_blocks = static_cast<uint32_t>(strips * chunks);
     blocks += a.col_blocks;
   }
   if (copy_count > 4) return hipErrorInvalidValue;
@@ -465,11 +603,14 @@ hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi35
   }
   if (blocks == 0) return hipSuccess;
   return of_dtype(dtype, [&](auto t) {
-    return launch_prepare_of<decltype(t)>(a, static_cast<uint32_t>(blocks), stream);
+    if (columns && whole_columns(columns->rows))
+      return launch_prepare_of<decltype(t), true>(a, static_cast<uint32_t>(blocks), stream);
+    return launch_prepare_of<decltype(t), false>(a, static_cast<uint32_t>(blocks), stream);
   });
 }
 
 hipError_t launch_quantize_columns_rest(const rns8_mi355x_quantize_args& g, hipStream_t stream) {
+  if (whole_columns(g.rows)) return hipSuccess;  // done by launch_prepare
   return of_dtype(g.dtype, [&](auto t) { return launch_columns_rest<decltype(t)>(cols_args(g), stream); });
 }
 

@@ -28,7 +28,8 @@ struct Plan {
   TileShape tiles;
 };
 
-Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
+// fragments: for the choice, a as it would be in fragment order.
+Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool fragments = false) {
   Plan p{};
   const bool inner = g.b_layout == RNS8_MI355X_B_INNER;
   p.lda = g.lda;
@@ -43,7 +44,7 @@ Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled) {
     // a copy: a launch, and its bytes read and written
     const double copies = (p.copy_a ? 2.0 + static_cast<double>(g.m) * static_cast<double>(g.k) / 2.5e6 : 0.0) +
                           (p.copy_b ? 2.0 + static_cast<double>(g.n) * static_cast<double>(g.k) / 2.5e6 : 0.0);
-    p.few_rows = scaled_rows_cost(g.m, g.n, g.k) <= p.tiles.cost + copies;
+    p.few_rows = scaled_rows_cost(g.m, g.n, g.k, fragments) <= p.tiles.cost + copies;
     if (p.few_rows) {
       p.copy_a = p.copy_b = false;
       return p;
@@ -78,6 +79,18 @@ int gemm_i8_copies(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, Operan
   if (p.copy_a) copies[count++] = {g.a, g.m, g.k, g.lda, ws + p.a_at, p.lda};
   if (p.copy_b) copies[count++] = {g.b, p.b_rows, p.b_cols, g.ldb, ws + p.b_at, p.ldb};
   return count;
+}
+
+// More than one tile of tokens is read by every workgroup: 48 tokens by 8192 x
+// 4096 13.1 us from rows, 10.7 in fragment order.
+bool gemm_i8_takes_fragments(const rns8_mi355x_gemm_i8_args& g) {
+  return g.m > 16 && g.n > 0 && make_plan(g, true, true).few_rows;
+}
+
+hipError_t launch_gemm_i8_fragments(const rns8_mi355x_gemm_i8_args& g, hipStream_t stream) {
+  ScaledGemm s{g.m, g.n, g.k, g.a, g.b, g.lda, g.ldb, false, g.a_scale, g.b_scale, g.bias, g.out, g.ldo, g.dtype};
+  s.fragments = true;
+  return launch_scaled_rows(s, stream);
 }
 
 hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool copied, hipStream_t stream) {

@@ -21,6 +21,7 @@ struct ScaledGemm {
   void* out;
   int64_t ldo;
   uint32_t dtype;
+  bool fragments = false;  // a in fragment order (launch_scaled_rows only)
 };
 
 // How the tile kernel splits a product: slices == 1 writes the output, more
@@ -38,7 +39,7 @@ hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int3
 
 // Few tokens (scaled_rows.hip): operands at any alignment, no workspace.
 bool scaled_rows_takes(int64_t m, int64_t n, int64_t k, bool inner);
-double scaled_rows_cost(int64_t m, int64_t n, int64_t k);  // predicted us
+double scaled_rows_cost(int64_t m, int64_t n, int64_t k, bool fragments);  // predicted us
 hipError_t launch_scaled_rows(const ScaledGemm& g, hipStream_t stream);
 
 // What operands read once arrive at, for the predicted times: bytes per us.

@@ -13,6 +13,7 @@
 //     into its LDS, while its first weights are on their way: less than the launch
 //     of a kernel of its own.
 #include <algorithm>
+#include <type_traits>
 
 #include "scaled_epilogue.hpp"
 #include "scaled_gemm.hpp"
@@ -52,7 +53,8 @@ __device__ __forceinline__ v4i load_cut(const int8_t* row, uint32_t c, uint32_t 
   return __builtin_bit_cast(v4i, w);
 }
 
-template <int kTokens16, int kChannels16, int kUnroll, bool kFused, typename T>
+// kFragments: q in fragment order.
+template <int kTokens16, int kChannels16, int kUnroll, bool kFused, bool kFragments, typename T>
 __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
   constexpr int MB = kTokens16, RB = kChannels16, U = kUnroll;
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];  // fused: m rows of k bytes; then the waves' sums
@@ -74,6 +76,9 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
     const int64_t t = min<int64_t>(16 * i + r, a.m - 1);
     qrow[i] = kFused ? lds + t * pitch : a.q + t * a.ldq;
   }
+  auto fragment = [&](uint32_t block, int i) {
+    return *reinterpret_cast<const v4i*>(a.q + (static_cast<uint64_t>(block) * MB + i) * 1024 + 16 * lane);
+  };
   struct Group {
     v4i w[U][RB];
     v4i q[kFused ? 1 : U][MB];
@@ -87,7 +92,12 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
       for (int j = 0; j < RB; ++j) __builtin_memcpy(&f.w[u][j], wrow[j] + c, 16);
       if constexpr (!kFused) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) __builtin_memcpy(&f.q[u][i], qrow[i] + c, 16);
+        for (int i = 0; i < MB; ++i) {
+          if constexpr (kFragments)
+            f.q[u][i] = fragment(min(b + u, last - 1), i);
+          else
+            __builtin_memcpy(&f.q[u][i], qrow[i] + c, 16);
+        }
       }
     }
   };
@@ -172,7 +182,13 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
     for (int j = 0; j < RB; ++j) w[j] = load_cut(wrow[j], c, k);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-      const v4i q = kFused ? *reinterpret_cast<const v4i*>(qrow[i] + c) : load_cut(qrow[i], c, k);
+      v4i q;
+      if constexpr (kFused)
+        q = *reinterpret_cast<const v4i*>(qrow[i] + c);
+      else if constexpr (kFragments)
+        q = fragment(blocks, i);
+      else
+        q = load_cut(qrow[i], c, k);
 #pragma unroll
       for (int j = 0; j < RB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], q, acc[i][j], 0, 0, 0);
     }
@@ -202,13 +218,13 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
     store4(static_cast<float*>(a.out) + at, a.n - channel, f);
 }
 
-template <int MB, int RB, int U, bool kFused, typename T>
+template <int MB, int RB, int U, bool kFused, bool kFragments, typename T>
 hipError_t launch(const RowsArgs& a, hipStream_t stream) {
   const int64_t blocks = (a.n + 16 * RB - 1) / (16 * RB);
   if (blocks > 0x3FFFFF) return hipErrorInvalidValue;
   const size_t sums = static_cast<size_t>(kWaves) * MB * RB * 64 * sizeof(v4i);
   const size_t rows = kFused ? static_cast<size_t>(a.m) * ((a.k + 63) / 64 * 64 + 16) : 0;
-  hipLaunchKernelGGL((scaled_rows_kernel<MB, RB, U, kFused, T>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
+  hipLaunchKernelGGL((scaled_rows_kernel<MB, RB, U, kFused, kFragments, T>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
                      static_cast<unsigned>(std::max(sums, rows)), stream, a);
   return hipGetLastError();
 }
@@ -221,11 +237,12 @@ bool scaled_rows_takes(int64_t m, int64_t n, int64_t k, bool inner) {
 
 // A start, then the larger of a workgroup's own time (its K, read once for
 // the weights and once for every 16 tokens) and the weights' from HBM beside
-// what more than 16 tokens add. Fitted to 50 shapes from 4 x 256 x 256 to 64 x
-// 8192 x 8192, within 15% at each: 48 tokens by 8192 x 4096 13.9 us for 13.1.
-double scaled_rows_cost(int64_t m, int64_t n, int64_t k) {
+// what more than 16 tokens add, a quarter of it from fragment order. Fitted to 50
+// shapes from 4 x 256 x 256 to 64 x 8192 x 8192, within 15% at each: 48 tokens by
+// 8192 x 4096 14.9 us for 13.1 from rows and 10.4 for 9.7 in fragment order.
+double scaled_rows_cost(int64_t m, int64_t n, int64_t k, bool fragments) {
   const double depth = static_cast<double>(k) / 8192, tokens16 = static_cast<double>((m + 15) / 16);
-  const double more = 3.6 * depth * (tokens16 - 1), own = depth * 5.6 + more;
+  const double more = (fragments ? 0.9 : 3.6) * depth * (tokens16 - 1), own = depth * 5.6 + more;
   return 3.4 + std::max(own, static_cast<double>(n) * static_cast<double>(k) / kBytesPerUs + more);
 }
 
@@ -251,10 +268,20 @@ hipError_t launch_scaled_rows(const ScaledGemm& g, hipStream_t stream) {
   // 15.6, 21.4 / 17.4, 36.8 / 25.6, 43.9 / 28.9; 4096 x 4096 6.5 / 8, 7.5 / 10,
   // 11.3 / 13.0, 13.1 / 15.1.
   const bool wide = g.m > 1 && g.n >= 32 * 256;
-  if (g.m <= 16) return wide ? launch<1, 2, 4, false, float>(a, stream) : launch<1, 1, 4, false, float>(a, stream);
-  if (g.m <= 32) return wide ? launch<2, 2, 4, false, float>(a, stream) : launch<2, 1, 4, false, float>(a, stream);
-  if (g.m <= 48) return wide ? launch<3, 2, 4, false, float>(a, stream) : launch<3, 1, 4, false, float>(a, stream);
-  return wide ? launch<4, 2, 4, false, float>(a, stream) : launch<4, 1, 4, false, float>(a, stream);
+  if (g.m <= 16)
+    return wide ? launch<1, 2, 4, false, false, float>(a, stream) : launch<1, 1, 4, false, false, float>(a, stream);
+  auto tokens = [&](auto fragments) {
+    constexpr bool kFragments = decltype(fragments)::value;
+    if (g.m <= 32)
+      return wide ? launch<2, 2, 4, false, kFragments, float>(a, stream)
+                  : launch<2, 1, 4, false, kFragments, float>(a, stream);
+    if (g.m <= 48)
+      return wide ? launch<3, 2, 4, false, kFragments, float>(a, stream)
+                  : launch<3, 1, 4, false, kFragments, float>(a, stream);
+    return wide ? launch<4, 2, 4, false, kFragments, float>(a, stream)
+                : launch<4, 1, 4, false, kFragments, float>(a, stream);
+  };
+  return g.fragments ? tokens(std::true_type{}) : tokens(std::false_type{});
 }
 
 // Two tokens at most, and no more bytes than the quantization is worth beside
@@ -283,9 +310,9 @@ hipError_t launch_linear_rows(const rns8_mi355x_linear_i8_args& g, hipStream_t s
   a.stop = quantized_stop(g.k, g.ldq);
   a.scale_out = g.x_scale;
   switch (g.dtype) {
-    case RNS8_MI355X_F32: return launch<1, 1, 8, true, float>(a, stream);
-    case RNS8_MI355X_F16: return launch<1, 1, 8, true, f16>(a, stream);
-    case RNS8_MI355X_BF16: return launch<1, 1, 8, true, bf16>(a, stream);
+    case RNS8_MI355X_F32: return launch<1, 1, 8, true, false, float>(a, stream);
+    case RNS8_MI355X_F16: return launch<1, 1, 8, true, false, f16>(a, stream);
+    case RNS8_MI355X_BF16: return launch<1, 1, 8, true, false, bf16>(a, stream);
     default: return hipErrorInvalidValue;
   }
 }
