@@ -37,9 +37,11 @@ Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool fragm
   p.tiles = choose_tile_shape(g.m, g.n, g.k);
   p.b_rows = inner ? g.k : g.n;
   p.b_cols = inner ? g.n : g.k;
-  // where b is n x k, a's chunks are read whole: they have to end in zeros
-  p.copy_a = g.k > 0 && !(in_place(g.a, g.lda) && (inner || a_zero_filled || g.k % 16 == 0));
+  p.copy_a = g.k > 0 && !in_place(g.a, g.lda);
   p.copy_b = g.k > 0 && !in_place(g.b, g.ldb);
+  // where b is n x k and k ends inside a chunk, one of the two has to end in
+  // zeros there, as copies do: the other's bytes then do not matter
+  if (!inner && g.k % 16 != 0 && !a_zero_filled && !p.copy_a && !p.copy_b) (g.m <= g.n ? p.copy_a : p.copy_b) = true;
   if (scaled_rows_takes(g.m, g.n, g.k, inner)) {
     // a copy: a launch, and its bytes read and written
     const double copies = (p.copy_a ? 2.0 + static_cast<double>(g.m) * static_cast<double>(g.k) / 2.5e6 : 0.0) +

@@ -11,7 +11,8 @@ namespace rns8x {
 
 // Operands as the kernels read them: 16-byte aligned rows at strides that are
 // multiples of 16 below 2^23. `k` may end inside a 16-byte chunk: where b is n x
-// k, a's bytes from k to the chunk's end are zeros and b's may hold anything.
+// k, a's or b's bytes from k to the chunk's end are zeros and the other's may hold
+// anything.
 struct ScaledGemm {
   int64_t m, n, k;
   const int8_t *a, *b;
