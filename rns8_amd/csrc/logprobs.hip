@@ -14,13 +14,14 @@
 // their gradient): a logit costs about ten vector operations, the exponential
 // counted as four, and the next loads are in flight beside them.
 //
-// Few rows are cut into parts of a few thousand logits, one workgroup each,
-// whose sums and alternatives a second kernel joins: 4 rows of 131072 would
-// occupy 4 of 256 CUs.
+// Few long rows are cut into parts of 4096 logits or more, one workgroup each, whose
+// sums and alternatives a second kernel joins: 4 rows of 131072 would occupy 4 of
+// 256 CUs.
 //
 // Alternatives: the n-th largest of any n different threads' maxima is a lower
 // bound of the part's n-th largest logit, so with 4 waves the least of the waves'
-// ceil(n/4)-th largest lane maxima is one. Only threads whose maximum reaches it
+// ceil(n/4)-th largest lane maxima is one (in a part so short that not every wave
+// has logits in all lanes: of the waves that do, which share n). Only threads whose maximum reaches it
 // hold candidates: short parts keep their logits in registers for that look,
 // longer ones read those threads' logits again (some tens of 256 threads). The
 // candidates are ordered by counting; where too many are equal (a part of one
@@ -170,6 +171,15 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
   return static_cast<uint64_t>(hi) << 32 | wave_reduce(lo, MaxU{});
 }
 
+// How many of the keys come before `key` (eight loads in flight: one at a time, a
+// list of 500 took 50 us).
+__device__ __forceinline__ uint32_t rank_among(const uint64_t* keys, uint32_t n, uint64_t key) {
+  uint32_t rank = 0;
+#pragma unroll 8
+  for (uint32_t j = 0; j < n; ++j) rank += keys[j] > key;
+  return rank;
+}
+
 struct Args {
   const void* logits;
   int64_t rows, vocab, ldl;
@@ -179,7 +189,7 @@ struct Args {
   float *logp, *entropy, *lse;
   int32_t* top_ids;
   float* top_logp;
-  int64_t parts, part_len;  // part_len: a multiple of kStride where parts > 1
+  int64_t parts, part_len;  // part_len: a multiple of 64 logits
   float* part_sums;         // [rows][parts][4]
   uint64_t* part_keys;      // [rows][parts][top]
 };
@@ -299,17 +309,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
     const bool lane_nan = t.s != t.s;  // a NaN among the lane's logits, which comes first
     t = wave_join(t, a.c);
     if (lane == 0) wave_sums[wave] = t;
-    if (a.top) {
-      // the wave's ceil(top / 4)-th largest lane maximum
+    // waves with logits in every lane; without any, the part has few enough logits
+    // for all of them to be candidates
+    const uint32_t full = static_cast<uint32_t>(min<int64_t>((last - first) / (64 * kVector), kWaves));
+    if (a.top && full) {
       float mine = lane_max, least = -INFINITY;
-      for (uint32_t k = 0; k < (a.top + kWaves - 1) / kWaves; ++k) {
+      for (uint32_t k = 0; k < (a.top + full - 1) / full; ++k) {
         least = wave_max(mine);
         const uint64_t who = __ballot(mine == least);
         if (lane == __ffsll(static_cast<unsigned long long>(who)) - 1) mine = -INFINITY;
       }
       if (lane == 0) wave_least[wave] = least;
-      if (threadIdx.x == 0) count = lane_count = 0;
     }
+    if (threadIdx.x == 0) count = lane_count = 0;
     __syncthreads();
     t = join_waves(wave_sums, a.c);
     if (threadIdx.x == 0) {
@@ -321,9 +333,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
       }
     }
     if (a.top) {
-      float from = wave_least[0];
+      float from = full ? wave_least[0] : -INFINITY;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) from = fminf(from, wave_least[w]);
+      for (uint32_t w = 1; w < kWaves; ++w) from = w < full ? fminf(from, wave_least[w]) : from;
       auto gather = [&](int64_t at, const Held<T>& h) {
 #pragma unroll
         for (int i = 0; i < kVector; ++i) {
@@ -370,8 +382,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
       if (n <= kMaxCandidates) {
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
           const uint64_t key = keys[i];
-          uint32_t rank = 0;
-          for (uint32_t j = 0; j < n; ++j) rank += keys[j] > key;
+          const uint32_t rank = rank_among(keys, n, key);
           if (rank < a.top) put(rank, key);
         }
         // (a part shorter than `top`: its list ends in zeros, below every key)
@@ -403,9 +414,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
 }
 
 // A workgroup loads a row's lists; its first wave joins the sums, lane p part p.
-// The lists are in order, so the top-th largest of their heads bounds the row's
-// alternatives from below: the keys from there on are gathered and ordered by
-// counting, as within a part.
+// The lists are in order: with each list's k-th key, k = ceil(top / parts), the
+// ceil(top / k)-th largest of those has at least `top` keys at or above it. The keys
+// from there on are gathered and ordered by counting, as within a part.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
   __shared__ uint64_t keys[kMaxTop * kMaxTop];
@@ -414,6 +425,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
   __shared__ Sums joined;
   const int lane = threadIdx.x & 63;
   const uint32_t parts = static_cast<uint32_t>(a.parts), total = parts * a.top;
+  const uint32_t each = (a.top + parts - 1) / parts, enough = a.top ? (a.top + each - 1) / each : 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const uint64_t* const lists = a.part_keys + row * total;
     constexpr uint32_t kHeld = kMaxTop * kMaxTop / kThreads;  // 16: parts and top are at most 64
@@ -430,20 +442,18 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
         float w[4];
         __builtin_memcpy(w, a.part_sums + 4 * (row * a.parts + lane), 16);
         t = {w[0], w[1], w[2]};
-        if (a.top) head = lists[lane * a.top];
+        if (a.top) head = lists[lane * a.top + each - 1];
       }
       t = wave_join(t, a.c);
       if (lane == 0) {
         write_row<T>(a, row, t);
         joined = t;
         count = 0;
-        from = 0;  // fewer parts than alternatives: every key
+        from = 0;  // where lists end before their k-th key: every key
       }
       keys[lane] = head;
       __builtin_amdgcn_wave_barrier();
-      uint32_t rank = 0;
-      for (uint32_t p = 0; p < parts; ++p) rank += keys[p] > head;
-      if (head && rank == a.top - 1) from = head;
+      if (head && rank_among(keys, parts, head) == enough - 1) from = head;
     }
     __syncthreads();
     if (a.top) {
@@ -457,8 +467,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
       const uint32_t n = count;
       for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t mine = keys[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += keys[j] > mine;
+        const uint32_t rank = rank_among(keys, n, mine);
         if (rank < a.top) write_alternative(a, row, rank, mine, t);
       }
     }
@@ -551,19 +560,29 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
   }
 }
 
-// Parts of a row: as many as give about `units` workgroups, none shorter than
-// `least` rounds.
-void cut_rows(int64_t rows, int64_t vocab, int64_t units, int64_t least, int64_t& parts, int64_t& len) {
-  const int64_t rounds = (vocab + kStride - 1) / kStride;
-  parts = std::max<int64_t>(1, std::min({(units + rows - 1) / rows, (rounds + least - 1) / least, kMaxParts}));
-  const int64_t per = (rounds + parts - 1) / parts;
-  parts = (rounds + per - 1) / per;
-  len = per * kStride;
+struct Cut {
+  int64_t parts, len;
+};
+
+// A row in even parts, whole cache lines of whichever type.
+Cut cut_row(int64_t vocab, int64_t parts) {
+  const int64_t len = ((vocab + parts - 1) / parts + 63) / 64 * 64;
+  return {(vocab + len - 1) / len, len};
 }
 
-// With alternatives a part may be one round, as it stays in registers.
-void forward_parts(int64_t rows, int64_t vocab, uint32_t top, int64_t& parts, int64_t& len) {
-  cut_rows(rows, vocab, 1024, top ? 1 : 4, parts, len);
+// A second launch and its reads of what the first wrote cost 2 to 4 us. bf16, 20
+// alternatives, one part against the number here: 4 rows of 131072 27 us and 12 (32
+// parts), 64 rows 29 and 16 (8 parts), 16 rows of 50001 16 and 13; but 4 rows of
+// 32768 12 both ways, and 400 rows of 100000 31 and 32 in two parts.
+Cut forward_cut(int64_t rows, int64_t vocab) {
+  if (vocab <= 32768) return cut_row(vocab, 1);
+  return cut_row(vocab, std::max<int64_t>(1, std::min({512 / rows, vocab / 4096, kMaxParts})));
+}
+
+// The gradient: about 1024 workgroups, no fewer than two rounds each.
+Cut backward_cut(int64_t rows, int64_t vocab) {
+  const int64_t most = (vocab + 2 * kStride - 1) / (2 * kStride);
+  return cut_row(vocab, std::max<int64_t>(1, std::min((1024 + rows - 1) / rows, most)));
 }
 
 dim3 grid_of(int64_t units) { return dim3(static_cast<unsigned>(std::min(units, kMaxBlocks))); }
@@ -571,15 +590,13 @@ dim3 grid_of(int64_t units) { return dim3(static_cast<unsigned>(std::min(units, 
 template <typename T>
 hipError_t launch_forward(const Args& a, hipStream_t stream) {
   const dim3 grid = grid_of(a.rows * a.parts), block(kThreads);
-  const int64_t rounds = a.part_len / kStride;
+  const int64_t rounds = (a.part_len + kStride - 1) / kStride;
   if (a.top == 0 || rounds > kHeldRounds)
     hipLaunchKernelGGL((logprobs_kernel<T, 0>), grid, block, 0, stream, a);
   else if (rounds <= 1)
     hipLaunchKernelGGL((logprobs_kernel<T, 1>), grid, block, 0, stream, a);
   else if (rounds <= 2)
     hipLaunchKernelGGL((logprobs_kernel<T, 2>), grid, block, 0, stream, a);
-  else if (rounds <= 4)
-    hipLaunchKernelGGL((logprobs_kernel<T, 4>), grid, block, 0, stream, a);
   else
     hipLaunchKernelGGL((logprobs_kernel<T, kHeldRounds>), grid, block, 0, stream, a);
   const hipError_t e = hipGetLastError();
@@ -602,17 +619,16 @@ hipError_t of_dtype(uint32_t dtype, F&& f) {
 
 uint64_t logprobs_bytes(const rns8_mi355x_logprobs_args& g) {
   if (g.rows == 0) return 0;
-  int64_t parts, len;
-  forward_parts(g.rows, g.vocab, g.top, parts, len);
+  const int64_t parts = forward_cut(g.rows, g.vocab).parts;
   return parts == 1 ? 0u : static_cast<uint64_t>(g.rows) * static_cast<uint64_t>(parts) * (16u + 8u * g.top);
 }
 
 hipError_t launch_logprobs(const rns8_mi355x_logprobs_args& g, hipStream_t stream) {
   if (g.rows == 0) return hipSuccess;
   if (g.top > kMaxTop || g.vocab < 1 || g.vocab > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const Cut cut = forward_cut(g.rows, g.vocab);
   Args a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.scale * kLog2E, g.top, g.logp, g.entropy, g.lse,
-         g.top_ids, g.top_logp, 1, 0, nullptr, nullptr};
-  forward_parts(g.rows, g.vocab, g.top, a.parts, a.part_len);
+         g.top_ids, g.top_logp, cut.parts, cut.len, nullptr, nullptr};
   a.part_sums = static_cast<float*>(g.workspace);
   a.part_keys = reinterpret_cast<uint64_t*>(a.part_sums + 4 * g.rows * a.parts);
   return of_dtype(g.dtype, [&](auto t) { return launch_forward<decltype(t)>(a, stream); });
@@ -620,14 +636,11 @@ hipError_t launch_logprobs(const rns8_mi355x_logprobs_args& g, hipStream_t strea
 
 hipError_t launch_logprobs_backward(const rns8_mi355x_logprobs_backward_args& g, hipStream_t stream) {
   if (g.rows == 0) return hipSuccess;
+  // in place a row's logits may be read twice: by the workgroup that writes them
+  const Cut cut = g.dlogits == g.logits ? cut_row(g.vocab, 1) : backward_cut(g.rows, g.vocab);
   BackArgs a{g.logits, g.rows, g.vocab, g.ldl, g.targets, g.scale, g.scale * kLog2E, g.lse, g.entropy, g.dlogp,
-             g.dentropy, g.dlogits, g.lddl, 1, 0, 0};
+             g.dentropy, g.dlogits, g.lddl, cut.parts, cut.len, 0};
   a.streamed = streams(2 * g.rows * g.vocab * (g.dtype == RNS8_MI355X_F32 ? 4 : 2), g.dlogits, g.lddl, g.dtype);
-  cut_rows(g.rows, g.vocab, 1024, 2, a.parts, a.part_len);
-  if (g.dlogits == g.logits) {  // in place a row's logits may be read twice: by the workgroup that writes them
-    a.parts = 1;
-    a.part_len = (g.vocab + kStride - 1) / kStride * kStride;
-  }
   return of_dtype(g.dtype, [&](auto t) {
     hipLaunchKernelGGL((logprobs_backward_kernel<decltype(t)>), grid_of(a.rows * a.parts), dim3(kThreads), 0, stream,
                        a);

@@ -125,6 +125,18 @@ def test_ties_and_special_rows(gpu_ctx, dtype, vocab):
     assert got["entropy"][2] == 0 and got["lse"][2] == -float("inf")
 
 
+@pytest.mark.parametrize("rows", [1, 3, 130, 700])
+@pytest.mark.parametrize("vocab", [511, 512, 513, 1543, 2041, 2057, 8200, 12969, 14847, 17493])
+@pytest.mark.parametrize("top", [1, 5, 20, 64])
+def test_alternatives_of_short_and_ragged_parts(gpu_ctx, rows, vocab, top):
+    logits = (3.0 * normal(rows + vocab, rows, vocab)).bfloat16()
+    if rows > 2:
+        logits[1, 40:] = -float("inf")
+        logits[2, : vocab - 10] = -float("inf")
+    targets = torch.randint(vocab, (rows,), device="cuda")
+    check(run(gpu_ctx, logits, targets, 1.0, top), definition(logits, targets, 1.0, top), logits, 1.0)
+
+
 def test_not_finite(gpu_ctx):
     v = normal(1, 6, 3000)
     v[1, 2999], v[2, 5], v[3, 100] = float("nan"), float("inf"), -float("inf")
