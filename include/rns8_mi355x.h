@@ -272,10 +272,12 @@ RNS8_API rns8_status rns8_mi355x_get_exact_proof(
  * They share these rules:
  *   - Every operator takes its arguments in one struct: struct_size and
  *     abi_version as in the other structs of this library, device pointers,
- *     and row strides (ld*) in elements. The device reads and writes only the
- *     columns named; a stride may be any value from the row length on, and no
- *     pointer needs more alignment than its element type. Outputs must not
- *     overlap inputs unless stated.
+ *     and row strides (ld*) in elements. The device writes only the columns
+ *     named and reads no others of floating operands; 8-bit operands may be
+ *     read in whole aligned 16-byte chunks, whose other bytes do not matter. A
+ *     stride may be any value from the row length on, and no pointer needs more
+ *     alignment than its element type. Outputs must not overlap inputs unless
+ *     stated.
  *   - `dtype` is the type of the floating operands marked `dtype` below.
  *     Sums, statistics and scales are computed and kept in 32 bits; an output
  *     is rounded once, to nearest even.
@@ -339,13 +341,15 @@ RNS8_API rns8_status rns8_mi355x_quantize_columns_workspace(const rns8_mi355x_qu
 
 /* The product of 8-bit matrices with scales:
  *   out[i][j] = a_scale[i] * b_scale[j] * sum_k a[i][k] b(k, j) + bias[j],
- * the sum exact in integers for every k (bytes may be -128), rounded once to
- * 32 bits. b is stored n x k (RNS8_MI355X_B_CHANNELS: one row for each output
+ * the sum exact in integers for every k (bytes may be -128) and rounded once to
+ * 32 bits, so a row of out is the same whatever other rows a call has. b is stored n x k (RNS8_MI355X_B_CHANNELS: one row for each output
  * channel, the usual layout of weights) or k x n (RNS8_MI355X_B_INNER). Any of
  * a_scale, b_scale (1) and bias (0) may be NULL. m, n >= 0, k >= 0 (an empty
- * sum is zero); m, n and k below 2^31, lda and ldb below 2^23. Operands whose
- * pointers and strides are multiples of 16 (and whose k is one) are read in
- * place; others are first copied into the workspace. */
+ * sum is zero); m, n and k below 2^31, lda and ldb below 2^23. Products of more
+ * than 64 rows read operands in place whose pointers and strides are multiples
+ * of 16 and copy others into the workspace first, and one of the two where b is
+ * n x k and k is no multiple of 16. Products of fewer rows may read in place
+ * at any alignment. */
 #define RNS8_MI355X_B_CHANNELS 0u
 #define RNS8_MI355X_B_INNER 1u
 typedef struct rns8_mi355x_gemm_i8_args {
@@ -377,8 +381,9 @@ RNS8_API rns8_status rns8_mi355x_gemm_i8_scaled_workspace(const rns8_mi355x_gemm
  * rns8_mi355x_quantize_rows (no multiplier) and multiplied with 8-bit weights
  * w (n x k, w_scale[n]):
  *   out[i][j] = x_scale[i] * w_scale[j] * sum_k q[i][k] w[j][k] + bias[j].
- * x_q (m x k at stride ldq) and x_scale[m] receive the quantized rows if given
- * (both or neither): what the backward pass reads. k >= 1. */
+ * x_q (m x k at stride ldq, zeros after each row as there) and x_scale[m] receive
+ * the quantized rows if given (both or neither): what the backward pass reads.
+ * k >= 1; k below 2^23 - 16, ldw and ldq below 2^23. */
 typedef struct rns8_mi355x_linear_i8_args {
   uint64_t struct_size;
   uint32_t abi_version;
@@ -412,7 +417,8 @@ RNS8_API rns8_status rns8_mi355x_linear_i8_workspace(const rns8_mi355x_linear_i8
  *   dbias[j] = sum_i dy[i][j].
  * dw is the gradient of the weights w * w_scale. dx, dw and dbias may each be
  * NULL (not all three); x_q and x_scale may be NULL without dw, w and w_scale
- * without dx. */
+ * without dx. With dx n, and with dw or dbias m, stays below 2^23 - 16; ldq and ldw
+ * below 2^23. */
 typedef struct rns8_mi355x_linear_i8_backward_args {
   uint64_t struct_size;
   uint32_t abi_version;

@@ -28,6 +28,11 @@ bool operand_ok(const void* p, int64_t rows, int64_t cols, int64_t ld, uint64_t 
 bool optional_ok(const void* p, int64_t rows, int64_t cols, int64_t ld, uint64_t size) {
   return !p || operand_ok(p, rows, cols, ld, size);
 }
+// An output may be an input itself, row for row; rows at another stride would
+// overwrite inputs that are still to be read.
+bool in_place_ok(const void* in, int64_t ldin, const void* out, int64_t ldout, int64_t rows) {
+  return in != out || !out || ldin == ldout || rows < 2;
+}
 bool floats_ok(const void* p, int64_t count) { return operand_ok(p, 1, count, count, sizeof(float)); }
 
 rns8_status check_workspace(const void* p, uint64_t have, uint64_t need) {
@@ -271,6 +276,8 @@ rns8_status check_norm(const rns8_mi355x_block_norm_args& a) {
   if (!optional_ok(a.h, a.rows, a.cols, a.ldh, size) || !optional_ok(a.y, a.rows, a.cols, a.ldy, size) ||
       !optional_ok(a.q, a.rows, a.cols, a.ldq, 1))
     return RNS8_INVALID_ARGUMENT;
+  if (!in_place_ok(a.x, a.ldx, a.h, a.ldh, a.rows) || !in_place_ok(a.residual, a.ldresidual, a.h, a.ldh, a.rows))
+    return RNS8_INVALID_ARGUMENT;
   if (!a.q != !a.q_scale) return RNS8_INVALID_ARGUMENT;
   if (a.rows > 0 && (pre ? !a.y && !a.q : !a.h)) return RNS8_INVALID_ARGUMENT;
   if (!pre && (a.y || a.q)) return RNS8_INVALID_ARGUMENT;
@@ -325,6 +332,7 @@ rns8_status check_logprobs_backward(const rns8_mi355x_logprobs_backward_args& a)
   if (!operand_ok(a.logits, a.rows, a.vocab, a.ldl, size) || !operand_ok(a.dlogits, a.rows, a.vocab, a.lddl, size) ||
       !floats_ok(a.lse, a.rows))
     return RNS8_INVALID_ARGUMENT;
+  if (!in_place_ok(a.logits, a.ldl, a.dlogits, a.lddl, a.rows)) return RNS8_INVALID_ARGUMENT;
   if (a.rows > 0 && !a.dlogp && !a.dentropy) return RNS8_INVALID_ARGUMENT;
   if (a.dlogp && (!floats_ok(a.dlogp, a.rows) || !ids_ok(a.targets, a.rows))) return RNS8_INVALID_ARGUMENT;
   if (a.dentropy && (!floats_ok(a.dentropy, a.rows) || !floats_ok(a.entropy, a.rows))) return RNS8_INVALID_ARGUMENT;

@@ -5,6 +5,17 @@
 
 namespace rns8x {
 
+// A sum with its scales and bias, in 32 bits. Every kernel of the product ends in
+// this, so a token's results do not depend on which of them its batch takes. (Left
+// alone, the compiler joins the last step and the conversion to 16 bits in some
+// kernels, which rounds once instead of twice.)
+template <typename S>
+__device__ __forceinline__ float scaled_value(S sum, float a_scale, float b_scale, float bias) {
+  float v = fmaf(static_cast<float>(sum) * a_scale, b_scale, bias);
+  asm("" : "+v"(v));  // (no instruction: the value as 32 bits hold it)
+  return v;
+}
+
 // Four neighbouring outputs of a row (`n` of them inside it).
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int64_t n, const float (&v)[4]) {

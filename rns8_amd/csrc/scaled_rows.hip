@@ -208,7 +208,7 @@ __global__ __launch_bounds__(kThreads) void scaled_rows_kernel(RowsArgs a) {
   const float sa = kFused ? (token ? scale[1] : scale[0]) : token_scale;
   float f[4];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) f[x] = static_cast<float>(sum[x]) * sa * sb[x] + bias[x];
+  for (int x = 0; x < 4; ++x) f[x] = scaled_value(sum[x], sa, sb[x], bias[x]);
   const int64_t at = token * a.ldo + channel;
   if (a.dtype == RNS8_MI355X_BF16)
     store4(static_cast<bf16*>(a.out) + at, a.n - channel, f);

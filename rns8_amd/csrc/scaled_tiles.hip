@@ -317,7 +317,7 @@ __global__ __launch_bounds__(C::kThreads, kMinBlocks) void scaled_tiles_kernel(T
     for (int i = 0; i < TM; ++i) sa[i] = args.a_scale && row0 + 16 * i < m ? args.a_scale[row0 + 16 * i] : 1.0f;
     auto value = [&](const Acc4& v, int i, const float (&sb)[4], const float (&bias)[4], float (&f)[4]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(static_cast<int>(v.v[e])) * sa[i] * sb[e] + bias[e];
+      for (int e = 0; e < 4; ++e) f[e] = scaled_value(static_cast<int>(v.v[e]), sa[i], sb[e], bias[e]);
     };
     auto write = [&](auto type) {
       using T = decltype(type);
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(256) void join_slices_kernel(JoinArgs a) {
     load4_or(a.b_scale, c, a.n, 1.0f, sb);
     load4_or(a.bias, c, a.n, 0.0f, bias);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(sum[e]) * sa * sb[e] + bias[e];
+    for (int e = 0; e < 4; ++e) f[e] = scaled_value(sum[e], sa, sb[e], bias[e]);
     store4(static_cast<T*>(a.out) + row * a.ldo + c, a.n - c, f);
   }
 }
