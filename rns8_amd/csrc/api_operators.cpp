@@ -169,6 +169,9 @@ struct BackwardParts {
   uint64_t bytes = 0;
 };
 
+// (n and k are at least 1)
+bool both_products(const rns8_mi355x_linear_i8_backward_args& a) { return a.dx && a.dw && a.m > 0; }
+
 void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts& p) {
   uint8_t* at = static_cast<uint8_t*>(a.workspace);
   auto take = [&](uint64_t bytes) {
@@ -198,8 +201,6 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.dx.a_scale = p.rows.scale;
     p.dx.out = a.dx;
     p.dx.ldo = a.lddx;
-    p.dx.workspace_bytes = gemm_i8_bytes(p.dx, true);
-    p.dx.workspace = take(p.dx.workspace_bytes);
   }
   if (a.dw || a.dbias) {
     p.columns.dtype = a.dtype;
@@ -226,11 +227,18 @@ void backward_parts(const rns8_mi355x_linear_i8_backward_args& a, BackwardParts&
     p.dw.a_scale = p.columns.scale;
     p.dw.out = a.dw;
     p.dw.ldo = a.lddw;
-    if (a.dw) {
-      p.dw.workspace_bytes = gemm_i8_bytes(p.dw, true);
-      p.dw.workspace = take(p.dw.workspace_bytes);
-    }
   }
+  uint64_t bytes[2] = {};
+  if (both_products(a)) {
+    gemm_i8_pair_bytes(p.dx, p.dw, bytes);
+  } else {
+    if (a.dx) bytes[0] = gemm_i8_bytes(p.dx, true);
+    if (a.dw) bytes[1] = gemm_i8_bytes(p.dw, true);
+  }
+  p.dx.workspace_bytes = bytes[0];
+  p.dx.workspace = take(bytes[0]);
+  p.dw.workspace_bytes = bytes[1];
+  p.dw.workspace = take(bytes[1]);
 }
 
 rns8_status check_linear_backward(const rns8_mi355x_linear_i8_backward_args& a) {
@@ -469,6 +477,7 @@ rns8_status rns8_mi355x_linear_i8_backward(rns8_context* ctx, const rns8_mi355x_
         if (a.dw) count += gemm_i8_copies(p.dw, true, copies + count);
         hipError_t e = launch_prepare(a.dx ? &p.rows : nullptr, columns ? &p.columns : nullptr, copies, count, s);
         if (e == hipSuccess && columns) e = launch_quantize_columns_rest(p.columns, s);
+        if (both_products(a)) return e != hipSuccess ? e : launch_gemm_i8_pair(p.dx, p.dw, s);
         if (e == hipSuccess && a.dx) e = launch_gemm_i8(p.dx, true, true, s);
         if (e == hipSuccess && a.dw) e = launch_gemm_i8(p.dw, true, true, s);
         return e;

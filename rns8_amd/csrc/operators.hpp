@@ -70,6 +70,11 @@ uint64_t gemm_i8_bytes(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled);
 // workspace; launch_gemm_i8 makes them itself unless `copied`.
 int gemm_i8_copies(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, OperandCopy* copies);
 hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& a, bool a_zero_filled, bool copied, hipStream_t stream);
+// Two products with rows in each, both with b k x n, zero-filled rows of a and their
+// copies made: in one launch where that is faster. Their workspaces are apart.
+void gemm_i8_pair_bytes(const rns8_mi355x_gemm_i8_args& x, const rns8_mi355x_gemm_i8_args& y, uint64_t (&bytes)[2]);
+hipError_t launch_gemm_i8_pair(const rns8_mi355x_gemm_i8_args& x, const rns8_mi355x_gemm_i8_args& y,
+                               hipStream_t stream);
 // Whether the product would rather have its rows in fragment order, and the product of such rows.
 bool gemm_i8_takes_fragments(const rns8_mi355x_gemm_i8_args& a);
 hipError_t launch_gemm_i8_fragments(const rns8_mi355x_gemm_i8_args& a, hipStream_t stream);

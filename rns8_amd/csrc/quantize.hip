@@ -145,10 +145,11 @@ struct ColsArgs {
 };
 
 // About 1024 workgroups of 256 columns, at least 16 rows each, and few enough
-// that joining them is a small part of the second kernel.
+// that joining them is a small part of the second kernel: 4096 x 4096 26.8 us in 32
+// chunks, 27.9 in 64; 16384 x 2048 44.7 and 41.3.
 int64_t column_chunks(int64_t rows, int64_t cols) {
   const int64_t col_blocks = (cols + 255) / 256;
-  return std::max<int64_t>(1, std::min({(1024 + col_blocks - 1) / col_blocks, (rows + 15) / 16, int64_t{64}}));
+  return std::max<int64_t>(1, std::min({(1024 + col_blocks - 1) / col_blocks, (rows + 15) / 16, int64_t{rows > 8192 ? 64 : 32}}));
 }
 
 // Eight columns from column c on of four rows `step` apart and their factors,
@@ -453,7 +454,7 @@ hipError_t launch_columns_rest(const ColsArgs& a, hipStream_t stream) {
 }
 
 // ---- rows, columns and copies in one launch -------------------------------------------
-// Workgroups of 256 threads in three ranges: rows to quantize; columns, 64 of
+// Workgroups of 256 threads in three ranges: rows to quantize; columns, 32 of
 // them whole or (256 columns, rows of a chunk) for their partials; copies. They
 // share nothing: one launch costs less than three, and small ones fill the chip
 // together.

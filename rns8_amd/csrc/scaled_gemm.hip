@@ -28,13 +28,15 @@ struct Plan {
   TileShape tiles;
 };
 
-// fragments: for the choice, a as it would be in fragment order.
-Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool fragments = false) {
+// fragments: for the choice, a as it would be in fragment order. tiles: how the
+// tile kernel splits it, where that is settled already.
+Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool fragments = false,
+               const TileShape* tiles = nullptr) {
   Plan p{};
   const bool inner = g.b_layout == RNS8_MI355X_B_INNER;
   p.lda = g.lda;
   p.ldb = g.ldb;
-  p.tiles = choose_tile_shape(g.m, g.n, g.k);
+  p.tiles = tiles ? *tiles : choose_tile_shape(g.m, g.n, g.k);
   p.b_rows = inner ? g.k : g.n;
   p.b_cols = inner ? g.n : g.k;
   p.copy_a = g.k > 0 && !in_place(g.a, g.lda);
@@ -65,6 +67,28 @@ Plan make_plan(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool fragm
   p.sums_at = take(p.tiles.bytes);
   p.bytes = at;
   return p;
+}
+
+ScaledGemm planned(const rns8_mi355x_gemm_i8_args& g, const Plan& p) {
+  int8_t* const ws = static_cast<int8_t*>(g.workspace);
+  ScaledGemm s{g.m, g.n, g.k, g.a, g.b, p.lda, p.ldb, g.b_layout == RNS8_MI355X_B_INNER, g.a_scale, g.b_scale, g.bias,
+               g.out, g.ldo, g.dtype};
+  if (p.copy_a) s.a = ws + p.a_at;
+  if (p.copy_b) s.b = ws + p.b_at;
+  if (g.k == 0) {  // no operand is read (their buffers are empty): any aligned address will do
+    s.a = s.b = static_cast<const int8_t*>(g.out) - reinterpret_cast<uintptr_t>(g.out) % 16;
+    s.lda = 0;
+    s.ldb = s.inner ? static_cast<int64_t>(round_up(static_cast<uint64_t>(g.n), 16)) : 0;
+  }
+  return s;
+}
+
+int32_t* sums_of(const rns8_mi355x_gemm_i8_args& g, const Plan& p) {
+  return reinterpret_cast<int32_t*>(static_cast<int8_t*>(g.workspace) + p.sums_at);
+}
+
+bool pair_shapes(const rns8_mi355x_gemm_i8_args& x, const rns8_mi355x_gemm_i8_args& y, TileShape (&shapes)[2]) {
+  return choose_pair_shapes({x.m, y.m}, {x.n, y.n}, {x.k, y.k}, shapes);
 }
 
 }  // namespace
@@ -98,9 +122,7 @@ hipError_t launch_gemm_i8_fragments(const rns8_mi355x_gemm_i8_args& g, hipStream
 hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled, bool copied, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return hipSuccess;
   const Plan p = make_plan(g, a_zero_filled);
-  int8_t* const ws = static_cast<int8_t*>(g.workspace);
-  ScaledGemm s{g.m, g.n, g.k, g.a, g.b, p.lda, p.ldb, g.b_layout == RNS8_MI355X_B_INNER, g.a_scale, g.b_scale, g.bias,
-               g.out, g.ldo, g.dtype};
+  const ScaledGemm s = planned(g, p);
   if (p.few_rows) return launch_scaled_rows(s, stream);
   if (!copied) {
     OperandCopy copies[2];
@@ -110,14 +132,27 @@ hipError_t launch_gemm_i8(const rns8_mi355x_gemm_i8_args& g, bool a_zero_filled,
       if (e != hipSuccess) return e;
     }
   }
-  if (p.copy_a) s.a = ws + p.a_at;
-  if (p.copy_b) s.b = ws + p.b_at;
-  if (g.k == 0) {  // no operand is read (their buffers are empty): any aligned address will do
-    s.a = s.b = static_cast<const int8_t*>(g.out) - reinterpret_cast<uintptr_t>(g.out) % 16;
-    s.lda = 0;
-    s.ldb = s.inner ? static_cast<int64_t>(round_up(static_cast<uint64_t>(g.n), 16)) : 0;
-  }
-  return launch_scaled_tiles(s, p.tiles, reinterpret_cast<int32_t*>(ws + p.sums_at), stream);
+  int32_t* const sums = sums_of(g, p);
+  return launch_scaled_tiles(&s, &p.tiles, &sums, 1, stream);
+}
+
+void gemm_i8_pair_bytes(const rns8_mi355x_gemm_i8_args& x, const rns8_mi355x_gemm_i8_args& y, uint64_t (&bytes)[2]) {
+  TileShape shapes[2];
+  pair_shapes(x, y, shapes);
+  bytes[0] = make_plan(x, true, false, &shapes[0]).bytes;
+  bytes[1] = make_plan(y, true, false, &shapes[1]).bytes;
+}
+
+hipError_t launch_gemm_i8_pair(const rns8_mi355x_gemm_i8_args& x, const rns8_mi355x_gemm_i8_args& y,
+                               hipStream_t stream) {
+  TileShape shapes[2];
+  const bool one_launch = pair_shapes(x, y, shapes);
+  const Plan p[2] = {make_plan(x, true, false, &shapes[0]), make_plan(y, true, false, &shapes[1])};
+  const ScaledGemm s[2] = {planned(x, p[0]), planned(y, p[1])};
+  int32_t* const sums[2] = {sums_of(x, p[0]), sums_of(y, p[1])};
+  if (one_launch) return launch_scaled_tiles(s, shapes, sums, 2, stream);
+  const hipError_t e = launch_scaled_tiles(&s[0], &shapes[0], &sums[0], 1, stream);
+  return e != hipSuccess ? e : launch_scaled_tiles(&s[1], &shapes[1], &sums[1], 1, stream);
 }
 
 }  // namespace rns8x

@@ -36,7 +36,11 @@ struct TileShape {
   double cost;  // predicted us
 };
 TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k);
-hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int32_t* partials, hipStream_t stream);
+// Shapes for two products with b stored k x n, and whether one launch takes both.
+bool choose_pair_shapes(const int64_t (&m)[2], const int64_t (&n)[2], const int64_t (&k)[2], TileShape (&shapes)[2]);
+// One product, or two of one tile with b stored k x n.
+hipError_t launch_scaled_tiles(const ScaledGemm* g, const TileShape* shapes, int32_t* const* partials, int count,
+                               hipStream_t stream);
 
 // Few tokens (scaled_rows.hip): operands at any alignment, no workspace.
 bool scaled_rows_takes(int64_t m, int64_t n, int64_t k, bool inner);

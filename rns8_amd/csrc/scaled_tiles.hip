@@ -107,8 +107,19 @@ struct TileArgs {
 
 __device__ __forceinline__ uint32_t div_u31(uint32_t n, DivU31 v) { return __umulhi(n << 1, v.mul) >> v.shift; }
 
+// One product or, with b stored k x n, two of one tile: the first `blocks`
+// workgroups are the first's. Two small ones share the chip, and of two large ones
+// the second's tiles start as the first's end. Both gradients of a layer of 118 x 8
+// x 35 (with their quantization) 15.0 us in two launches, 10.2 in one; of 1024^3
+// 29.3 and 23.1; of 4096^3 172.8 and 170.4. (With b stored n x k the kernel takes
+// the first's arguments without waiting for `blocks`, 0.5 us.)
+struct TilePair {
+  TileArgs product[2];
+  uint32_t blocks;
+};
+
 template <typename C, int kMinBlocks>
-__global__ __launch_bounds__(C::kThreads, kMinBlocks) void scaled_tiles_kernel(TileArgs args) {
+__global__ __launch_bounds__(C::kThreads, kMinBlocks) void scaled_tiles_kernel(TilePair pair_args) {
   constexpr int TM = C::TM, TN = C::TN, BM = C::BM, BN = C::BN, BK = C::BK;
   __shared__ __attribute__((aligned(16))) int8_t lds[C::kLds];
 
@@ -118,15 +129,18 @@ __global__ __launch_bounds__(C::kThreads, kMinBlocks) void scaled_tiles_kernel(T
   const int wave_m = wave / C::WN;
   const int wave_n = wave % C::WN;
 
-  const uint32_t grid = gridDim.x;
+  const bool second = C::kInner && blockIdx.x >= pair_args.blocks;
+  const TileArgs& args = pair_args.product[second ? 1 : 0];
+  const uint32_t grid = !C::kInner ? gridDim.x : second ? gridDim.x - pair_args.blocks : pair_args.blocks;
+  const uint32_t block = second ? blockIdx.x - pair_args.blocks : blockIdx.x;
   uint32_t u_first, u_step, u_end;
   if ((grid & 7u) == 0u) {
-    const uint32_t xcd = blockIdx.x & 7u;
-    u_first = static_cast<uint32_t>((static_cast<uint64_t>(xcd) * args.units) / 8) + (blockIdx.x >> 3);
+    const uint32_t xcd = block & 7u;
+    u_first = static_cast<uint32_t>((static_cast<uint64_t>(xcd) * args.units) / 8) + (block >> 3);
     u_end = static_cast<uint32_t>((static_cast<uint64_t>(xcd + 1) * args.units) / 8);
     u_step = grid >> 3;
   } else {
-    u_first = blockIdx.x;
+    u_first = block;
     u_end = args.units;
     u_step = grid;
   }
@@ -482,13 +496,19 @@ struct JoinArgs {
   int64_t m, n, ldp, ldo;
   const float *a_scale, *b_scale, *bias;
   void* out;
+  uint32_t dtype;
+};
+
+struct JoinPair {
+  JoinArgs product[2];
+  uint32_t blocks;  // the first's
 };
 
 template <typename T>
-__global__ __launch_bounds__(256) void join_slices_kernel(JoinArgs a) {
+__device__ __forceinline__ void join_slices(const JoinArgs& a, uint32_t block, uint32_t blocks) {
   const int64_t quads = a.ldp / 4;
-  for (int64_t q = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; q < a.m * quads;
-       q += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t q = static_cast<int64_t>(block) * 256 + threadIdx.x; q < a.m * quads;
+       q += static_cast<int64_t>(blocks) * 256) {
     const int64_t row = q / quads, c = 4 * (q - row * quads);
     if (c >= a.n) continue;
     int64_t sum[4] = {};
@@ -513,31 +533,51 @@ __global__ __launch_bounds__(256) void join_slices_kernel(JoinArgs a) {
   }
 }
 
-template <int TM, int TN, int WN, int kMinBlocks, bool kInner>
-hipError_t launch_cfg(TileArgs a, const TileShape& shape, hipStream_t stream) {
-  using Cf = Cfg<TM, TN, WN, kInner>;
+__global__ __launch_bounds__(256) void join_slices_kernel(JoinPair p) {
+  const bool second = blockIdx.x >= p.blocks;
+  const JoinArgs& a = p.product[second ? 1 : 0];
+  const uint32_t block = second ? blockIdx.x - p.blocks : blockIdx.x;
+  const uint32_t blocks = second ? gridDim.x - p.blocks : p.blocks;
+  if (a.dtype == RNS8_MI355X_F32)
+    join_slices<float>(a, block, blocks);
+  else if (a.dtype == RNS8_MI355X_F16)
+    join_slices<f16>(a, block, blocks);
+  else
+    join_slices<bf16>(a, block, blocks);
+}
+
+// The product's tiles and units; the workgroups it takes (0: too many units).
+template <typename Cf, int kMinBlocks>
+uint32_t split_units(TileArgs& a, uint32_t slices) {
   const uint32_t tiles_m = (a.m + Cf::BM - 1) / Cf::BM, tiles_n = (a.n + Cf::BN - 1) / Cf::BN;
-  const uint64_t tiles = static_cast<uint64_t>(tiles_m) * tiles_n, units = tiles * shape.slices;
-  if (units == 0 || units > 0x7FFFFFFFull) return hipErrorInvalidValue;
+  const uint64_t tiles = static_cast<uint64_t>(tiles_m) * tiles_n, units = tiles * slices;
+  if (units == 0 || units > 0x7FFFFFFFull) return 0;
   a.units = static_cast<uint32_t>(units);
   a.tiles_m = tiles_m;
   a.tiles = make_div_u31(static_cast<uint32_t>(tiles));
   a.group = make_div_u31(static_cast<uint32_t>(Cf::kGroupM) * tiles_n);
   a.rows = make_div_u31(Cf::kGroupM);
   a.tail = make_div_u31(tiles_m - (tiles_m - 1) / Cf::kGroupM * Cf::kGroupM);
-  const uint64_t grid = persistent_grid(units, static_cast<uint64_t>(device_cu_count()) * kMinBlocks);
-  hipLaunchKernelGGL((scaled_tiles_kernel<Cf, kMinBlocks>), dim3(static_cast<unsigned>(grid)), dim3(Cf::kThreads), 0,
-                     stream, a);
+  return static_cast<uint32_t>(persistent_grid(units, static_cast<uint64_t>(device_cu_count()) * kMinBlocks));
+}
+
+template <int TM, int TN, int WN, int kMinBlocks, bool kInner>
+hipError_t launch_cfg(TilePair p, const uint32_t* slices, int count, hipStream_t stream) {
+  using Cf = Cfg<TM, TN, WN, kInner>;
+  p.blocks = split_units<Cf, kMinBlocks>(p.product[0], slices[0]);
+  const uint32_t more = count > 1 ? split_units<Cf, kMinBlocks>(p.product[1], slices[1]) : 0;
+  if (p.blocks == 0 || (count > 1 && more == 0)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((scaled_tiles_kernel<Cf, kMinBlocks>), dim3(p.blocks + more), dim3(Cf::kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
 template <bool kInner>
-hipError_t launch_tile(const TileArgs& a, const TileShape& s, hipStream_t stream) {
-  if (s.bm == 256 && s.bn == 256) return launch_cfg<8, 8, 2, 1, kInner>(a, s, stream);
-  if (s.bm == 256 && s.bn == 128) return launch_cfg<8, 4, 2, 1, kInner>(a, s, stream);
-  if (s.bm == 128 && s.bn == 256) return launch_cfg<4, 8, 2, 1, kInner>(a, s, stream);
-  if (s.bm == 128 && s.bn == 128) return launch_cfg<4, 4, 2, 2, kInner>(a, s, stream);
-  if (s.bm == 64 && s.bn == 64) return launch_cfg<2, 4, 1, 4, kInner>(a, s, stream);
+hipError_t launch_tile(const TilePair& p, const TileShape& s, const uint32_t* slices, int count, hipStream_t stream) {
+  if (s.bm == 256 && s.bn == 256) return launch_cfg<8, 8, 2, 1, kInner>(p, slices, count, stream);
+  if (s.bm == 256 && s.bn == 128) return launch_cfg<8, 4, 2, 1, kInner>(p, slices, count, stream);
+  if (s.bm == 128 && s.bn == 256) return launch_cfg<4, 8, 2, 1, kInner>(p, slices, count, stream);
+  if (s.bm == 128 && s.bn == 128) return launch_cfg<4, 4, 2, 2, kInner>(p, slices, count, stream);
+  if (s.bm == 64 && s.bn == 64) return launch_cfg<2, 4, 1, 4, kInner>(p, slices, count, stream);
   return hipErrorInvalidValue;
 }
 
@@ -572,53 +612,87 @@ double tile_cost(const TileCost& c, int64_t m, int64_t n, int64_t k, double unit
 
 }  // namespace
 
-TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k) {
-  TileShape best{};
+namespace {
+
+// The best cut of a product into this kind of tile, if it beats `best`.
+void choose_slices(const TileCost& c, int64_t m, int64_t n, int64_t k, TileShape& best) {
   const int64_t need = std::max<int64_t>(1, (k + kExactK - 1) / kExactK);
-  for (const TileCost& c : kTileCosts) {
-    const double tiles = static_cast<double>((m + c.bm - 1) / c.bm) * static_cast<double>((n + c.bn - 1) / c.bn);
-    for (const int64_t wanted : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      int64_t s = std::max(wanted, need);
-      if (s > 1 && k < 256 * s) continue;  // slices of two chunks at least
-      int64_t k_slice = k;
-      if (s > 1) {
-        k_slice = ((k + s - 1) / s + 127) / 128 * 128;
-        k_slice = std::min<int64_t>(k_slice, kExactK / 128 * 128);
-        s = (k + k_slice - 1) / k_slice;
-      }
-      const double units = tiles * static_cast<double>(s);
-      if (units > 0x7FFFFFFF) continue;
-      double cost = tile_cost(c, m, n, k, units, k_slice);
-      // the join: a launch, and the partial sums written and read
-      if (s > 1)
-        cost += 2.2 + 0.03 * static_cast<double>(s) +
-                static_cast<double>(s) * static_cast<double>(m) * static_cast<double>(n) * 8 / 4e6;
-      if (best.cost != 0 && cost >= best.cost) continue;
-      best.cost = cost;
-      best.bm = c.bm;
-      best.bn = c.bn;
-      best.slices = static_cast<uint32_t>(s);
-      best.k_slice = k_slice;
+  const double tiles = static_cast<double>((m + c.bm - 1) / c.bm) * static_cast<double>((n + c.bn - 1) / c.bn);
+  for (const int64_t wanted : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    int64_t s = std::max(wanted, need);
+    if (s > 1 && k < 256 * s) continue;  // slices of two chunks at least
+    int64_t k_slice = k;
+    if (s > 1) {
+      k_slice = ((k + s - 1) / s + 127) / 128 * 128;
+      k_slice = std::min<int64_t>(k_slice, kExactK / 128 * 128);
+      s = (k + k_slice - 1) / k_slice;
     }
+    const double units = tiles * static_cast<double>(s);
+    if (units > 0x7FFFFFFF) continue;
+    double cost = tile_cost(c, m, n, k, units, k_slice);
+    // the join: a launch, and the partial sums written and read
+    if (s > 1)
+      cost += 2.2 + 0.03 * static_cast<double>(s) +
+              static_cast<double>(s) * static_cast<double>(m) * static_cast<double>(n) * 8 / 4e6;
+    if (best.cost != 0 && cost >= best.cost) continue;
+    best.cost = cost;
+    best.bm = c.bm;
+    best.bn = c.bn;
+    best.slices = static_cast<uint32_t>(s);
+    best.k_slice = k_slice;
   }
   best.ldp = (n + 3) / 4 * 4;
   best.bytes = best.slices > 1 ? static_cast<uint64_t>(best.slices) * static_cast<uint64_t>(m) *
                                      static_cast<uint64_t>(best.ldp) * sizeof(int32_t)
                                : 0u;
+}
+
+}  // namespace
+
+TileShape choose_tile_shape(int64_t m, int64_t n, int64_t k) {
+  TileShape best{};
+  for (const TileCost& c : kTileCosts) choose_slices(c, m, n, k, best);
   return best;
 }
 
-hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int32_t* partials, hipStream_t stream) {
+// In one launch where that is predicted to take less than two: products that fit
+// on the chip together take as long as the longer one, others save a start.
+bool choose_pair_shapes(const int64_t (&m)[2], const int64_t (&n)[2], const int64_t (&k)[2], TileShape (&shapes)[2]) {
+  for (int i = 0; i < 2; ++i) shapes[i] = choose_tile_shape(m[i], n[i], k[i]);
+  double least = shapes[0].cost + shapes[1].cost;
+  bool one = false;
+  for (const TileCost& c : kTileCosts) {
+    TileShape s[2]{};
+    double units = 0;
+    for (int i = 0; i < 2; ++i) {
+      choose_slices(c, m[i], n[i], k[i], s[i]);
+      units += static_cast<double>((m[i] + c.bm - 1) / c.bm) * static_cast<double>((n[i] + c.bn - 1) / c.bn) * s[i].slices;
+    }
+    if (s[0].cost == 0 || s[1].cost == 0) continue;
+    const double together = units <= 256.0 * c.resident ? std::max(s[0].cost, s[1].cost) : s[0].cost + s[1].cost - c.start / 2;
+    if (together >= least) continue;
+    least = together;
+    one = true;
+    shapes[0] = s[0];
+    shapes[1] = s[1];
+  }
+  return one;
+}
+
+namespace {
+
+// The kernel's arguments, if it can take the product.
+bool tile_args(const ScaledGemm& g, const TileShape& shape, int32_t* partials, TileArgs& a) {
   const int64_t limit = int64_t{1} << 23;
   if (g.m <= 0 || g.n <= 0 || g.k < 0 || g.lda % 16 || g.ldb % 16 || g.lda >= limit || g.ldb >= limit ||
       reinterpret_cast<uintptr_t>(g.a) % 16 || reinterpret_cast<uintptr_t>(g.b) % 16 || g.m > 0x7FFFFFFF ||
-      g.n > 0x7FFFFFFF - 256 || g.k > 0x7FFFFFFF - 256)
-    return hipErrorInvalidValue;
+      g.n > 0x7FFFFFFF - 256 || g.k > 0x7FFFFFFF - 256 || g.dtype > RNS8_MI355X_BF16)
+    return false;
   const int64_t k16 = (g.k + 15) / 16 * 16;
-  if (g.lda < k16 || (g.inner ? g.ldb < (g.n + 15) / 16 * 16 : g.ldb < k16)) return hipErrorInvalidValue;
+  if (g.lda < k16 || (g.inner ? g.ldb < (g.n + 15) / 16 * 16 : g.ldb < k16)) return false;
   if (shape.slices == 0 || shape.k_slice > kExactK || (shape.slices > 1 && (!partials || shape.k_slice % 128)))
-    return hipErrorInvalidValue;
-  TileArgs a{};
+    return false;
+  a = TileArgs{};
   a.a = g.a;
   a.b = g.b;
   a.a_scale = g.a_scale;
@@ -637,17 +711,32 @@ hipError_t launch_scaled_tiles(const ScaledGemm& g, const TileShape& shape, int3
   a.dtype = g.dtype;
   a.k_slice = static_cast<uint32_t>(shape.slices > 1 ? shape.k_slice : k16);
   a.pairs = static_cast<uint32_t>(std::max<int64_t>(1, (a.k_slice + 127) / 128));
-  hipError_t e = g.inner ? launch_tile<true>(a, shape, stream) : launch_tile<false>(a, shape, stream);
-  if (e != hipSuccess || shape.slices == 1) return e;
-  const JoinArgs j{partials, shape.slices, g.m, g.n, shape.ldp, g.ldo, g.a_scale, g.b_scale, g.bias, g.out};
-  const int64_t blocks = (g.m * (shape.ldp / 4) + 255) / 256;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)));
-  switch (g.dtype) {
-    case RNS8_MI355X_F32: hipLaunchKernelGGL(join_slices_kernel<float>, grid, dim3(256), 0, stream, j); break;
-    case RNS8_MI355X_F16: hipLaunchKernelGGL(join_slices_kernel<f16>, grid, dim3(256), 0, stream, j); break;
-    case RNS8_MI355X_BF16: hipLaunchKernelGGL(join_slices_kernel<bf16>, grid, dim3(256), 0, stream, j); break;
-    default: return hipErrorInvalidValue;
+  return true;
+}
+
+}  // namespace
+
+hipError_t launch_scaled_tiles(const ScaledGemm* g, const TileShape* shapes, int32_t* const* partials, int count,
+                               hipStream_t stream) {
+  TilePair p{};
+  JoinPair j{};
+  uint32_t slices[2] = {}, join_blocks[2] = {};
+  int joins = 0;
+  for (int i = 0; i < count; ++i) {
+    if (g[i].inner != g[0].inner || (i > 0 && !g[i].inner) || shapes[i].bm != shapes[0].bm || shapes[i].bn != shapes[0].bn ||
+        !tile_args(g[i], shapes[i], partials[i], p.product[i]))
+      return hipErrorInvalidValue;
+    slices[i] = shapes[i].slices;
+    if (slices[i] == 1) continue;
+    j.product[joins] = {partials[i], slices[i], g[i].m, g[i].n, shapes[i].ldp, g[i].ldo, g[i].a_scale, g[i].b_scale,
+                        g[i].bias, g[i].out, g[i].dtype};
+    join_blocks[joins++] = static_cast<uint32_t>(std::min<int64_t>((g[i].m * (shapes[i].ldp / 4) + 255) / 256, 1 << 20));
   }
+  const hipError_t e = g[0].inner ? launch_tile<true>(p, shapes[0], slices, count, stream)
+                                  : launch_tile<false>(p, shapes[0], slices, count, stream);
+  if (e != hipSuccess || joins == 0) return e;
+  j.blocks = join_blocks[0];
+  hipLaunchKernelGGL(join_slices_kernel, dim3(join_blocks[0] + join_blocks[1]), dim3(256), 0, stream, j);
   return hipGetLastError();
 }
 
