@@ -12,7 +12,10 @@
 // lowest (masks) take v - m first instead, where c m would overflow. 32 bits
 // hold every sum. Both kernels are bound by reading the logits (and writing
 // their gradient): a logit costs about ten vector operations, the exponential
-// counted as four, and the next loads are in flight beside them.
+// counted as four, and the next loads are in flight beside them. bf16, 4096 x 32768
+// 50 us (5.3 TB/s) and the gradient 84 (6.4 TB/s); f32, 1000 x 50001 with 5
+// alternatives 43 us (4.6 TB/s); 4 x 131072 with 20 alternatives 7.5 and 4.9 for the
+// join.
 //
 // Few long rows are cut into parts of 4096 logits or more, one workgroup each, whose
 // sums and alternatives a second kernel joins: 4 rows of 131072 would occupy 4 of

@@ -8,10 +8,14 @@
 //     l % 16 at 16 (l / 16) of each 64 of K (16 rows x 64 bytes to a load), at any
 //     alignment. The next group's loads are issued before a group is multiplied.
 //   * a (in 8 bits) is small and read the same way, from the caches; 32 channels
-//     to a wave halve that traffic where there are more than 16 tokens.
+//     to a wave halve that traffic where there are more than 16 tokens, and the
+//     linear layer then stores its rows in fragment order, whole cache lines to a
+//     load.
 //   * One or two tokens of a linear layer are quantized here, by every workgroup
 //     into its LDS, while its first weights are on their way: less than the launch
 //     of a kernel of its own.
+// Measured: one token (bf16, quantized here) by 8192 x 8192 16.3 us with its launch
+// (67 MB: 4.1 TB/s); 48 tokens by 8192 x 4096 in fragment order 10.4 us.
 #include <algorithm>
 #include <type_traits>
 

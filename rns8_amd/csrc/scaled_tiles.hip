@@ -19,6 +19,10 @@
 //   * Few tiles: K is cut into slices whose int32 sums go to a workspace; a
 //     second kernel adds them in 64 bits and runs the epilogue. The result does
 //     not depend on the cut.
+//   * Both gradients of a linear layer run in one launch (TilePair).
+// Measured (bf16 outputs): 8192^3 405 us (2.7 POP/s, 0.61 of the cycles in MFMA),
+// 4096^3 64 us (2.1 POP/s: one tile to a CU, its start and epilogue 11 us of it),
+// 1000 x 1101 x 903 9.5 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
