@@ -8,9 +8,9 @@
 // S and W are kept for a running maximum: when c m rises by t, S becomes S 2^-t
 // and W becomes (W - t S) 2^-t, so one pass over the row is enough. d is one
 // fused multiply-add against the rounded c m, which is what lse starts from, so
-// its error goes with its own size; rows of nothing but values near the type's
-// lowest (masks) take v - m first instead, where c m would overflow. 32 bits
-// hold every sum. Both kernels are bound by reading the logits (and writing
+// its error goes with its own size; where c m is so large that its rounding alone
+// would be an exponent of its own (rows of nothing but a mask's value), v - m comes
+// first instead. 32 bits hold every sum. Both kernels are bound by reading the logits (and writing
 // their gradient): a logit costs about ten vector operations, the exponential
 // counted as four, and the next loads are in flight beside them. bf16, 4096 x 32768
 // 50 us (5.3 TB/s) and the gradient 84 (6.4 TB/s); f32, 1000 x 50001 with 5
@@ -57,19 +57,24 @@ struct Sums {
 
 __device__ __forceinline__ bool is_empty(Sums t) { return t.m == -INFINITY && t.s == 0.0f; }
 
-// d for a logit against the maximum m: c v - c m. Below kLow c m may overflow:
-// the difference comes first there (m = -infinity: nothing but ruled-out tokens,
-// d = -infinity).
-constexpr float kLow = -1e37f;
+// d for a logit against the maximum m: c v - c m. Up to kFused the rounding of c m
+// moves d by 2^-5 at most; beyond it that grows past any exponent (2^8 at 1e10),
+// and c m may overflow: the difference comes first there, and the sums start from
+// c m itself (m = -infinity: nothing but ruled-out tokens, d = -infinity).
+constexpr float kFused = 0x1p20f;
+__device__ __forceinline__ bool is_fused(float m, float c) { return fabsf(m * c) < kFused; }
 __device__ __forceinline__ float exponent(float v, float m, float c) {
-  if (m > kLow) return fmaf(v, c, -(m * c));
+  if (is_fused(m, c)) return fmaf(v, c, -(m * c));
   return m == -INFINITY ? v : (v - m) * c;
 }
 
 // `a` for a maximum m >= a.m.
 __device__ __forceinline__ Sums rescale(Sums a, float m, float c) {
   if (a.m == m || a.m == -INFINITY) return {m, a.s, a.w};
-  const float t = a.m > kLow ? a.m * c - m * c : (a.m - m) * c, e = exp2_fast(t);
+  const bool to_fused = is_fused(m, c);
+  const float t = is_fused(a.m, c) ? (to_fused ? a.m * c - m * c : fmaf(-m, c, a.m * c))
+                                   : (to_fused ? fmaf(a.m, c, -(m * c)) : (a.m - m) * c);
+  const float e = exp2_fast(t);
   // (sums that the maximum has left behind by more than floats hold: t s may be infinite)
   return {m, a.s * e, e > 0.0f ? (a.w + t * a.s) * e : 0.0f};
 }
@@ -105,7 +110,7 @@ __device__ __forceinline__ Sums join_waves(const Sums* wave_sums, float c) {
 }
 
 // Adds kCount logits. The decisions are the wave's, so that none of them costs
-// more than a compare and a branch: a new maximum, a maximum below kLow, and
+// more than a compare and a branch: a new maximum, a maximum past kFused, and
 // ruled-out tokens, whose 2^d d is 0 times infinity: the chunk's own W is then
 // NaN, its terms are taken again with d held above -200 (2^-200 is 0 in 32 bits,
 // and so is its term), and so are those of the wave's later chunks at once
@@ -118,7 +123,7 @@ __device__ __forceinline__ void add_logits(Sums& t, const float (&v)[kCount], fl
   if (__any(m > t.m)) t = rescale(t, m, c);
   const float base = -(m * c);
   float s[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};  // two chains of additions
-  if (__any(!(m > kLow))) {
+  if (__any(!(fabsf(base) < kFused))) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
       const float d = exponent(v[i], m, c), e = exp2_fast(d);
@@ -198,7 +203,7 @@ struct Args {
 };
 
 __device__ __forceinline__ float lse_of(Sums t, float scale, float c, float log_s) {
-  return t.m > kLow ? kLn2 * (t.m * c + log_s) : t.m == -INFINITY ? kLn2 * log_s : t.m * scale + kLn2 * log_s;
+  return is_fused(t.m, c) ? kLn2 * (t.m * c + log_s) : t.m == -INFINITY ? kLn2 * log_s : t.m * scale + kLn2 * log_s;
 }
 
 // The log-probability of a logit.
@@ -527,7 +532,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
       __syncthreads();
       from = t.m == -INFINITY ? 0.0f : t.m;
       // (the sums' origin is the rounded c m; here it is m itself)
-      const float off = t.m > kLow ? fmaf(t.m, a.c, -(t.m * a.c)) : 0.0f;
+      const float off = is_fused(t.m, a.c) ? fmaf(t.m, a.c, -(t.m * a.c)) : 0.0f;
       log_s = is_empty(t) ? 0.0f : kLn2 * (log2f(t.s) - off);
     }
     auto grad = [&](int64_t at, float (&v)[kVector]) {

@@ -298,3 +298,59 @@ def test_refusals(gpu_ctx):
         assert e.value.status == r.abi.INVALID_ARGUMENT, kwargs
     with pytest.raises(r.Rns8Error):
         ops.TokenLogprobsBackward(gpu_ctx, logits=v, lse=f, dlogits=v)()
+
+
+# masks' values and scales for which scale * value lies on both sides of 2^20 / log2(e), up to the type's limits
+LARGE = [(-1e5, 1.0), (-7e5, 1.0), (-7.5e5, 1.0), (-1e6, 1.0), (-1e9, 1.0), (-1e10, 0.7), (-1e20, 1.0), (-1e36, 1000.0),
+         (3e5, 1.0), (1e10, 1.0), (3e38, 1.0), (3e38, 0.5), (-3e4, 40.0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value,scale", LARGE)
+@pytest.mark.parametrize("vocab", [700, 70000])
+def test_rows_of_one_large_value(gpu_ctx, dtype, value, scale, vocab):
+    """Equal logits spread evenly however large they are; one that stands out by 2^-4 of the value takes everything.
+
+    Differences of equal numbers are exact, so the logarithm of vocab (below 12, log2 below 17) is off by the sum's
+    and the logarithm's few steps alone; lse has six roundings of |z| (scale's own among them)."""
+    v = torch.full((3, vocab), value, device="cuda").to(dtype)
+    v[1, vocab - 3] = value * (1 - 2.0 ** -4) if value < 0 else value
+    if value > 0:
+        v[1, :vocab - 3], v[1, vocab - 2:] = value * (1 - 2.0 ** -4), -value
+    v[2, ::2] = -float("inf")
+    targets = torch.tensor([7, vocab - 3, 1], device="cuda")
+    fwd = run(gpu_ctx, v, targets, scale, 3)
+    n = torch.log(torch.tensor([vocab, 1.0, vocab / 2], dtype=torch.float64))
+    assert_close(fwd["logp"].cpu(), -n, 128 * U32, "logp")
+    assert_close(fwd["entropy"].cpu(), n, 128 * U32, "entropy")
+    z = v.double().amax(1).cpu() * scale
+    fits = z.abs() < 3.4e38
+    assert ((fwd["lse"].cpu().double() - z - n).abs() <= 8 * U32 * z.abs() + 128 * U32)[fits].all()
+    assert fwd["top_ids"].tolist() == [[0, 1, 2], [vocab - 3, 0, 1], [1, 3, 5]]
+    assert (fwd["top_logp"][:, 0].cpu().double() + n).abs().max() <= 128 * U32
+    if not fits.all():
+        return
+    ones, d = torch.ones(3, device="cuda"), torch.empty_like(v)
+    ops.TokenLogprobsBackward(gpu_ctx, logits=v, lse=fwd["lse"], entropy=fwd["entropy"], targets=targets, dlogp=ones,
+                              dentropy=ones, dlogits=d, scale=scale)()
+    ready()
+    want = torch.zeros(3, vocab, dtype=torch.float64, device="cuda")
+    want[0], want[2, 1::2] = -scale / vocab, -2 * scale / vocab
+    want[0, 7] += scale
+    want[2, 1] += scale
+    p = torch.zeros_like(want)
+    p[0], p[1, vocab - 3], p[2, 1::2] = 1 / vocab, 1.0, 2 / vocab
+    # log p, entropy and p itself, each off as above
+    assert_close(d, want, 3 * 128 * U32 * scale * p + U32 * want.abs(), "dlogits")
+
+
+def test_maxima_that_rise_past_the_fused_range(gpu_ctx):
+    """Logits that rise from -1e10 to 1e10 along a row: each part's sums follow maxima of every size."""
+    up = torch.logspace(0, 10, 4500, device="cuda", dtype=torch.float64).float()
+    v = torch.cat((-up.flip(0), up, up[-1:]))[None].repeat(2, 1)
+    v[1] = v[1].flip(0)
+    top = torch.tensor([9000, 1], device="cuda")
+    fwd = run(gpu_ctx, v, top, 1.0, 3)
+    assert (fwd["logp"].double() + torch.log(torch.tensor(2.0))).abs().max() <= 128 * U32
+    assert (fwd["entropy"].double() - torch.log(torch.tensor(2.0))).abs().max() <= 128 * U32
+    assert fwd["top_ids"].tolist() == [[8999, 9000, 8998], [0, 1, 2]]
