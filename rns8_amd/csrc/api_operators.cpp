@@ -90,6 +90,13 @@ struct LinearParts {
   uint64_t bytes = 0;
 };
 
+// Which way a call goes, for its workspace and for its launches alike: no
+// outputs and no rows to keep, one kernel for all of it, or the parts below.
+bool linear_is_empty(const rns8_mi355x_linear_i8_args& a) { return a.m == 0 || (a.n == 0 && !a.x_q); }
+bool linear_in_one_kernel(const rns8_mi355x_linear_i8_args& a) {
+  return a.m > 0 && a.n > 0 && linear_rows_takes(a.m, a.n, a.k);
+}
+
 // Quantized rows that a product may read whole 16-byte chunks of.
 int64_t padded_row(int64_t cols) { return static_cast<int64_t>(round_up(static_cast<uint64_t>(cols), 16)); }
 
@@ -379,7 +386,7 @@ rns8_status no_workspace(const A&) {
 }
 
 uint64_t linear_bytes(rns8_mi355x_linear_i8_args a) {
-  if (linear_rows_takes(a.m, a.n, a.k)) return 0;
+  if (linear_is_empty(a) || linear_in_one_kernel(a)) return 0;
   a.workspace = nullptr;
   LinearParts p;
   linear_parts(a, p);
@@ -442,7 +449,8 @@ rns8_status rns8_mi355x_linear_i8(rns8_context* ctx, const rns8_mi355x_linear_i8
         return check_workspace(a.workspace, a.workspace_bytes, linear_bytes(a));
       },
       [](const rns8_mi355x_linear_i8_args& a, hipStream_t s) {
-        if (a.m > 0 && a.n > 0 && linear_rows_takes(a.m, a.n, a.k)) return launch_linear_rows(a, s);
+        if (linear_is_empty(a)) return hipSuccess;
+        if (linear_in_one_kernel(a)) return launch_linear_rows(a, s);
         LinearParts p;
         linear_parts(a, p);
         if (p.fragments) {
