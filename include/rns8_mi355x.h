@@ -11,7 +11,9 @@
  *
  * Conventions
  *   - `stream` is a hipStream_t passed as void*; NULL selects the context's
- *     own stream. Work is ordered on that stream only.
+ *     own stream, which waits for no other. Work is ordered on that stream
+ *     only. The device's default stream, whose handle is NULL elsewhere, is
+ *     RNS8_MI355X_DEFAULT_STREAM here (hipStreamLegacy's value).
  *   - Device pointers must be accessible from the context's device.
  *   - Range violations are reported through `d_status`: a device uint32_t
  *     that the caller zeroes before the call; the export kernel sets it
@@ -29,6 +31,8 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+#define RNS8_MI355X_DEFAULT_STREAM ((void*)1)
 
 /* Prefix a plan created from `desc` would select (validation and prefix
  * selection of rns8_create_plan, reference api_plan_public_api.inc:3-73 and

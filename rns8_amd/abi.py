@@ -397,6 +397,7 @@ B_CHANNELS = 0
 B_INNER = 1
 NORM_POST = 1
 NORM_PRE = 2
+DEFAULT_STREAM = 1  # as a stream's handle: the device's default stream
 
 
 class QuantizeArgs(C.Structure):

@@ -311,6 +311,7 @@ void free_device(void* p) {
 }
 
 hipStream_t pick_stream(const rns8_context& ctx, void* stream) {
+  if (stream == RNS8_MI355X_DEFAULT_STREAM) return nullptr;
   return stream ? static_cast<hipStream_t>(stream) : ctx.stream;
 }
 

@@ -15,11 +15,11 @@ Operands are tensors in device memory: any objects with torch's data_ptr(),
 shape, stride(), dtype and is_cuda. Rows may be strided; the elements of a row
 are next to each other. A torch.cuda.Stream is passed as its cuda_stream (in a
 process that imports torch before this library is loaded: both then share one
-HIP runtime). Torch's default stream has the handle 0, which this library reads
-as the context's own stream; that one does not wait for torch's, so a program on
-the default stream synchronizes between the two. A workspace is allocated when
-the object is made, unless one is given, and the object must outlive its calls
-on the GPU.
+HIP runtime). Torch's default stream has the handle 0: it runs the operator on
+that stream, in order with torch's work there. The context's own stream waits for
+no other, so a program that leaves the stream out synchronizes between the two. A
+workspace is allocated when the object is made, unless one is given, and the
+object must outlive its calls on the GPU.
 """
 from __future__ import annotations
 
@@ -119,7 +119,8 @@ class _Call:
                 self.args.workspace, self.args.workspace_bytes = self._own, need.value
 
     def __call__(self, stream: int | None = None) -> None:
-        status = self._fn(self.ctx.ptr, self._ref, stream)
+        # (the C interface reads a handle of 0 as none)
+        status = self._fn(self.ctx.ptr, self._ref, abi.DEFAULT_STREAM if stream == 0 else stream)
         if status:
             check(status, self._entry)
 

@@ -33,3 +33,26 @@ def test_a_layer_without_channels(gpu_ctx, m, k, keep):
     if keep:
         q, s = quantize(x.float(), 1)
         assert torch.equal(kept.t[:, :k], q) and torch.equal(scale, s) and kept.untouched()
+
+
+def test_on_the_default_stream(gpu_ctx):
+    """The handle that torch gives for its default stream: behind torch's work there, and before what follows."""
+    if len({line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line}) != 1:
+        pytest.skip("torch was loaded after the library: two HIP runtimes, whose streams differ")
+    handle = torch.cuda.current_stream().cuda_stream
+    assert handle == 0
+    big = torch.randn(8192, 8192, device="cuda")
+    x, scale = torch.zeros(300, 512, device="cuda"), torch.zeros(300, device="cuda")
+    call = ops.QuantizeRows(gpu_ctx, x=x, q=torch.empty(300, 512, dtype=torch.int8, device="cuda"), scale=scale)
+    big @ big
+    ready()
+    got = []
+    for value in (3.0, 5.0, 7.0):
+        for _ in range(4):  # some milliseconds
+            big @ big
+        x.fill_(value)
+        call(handle)
+        got.append(scale.clone())
+    ready()
+    for value, scale in zip((3.0, 5.0, 7.0), got):
+        assert torch.equal(scale, torch.full_like(scale, value) / torch.full_like(scale, 127.0))

@@ -76,3 +76,22 @@ def test_a_layer_without_channels(enqueued, m, k):
 def test_a_layer_without_tokens(enqueued, n, keep):
     (got,) = enqueued("linear_i8", linear(0, n, 64, keep))
     assert got[:4] == (abi.SUCCESS, 0, abi.SUCCESS, 0)
+
+
+def test_streams(enqueued):
+    """No stream is the context's own (4096 here), the default stream's name is the default stream."""
+    calls = [linear(300, 500, 64, stream=s) for s in (0, abi.DEFAULT_STREAM, 8192)]
+    assert [a.stream for a in enqueued("linear_i8", *calls)] == [4096, 0, 8192]
+
+
+def test_python_handles(monkeypatch):
+    """A call without a stream names none; a handle of 0 is the default stream's."""
+    from rns8_amd import operators
+
+    seen = []
+    call = object.__new__(operators.QuantizeRows)
+    call.ctx = type("Context", (), {"ptr": None})()
+    call._ref = None
+    call._fn = lambda ctx, args, stream: seen.append(stream) or abi.SUCCESS
+    call(), call(None), call(0), call(8192)
+    assert seen == [None, None, abi.DEFAULT_STREAM, 8192]
