@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from operator_cases import Guarded, quantize
+from operator_cases import U32, Guarded, assert_close, quantize
 from rns8_amd import operators as ops
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +56,48 @@ def test_on_the_default_stream(gpu_ctx):
     ready()
     for value, scale in zip((3.0, 5.0, 7.0), got):
         assert torch.equal(scale, torch.full_like(scale, value) / torch.full_like(scale, 127.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset,scale", [(0, 1.0), (50, 1.0), (100, 1.0), (1000, 1.0), (-1000, 0.5), (2000, 2.0),
+                                          (4000, 1.0), (-4000, 1.0), (100000, 1.0)])
+@pytest.mark.parametrize("rows,vocab", [(40, 1000), (3, 50001)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_gradient_of_logits_on_a_common_offset(gpu_ctx, dtype, offset, scale, rows, vocab, in_place):
+    """An offset that all logits of a row share changes no probability, so it is no excuse for an error.
+
+    With D = max |z - max z| and L = max -log p of a row, an exponential's argument is off by 2^-24 (4 (D + L)), lse by
+    32 of these units at most where the row is not summed again (|lse| <= 64), the sum and its logarithm by 512."""
+    v = (2.5 / scale * normal(rows, rows, vocab) + offset / scale).to(dtype)
+    v[:, 7] = v.amax(1) + 1 / scale
+    targets = torch.arange(rows, device="cuda")
+    targets[1] = 7
+    gl, ge = normal(3, rows), normal(4, rows)
+    out = {k: torch.empty(rows, device="cuda") for k in ("logp", "entropy", "lse")}
+    d, e_ = v.clone(), v.clone()
+    ready()
+    ops.TokenLogprobs(gpu_ctx, logits=v, targets=targets, scale=scale, **out)()
+    more = dict(lse=out["lse"], scale=scale)
+    ops.TokenLogprobsBackward(gpu_ctx, logits=d if in_place else v, targets=targets, dlogp=gl, dlogits=d, **more)()
+    ops.TokenLogprobsBackward(gpu_ctx, logits=e_ if in_place else v, entropy=out["entropy"], dentropy=ge, dlogits=e_,
+                              **more)()
+    ready()
+    z = v.double() * float(torch.tensor(scale))
+    logp = torch.log_softmax(z, 1)
+    p = logp.exp()
+    entropy = -(p * logp).sum(1)
+    size = (z.amax(1) - z.amin(1))[:, None]
+    off = U32 * (4 * (size - logp.amin(1, keepdim=True)) + 32 + 512)
+    given = logp.gather(1, targets[:, None])[:, 0]
+    assert_close(out["logp"], given, off[:, 0], "logp")
+    assert_close(out["entropy"], entropy, (2 * off * (1 + size))[:, 0], "entropy")
+    want = -scale * gl.double()[:, None] * p
+    slack = off * want.abs()
+    hit = torch.zeros_like(p).scatter_(1, targets[:, None], 1.0)
+    want, slack = want + scale * gl.double()[:, None] * hit, slack + 2 * U32 * scale * gl.double().abs()[:, None] * hit
+    assert_close(d, want, slack, "dlogits of logp")
+    terms = scale * ge.double().abs()[:, None] * p
+    want = -scale * ge.double()[:, None] * p * (logp + entropy[:, None])
+    assert_close(e_, want, terms * (off * (logp.abs() + entropy[:, None]) + 2 * off * (2 + size)), "dlogits of entropy")
+    if dtype == torch.float32:  # what the target gains the others lose
+        assert (d.double().sum(1).abs() <= scale * gl.double().abs() * (off[:, 0] + 4 * U32)).all()
