@@ -349,7 +349,8 @@ RNS8_API rns8_status rns8_mi355x_quantize_columns_workspace(const rns8_mi355x_qu
  * 32 bits, so a row of out is the same whatever other rows a call has. b is stored n x k (RNS8_MI355X_B_CHANNELS: one row for each output
  * channel, the usual layout of weights) or k x n (RNS8_MI355X_B_INNER). Any of
  * a_scale, b_scale (1) and bias (0) may be NULL. m, n >= 0, k >= 0 (an empty
- * sum is zero); m, n and k below 2^31, lda and ldb below 2^23. Products of more
+ * sum is zero); m below 2^31, n below 2^31 - 256, k (and n where b is k x n) at
+ * most 2^23 - 16, lda and ldb below 2^23. Products of more
  * than 64 rows read operands in place whose pointers and strides are multiples
  * of 16 and copy others into the workspace first, and one of the two where b is
  * n x k and k is no multiple of 16. Products of fewer rows may read in place
@@ -387,7 +388,7 @@ RNS8_API rns8_status rns8_mi355x_gemm_i8_scaled_workspace(const rns8_mi355x_gemm
  *   out[i][j] = x_scale[i] * w_scale[j] * sum_k q[i][k] w[j][k] + bias[j].
  * x_q (m x k at stride ldq, zeros after each row as there) and x_scale[m] receive
  * the quantized rows if given (both or neither): what the backward pass reads.
- * k >= 1; k below 2^23 - 16, ldw and ldq below 2^23. */
+ * k >= 1; n below 2^31 - 256, k below 2^23 - 16, ldw and ldq below 2^23. */
 typedef struct rns8_mi355x_linear_i8_args {
   uint64_t struct_size;
   uint32_t abi_version;
@@ -421,8 +422,8 @@ RNS8_API rns8_status rns8_mi355x_linear_i8_workspace(const rns8_mi355x_linear_i8
  *   dbias[j] = sum_i dy[i][j].
  * dw is the gradient of the weights w * w_scale. dx, dw and dbias may each be
  * NULL (not all three); x_q and x_scale may be NULL without dw, w and w_scale
- * without dx. With dx n, and with dw or dbias m, stays below 2^23 - 16; ldq and ldw
- * below 2^23. */
+ * without dx. With dx n, and with dw or dbias m, stays below 2^23 - 16, and with dx
+ * or dw k at most that; ldq and ldw below 2^23. */
 typedef struct rns8_mi355x_linear_i8_backward_args {
   uint64_t struct_size;
   uint32_t abi_version;

@@ -74,7 +74,8 @@ rns8_status check_gemm(const rns8_mi355x_gemm_i8_args& a) {
   if ((a.a_scale && !floats_ok(a.a_scale, a.m)) || (a.b_scale && !floats_ok(a.b_scale, a.n)) ||
       (a.bias && !floats_ok(a.bias, a.n)))
     return RNS8_INVALID_ARGUMENT;
-  if (a.m > kMaxSize || a.n > kMaxSize || a.k > kMaxSize || a.lda >= kMaxByteStride || a.ldb >= kMaxByteStride)
+  if (a.m > kMaxSize || a.n > (inner ? kMaxByteRow : kMaxProductCols) || a.k > kMaxByteRow || a.lda >= kMaxByteStride ||
+      a.ldb >= kMaxByteStride)
     return RNS8_UNSUPPORTED_BACKEND;
   return RNS8_SUCCESS;
 }
@@ -162,7 +163,7 @@ rns8_status check_linear(const rns8_mi355x_linear_i8_args& a) {
     return RNS8_INVALID_ARGUMENT;
   if (!a.x_q != !a.x_scale) return RNS8_INVALID_ARGUMENT;
   if (a.x_q && (!operand_ok(a.x_q, a.m, a.k, a.ldq, 1) || !floats_ok(a.x_scale, a.m))) return RNS8_INVALID_ARGUMENT;
-  if (a.m > kMaxSize || a.n > kMaxSize || a.k >= kMaxByteStride - 16 || a.ldw >= kMaxByteStride ||
+  if (a.m > kMaxSize || a.n > kMaxProductCols || a.k >= kMaxByteRow || a.ldw >= kMaxByteStride ||
       (a.x_q && a.ldq >= kMaxByteStride))
     return RNS8_UNSUPPORTED_BACKEND;
   return RNS8_SUCCESS;
@@ -259,9 +260,9 @@ rns8_status check_linear_backward(const rns8_mi355x_linear_i8_backward_args& a) 
                !floats_ok(a.x_scale, a.m)))
     return RNS8_INVALID_ARGUMENT;
   if (a.dbias && !floats_ok(a.dbias, a.n)) return RNS8_INVALID_ARGUMENT;
-  const int64_t most = kMaxByteStride - 16;
-  if (a.k > kMaxSize || (a.dx && (a.n >= most || a.ldw >= kMaxByteStride)) ||
-      ((a.dw || a.dbias) && (a.m >= most || a.n > kMaxSize)) || (a.dw && a.ldq >= kMaxByteStride) || a.m > kMaxSize)
+  if (a.k > ((a.dx || a.dw) ? kMaxByteRow : kMaxSize) || (a.dx && (a.n >= kMaxByteRow || a.ldw >= kMaxByteStride)) ||
+      ((a.dw || a.dbias) && (a.m >= kMaxByteRow || a.n > kMaxSize)) || (a.dw && a.ldq >= kMaxByteStride) ||
+      a.m > kMaxSize)
     return RNS8_UNSUPPORTED_BACKEND;
   return RNS8_SUCCESS;
 }

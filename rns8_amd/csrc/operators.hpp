@@ -78,6 +78,10 @@ hipError_t launch_gemm_i8_pair(const rns8_mi355x_gemm_i8_args& x, const rns8_mi3
 // Whether the product would rather have its rows in fragment order, and the product of such rows.
 bool gemm_i8_takes_fragments(const rns8_mi355x_gemm_i8_args& a);
 hipError_t launch_gemm_i8_fragments(const rns8_mi355x_gemm_i8_args& a, hipStream_t stream);
+// What the product's kernels take: rows of 8-bit operands whose copies, at a
+// multiple of 16 bytes, stay below 2^23, and columns whose tiles end below 2^31.
+constexpr int64_t kMaxByteRow = (int64_t{1} << 23) - 16;
+constexpr int64_t kMaxProductCols = 0x7FFFFFFF - 256;
 
 // The linear layer for one or two tokens in one kernel (scaled_rows.hip).
 bool linear_rows_takes(int64_t m, int64_t n, int64_t k);

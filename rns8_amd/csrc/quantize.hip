@@ -143,8 +143,14 @@ struct ColsArgs {
   uint32_t* amax_part;  // [chunks][cols]
   float* sum_part;      // [chunks][cols]
   int64_t chunks, chunk_rows;
-  int64_t tiles_c;
+  int64_t tiles, tiles_c;
+  int64_t first;  // the first tile of this launch
 };
+
+// Tiles or strips of columns to a launch: workgroups of 256 threads, with room for
+// what else it does below 2^32 threads. More of them take more launches (walked in
+// the kernels, they would cost every call registers: 8192 x 8192 75 us for 67).
+constexpr int64_t kMaxUnits = int64_t{1} << 23;
 
 // About 1024 workgroups of 256 columns, at least 16 rows each, and few enough
 // that joining them is a small part of the second kernel: 4096 x 4096 26.8 us in 32
@@ -248,8 +254,8 @@ __global__ __launch_bounds__(256) void quantize_columns_kernel(ColsArgs a) {
   __shared__ uint32_t tile[kTile * kPitch];  // [column][four rows]
   __shared__ uint32_t amax_lds[kTile];
   __shared__ float sum_lds[kTile];
-  const int64_t tile_r = blockIdx.x / a.tiles_c;
-  const int64_t c0 = (blockIdx.x - tile_r * a.tiles_c) * kTile, r0 = tile_r * kTile;
+  const int64_t unit = a.first + blockIdx.x, tile_r = unit / a.tiles_c;
+  const int64_t c0 = (unit - tile_r * a.tiles_c) * kTile, r0 = tile_r * kTile;
   const int vec = threadIdx.x & 15, quad = threadIdx.x >> 4;  // 16 vectors of 8 columns by 16 groups of four rows
   const int64_t c = c0 + 8 * vec;
   // the whole tile is on its way while the columns' scales are joined
@@ -447,12 +453,14 @@ __device__ __forceinline__ void quantize_whole_columns(const ColsArgs& a, int64_
 }
 
 template <typename T>
-hipError_t launch_columns_rest(const ColsArgs& a, hipStream_t stream) {
-  const int64_t tiles_r = a.stop > 0 ? (a.stop + kTile - 1) / kTile : 1;  // no rows: scales and sums alone
-  if (tiles_r > kMaxBlocks / a.tiles_c) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((quantize_columns_kernel<T>), dim3(static_cast<unsigned>(tiles_r * a.tiles_c)), dim3(256), 0,
-                     stream, a);
-  return hipGetLastError();
+hipError_t launch_columns_rest(ColsArgs a, hipStream_t stream) {
+  for (; a.first < a.tiles; a.first += kMaxUnits) {
+    const dim3 grid(static_cast<unsigned>(std::min(a.tiles - a.first, kMaxUnits)));
+    hipLaunchKernelGGL((quantize_columns_kernel<T>), grid, dim3(256), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 // ---- rows, columns and copies in one launch -------------------------------------------
@@ -543,6 +551,7 @@ ColsArgs cols_args(const rns8_mi355x_quantize_args& g) {
   a.amax_part = static_cast<uint32_t*>(g.workspace);
   a.sum_part = reinterpret_cast<float*>(a.amax_part + a.chunks * a.cols);
   a.tiles_c = (g.cols + kTile - 1) / kTile;
+  a.tiles = std::max<int64_t>(1, (a.stop + kTile - 1) / kTile) * a.tiles_c;  // no rows: scales and sums alone
   return a;
 }
 
@@ -580,6 +589,7 @@ hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi35
   PrepareArgs a{};
   uint32_t dtype = RNS8_MI355X_F32;
   uint64_t blocks = 0;
+  int64_t col_units = 0;
   if (rows && rows->rows > 0) {
     dtype = rows->dtype;
     a.rows = rows_args(*rows);
@@ -593,9 +603,11 @@ hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi35
     const bool whole = whole_columns(columns->rows);
     const int64_t width = whole ? kWholeCols : 256, chunks = whole ? 1 : a.cols.chunks;
     const int64_t strips = (columns->cols + width - 1) / width;
-    if (strips > kMaxBlocks / 4 / chunks) return hipErrorInvalidValue;
+    // (columns below 2^31: at most 2^26 strips of whole columns, and 2^23 units of
+    // partials, which a launch holds: more than 2^12 strips are of one chunk each)
+    col_units = strips * chunks;
     a.col_strips = static_cast<uint32_t>(strips);
-    a.col_blocks = static_cast<uint32_t>(strips * chunks);
+    a.col_blocks = static_cast<uint32_t>(std::min(col_units, kMaxUnits));
     blocks += a.col_blocks;
   }
   if (copy_count > 4) return hipErrorInvalidValue;
@@ -606,9 +618,23 @@ hipError_t launch_prepare(const rns8_mi355x_quantize_args* rows, const rns8_mi35
   }
   if (blocks == 0) return hipSuccess;
   return of_dtype(dtype, [&](auto t) {
-    if (columns && whole_columns(columns->rows))
-      return launch_prepare_of<decltype(t), true>(a, static_cast<uint32_t>(blocks), stream);
-    return launch_prepare_of<decltype(t), false>(a, static_cast<uint32_t>(blocks), stream);
+    if (!columns || !whole_columns(columns->rows))
+      return launch_prepare_of<decltype(t), false>(a, static_cast<uint32_t>(blocks), stream);
+    hipError_t e = launch_prepare_of<decltype(t), true>(a, static_cast<uint32_t>(blocks), stream);
+    // columns past the first launch's: matrices of their own
+    a.row_blocks = 0;
+    std::fill_n(a.copy_blocks, 4, 0u);
+    while (e == hipSuccess && (col_units -= kMaxUnits) > 0) {
+      constexpr int64_t kDone = kMaxUnits * kWholeCols;
+      a.cols.x = static_cast<const decltype(t)*>(a.cols.x) + kDone;
+      a.cols.cols -= kDone;
+      a.cols.q += kDone * a.cols.ldq;
+      a.cols.scale += kDone;
+      if (a.cols.sums) a.cols.sums += kDone;
+      a.col_blocks = static_cast<uint32_t>(std::min(col_units, kMaxUnits));
+      e = launch_prepare_of<decltype(t), true>(a, a.col_blocks, stream);
+    }
+    return e;
   });
 }
 

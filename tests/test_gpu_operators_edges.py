@@ -101,3 +101,24 @@ def test_gradient_of_logits_on_a_common_offset(gpu_ctx, dtype, offset, scale, ro
     assert_close(e_, want, terms * (off * (logp.abs() + entropy[:, None]) + 2 * off * (2 + size)), "dlogits of entropy")
     if dtype == torch.float32:  # what the target gains the others lose
         assert (d.double().sum(1).abs() <= scale * gl.double().abs() * (off[:, 0] + 4 * U32)).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(2**28 + 1000, 1), (2**30 + 1000, 1), (2, 2**24 + 50), (1, 2**28 + 50)])
+def test_columns_past_the_workgroups_of_a_launch(gpu_ctx, rows, cols):
+    """As many tiles, or strips of whole columns, as take more than one launch; whole numbers add up exactly in 32 bits."""
+    x = torch.randint(-7, 8, (rows, cols), device="cuda", dtype=torch.int8)
+    if cols == 1:
+        x[::2, 0] = -x[1::2, 0]
+        x[12345, 0], x[12344, 0] = 127, -127
+    v = x.half()
+    q = torch.full((cols, rows), 99, dtype=torch.int8, device="cuda")
+    scale, sums = torch.empty(2, cols, device="cuda")
+    ready()
+    ops.QuantizeColumns(gpu_ctx, x=v, q=q, scale=scale, sums=sums)()
+    ready()
+    assert torch.equal(sums, x.sum(0).float())
+    if cols == 1:
+        assert scale.item() == 1.0 and torch.equal(q[0], x[:, 0])
+    else:
+        want, want_scale = quantize(v.float(), 0)
+        assert torch.equal(scale, want_scale) and torch.equal(q, want.t())

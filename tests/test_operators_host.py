@@ -95,3 +95,71 @@ def test_python_handles(monkeypatch):
     call._fn = lambda ctx, args, stream: seen.append(stream) or abi.SUCCESS
     call(), call(None), call(0), call(8192)
     assert seen == [None, None, abi.DEFAULT_STREAM, 8192]
+
+
+# ---- limits ---------------------------------------------------------------------------------
+
+
+def columns(rows, cols):
+    return dict(dtype=abi.F16, rows=rows, cols=cols, x=P if rows else 0, ldx=cols, q=P if rows else 0, ldq=max(rows, 1),
+                scale=P, sums=P)
+
+
+@pytest.mark.parametrize("rows,cols", [(2**20 + 1, 32768), (2**31 - 1, 1), (2**28 + 1000, 100), (0, 2**31 - 1),
+                                       (1, 2**31 - 1), (2, 2**24 + 50), (512, 2**26), (513, 2**28), (600, 2**22 + 1)])
+def test_columns_of_any_size_that_is_promised(enqueued, rows, cols):
+    """Strips of 32 whole columns or, past 512 rows, partials and then tiles of 128 x 128: no launch is refused, and none
+    has 2^32 threads."""
+    (got,) = enqueued("quantize_columns", columns(rows, cols))
+    assert got[:3:2] == (abi.SUCCESS, abi.SUCCESS) and got.blocks < 2**32 // 256
+    units = -(-cols // 32) if 0 < rows <= 512 else max(1, -(-rows // 128)) * -(-cols // 128)
+    launches = -(-units // 2**23) + (0 if 0 < rows <= 512 else 1)
+    assert got.launches == launches
+
+
+LONGEST = 2**23 - 16  # a row of 8-bit operands
+
+
+def product(m, n, k, layout=abi.B_CHANNELS, pad=1):
+    return dict(dtype=abi.F32, m=m, n=n, k=k, a=P, lda=k + pad, b=P, ldb=(n if layout else k) + pad, b_layout=layout, out=P,
+                ldo=n)
+
+
+@pytest.mark.parametrize("call,refused", [
+    (product(300, 500, LONGEST), False), (product(300, 500, LONGEST, pad=0), False), (product(300, 500, LONGEST + 1), True),
+    (product(300, 500, 2**23 - 1, pad=0), True), (product(300, LONGEST, 500, abi.B_INNER), False),
+    (product(300, LONGEST + 1, 500, abi.B_INNER), True), (product(1, 2**31 - 257, 1), False),
+    (product(1, 2**31 - 256, 1), True), (product(2**31 - 1, 1, 1), False)])
+def test_limits_of_products(enqueued, call, refused):
+    (got,) = enqueued("gemm_i8_scaled", call)
+    if refused:
+        assert got[:4] == (abi.UNSUPPORTED_BACKEND, 0, abi.UNSUPPORTED_BACKEND, 0)
+    else:
+        assert got.query == got.status == abi.SUCCESS and got.launches >= 1
+
+
+def gradients(m, n, k, pad=1, **more):
+    c = dict(dtype=abi.F32, m=m, n=n, k=k, dy=P, lddy=n, x_q=P, ldq=k + pad, x_scale=P, w=P, ldw=k + pad, w_scale=P, dx=P,
+             lddx=k, dw=P, lddw=k, dbias=P)
+    return c | more
+
+
+@pytest.mark.parametrize("call,refused", [
+    (gradients(300, 500, LONGEST), False), (gradients(300, 500, LONGEST + 1), True),
+    (gradients(300, 500, LONGEST + 1, dx=0), True), (gradients(300, 500, LONGEST + 1, dw=0), True),
+    (gradients(300, 500, LONGEST + 1, dx=0, dw=0), False), (gradients(LONGEST - 1, 500, 20), False),
+    (gradients(LONGEST, 500, 20), True), (gradients(300, LONGEST, 20), True), (gradients(300, LONGEST - 1, 20), False)])
+def test_limits_of_gradients(enqueued, call, refused):
+    (got,) = enqueued("linear_i8_backward", call)
+    if refused:
+        assert got[:4] == (abi.UNSUPPORTED_BACKEND, 0, abi.UNSUPPORTED_BACKEND, 0)
+    else:
+        assert got.query == got.status == abi.SUCCESS and got.launches >= 1
+
+
+def test_limits_of_layers(enqueued):
+    fits = [linear(1, 2**31 - 257, 1), linear(300, 500, LONGEST - 1), linear(300, 2**31 - 257, 20)]
+    over = [linear(1, 2**31 - 256, 1), linear(300, 500, LONGEST), linear(300, 2**31 - 256, 20)]
+    assert all(a.query == a.status == abi.SUCCESS and a.launches for a in enqueued("linear_i8", *fits))
+    refused = (abi.UNSUPPORTED_BACKEND, 0, abi.UNSUPPORTED_BACKEND, 0)
+    assert all(a[:4] == refused for a in enqueued("linear_i8", *over))
