@@ -555,8 +555,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
 #pragma unroll
       for (int i = 0; i < kVector; ++i) {
         const float logp = fmaf(v[i] - from, a.scale, -log_s), p = exp2_fast(logp * kLog2E);
-        // (p = 0 far below any logit that counts: its factor stays finite)
-        d[i] = -a.scale * p * fmaf(fmaxf(logp, -1e30f), ge, rest);
+        // (p is 0 in 32 bits below -104: its factor stays finite, also times a large ge)
+        d[i] = -a.scale * p * fmaf(fmaxf(logp, -200.0f), ge, rest);
       }
       if (asked && static_cast<uint64_t>(target - at) < kVector) {
 #pragma unroll

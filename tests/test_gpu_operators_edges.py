@@ -122,3 +122,26 @@ def test_columns_past_the_workgroups_of_a_launch(gpu_ctx, rows, cols):
     else:
         want, want_scale = quantize(v.float(), 0)
         assert torch.equal(scale, want_scale) and torch.equal(q, want.t())
+
+
+@pytest.mark.parametrize("weight", [1.0, 2.0 ** 30, -(2.0 ** 66), 2.0 ** 116])
+def test_large_weights_of_the_entropy_beside_masks(gpu_ctx, weight):
+    """A ruled-out token gets 0 whatever the weight is; the others' gradients grow with it (a power of two times those of 1)."""
+    v = normal(1, 5, 3000)
+    v[:, ::3], v[1, 1::3], v[2, 4] = -float("inf"), torch.finfo(torch.float32).min, -500.0
+    lse, entropy = torch.empty(2, 5, device="cuda")
+    ready()
+    ops.TokenLogprobs(gpu_ctx, logits=v, lse=lse, entropy=entropy)()
+    got = []
+    for w in (1.0, weight):
+        d, g = torch.empty_like(v), torch.full((5,), w, device="cuda")
+        ready()
+        ops.TokenLogprobsBackward(gpu_ctx, logits=v, lse=lse, entropy=entropy, dentropy=g, dlogits=d)()
+        ready()
+        got.append(d)
+    none = torch.softmax(v.double(), 1) < 2.0 ** -150
+    assert none[:, ::3].all() and none[1, 1::3].all() and none[2, 4]
+    assert not got[1][none].any()
+    # (values that are denormal for a weight of 1 have lost digits that they keep for a large one)
+    normal_ones = got[0].abs() > 2.0 ** -126
+    assert torch.equal(got[1][normal_ones], got[0][normal_ones] * weight)
