@@ -145,3 +145,27 @@ def test_large_weights_of_the_entropy_beside_masks(gpu_ctx, weight):
     # (values that are denormal for a weight of 1 have lost digits that they keep for a large one)
     normal_ones = got[0].abs() > 2.0 ** -126
     assert torch.equal(got[1][normal_ones], got[0][normal_ones] * weight)
+
+
+@pytest.mark.parametrize("size", [1e-18, 1e-15, 1e-13, 1e-10, 1.0, 1e10, 1e13, 1e14, 1e15, 1e17])
+@pytest.mark.parametrize("flags", [ops.NORM_POST, ops.NORM_PRE])
+@pytest.mark.parametrize("rows,cols", [(5, 200), (40, 5000)])
+def test_norm_gradients_of_rows_of_any_size(gpu_ctx, size, flags, rows, cols):
+    """Rows whose squares 32 bits hold: r, but not its cube. With n = x r, each of
+    dx = r (w d - n mean(w d n)) and dw = sum d n is off by 128 (over rows 256) units of its terms, as any norm's gradients."""
+    x, d, w = size * normal(1, rows, cols), normal(2, rows, cols), 1 + 0.3 * normal(3, cols)
+    rstd, h, y, dx = torch.empty(2, rows, device="cuda"), *torch.empty(3, rows, cols, device="cuda")
+    dw = torch.empty(cols, device="cuda")
+    pre = flags == ops.NORM_PRE
+    given = dict(x=x, flags=flags, eps=0.0, **({"pre_weight": w} if pre else {"post_weight": w}))
+    ready()
+    ops.BlockNorm(gpu_ctx, **given, h=h, y=y if pre else None, rstd=rstd)()
+    ops.BlockNormBackward(gpu_ctx, **given, rstd=rstd, dx=dx, **(dict(dy=d, dpre_weight=dw) if pre else
+                                                                 dict(dh=d, dpost_weight=dw)))()
+    ready()
+    r = x.double().square().mean(1, keepdim=True).rsqrt()
+    n, wd = x.double() * r, w.double() * d.double()
+    assert_close(dx, r * (wd - n * (wd * n).mean(1, keepdim=True)),
+                 128 * U32 * r * (wd.abs() + n.abs() * (wd * n).abs().mean(1, keepdim=True)), "dx")
+    terms = d.double() * n
+    assert_close(dw, terms.sum(0), 256 * U32 * terms.abs().sum(0), "dw")
