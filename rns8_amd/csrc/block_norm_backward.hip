@@ -60,21 +60,22 @@ __global__ __launch_bounds__(row_block(kThreads)) void block_norm_backward_kerne
     const float r1 = a.has_post ? a.rstd[row] : 1.0f;
     const float r2 = a.has_pre ? a.rstd[a.rows + row] : 0.0f;
     auto gate = [&](int j, int i) { return gate_at<kGates>(r, w, j, i); };
-    float h[kVectors][8];
-    float dot = 0.0f;
+    float h[kVectors][8] = {};  // (without a norm of h nothing depends on it, also where it is infinite)
+    float dot = 0.0f, k2 = 0.0f;
+    if (a.has_pre) {
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j)
+      for (int j = 0; j < kVectors; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = r.x.v[j].at(i) * r1 * w.post.v[j].at(i);
-        const float dy = r.dy.v[j].at(i);
-        h[j][i] = (a.keep * r.res.v[j].at(i) + a.branch * gate(j, i) * f) * r2;
-        dot += w.pre.v[j].at(i) * dy * h[j][i];
-        sum_pre[j][i] += dy * h[j][i];
-      }
-    float k2 = 0.0f;
-    if (a.has_pre) k2 = r2 * (row_sum<kThreads>(dot, scratch) * inv_cols);
-    dot = 0.0f;
+        for (int i = 0; i < 8; ++i) {
+          const float f = r.x.v[j].at(i) * r1 * w.post.v[j].at(i);
+          const float dy = r.dy.v[j].at(i);
+          h[j][i] = (a.keep * r.res.v[j].at(i) + a.branch * gate(j, i) * f) * r2;
+          dot += w.pre.v[j].at(i) * dy * h[j][i];
+          sum_pre[j][i] += dy * h[j][i];
+        }
+      k2 = r2 * (row_sum<kThreads>(dot, scratch) * inv_cols);
+      dot = 0.0f;
+    }
     // h, by r2 so far, becomes w_post df
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
@@ -103,15 +104,16 @@ __global__ __launch_bounds__(row_block(kThreads)) void block_norm_backward_kerne
         store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dgate_rows) + row * a.lddgate, a.cols, j, lane, out, false);
     }
     if (!a.dx) return;
-    float k1 = 0.0f;
-    if (a.has_post) k1 = r1 * (row_sum<kThreads>(dot, scratch) * inv_cols);
+    if (a.has_post) {
+      const float k1 = r1 * (row_sum<kThreads>(dot, scratch) * inv_cols);
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      float out[8];
+      for (int j = 0; j < kVectors; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = r1 * h[j][i] - r.x.v[j].at(i) * r1 * k1;
-      store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dx) + row * a.lddx, a.cols, j, lane, out, a.stream_dx);
+        for (int i = 0; i < 8; ++i) h[j][i] = r1 * h[j][i] - r.x.v[j].at(i) * r1 * k1;
     }
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j)
+      store_vector<kThreads, T, kVectors>(static_cast<T*>(a.dx) + row * a.lddx, a.cols, j, lane, h[j], a.stream_dx);
   });
   const int64_t group = row_is_shared(kThreads) ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
 #pragma unroll

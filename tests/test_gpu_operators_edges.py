@@ -169,3 +169,23 @@ def test_norm_gradients_of_rows_of_any_size(gpu_ctx, size, flags, rows, cols):
                  128 * U32 * r * (wd.abs() + n.abs() * (wd * n).abs().mean(1, keepdim=True)), "dx")
     terms = d.double() * n
     assert_close(dw, terms.sum(0), 256 * U32 * terms.abs().sum(0), "dw")
+
+
+@pytest.mark.parametrize("flags", [0, ops.NORM_POST])
+@pytest.mark.parametrize("cols", [100, 9000])
+def test_gradients_past_infinite_values_that_no_norm_reads(gpu_ctx, flags, cols):
+    """Without a norm of h, dresidual is residual_scale dh, and without one of x, dx is branch_scale gate dh: whatever the
+    block's output and the residual hold."""
+    x, res, gate, dh = (normal(i, 6, cols) for i in range(4))
+    x[1, 3], x[2, 7], res[3, 5], res[4, 6] = float("inf"), float("nan"), -float("inf"), float("nan")
+    rstd, h, dx, dres = torch.empty(2, 6, device="cuda"), *torch.empty(3, 6, cols, device="cuda")
+    given = dict(x=x, residual=res, gate=gate, flags=flags, branch_scale=0.5, residual_scale=4.0)
+    ready()
+    ops.BlockNorm(gpu_ctx, **given, h=h, rstd=rstd)()
+    ops.BlockNormBackward(gpu_ctx, **given, rstd=rstd, dh=dh, dx=dx, dresidual=dres)()
+    ready()
+    assert torch.equal(dres, 4.0 * dh)
+    if not flags:
+        assert torch.equal(dx, 0.5 * gate * dh)
+    else:
+        assert torch.isnan(dx).any(1).tolist() == [False, True, True, False, False, False]
