@@ -13,7 +13,9 @@ the stream given:
 
 Operands are tensors in device memory: any objects with torch's data_ptr(),
 shape, stride(), dtype and is_cuda. Rows may be strided; the elements of a row
-are next to each other. A torch.cuda.Stream is passed as its cuda_stream (in a
+are next to each other. Quantized rows that a call writes are followed by zeros up
+to padded(cols) or the next row, whichever is first, also where q is a view that
+ends before them (q[:, :cols] of a padded buffer). A torch.cuda.Stream is passed as its cuda_stream (in a
 process that imports torch before this library is loaded: both then share one
 HIP runtime). Torch's default stream has the handle 0: it runs the operator on
 that stream, in order with torch's work there. The context's own stream waits for
@@ -62,8 +64,10 @@ class _Operands:
         self.keep.append(t)
         return t.data_ptr() or None
 
-    def matrix(self, field, ld, t, rows, cols, kind=None, wider=False):
-        """A rows x cols operand into args.<field> and its row stride into args.<ld>."""
+    def matrix(self, field, ld, t, rows, cols, kind=None, wider=False, padding=False):
+        """A rows x cols operand into args.<field> and its row stride into args.<ld>.
+
+        padding: bytes that are written with zeros after each row, up to its stride (padded(cols) at most)."""
         if t is None:
             setattr(self.args, ld, cols)
             return
@@ -75,8 +79,19 @@ class _Operands:
         stride = t.stride(0) if rows > 1 else max(t.stride(0), shape[1])
         if stride < shape[1]:
             raise ValueError(f"{field}: rows overlap")
+        if padding and rows and not self._has_room(t, (rows - 1) * stride + min(stride, padded(cols))):
+            if rows > 1:
+                raise ValueError(f"{field}: its storage ends before the zeros after the last row")
+            stride = shape[1]
         setattr(self.args, field, self._pointer(field, t, kind or self.kind))
         setattr(self.args, ld, stride)
+
+    @staticmethod
+    def _has_room(t, length):
+        """Whether `length` bytes from t's first on are in its storage (of tensors that have one)."""
+        if not hasattr(t, "untyped_storage"):
+            return True
+        return t.storage_offset() + length <= t.untyped_storage().nbytes()
 
     def vector(self, field, t, count, kind="float32"):
         if t is None:
@@ -143,7 +158,7 @@ class QuantizeRows(_Call):
         rows, cols = x.shape
         self.args.rows, self.args.cols = rows, cols
         o.matrix("x", "ldx", x, rows, cols)
-        o.matrix("q", "ldq", q, rows, cols, "int8", wider=True)
+        o.matrix("q", "ldq", q, rows, cols, "int8", wider=True, padding=True)
         o.vector("scale", scale, rows)
         o.vector("multiplier", multiplier, cols)
         self._finish(o)
@@ -160,7 +175,7 @@ class QuantizeColumns(_Call):
         rows, cols = x.shape
         self.args.rows, self.args.cols = rows, cols
         o.matrix("x", "ldx", x, rows, cols)
-        o.matrix("q", "ldq", q, cols, rows, "int8", wider=True)
+        o.matrix("q", "ldq", q, cols, rows, "int8", wider=True, padding=True)
         o.vector("scale", scale, cols)
         o.vector("multiplier", multiplier, rows)
         o.vector("sums", sums, cols)
@@ -203,7 +218,7 @@ class LinearI8(_Call):
         o.vector("w_scale", w_scale, n)
         o.vector("bias", bias, n)
         o.matrix("out", "ldo", out, m, n)
-        o.matrix("x_q", "ldq", x_q, m, k, "int8", wider=True)
+        o.matrix("x_q", "ldq", x_q, m, k, "int8", wider=True, padding=True)
         o.vector("x_scale", x_scale, m)
         self._finish(o, workspace)
 
@@ -263,7 +278,7 @@ class BlockNorm(_Call):
                                   residual_scale)
         o.matrix("h", "ldh", h, rows, cols)
         o.matrix("y", "ldy", y, rows, cols)
-        o.matrix("q", "ldq", q, rows, cols, "int8", wider=True)
+        o.matrix("q", "ldq", q, rows, cols, "int8", wider=True, padding=True)
         o.vector("q_scale", q_scale, rows)
         o.vector("rstd", rstd, 2 * rows)
         self._finish(o)
