@@ -54,11 +54,14 @@ class _Operands:
         self.kind = kind
         args.dtype = _DTYPES[kind]
 
-    def _pointer(self, what, t, kind):
+    def _on_device(self, what, t):
         if not getattr(t, "is_cuda", False):
             raise ValueError(f"{what} is not in device memory")
         if t.device.index not in (None, self.device):
             raise ValueError(f"{what} is on device {t.device.index}, the context on {self.device}")
+
+    def _pointer(self, what, t, kind):
+        self._on_device(what, t)
         if _name(t) != kind:
             raise ValueError(f"{what} is of type {_name(t)}: {kind} is wanted")
         self.keep.append(t)
@@ -123,8 +126,9 @@ class _Call:
             check(getattr(lib(), self._query)(self._ref, C.byref(need)), self._query)
             self.workspace_bytes = need.value
             if workspace is not None:
-                if not workspace.is_cuda or not workspace.is_contiguous():
-                    raise ValueError("the workspace has to be contiguous device memory")
+                operands._on_device("the workspace", workspace)
+                if not workspace.is_contiguous():
+                    raise ValueError("the workspace has to be contiguous")
                 self._keep.append(workspace)
                 self.args.workspace = workspace.data_ptr()
                 self.args.workspace_bytes = workspace.numel() * workspace.element_size()

@@ -78,3 +78,14 @@ def test_rows_that_are_only_read_need_no_room():
                                 w_scale=Device(torch.zeros(8)), dw=Device(torch.zeros(8, 6)),
                                 workspace=Device(torch.zeros(1)))
     assert call.args.ldq == 16 and call.args.dtype == abi.F32
+
+
+@pytest.mark.parametrize("what", ["device", "host", "strides"])
+def test_workspaces_that_a_call_cannot_use(what):
+    x, w = Device(torch.zeros(70, 64)), Device(torch.zeros(80, 64, dtype=torch.int8))
+    layer = dict(x=x, w=w, w_scale=Device(torch.zeros(80)), out=Device(torch.zeros(70, 80)))
+    given = {"device": Device(torch.zeros(1 << 16), index=1), "host": torch.zeros(1 << 16),
+             "strides": Device(torch.zeros(1 << 16, 2)[:, 0])}[what]
+    with pytest.raises(ValueError, match="workspace"):
+        ops.LinearI8(Context(), **layer, workspace=given)
+    ops.LinearI8(Context(), **layer, workspace=Device(torch.zeros(1 << 16)))
