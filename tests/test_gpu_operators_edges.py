@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from operator_cases import U32, Guarded, assert_close, quantize
+from operator_cases import TYPES, U32, Guarded, assert_close, place, quantize
 from rns8_amd import operators as ops
 
 pytestmark = pytest.mark.gpu
@@ -10,6 +10,11 @@ pytestmark = pytest.mark.gpu
 
 def normal(seed, *shape):
     return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def integers(seed, *shape, low=-128, high=128):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(low, high, shape, generator=g, device="cuda").to(torch.int8)
 
 
 def ready():
@@ -189,3 +194,66 @@ def test_gradients_past_infinite_values_that_no_norm_reads(gpu_ctx, flags, cols)
         assert torch.equal(dx, 0.5 * gate * dh)
     else:
         assert torch.isnan(dx).any(1).tolist() == [False, True, True, False, False, False]
+
+
+# kept rows of the quantized activations: next to each other, at an odd address, with room for some of the zeros, and
+# at a stride of whole 16 bytes from an address that is none
+KEPT = [(0, 0), (0, 3), (5, 1), (None, 5)]
+
+
+def kept_rows(values, m, k, pad, offset):
+    pad = -k % 16 if pad is None else pad
+    kept = Guarded(m, k, torch.int8, pad, offset, -99)
+    if values is not None:
+        kept.t.copy_(values)
+        kept.was = kept.buf.clone()
+    return kept
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 1000), (2, 40, 70), (17, 300, 1000), (48, 130, 77), (64, 8200, 129),
+                                   (70, 300, 130), (300, 257, 641), (530, 130, 1000), (300, 64, 15)])
+@pytest.mark.parametrize("pad,offset", KEPT)
+@pytest.mark.parametrize("w_pad", [0, 3])
+def test_layers_that_keep_rows_at_any_alignment(gpu_ctx, m, n, k, pad, offset, w_pad):
+    """A product's sum is exact: its scales and bias are three 32-bit operations, and the rounding of the sum one more."""
+    dtype = TYPES[(m + k) % 3]
+    x, w = normal(m, m, k).to(dtype), place(integers(n, n, k), w_pad, w_pad)
+    ws, bias = torch.exp(normal(4, n)) / k, normal(5, n)
+    kept, scale, out = kept_rows(None, m, k, pad, offset), torch.empty(m, device="cuda"), Guarded(m, n, dtype)
+    ready()
+    ops.LinearI8(gpu_ctx, x=x, w=w.t, w_scale=ws, bias=bias, out=out.t, x_q=kept.t, x_scale=scale)()
+    ready()
+    q, s = quantize(x.float(), 1)
+    stop = min(kept.ld, ops.padded(k))
+    rows = torch.as_strided(kept.buf, (m, stop), (kept.ld, 1), kept.at)
+    assert torch.equal(rows[:, :k], q) and not rows[:, k:].any() and torch.equal(scale, s) and kept.untouched(stop)
+    want = (q.double() @ w.t.double().t().contiguous()) * s.double()[:, None] * ws.double()
+    assert_close(out.t, want + bias.double(), 4 * U32 * (want.abs() + bias.double().abs()), "out")
+    assert out.untouched()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 97), (5, 33, 70), (100, 130, 257), (300, 257, 129), (513, 256, 520),
+                                   (1030, 300, 200), (70, 40, 15)])
+@pytest.mark.parametrize("pad,offset", KEPT)
+@pytest.mark.parametrize("wanted", ["all", "dw"])
+def test_gradients_from_kept_rows_at_any_alignment(gpu_ctx, m, n, k, pad, offset, wanted):
+    """As the layer: exact sums, and the quantized gradients' own bytes and scales."""
+    dtype = TYPES[(m + n) % 3]
+    dy, xq, xs = normal(m + 1, m, n).to(dtype), integers(k, m, k), torch.exp(normal(6, m))
+    w, ws, kept = place(integers(n, n, k), 1, 1), torch.exp(normal(7, n)), kept_rows(xq, m, k, pad, offset)
+    dx, dw, db = Guarded(m, k, dtype), Guarded(n, k, torch.float32), torch.full((n,), 9.0, device="cuda")
+    more = dict(dx=dx.t, dbias=db) if wanted == "all" else {}
+    ready()
+    ops.LinearI8Backward(gpu_ctx, dy=dy, x_q=kept.t, x_scale=xs, w=w.t, w_scale=ws, dw=dw.t, **more)()
+    ready()
+    d = dy.float()
+    hq, hs = quantize(d * xs[:, None], 0)
+    want = (hq.double().t().contiguous() @ xq.double()) * hs.double()[:, None]
+    assert_close(dw.t, want, 4 * U32 * want.abs(), "dw")
+    if wanted == "all":
+        gq, gs = quantize(d * ws, 1)
+        want = (gq.double() @ w.t.double()) * gs.double()[:, None]
+        assert_close(dx.t, want, 4 * U32 * want.abs(), "dx")
+        assert_close(db, d.double().sum(0), m * U32 * d.double().abs().sum(0), "dbias")
+    assert kept.untouched() and dx.untouched() and dw.untouched()
+    assert torch.equal(kept.t, xq)

@@ -163,3 +163,14 @@ def test_limits_of_layers(enqueued):
     assert all(a.query == a.status == abi.SUCCESS and a.launches for a in enqueued("linear_i8", *fits))
     refused = (abi.UNSUPPORTED_BACKEND, 0, abi.UNSUPPORTED_BACKEND, 0)
     assert all(a[:4] == refused for a in enqueued("linear_i8", *over))
+
+
+@pytest.mark.parametrize("m,n,k", [(70, 300, 130), (300, 257, 641), (530, 130, 1000), (300, 64, 15)])
+def test_layers_copy_what_they_cannot_read_in_place(enqueued, m, n, k):
+    """Kept rows, weights, both or neither: each copy is a launch, or part of the quantization's where it is the weights'."""
+    at = dict(ldq=-(-k // 16) * 16, ldw=-(-k // 16) * 16)
+    none, rows, weights, both = enqueued("linear_i8", *(linear(m, n, k, keep=True, **(at | c)) for c in (
+        {}, {"x_q": P + 1}, {"w": P + 1}, {"x_q": P + 1, "w": P + 1})))
+    assert {a.status for a in (none, rows, weights, both)} == {abi.SUCCESS}
+    assert [a.launches - none.launches for a in (rows, weights, both)] == [1, 0, 2]
+    assert none.bytes < weights.bytes < both.bytes and none.bytes < rows.bytes < both.bytes
