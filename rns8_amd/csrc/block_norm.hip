@@ -149,7 +149,7 @@ hipError_t launch_block_norm(const rns8_mi355x_block_norm_args& g, hipStream_t s
   a.stream_h = streams(moved, g.h, g.ldh, g.dtype);
   a.stream_y = streams(moved, g.y, g.ldy, g.dtype);
   return of_dtype(g.dtype, [&](auto t) {
-    return with_row_shape(choose_row_shape(g.rows, g.cols, sizeof(t)), [&](auto threads, auto vectors) {
+    return with_row_shape<ChosenShapes<sizeof(t)>>(choose_row_shape(g.rows, g.cols, sizeof(t)), [&](auto threads, auto vectors) {
       constexpr int kThreads = decltype(threads)::value;
       const dim3 grid = forward_grid(kThreads, decltype(vectors)::value, a.rows), block(row_block(kThreads));
       if (a.gate && a.ldgate != 0)

@@ -163,6 +163,11 @@ __global__ __launch_bounds__(1024) void sum_groups_kernel(SumArgs a) {
 
 // One vector per thread as far as that goes: sums and two rows stay in registers.
 RowShape backward_shape(int64_t cols) { return row_shape(cols, cols <= 4096 ? 1 : 2); }
+struct BackwardShapes {
+  static constexpr bool has(int threads, int vectors) {
+    return threads < 512 ? vectors == 1 : threads == 512 ? vectors <= 2 : vectors >= 2;
+  }
+};
 
 // Row groups of a backward launch: enough to fill the chip, few enough that their
 // partial sums, written once and read once, stay small beside the rows, and all of
@@ -247,7 +252,7 @@ hipError_t launch_block_norm_backward(const rns8_mi355x_block_norm_backward_args
   a.part_gate = part_of(g.ldgate == 0 ? static_cast<float*>(g.dgate) : nullptr);
   if (g.rows > 0) {
     const hipError_t e = of_dtype(g.dtype, [&](auto t) {
-      return with_row_shape(shape, [&](auto threads, auto vectors) {
+      return with_row_shape<BackwardShapes>(shape, [&](auto threads, auto vectors) {
         constexpr int kThreads = decltype(threads)::value;
         const dim3 grid = backward_grid(g.rows, shape), block(row_block(kThreads));
         if (a.gate && a.ldgate != 0)

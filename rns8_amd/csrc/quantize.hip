@@ -120,7 +120,7 @@ hipError_t launch_rows(const RowsArgs& a, hipStream_t stream) {
 template <typename T>
 hipError_t launch_rows_of(const RowsArgs& a, hipStream_t stream) {
   if (a.cols > 32768) return launch_rows<T, 1024, 0>(a, stream);
-  return with_row_shape(choose_row_shape(a.rows, a.cols, sizeof(T)), [&](auto threads, auto vectors) {
+  return with_row_shape<ChosenShapes<sizeof(T)>>(choose_row_shape(a.rows, a.cols, sizeof(T)), [&](auto threads, auto vectors) {
     return launch_rows<T, decltype(threads)::value, decltype(vectors)::value>(a, stream);
   });
 }
@@ -514,8 +514,10 @@ template <typename T, int kThreads, int kVectors, bool kWhole>
 hipError_t launch_prepare_as(const PrepareArgs& a, uint32_t blocks, hipStream_t stream) {
   if (a.rows.multiplier)
     hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, true, kWhole>), dim3(blocks), dim3(256), 0, stream, a);
-  else
+  else if constexpr (!kWhole || (kThreads == 64 && kVectors == 1))
     hipLaunchKernelGGL((prepare_kernel<T, kThreads, kVectors, false, kWhole>), dim3(blocks), dim3(256), 0, stream, a);
+  else  // rows beside columns are a gradient's, and have a multiplier
+    return hipErrorInvalidValue;
   return hipGetLastError();
 }
 

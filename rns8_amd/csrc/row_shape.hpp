@@ -33,17 +33,29 @@ inline RowShape choose_row_shape(int64_t rows, int64_t cols, int element_size) {
   return row_shape(cols, rows < 512 || element_size == 4 ? 1 : 2);
 }
 
-// f(threads, vectors) with the shape as compile-time constants.
-template <typename F>
+// The shapes that choose_row_shape gives for elements of this size.
+template <int kElementSize>
+struct ChosenShapes {
+  static constexpr bool has(int threads, int vectors) {
+    return vectors == 1 || threads == 1024 || (vectors == 2 && kElementSize < 4);
+  }
+};
+
+// f(threads, vectors) with the shape, one that Shapes has, as compile-time constants.
+template <typename Shapes, typename F>
 hipError_t with_row_shape(RowShape s, F&& f) {
   auto vectors = [&](auto threads) {
-    if (s.vectors == 1) return f(threads, std::integral_constant<int, 1>{});
-    if constexpr (decltype(threads)::value < 1024) {
-      return f(threads, std::integral_constant<int, 2>{});
-    } else {
-      if (s.vectors == 2) return f(threads, std::integral_constant<int, 2>{});
-      return f(threads, std::integral_constant<int, 4>{});
+    constexpr int kThreads = decltype(threads)::value;
+    if constexpr (Shapes::has(kThreads, 1)) {
+      if (s.vectors == 1) return f(threads, std::integral_constant<int, 1>{});
     }
+    if constexpr (Shapes::has(kThreads, 2)) {
+      if (s.vectors == 2) return f(threads, std::integral_constant<int, 2>{});
+    }
+    if constexpr (Shapes::has(kThreads, 4)) {
+      if (s.vectors == 4) return f(threads, std::integral_constant<int, 4>{});
+    }
+    return hipErrorInvalidValue;
   };
   if (s.threads == 64) return vectors(std::integral_constant<int, 64>{});
   if (s.threads == 128) return vectors(std::integral_constant<int, 128>{});

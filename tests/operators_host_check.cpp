@@ -8,7 +8,8 @@
 //   <query status> <workspace bytes> <status> <launches> <most workgroups in one> <stream of the last>
 //
 // where the call is given a workspace of the size that the query answered. The
-// context's own stream has the handle 4096.
+// context's own stream has the handle 4096. The line "kernels" prints how often
+// each kernel of the library was launched so far, and an empty line after them.
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>
 
@@ -16,6 +17,7 @@
 #include <cstring>
 #include <iostream>
 #include <map>
+#include <set>
 #include <sstream>
 #include <string>
 
@@ -29,6 +31,12 @@ hipStream_t last_stream = nullptr;
 dim3 grid_of_call, block_of_call;
 size_t shared_of_call;
 hipStream_t stream_of_call;
+// kernels by the host's address of theirs (filled before main, so made on first use)
+std::map<const void*, std::string>& kernel_names() {
+  static std::map<const void*, std::string> names;
+  return names;
+}
+std::map<std::string, long> kernel_launches;
 }  // namespace
 
 extern "C" {
@@ -46,8 +54,12 @@ hipError_t __hipPopCallConfiguration(dim3* grid, dim3* block, size_t* shared, hi
   *stream = stream_of_call;
   return hipSuccess;
 }
-hipError_t hipLaunchKernel(const void*, dim3 grid, dim3, void**, size_t, hipStream_t stream) {
+void __hipRegisterFunction(void**, const void* host, char*, const char* name, unsigned, void*, void*, void*, void*, int*) {
+  kernel_names()[host] = name;
+}
+hipError_t hipLaunchKernel(const void* kernel, dim3 grid, dim3, void**, size_t, hipStream_t stream) {
   ++launches;
+  ++kernel_launches[kernel_names()[kernel]];
   const uint64_t blocks = static_cast<uint64_t>(grid.x) * grid.y * grid.z;
   if (blocks > most_blocks) most_blocks = blocks;
   last_stream = stream;
@@ -136,6 +148,29 @@ bool answer(const std::string& what, const Values& v) {
     rns8_mi355x_quantize_args a{};
     SET(rows), SET(cols), SET(x), SET(ldx), SET(multiplier), SET(q), SET(ldq), SET(scale);
     ask(a, v, OPERATOR_WITHOUT_WORKSPACE(quantize_rows));
+  } else if (what == "block_norm") {
+    rns8_mi355x_block_norm_args a{};
+    SET(rows), SET(cols), SET(flags), SET(branch_scale), SET(residual_scale), SET(x), SET(ldx), SET(gate), SET(ldgate);
+    SET(h), SET(ldh), SET(y), SET(ldy);
+    ask(a, v, OPERATOR_WITHOUT_WORKSPACE(block_norm));
+  } else if (what == "block_norm_backward") {
+    rns8_mi355x_block_norm_backward_args a{};
+    SET(rows), SET(cols), SET(flags), SET(branch_scale), SET(residual_scale), SET(x), SET(ldx), SET(gate), SET(ldgate);
+    SET(rstd), SET(dy), SET(lddy), SET(dx), SET(lddx), SET(dpre_weight);
+    ask(a, v, OPERATOR(block_norm_backward));
+  } else if (what == "token_logprobs") {
+    rns8_mi355x_logprobs_args a{};
+    SET(rows), SET(vocab), SET(logits), SET(ldl), SET(scale), SET(top), SET(lse), SET(top_ids);
+    ask(a, v, OPERATOR(token_logprobs));
+  } else if (what == "token_logprobs_backward") {
+    rns8_mi355x_logprobs_backward_args a{};
+    SET(rows), SET(vocab), SET(logits), SET(ldl), SET(targets), SET(scale), SET(lse), SET(dlogp), SET(dlogits), SET(lddl);
+    ask(a, v, OPERATOR_WITHOUT_WORKSPACE(token_logprobs_backward));
+  } else if (what == "kernels") {
+    std::set<std::string> names;
+    for (const auto& k : kernel_names()) names.insert(k.second);
+    for (const auto& name : names) std::cout << name << " " << kernel_launches[name] << "\n";
+    std::cout << "\n";
   } else {
     return false;
   }

@@ -42,11 +42,18 @@ def enqueued(tmp_path_factory):
                     str(ROOT / "tests" / "operators_host_check.cpp"), *map(str, OBJS), "-L/opt/rocm/lib",
                     "-Wl,-rpath,/opt/rocm/lib", "-lamdhip64", "-pthread", "-o", str(exe)], check=True)
 
+    def run_all(lines):
+        res = subprocess.run([str(exe)], input="\n".join([*lines, "kernels"]) + "\n", capture_output=True, text=True,
+                             timeout=120, check=True)
+        answers, names = res.stdout.splitlines()[:len(lines)], res.stdout.splitlines()[len(lines):]
+        return [Answer(*map(int, line.split())) for line in answers], {k: int(n) for k, n in map(str.split, names[:-1])}
+
     def run(what, *calls):
         text = "\n".join(" ".join([what, *(f"{k} {v}" for k, v in c.items())]) for c in calls) + "\n"
         res = subprocess.run([str(exe)], input=text, capture_output=True, text=True, timeout=60, check=True)
         return [Answer(*map(int, line.split())) for line in res.stdout.splitlines()]
 
+    run.all = run_all
     return run
 
 
@@ -174,3 +181,68 @@ def test_layers_copy_what_they_cannot_read_in_place(enqueued, m, n, k):
     assert {a.status for a in (none, rows, weights, both)} == {abi.SUCCESS}
     assert [a.launches - none.launches for a in (rows, weights, both)] == [1, 0, 2]
     assert none.bytes < weights.bytes < both.bytes and none.bytes < rows.bytes < both.bytes
+
+
+# ---- kernels ---------------------------------------------------------------------------------
+
+OPERATOR_KERNELS = ("quantize_rows_kernel", "prepare_kernel", "quantize_columns_kernel", "copy_rows_kernel",
+                    "scaled_tiles_kernel", "join_slices_kernel", "scaled_rows_kernel", "block_norm_kernel",
+                    "block_norm_backward_kernel", "sum_groups_kernel", "logprobs_kernel", "join_parts_kernel",
+                    "logprobs_backward_kernel")
+
+
+def many_calls():
+    """Calls of every operator over types, sizes on both sides of each rule, and options."""
+    def line(what, **fields):
+        return " ".join([what, *(f"{k} {v}" for k, v in fields.items())])
+
+    for dtype in (abi.F32, abi.F16, abi.BF16):
+        for rows in (1, 40, 600):
+            for cols in (5, 500, 1000, 1100, 2000, 3000, 4096, 5000, 8000, 9000, 16000, 17000, 30000, 40000):
+                for multiplier in (0, P):
+                    yield line("quantize_rows", dtype=dtype, rows=rows, cols=cols, x=P, ldx=cols, multiplier=multiplier,
+                               q=P, ldq=cols, scale=P)
+                if cols > 32768:
+                    continue
+                for ldgate in (0, cols):
+                    norm = dict(dtype=dtype, rows=rows, cols=cols, flags=3, branch_scale=1, residual_scale=1, x=P,
+                                ldx=cols, gate=P, ldgate=ldgate)
+                    yield line("block_norm", **norm, h=P, ldh=cols, y=P, ldy=cols)
+                    yield line("block_norm_backward", **norm, rstd=P, dy=P, lddy=cols, dx=P, lddx=cols, dpre_weight=P)
+        for rows in (1, 5, 600):
+            for vocab in (100, 2500, 7000, 30000, 50000, 130000):
+                for top in (0, 5):
+                    yield line("token_logprobs", dtype=dtype, rows=rows, vocab=vocab, logits=P, ldl=vocab, scale=1,
+                               lse=P, top=top, top_ids=P if top else 0)
+                yield line("token_logprobs_backward", dtype=dtype, rows=rows, vocab=vocab, logits=P, ldl=vocab, targets=P,
+                           scale=1, lse=P, dlogp=P, dlogits=P, lddl=vocab)
+        for m in (1, 2, 16, 17, 40, 60, 100, 300, 1000, 4096):
+            for n in (40, 300, 1100, 4096, 8200):
+                for k in (10, 64, 900, 1500, 3000, 8000, 12000):
+                    yield line("linear_i8", **(linear(m, n, k) | dict(dtype=dtype)))
+                    yield line("linear_i8", **(linear(m, n, k, keep=True, ldw=k + 1) | dict(dtype=dtype)))
+        for m in (40, 600, 1500):
+            for n in (40, 700, 1100, 3000, 5000, 9000):
+                for k in (64, 1000, 4096):
+                    for some in ({}, {"dw": 0, "dbias": 0}, {"dx": 0}):
+                        yield line("linear_i8_backward", **(gradients(m, n, k) | dict(dtype=dtype) | some))
+    for layout in (abi.B_CHANNELS, abi.B_INNER):
+        for m in (64, 256, 500, 1000, 2048, 4096, 8192):
+            for n in (64, 128, 300, 1000, 2048, 4096, 8192):
+                for k in (64, 1000, 4096, 30000, 200000):
+                    yield line("gemm_i8_scaled", **product(m, n, k, layout))
+        for m, n, k in ((277, 40555, 721), (1362, 5607, 2070)):
+            yield line("gemm_i8_scaled", **product(m, n, k, layout))
+    for rows in (0, 100, 600, 20000):
+        for dtype in (abi.F32, abi.F16, abi.BF16):
+            yield line("quantize_columns", **(columns(rows, 300) | dict(dtype=dtype)))
+
+
+def test_every_kernel_is_reached(enqueued):
+    """No instantiation of an operator's kernel is left that no call takes."""
+    answers, kernels = enqueued.all(list(many_calls()))
+    assert all(a.query == a.status == abi.SUCCESS and a.launches for a in answers)
+    mine = {k: n for k, n in kernels.items() if any(f"{len(name)}{name}" in k for name in OPERATOR_KERNELS)}
+    assert all(any(f"{len(name)}{name}" in k for k in mine) for name in OPERATOR_KERNELS)
+    unreached = [k for k, n in mine.items() if n == 0]
+    assert not unreached, "\n".join(unreached)
