@@ -158,70 +158,6 @@ __device__ __forceinline__ void add_logits(Sums& t, const float (&v)[kCount], fl
   t.w += w[0] + w[1];
 }
 
-template <typename T>
-struct Held {
-  T v[kVector];
-};
-
-// The logits [at, at + kVector) of a row, ruled out from `last` on.
-template <typename T>
-__device__ __forceinline__ void load_held(const T* z, int64_t at, int64_t last, Held<T>& h) {
-  if (at + kVector <= last) {
-    __builtin_memcpy(h.v, z + at, sizeof(h.v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVector; ++i) h.v[i] = at + i < last ? z[at + i] : static_cast<T>(-INFINITY);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void floats_of(const Held<T>& h, float (&v)[kVector]) {
-#pragma unroll
-  for (int i = 0; i < kVector; ++i) v[i] = static_cast<float>(h.v[i]);
-}
-
-// Adds this thread's share of the logits [first, last) of a row: two vectors at a
-// time, the next two in flight (the last are loaded twice).
-template <typename T>
-__device__ __forceinline__ void add_span(Sums& t, const T* z, int64_t first, int64_t last, float c, bool& terms_held) {
-  const int64_t at = first + kVector * threadIdx.x;
-  const int64_t whole = last - at >= kVector ? (last - at - kVector) / kStride + 1 : 0;
-  Held<T> x[2], y[2];
-  auto load_pair = [&](int64_t i, Held<T> (&h)[2]) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) __builtin_memcpy(h[k].v, z + at + min(i + k, whole - 1) * kStride, sizeof(h[k].v));
-  };
-  auto add_pair = [&](int64_t i, const Held<T> (&h)[2]) {
-    float u[2 * kVector];
-#pragma unroll
-    for (int k = 0; k < kVector; ++k) {
-      u[k] = static_cast<float>(h[0].v[k]);
-      u[kVector + k] = static_cast<float>(h[1].v[k]);
-    }
-    if (i + 1 >= whole) {  // the second was loaded twice
-#pragma unroll
-      for (int k = 0; k < kVector; ++k) u[kVector + k] = -INFINITY;
-    }
-    add_logits(t, u, c, terms_held);
-  };
-  if (whole > 0) {
-    load_pair(0, x);
-    for (int64_t i = 0; i < whole; i += 4) {
-      load_pair(i + 2, y);
-      add_pair(i, x);
-      if (i + 2 >= whole) break;
-      load_pair(i + 4, x);
-      add_pair(i + 2, y);
-    }
-  }
-  const int64_t rest = at + whole * kStride;
-  if (rest < last) {  // the vector that the part's end cuts
-    load_held(z, rest, last, x[0]);
-    float v[kVector];
-    floats_of(x[0], v);
-    add_logits(t, v, c, terms_held);
-  }
-}
-
 // Order of the alternatives as one unsigned integer: the logit's order (NaNs
 // above infinity, 0 and -0 equal) above the complement of the index. Neither 0 nor all ones.
 __device__ __forceinline__ uint64_t rank_key(float v, uint32_t index) {
@@ -299,6 +235,11 @@ __device__ __forceinline__ void write_alternative(const Args& a, int64_t row, ui
   if (a.top_logp) a.top_logp[row * a.top + rank] = logp_of(ranked_logit(key), t, a.c);
 }
 
+template <typename T>
+struct Held {
+  T v[kVector];
+};
+
 // kRounds: rounds of a part held in registers (0: every part is read again for
 // its alternatives, if any are asked for).
 template <typename T, int kRounds>
@@ -317,18 +258,66 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
     bool terms_held = false;
     constexpr int kHold = kRounds > 0 ? kRounds : 1;
     Held<T> held[kHold];
-    auto load = [&](int64_t at, Held<T>& h) { load_held(z, at, last, h); };
+    auto load = [&](int64_t at, Held<T>& h) {
+      if (at + kVector <= last) {
+        __builtin_memcpy(h.v, z + at, sizeof(h.v));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVector; ++i) h.v[i] = at + i < last ? z[at + i] : static_cast<T>(-INFINITY);
+      }
+    };
+    auto floats = [&](const Held<T>& h, float (&v)[kVector]) {
+#pragma unroll
+      for (int i = 0; i < kVector; ++i) v[i] = static_cast<float>(h.v[i]);
+    };
+    float v[kVector];
     if constexpr (kRounds > 0) {
-      float v[kVector];
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) load(first + r * kStride + kVector * threadIdx.x, held[r]);
 #pragma unroll
       for (int r = 0; r < kRounds; ++r) {
-        floats_of(held[r], v);
+        floats(held[r], v);
         add_logits(t, v, a.c, terms_held);
       }
     } else {
-      add_span(t, z, first, last, a.c, terms_held);
+      // two vectors at a time, the next two in flight (the last are loaded twice)
+      const int64_t at = first + kVector * threadIdx.x;
+      const int64_t whole = last - at >= kVector ? (last - at - kVector) / kStride + 1 : 0;
+      Held<T> x[2], y[2];
+      auto load_pair = [&](int64_t i, Held<T> (&h)[2]) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          __builtin_memcpy(h[k].v, z + at + min(i + k, whole - 1) * kStride, sizeof(h[k].v));
+      };
+      auto add_pair = [&](int64_t i, const Held<T> (&h)[2]) {
+        float u[2 * kVector];
+#pragma unroll
+        for (int k = 0; k < kVector; ++k) {
+          u[k] = static_cast<float>(h[0].v[k]);
+          u[kVector + k] = static_cast<float>(h[1].v[k]);
+        }
+        if (i + 1 >= whole) {  // the second was loaded twice
+#pragma unroll
+          for (int k = 0; k < kVector; ++k) u[kVector + k] = -INFINITY;
+        }
+        add_logits(t, u, a.c, terms_held);
+      };
+      if (whole > 0) {
+        load_pair(0, x);
+        for (int64_t i = 0; i < whole; i += 4) {
+          load_pair(i + 2, y);
+          add_pair(i, x);
+          if (i + 2 >= whole) break;
+          load_pair(i + 4, x);
+          add_pair(i + 2, y);
+        }
+      }
+      const int64_t rest = at + whole * kStride;
+      if (rest < last) {  // the vector that the part's end cuts
+        load(rest, held[0]);
+        floats(held[0], v);
+        add_logits(t, v, a.c, terms_held);
+      }
     }
     const float lane_max = t.m;
     const bool lane_nan = t.s != t.s;  // a NaN among the lane's logits, which comes first
@@ -507,8 +496,9 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(Args a) {
 // log p of 20 is off by. Beyond (logits on a large common offset, rows of nothing
 // but a mask's lowest value) the row's maximum and sum are computed again, and log p
 // starts from the maximum, as in the forward pass: another read of the row by every
-// workgroup that has a part of it (bf16, all rows such: 4096 x 32768 119 us for 82,
-// 4 x 131072 in 32 parts 20 for 3).
+// workgroup that has a part of it (bf16, all rows such: 4096 x 32768 130 us for 84,
+// 4 x 131072 in 32 parts 30 for 3; with the forward pass's four vectors in flight 119
+// and 20, but 40 more registers, which cost f32 rows that need no such read 4%).
 constexpr float kLargeLse = 64.0f;
 
 struct BackArgs {
@@ -540,7 +530,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(BackArgs a)
     if (fabsf(log_s) > kLargeLse) {
       Sums t{-INFINITY, 0.0f, 0.0f};
       bool terms_held = false;
-      add_span(t, z, 0, a.vocab, a.c, terms_held);
+      for (int64_t at = kVector * threadIdx.x; at < a.vocab; at += kStride) {
+        float v[kVector];
+        load_upto8(z + at, a.vocab - at, v, -INFINITY);
+        add_logits(t, v, a.c, terms_held);
+      }
       t = wave_join(t, a.c);
       if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = t;
       __syncthreads();
