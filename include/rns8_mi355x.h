@@ -468,7 +468,8 @@ RNS8_API rns8_status rns8_mi355x_linear_i8_backward_workspace(
  * rns8_mi355x_quantize_rows. h may be NULL with NORM_PRE, and may be x or
  * residual itself (in place, at equal strides). rstd, if given, receives r1
  * (rows values) and then r2 (rows values) for the backward pass. Rows are at
- * most 32768 long. */
+ * most 32768 long. Their sums of squares are 32-bit values: one past 2^128 gives
+ * r = 0, and with eps = 0 one that vanishes (values below 1e-22) r = infinity. */
 #define RNS8_MI355X_NORM_POST 1u
 #define RNS8_MI355X_NORM_PRE 2u
 typedef struct rns8_mi355x_block_norm_args {
@@ -593,7 +594,7 @@ RNS8_API rns8_status rns8_mi355x_token_logprobs_workspace(const rns8_mi355x_logp
 /* The gradient of logp and entropy, from the forward pass's lse and entropy:
  *   dlogits[v] = scale * (dlogp * ([v = target] - p[v]) - dentropy * p[v] * (log p[v] + entropy)).
  * Ruled-out tokens and rows without a finite lse from ruled-out tokens alone
- * get 0; a row whose target asks for none has no gradient from logp. dlogp and
+ * get 0; a row whose lse is NaN gets NaN throughout; a row whose target asks for none has no gradient from logp. dlogp and
  * dentropy may be NULL (0; not both); entropy may be NULL without dentropy.
  * dlogits may be logits itself, at an equal stride. */
 typedef struct rns8_mi355x_logprobs_backward_args {

@@ -7,8 +7,9 @@
 // Bound by HBM: a row is read once into registers, crosses one reduction for each
 // norm (and one for its 8-bit form) and is written once, while the next row is on
 // its way. The weights and a one-row gate stay in registers over a workgroup's rows.
-// bf16, 8192 x 4096 49 us (268 MB: 5.5 TB/s); 8192 x 8192 with h and 8-bit rows 92 us
-// (470 MB: 5.1 TB/s); one token of 4096 3.5 us.
+// bf16, 8192 x 4096 50 us (268 MB: 5.3 TB/s); 8192 x 8192 with h and 8-bit rows 91 us
+// (470 MB: 5.1 TB/s); one token of 4096 3.5 us. Rows past 16384 (four vectors to each
+// of 1024 threads) keep more than a CU's registers hold, and spill.
 #include <algorithm>
 
 #include "block_norm.hpp"

@@ -10,7 +10,7 @@
 // norm and leave as two. The sums over rows take half of the registers, so the
 // next row's loads are those of the CU's other workgroups (holding the next
 // row beside this one left room for one workgroup of 512 to a CU: 8192 x 4096
-// 114 us against 93). bf16, 8192 x 4096 75 us (335 MB: 4.5 TB/s) and 6 for the sums;
+// 114 us against 93). bf16, 8192 x 4096 76 us (335 MB: 4.4 TB/s) and 6 for the sums;
 // f32, 1000 x 1101 with gates 14 and 4. Rows past 8192 spill (16384 f32 columns are
 // 2 MB of row, weights and sums to a CU's 512 KB of registers).
 #include <algorithm>

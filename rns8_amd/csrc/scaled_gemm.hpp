@@ -26,7 +26,8 @@ struct ScaledGemm {
 };
 
 // How the tile kernel splits a product: slices == 1 writes the output, more
-// leave int32 partial sums [slices][m][ldp] that launch_join_slices adds.
+// leave int32 partial sums [slices][m][ldp], which launch_scaled_tiles adds in a
+// second launch.
 struct TileShape {
   uint32_t bm, bn;  // the tile
   uint32_t slices;

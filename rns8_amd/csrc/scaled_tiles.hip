@@ -20,9 +20,9 @@
 //     second kernel adds them in 64 bits and runs the epilogue. The result does
 //     not depend on the cut.
 //   * Both gradients of a linear layer run in one launch (TilePair).
-// Measured (bf16 outputs): 8192^3 405 us (2.7 POP/s, 0.61 of the cycles in MFMA),
-// 4096^3 64 us (2.1 POP/s: one tile to a CU, its start and epilogue 11 us of it),
-// 1000 x 1101 x 903 9.5 us.
+// Measured (bf16 outputs, medians): 8192^3 408 us (2.7 POP/s, 0.66 of the cycles in
+// MFMA), 4096^3 61 us (2.25 POP/s, 0.46 of them: one tile to a CU, nothing beside its
+// start and epilogue), 1000 x 1101 x 903 9.5 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -113,7 +113,9 @@ __device__ __forceinline__ uint32_t div_u31(uint32_t n, DivU31 v) { return __umu
 
 // One product or, with b stored k x n, two of one tile: the first `blocks`
 // workgroups are the first's. Two small ones share the chip, and of two large ones
-// the second's tiles start as the first's end. Both gradients of a layer of 118 x 8
+// the second's tiles start as the first's end (with loads of their own: the LDS of a
+// CU holds one workgroup of the largest tiles, so nothing of the second's is on its way
+// before). Both gradients of a layer of 118 x 8
 // x 35 (with their quantization) 15.0 us in two launches, 10.2 in one; of 1024^3
 // 29.3 and 23.1; of 4096^3 172.8 and 170.4. (With b stored n x k the kernel takes
 // the first's arguments without waiting for `blocks`, 0.5 us.)
