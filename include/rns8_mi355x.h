@@ -621,6 +621,154 @@ RNS8_API rns8_status rns8_mi355x_token_logprobs_backward(
     const rns8_mi355x_logprobs_backward_args* args,
     void* stream);
 
+/* ---- operators on 4-bit microscaled matrices ("MX4") ---------------------------
+ *
+ * A block of 32 neighbouring values of a row (the last of a row may have fewer)
+ * shares one power of two, and each value has 4 bits:
+ *   v ~ level * 2^e,  level in {0, 1/2, 1, 3/2, 2, 3, 4, 6} with a sign,
+ *   e = floor(log2(max |v|)) - 2, at least -127,
+ * level the nearest to v / 2^e, of two as near the one with the even code, at most
+ * 6. A code is the level's index above plus 8 for a sign, e is held as the byte e +
+ * 127. A block that holds an infinity or a NaN gives codes 0 and the byte 255,
+ * which makes whatever is computed from it NaN. (These are the OCP microscaling
+ * formats' MXFP4 elements and scales.)
+ *
+ * An MX4 matrix of rows x cols is one buffer of RNS8_MI355X_MX4_BYTES(rows, cols)
+ * bytes, 16-byte aligned, in the order in which the matrix cores take it: units
+ * of 16 rows x 256 columns, 2176 bytes each, the units of 16 rows one after the
+ * other. Column c of row r of a unit has its code in the 4 bits (the low ones
+ * where c is even) of byte 1024 (c / 128) + 16 L + (c % 32) / 2 and its scale in
+ * byte 2048 + 2 L + c / 128, L = r % 16 + 16 ((c % 128) / 32). What lies past the
+ * matrix in its units is zeros. 16 rows at a multiple of 16 are themselves an MX4
+ * matrix.
+ *
+ * The rules of the operators above hold here too. rows and cols of an MX4 matrix
+ * are below 2^31 - 256 and those that a product sums over at most 2^23. */
+#define RNS8_MI355X_MX4_UNIT 2176
+#define RNS8_MI355X_MX4_BYTES(rows, cols) \
+  (((uint64_t)(rows) + 15u) / 16u * (((uint64_t)(cols) + 255u) / 256u) * RNS8_MI355X_MX4_UNIT)
+
+/* Floating rows to MX4 and back.
+ *   - rns8_mi355x_quantize_mx4: q receives x (rows x cols), q_t its transpose (cols
+ *     x rows, blocks along the rows of x); either may be NULL, not both.
+ *   - rns8_mi355x_dequantize_mx4: x receives the values of q (rows x cols), NaN
+ *     for blocks whose scale is 255; q_t is NULL.
+ * Values that MX4 holds are unchanged by a quantization (their blocks' scales may
+ * be smaller than they were). rows >= 0, cols >= 1. */
+typedef struct rns8_mi355x_mx4_args {
+  uint64_t struct_size;
+  uint32_t abi_version;
+  uint32_t dtype;
+  int64_t rows;
+  int64_t cols;
+  void* x; /* dtype, rows x cols; quantize_mx4 only reads it */
+  int64_t ldx;
+  uint8_t* q;   /* MX4, rows x cols */
+  uint8_t* q_t; /* MX4, cols x rows */
+} rns8_mi355x_mx4_args;
+
+RNS8_API rns8_status rns8_mi355x_quantize_mx4(rns8_context* ctx, const rns8_mi355x_mx4_args* args, void* stream);
+RNS8_API rns8_status rns8_mi355x_dequantize_mx4(rns8_context* ctx, const rns8_mi355x_mx4_args* args, void* stream);
+
+/* Rows as checkpoints hold them into q: `data` has the codes, two to a byte (an
+ * even column in the low bits; ceil(cols / 2) bytes of a row are read), `scale`
+ * the scales' bytes (ceil(cols / 32) of a row). Both have strides in bytes and any
+ * alignment. rows >= 0, cols >= 1. */
+typedef struct rns8_mi355x_pack_mx4_args {
+  uint64_t struct_size;
+  uint32_t abi_version;
+  uint32_t dtype; /* 0: there are no floating operands */
+  int64_t rows;
+  int64_t cols;
+  const uint8_t* data;
+  int64_t ldd;
+  const uint8_t* scale;
+  int64_t lds;
+  uint8_t* q; /* MX4, rows x cols */
+} rns8_mi355x_pack_mx4_args;
+
+RNS8_API rns8_status rns8_mi355x_pack_mx4(rns8_context* ctx, const rns8_mi355x_pack_mx4_args* args, void* stream);
+
+/* The product of MX4 matrices:
+ *   out[i][j] = sum_k a[i][k] b[j][k] + bias[j],
+ * b with one row for each output channel. Products of two codes are exact, sums
+ * are 32-bit. m, n, k >= 0 (an empty sum is zero). */
+typedef struct rns8_mi355x_gemm_mx4_args {
+  uint64_t struct_size;
+  uint32_t abi_version;
+  uint32_t dtype;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  const uint8_t* a;  /* MX4, m x k */
+  const uint8_t* b;  /* MX4, n x k */
+  const float* bias; /* n, or NULL */
+  void* out;         /* dtype, m x n */
+  int64_t ldo;
+  void* workspace;
+  uint64_t workspace_bytes;
+} rns8_mi355x_gemm_mx4_args;
+
+RNS8_API rns8_status rns8_mi355x_gemm_mx4(rns8_context* ctx, const rns8_mi355x_gemm_mx4_args* args, void* stream);
+RNS8_API rns8_status rns8_mi355x_gemm_mx4_workspace(const rns8_mi355x_gemm_mx4_args* args, uint64_t* bytes);
+
+/* A linear layer: x's rows rounded as by rns8_mi355x_quantize_mx4, times MX4
+ * weights w (n x k), with bias. k >= 1. */
+typedef struct rns8_mi355x_linear_mx4_args {
+  uint64_t struct_size;
+  uint32_t abi_version;
+  uint32_t dtype;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  const void* x; /* dtype, m x k */
+  int64_t ldx;
+  const uint8_t* w;  /* MX4, n x k */
+  const float* bias; /* n, or NULL */
+  void* out;         /* dtype, m x n */
+  int64_t ldo;
+  void* workspace;
+  uint64_t workspace_bytes;
+} rns8_mi355x_linear_mx4_args;
+
+RNS8_API rns8_status rns8_mi355x_linear_mx4(rns8_context* ctx, const rns8_mi355x_linear_mx4_args* args, void* stream);
+RNS8_API rns8_status rns8_mi355x_linear_mx4_workspace(const rns8_mi355x_linear_mx4_args* args, uint64_t* bytes);
+
+/* Its gradients, in MX4 products too, the roundings passed straight through. R is
+ * the rounding along rows, so that each product sums over blocks of its own:
+ *   dx = R(dy) R(w^T)^T, R(w^T) the MX4 matrix w_t (k x n),
+ *   dw = R(dy^T) R(x^T)^T,  dbias[j] = sum_i dy[i][j].
+ * dx, dw and dbias may each be NULL (not all three); x may be NULL without dw, w_t
+ * without dx. n, k >= 1. */
+typedef struct rns8_mi355x_linear_mx4_backward_args {
+  uint64_t struct_size;
+  uint32_t abi_version;
+  uint32_t dtype;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  const void* dy; /* dtype, m x n */
+  int64_t lddy;
+  const void* x; /* dtype, m x k */
+  int64_t ldx;
+  const uint8_t* w_t; /* MX4, k x n */
+  void* dx;           /* dtype, m x k */
+  int64_t lddx;
+  float* dw; /* n x k */
+  int64_t lddw;
+  float* dbias; /* n */
+  void* workspace;
+  uint64_t workspace_bytes;
+} rns8_mi355x_linear_mx4_backward_args;
+
+RNS8_API rns8_status rns8_mi355x_linear_mx4_backward(
+    rns8_context* ctx,
+    const rns8_mi355x_linear_mx4_backward_args* args,
+    void* stream);
+RNS8_API rns8_status rns8_mi355x_linear_mx4_backward_workspace(
+    const rns8_mi355x_linear_mx4_backward_args* args,
+    uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -397,6 +397,7 @@ B_CHANNELS = 0
 B_INNER = 1
 NORM_POST = 1
 NORM_PRE = 2
+MX4_UNIT = 2176  # bytes of 16 rows x 256 columns
 DEFAULT_STREAM = 1  # as a stream's handle: the device's default stream
 
 
@@ -467,6 +468,38 @@ class LogprobsBackwardArgs(C.Structure):
                 ("vocab", C.c_int64), ("logits", C.c_void_p), ("ldl", C.c_int64), ("targets", C.c_void_p),
                 ("scale", C.c_float), ("reserved", C.c_uint32), ("lse", C.c_void_p), ("entropy", C.c_void_p),
                 ("dlogp", C.c_void_p), ("dentropy", C.c_void_p), ("dlogits", C.c_void_p), ("lddl", C.c_int64)]
+
+
+class Mx4Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("q", C.c_void_p), ("q_t", C.c_void_p)]
+
+
+class PackMx4Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("data", C.c_void_p), ("ldd", C.c_int64), ("scale", C.c_void_p),
+                ("lds", C.c_int64), ("q", C.c_void_p)]
+
+
+class GemmMx4Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("m", C.c_int64),
+                ("n", C.c_int64), ("k", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("bias", C.c_void_p),
+                ("out", C.c_void_p), ("ldo", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class LinearMx4Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("m", C.c_int64),
+                ("n", C.c_int64), ("k", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("w", C.c_void_p),
+                ("bias", C.c_void_p), ("out", C.c_void_p), ("ldo", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class LinearMx4BackwardArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("m", C.c_int64),
+                ("n", C.c_int64), ("k", C.c_int64), ("dy", C.c_void_p), ("lddy", C.c_int64), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w_t", C.c_void_p), ("dx", C.c_void_p), ("lddx", C.c_int64), ("dw", C.c_void_p),
+                ("lddw", C.c_int64), ("dbias", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
 
 
 _P = C.c_void_p
@@ -550,6 +583,15 @@ PROTOTYPES = {
     "rns8_mi355x_token_logprobs": (_U32, [_P, C.POINTER(LogprobsArgs), _P]),
     "rns8_mi355x_token_logprobs_workspace": (_U32, [C.POINTER(LogprobsArgs), C.POINTER(_U64)]),
     "rns8_mi355x_token_logprobs_backward": (_U32, [_P, C.POINTER(LogprobsBackwardArgs), _P]),
+    "rns8_mi355x_quantize_mx4": (_U32, [_P, C.POINTER(Mx4Args), _P]),
+    "rns8_mi355x_dequantize_mx4": (_U32, [_P, C.POINTER(Mx4Args), _P]),
+    "rns8_mi355x_pack_mx4": (_U32, [_P, C.POINTER(PackMx4Args), _P]),
+    "rns8_mi355x_gemm_mx4": (_U32, [_P, C.POINTER(GemmMx4Args), _P]),
+    "rns8_mi355x_gemm_mx4_workspace": (_U32, [C.POINTER(GemmMx4Args), C.POINTER(_U64)]),
+    "rns8_mi355x_linear_mx4": (_U32, [_P, C.POINTER(LinearMx4Args), _P]),
+    "rns8_mi355x_linear_mx4_workspace": (_U32, [C.POINTER(LinearMx4Args), C.POINTER(_U64)]),
+    "rns8_mi355x_linear_mx4_backward": (_U32, [_P, C.POINTER(LinearMx4BackwardArgs), _P]),
+    "rns8_mi355x_linear_mx4_backward_workspace": (_U32, [C.POINTER(LinearMx4BackwardArgs), C.POINTER(_U64)]),
 }
 
 LIB_PATH = Path(__file__).resolve().parent / "librns8.so"

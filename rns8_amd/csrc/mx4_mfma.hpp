@@ -1,0 +1,84 @@
+// The scaled MFMA on MX4 fragments, and the rounding of a lane's own block.
+#pragma once
+
+#include "mx4.hpp"
+
+namespace rns8x {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// What a lane has of a unit: a block of each fragment, and their scales (low byte
+// the first's).
+struct Mx4Unit {
+  i32x4 codes[2];
+  uint32_t scales;
+};
+
+__device__ __forceinline__ Mx4Unit load_unit(const uint8_t* unit, int lane) {
+  Mx4Unit u;
+  u.codes[0] = *reinterpret_cast<const i32x4*>(unit + 16 * lane);
+  u.codes[1] = *reinterpret_cast<const i32x4*>(unit + 1024 + 16 * lane);
+  u.scales = *reinterpret_cast<const uint16_t*>(unit + kMx4Scales + 2 * lane);
+  return u;
+}
+
+// acc[row of b][row of a] += sum over 128 columns; kFragment: which byte of the
+// scales is this fragment's. Lane L then has rows 4 (L / 16) + e of b and row L % 16
+// of a.
+template <int kFragment>
+__device__ __forceinline__ f32x4 mx4_mfma(i32x4 b, i32x4 a, f32x4 acc, uint32_t b_scales, uint32_t a_scales) {
+  const i32x8 b8 = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
+  const i32x8 a8 = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+  constexpr int kFp4 = 4;
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b8, a8, acc, kFp4, kFp4, kFragment, static_cast<int>(b_scales),
+                                                          kFragment, static_cast<int>(a_scales));
+}
+
+struct Mx4Block {
+  i32x4 codes;
+  uint32_t scale;
+};
+
+// Columns [c, c + 32) of a row of k values (zeros past its end).
+template <typename T>
+__device__ __forceinline__ Mx4Block round_block(const T* row, uint32_t c, uint32_t k) {
+  constexpr int kWords = 8 * sizeof(T);
+  uint32_t raw[kWords] = {};
+  if (c + 32 <= k) {
+    __builtin_memcpy(raw, row + c, sizeof(raw));
+  } else if (c < k) {
+    T t[32] = {};
+#pragma unroll
+    for (uint32_t e = 0; e < 32; ++e)
+      if (c + e < k) t[e] = row[c + e];
+    __builtin_memcpy(raw, t, sizeof(raw));
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) m = larger<T>(m, magnitudes<T>(raw[w]));
+  if constexpr (sizeof(T) == 2) m = larger<T>(m, m >> 16) & 0xFFFFu;
+  const Mx4Scale s = mx4_scale(float_bits<T>(m));
+  Mx4Block out;
+  out.scale = s.code;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t codes = 0;
+    auto pair = [&](auto byte) {
+      constexpr int b = decltype(byte)::value;
+      if constexpr (sizeof(T) == 4)
+        codes = mx4_codes<b>(codes, as_float(raw[8 * q + 2 * b]), as_float(raw[8 * q + 2 * b + 1]), s.scale);
+      else
+        codes = mx4_codes<b, T>(codes, raw[4 * q + b], s.scale);
+    };
+    pair(std::integral_constant<int, 0>{});
+    pair(std::integral_constant<int, 1>{});
+    pair(std::integral_constant<int, 2>{});
+    pair(std::integral_constant<int, 3>{});
+    out.codes[q] = s.code == 255u ? 0 : static_cast<int>(codes);
+  }
+  return out;
+}
+
+}  // namespace rns8x

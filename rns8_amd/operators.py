@@ -1,4 +1,4 @@
-"""Operators of language models around the 8-bit product, on device tensors.
+"""Operators of language models around 8-bit and 4-bit products, on device tensors.
 
 Each class here is one call of the C entry point of the same name
 (include/rns8_mi355x.h, which states what it computes): it takes its operands
@@ -17,7 +17,8 @@ are next to each other. Quantized rows that a call writes are followed by zeros 
 to padded(cols) or the next row, whichever is first, also where q is a view that
 ends before them (q[:, :cols] of a padded buffer). A torch.cuda.Stream is passed as its cuda_stream (in a
 process that imports torch before this library is loaded: both then share one
-HIP runtime). Torch's default stream has the handle 0: it runs the operator on
+HIP runtime). A 4-bit microscaled (MX4) matrix is a contiguous uint8 tensor of
+mx4_bytes(rows, cols) bytes. Torch's default stream has the handle 0: it runs the operator on
 that stream, in order with torch's work there. The context's own stream waits for
 no other, so a program that leaves the stream out synchronizes between the two. A
 workspace is allocated when the object is made, unless one is given, and the
@@ -38,6 +39,11 @@ def padded(cols: int) -> int:
     return (cols + 15) // 16 * 16
 
 
+def mx4_bytes(rows: int, cols: int) -> int:
+    """The bytes of a 4-bit microscaled (MX4) matrix: a contiguous uint8 tensor holds one."""
+    return (rows + 15) // 16 * ((cols + 255) // 256) * abi.MX4_UNIT
+
+
 def _name(t) -> str:
     return str(t.dtype).rsplit(".", 1)[-1]
 
@@ -48,6 +54,8 @@ class _Operands:
     def __init__(self, ctx, args, first):
         self.args, self.keep = args, []
         self.device = ctx.device_info().device_id
+        if first is None:  # (no floating operands)
+            return
         kind = _name(first)
         if kind not in _DTYPES:
             raise ValueError(f"operands of type {kind}: float32, float16 or bfloat16 are wanted")
@@ -95,6 +103,15 @@ class _Operands:
         if not hasattr(t, "untyped_storage"):
             return True
         return t.storage_offset() + length <= t.untyped_storage().nbytes()
+
+    def mx4(self, field, t, rows, cols, count=1):
+        """`count` MX4 matrices of rows x cols, one after the other, into args.<field>."""
+        if t is None:
+            return
+        need = count * mx4_bytes(rows, cols)
+        if t.numel() != need or not t.is_contiguous():
+            raise ValueError(f"{field} has shape {tuple(t.shape)}: {need} bytes next to each other are wanted")
+        setattr(self.args, field, self._pointer(field, t, "uint8"))
 
     def vector(self, field, t, count, kind="float32"):
         if t is None:
@@ -353,3 +370,102 @@ class TokenLogprobsBackward(_Call):
         o.vector("dlogp", dlogp, rows)
         o.vector("dentropy", dentropy, rows)
         self._finish(o)
+
+
+class QuantizeMx4(_Call):
+    """Rows of x (q) and of its transpose (q_t) as MX4 matrices (rns8_mi355x_quantize_mx4)."""
+
+    _entry, _args = "rns8_mi355x_quantize_mx4", abi.Mx4Args
+
+    def __init__(self, ctx, *, x, q=None, q_t=None):
+        o = self._begin(ctx, x)
+        rows, cols = x.shape
+        self.args.rows, self.args.cols = rows, cols
+        o.matrix("x", "ldx", x, rows, cols)
+        o.mx4("q", q, rows, cols)
+        o.mx4("q_t", q_t, cols, rows)
+        self._finish(o)
+
+
+class DequantizeMx4(_Call):
+    """The values of an MX4 matrix (rns8_mi355x_dequantize_mx4)."""
+
+    _entry, _args = "rns8_mi355x_dequantize_mx4", abi.Mx4Args
+
+    def __init__(self, ctx, *, q, out):
+        o = self._begin(ctx, out)
+        rows, cols = out.shape
+        self.args.rows, self.args.cols = rows, cols
+        o.matrix("x", "ldx", out, rows, cols)
+        o.mx4("q", q, rows, cols)
+        self._finish(o)
+
+
+class PackMx4(_Call):
+    """Rows of codes, two to a byte, and of scales as an MX4 matrix (rns8_mi355x_pack_mx4)."""
+
+    _entry, _args = "rns8_mi355x_pack_mx4", abi.PackMx4Args
+
+    def __init__(self, ctx, *, data, scale, q, cols):
+        o = self._begin(ctx, None)
+        rows = data.shape[0]
+        self.args.rows, self.args.cols = rows, cols
+        o.matrix("data", "ldd", data, rows, (cols + 1) // 2, "uint8")
+        o.matrix("scale", "lds", scale, rows, (cols + 31) // 32, "uint8")
+        o.mx4("q", q, rows, cols)
+        self._finish(o)
+
+
+class GemmMx4(_Call):
+    """The product of MX4 matrices, a (m x k) and b (n x k), into out (m x n) (rns8_mi355x_gemm_mx4)."""
+
+    _entry, _args = "rns8_mi355x_gemm_mx4", abi.GemmMx4Args
+    _query = "rns8_mi355x_gemm_mx4_workspace"
+
+    def __init__(self, ctx, *, a, b, k, out, bias=None, workspace=None):
+        o = self._begin(ctx, out)
+        m, n = out.shape
+        self.args.m, self.args.n, self.args.k = m, n, k
+        o.mx4("a", a, m, k)
+        o.mx4("b", b, n, k)
+        o.matrix("out", "ldo", out, m, n)
+        o.vector("bias", bias, n)
+        self._finish(o, workspace)
+
+
+class LinearMx4(_Call):
+    """A linear layer: x's rows rounded to MX4 times MX4 weights w (n x k) (rns8_mi355x_linear_mx4)."""
+
+    _entry, _args = "rns8_mi355x_linear_mx4", abi.LinearMx4Args
+    _query = "rns8_mi355x_linear_mx4_workspace"
+
+    def __init__(self, ctx, *, x, w, out, bias=None, workspace=None):
+        o = self._begin(ctx, x)
+        (m, k), n = x.shape, out.shape[1]
+        self.args.m, self.args.n, self.args.k = m, n, k
+        o.matrix("x", "ldx", x, m, k)
+        o.mx4("w", w, n, k)
+        o.vector("bias", bias, n)
+        o.matrix("out", "ldo", out, m, n)
+        self._finish(o, workspace)
+
+
+class LinearMx4Backward(_Call):
+    """Its gradients; w_t: the transposed weights (k x n) as an MX4 matrix (rns8_mi355x_linear_mx4_backward)."""
+
+    _entry, _args = "rns8_mi355x_linear_mx4_backward", abi.LinearMx4BackwardArgs
+    _query = "rns8_mi355x_linear_mx4_backward_workspace"
+
+    def __init__(self, ctx, *, dy, x=None, w_t=None, dx=None, dw=None, dbias=None, workspace=None):
+        o = self._begin(ctx, dy)
+        m, n = dy.shape
+        shaped = next((t for t in (dx, dw, x) if t is not None), None)
+        k = shaped.shape[1] if shaped is not None else 1
+        self.args.m, self.args.n, self.args.k = m, n, k
+        o.matrix("dy", "lddy", dy, m, n)
+        o.matrix("x", "ldx", x, m, k)
+        o.mx4("w_t", w_t, k, n)
+        o.matrix("dx", "lddx", dx, m, k)
+        o.matrix("dw", "lddw", dw, n, k, "float32")
+        o.vector("dbias", dbias, n)
+        self._finish(o, workspace)
