@@ -769,6 +769,52 @@ RNS8_API rns8_status rns8_mi355x_linear_mx4_backward_workspace(
     const rns8_mi355x_linear_mx4_backward_args* args,
     uint64_t* bytes);
 
+/* A mixture-of-experts layer for few tokens, its experts' weights MX4 matrices:
+ *   scores[t][e] = sum_c x[t][c] router[e][c]              (64-bit sums, then 32 bits)
+ *   ids[t]: the `top` experts of the largest scores, falling, of equal ones the
+ *     lower index first (a NaN counts as the largest),
+ *   weights[t][s] = exp(scores[t][ids[t][s]]) / sum_e exp(scores[t][e]), with
+ *     RNS8_MI355X_EXPERTS_NORMALIZE the sum over the chosen experts alone,
+ *   out[t] = sum_s weights[t][s] down[e] (silu(gate[e] x[t]) * (up[e] x[t])),  e = ids[t][s],
+ *   silu(v) = v / (1 + exp(-v)).
+ * x is not rounded: few tokens wait for the weights alone. Sums are 32-bit; a
+ * hidden value is kept in 16 bits of precision (24 where dtype is float). Without a
+ * router, ids and weights are inputs: an id below 0 or not below `experts` is a
+ * slot that adds nothing (its expert is elsewhere), and an expert that a token has
+ * twice counts twice. With one they are outputs, and each may be NULL. gate and
+ * up hold one inner x width matrix for each expert, down one width x inner, one
+ * after the other. A score that is not finite, or a value of a token, makes that
+ * token's row alone NaN (or infinite). tokens at most 64, experts at most 1024,
+ * top at most 16 and at most `experts`, width and inner at most 65536. */
+#define RNS8_MI355X_EXPERTS_NORMALIZE 1u
+typedef struct rns8_mi355x_experts_mx4_args {
+  uint64_t struct_size;
+  uint32_t abi_version;
+  uint32_t dtype;
+  int64_t tokens;
+  int64_t experts;
+  int64_t width;
+  int64_t inner;
+  uint32_t top;
+  uint32_t flags;
+  const void* x; /* dtype, tokens x width */
+  int64_t ldx;
+  const void* router; /* dtype, experts x width, or NULL */
+  int64_t ldrouter;
+  const uint8_t* gate; /* MX4, experts of inner x width */
+  const uint8_t* up;   /* MX4, experts of inner x width */
+  const uint8_t* down; /* MX4, experts of width x inner */
+  void* out;           /* dtype, tokens x width */
+  int64_t ldo;
+  int32_t* ids;   /* tokens x top, dense */
+  float* weights; /* tokens x top, dense */
+  void* workspace;
+  uint64_t workspace_bytes;
+} rns8_mi355x_experts_mx4_args;
+
+RNS8_API rns8_status rns8_mi355x_experts_mx4(rns8_context* ctx, const rns8_mi355x_experts_mx4_args* args, void* stream);
+RNS8_API rns8_status rns8_mi355x_experts_mx4_workspace(const rns8_mi355x_experts_mx4_args* args, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -397,6 +397,7 @@ B_CHANNELS = 0
 B_INNER = 1
 NORM_POST = 1
 NORM_PRE = 2
+EXPERTS_NORMALIZE = 1
 MX4_UNIT = 2176  # bytes of 16 rows x 256 columns
 DEFAULT_STREAM = 1  # as a stream's handle: the device's default stream
 
@@ -502,6 +503,15 @@ class LinearMx4BackwardArgs(C.Structure):
                 ("workspace_bytes", C.c_uint64)]
 
 
+class ExpertsMx4Args(C.Structure):
+    _fields_ = [("struct_size", C.c_uint64), ("abi_version", C.c_uint32), ("dtype", C.c_uint32), ("tokens", C.c_int64),
+                ("experts", C.c_int64), ("width", C.c_int64), ("inner", C.c_int64), ("top", C.c_uint32),
+                ("flags", C.c_uint32), ("x", C.c_void_p), ("ldx", C.c_int64), ("router", C.c_void_p),
+                ("ldrouter", C.c_int64), ("gate", C.c_void_p), ("up", C.c_void_p), ("down", C.c_void_p),
+                ("out", C.c_void_p), ("ldo", C.c_int64), ("ids", C.c_void_p), ("weights", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _U64 = C.c_uint64
@@ -592,6 +602,8 @@ PROTOTYPES = {
     "rns8_mi355x_linear_mx4_workspace": (_U32, [C.POINTER(LinearMx4Args), C.POINTER(_U64)]),
     "rns8_mi355x_linear_mx4_backward": (_U32, [_P, C.POINTER(LinearMx4BackwardArgs), _P]),
     "rns8_mi355x_linear_mx4_backward_workspace": (_U32, [C.POINTER(LinearMx4BackwardArgs), C.POINTER(_U64)]),
+    "rns8_mi355x_experts_mx4": (_U32, [_P, C.POINTER(ExpertsMx4Args), _P]),
+    "rns8_mi355x_experts_mx4_workspace": (_U32, [C.POINTER(ExpertsMx4Args), C.POINTER(_U64)]),
 }
 
 LIB_PATH = Path(__file__).resolve().parent / "librns8.so"

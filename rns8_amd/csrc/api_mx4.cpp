@@ -160,6 +160,27 @@ hipError_t enqueue_backward(const rns8_mi355x_linear_mx4_backward_args& a, hipSt
   return e;
 }
 
+// ---- experts ---------------------------------------------------------------------------------
+rns8_status check_experts(const rns8_mi355x_experts_mx4_args& a) {
+  if (a.tokens < 0 || a.experts < 1 || a.width < 1 || a.inner < 1 || a.top < 1 || (a.flags & ~RNS8_MI355X_EXPERTS_NORMALIZE) != 0 ||
+      static_cast<int64_t>(a.top) > a.experts)
+    return RNS8_INVALID_ARGUMENT;
+  if (a.tokens > kMaxExpertTokens || a.experts > kMaxExperts || a.top > kMaxExpertTop || a.width > kMaxExpertSize ||
+      a.inner > kMaxExpertSize)
+    return RNS8_UNSUPPORTED_BACKEND;
+  const uint64_t size = element_size(a.dtype);
+  if (!operand_ok(a.x, a.tokens, a.width, a.ldx, size) || !operand_ok(a.out, a.tokens, a.width, a.ldo, size) ||
+      !optional_ok(a.router, a.experts, a.width, a.ldrouter, size))
+    return RNS8_INVALID_ARGUMENT;
+  if (!mx4_ok(a.gate, a.inner, a.width) || !mx4_ok(a.up, a.inner, a.width) || !mx4_ok(a.down, a.width, a.inner))
+    return RNS8_INVALID_ARGUMENT;
+  const int64_t pairs = a.tokens * a.top;
+  if (!a.router && pairs > 0 && (!a.ids || !a.weights)) return RNS8_INVALID_ARGUMENT;
+  return optional_ok(a.ids, 1, pairs, pairs, sizeof(int32_t)) && optional_ok(a.weights, 1, pairs, pairs, sizeof(float))
+             ? RNS8_SUCCESS
+             : RNS8_INVALID_ARGUMENT;
+}
+
 }  // namespace
 }  // namespace rns8x
 
@@ -226,6 +247,19 @@ rns8_status rns8_mi355x_linear_mx4_backward(rns8_context* ctx, const rns8_mi355x
 
 rns8_status rns8_mi355x_linear_mx4_backward_workspace(const rns8_mi355x_linear_mx4_backward_args* args, uint64_t* bytes) {
   return workspace_query(args, bytes, check_linear_backward, backward_bytes);
+}
+
+rns8_status rns8_mi355x_experts_mx4(rns8_context* ctx, const rns8_mi355x_experts_mx4_args* args, void* stream) {
+  return run_operator(
+      ctx, args, stream, check_experts,
+      [](const rns8_mi355x_experts_mx4_args& a) {
+        return check_workspace(a.workspace, a.workspace_bytes, experts_mx4_bytes(a));
+      },
+      launch_experts_mx4);
+}
+
+rns8_status rns8_mi355x_experts_mx4_workspace(const rns8_mi355x_experts_mx4_args* args, uint64_t* bytes) {
+  return workspace_query(args, bytes, check_experts, experts_mx4_bytes);
 }
 
 }  // extern "C"

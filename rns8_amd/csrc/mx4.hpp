@@ -132,4 +132,10 @@ constexpr int64_t kMx4Rows = 64, kMx4FusedRows = 16;
 bool linear_mx4_in_one_kernel(int64_t m, int64_t n);
 hipError_t launch_mx4_rows(const Mx4Gemm& g, hipStream_t stream);
 
+// ---- experts (mx4_experts.hip) ------------------------------------------------------------
+constexpr int64_t kMaxExpertTokens = 64, kMaxExperts = 1024, kMaxExpertSize = 65536;
+constexpr uint32_t kMaxExpertTop = 16;
+uint64_t experts_mx4_bytes(const rns8_mi355x_experts_mx4_args& a);
+hipError_t launch_experts_mx4(const rns8_mi355x_experts_mx4_args& a, hipStream_t stream);
+
 }  // namespace rns8x

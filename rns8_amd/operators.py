@@ -469,3 +469,33 @@ class LinearMx4Backward(_Call):
         o.matrix("dw", "lddw", dw, n, k, "float32")
         o.vector("dbias", dbias, n)
         self._finish(o, workspace)
+
+
+class ExpertsMx4(_Call):
+    """A mixture-of-experts layer for at most 64 tokens (rns8_mi355x_experts_mx4).
+
+    gate, up and down have a row of bytes for each expert: MX4 matrices of inner x
+    width, inner x width and width x inner. With router (experts x width), ids and
+    weights (tokens x top) are outputs, and top says how many where neither is given."""
+
+    _entry, _args = "rns8_mi355x_experts_mx4", abi.ExpertsMx4Args
+    _query = "rns8_mi355x_experts_mx4_workspace"
+
+    def __init__(self, ctx, *, x, gate, up, down, inner, out, router=None, ids=None, weights=None, top=None,
+                 normalize=True, workspace=None):
+        o = self._begin(ctx, x)
+        (tokens, width), experts = x.shape, gate.shape[0]
+        if top is None:
+            top = next((t.shape[1] for t in (ids, weights) if t is not None), 0)
+        a = self.args
+        a.tokens, a.experts, a.width, a.inner, a.top = tokens, experts, width, inner, top
+        a.flags = abi.EXPERTS_NORMALIZE if normalize else 0
+        o.matrix("x", "ldx", x, tokens, width)
+        o.matrix("router", "ldrouter", router, experts, width)
+        o.mx4("gate", gate, inner, width, experts)
+        o.mx4("up", up, inner, width, experts)
+        o.mx4("down", down, width, inner, experts)
+        o.matrix("out", "ldo", out, tokens, width)
+        o.vector("ids", ids, tokens * top, "int32")
+        o.vector("weights", weights, tokens * top)
+        self._finish(o, workspace)
