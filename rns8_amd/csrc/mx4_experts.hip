@@ -1,22 +1,27 @@
 // A mixture-of-experts layer for few tokens on MX4 weights (gfx950). Bound by
 // reading the chosen experts' weights once.
 //
-// Four launches:
 //   * stage: the router's scores, summed in 64 bits (two experts whose scores are next
 //     to each other keep their order whatever the batch), and x as rows of bf16 parts
-//     that add up to it exactly (bf16 1, half 2, float 3), zeros up to whole units;
-//   * route: one workgroup chooses the experts and lists the (expert, token) pairs,
-//     experts with a token first to last, each one's tokens in order;
-//   * hidden: gate and up for 16 rows of one expert to a workgroup, its eight waves a
-//     share of the width each; silu(gate) up times the token's weight goes to the
-//     workspace, again as bf16 parts (two: 16 bits; float three);
-//   * down: 16 channels to a workgroup, its waves a share of all experts' rows; a wave
-//     adds an expert's result to its own table of tokens in LDS, the tables are added
-//     in order.
+//     that add up to it exactly (bf16 1, half 2, float 3), zeros up to whole units.
+//   * hidden: every workgroup lists the (expert, token) pairs for itself (in LDS: less than
+//     a launch), experts with a token first to last, each one's tokens in order; of few
+//     tokens it also chooses the experts. Then 16 rows of one expert's gate and up at a
+//     time; silu(gate) up times the token's weight goes to the workspace, again as bf16
+//     parts (two: 16 bits; float three).
+//   * down, few pairs: 16 channels to a workgroup, its waves a share of all experts' rows,
+//     the hidden values in LDS; a wave adds an expert's result to its own table of
+//     tokens, the tables are added in order. Three launches.
+//   * down, many pairs: 32 channels of one expert at a time, and its tokens' results go to
+//     the workspace; a last kernel adds each token's, by its slots. Five launches with the
+//     choice.
 // Weights go from HBM into registers as whole units, are turned to bf16 there (exact:
 // v_cvt_scalef32_pk_bf16_fp4 applies the scale) and meet the tokens' parts in
 // v_mfma_f32_16x16x32_bf16. The tokens of an expert are the MFMA's columns: an expert
-// with few tokens costs few.
+// with few tokens costs few. Sixteen rows are one wave's where there are many, and
+// otherwise eight waves', each with a share of the sum. Loads return in order, and who
+// waits for tokens from memory has waited for all weights asked for before: tokens lie
+// in LDS, so that a wave always has the next units' weights in flight.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,15 +36,16 @@ namespace {
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxPairs = kMaxExpertTokens * kMaxExpertTop;
-constexpr int kMaxFrags = kMaxExpertTokens / 16;
 
 // Who computes what: pairs sorted by expert, then token.
 struct Routing {
   uint32_t active;  // experts with a token
-  uint16_t expert[kMaxPairs], start[kMaxPairs + 1];  // of an active expert; its pairs are [start[i], start[i + 1])
-  uint16_t token[kMaxPairs];
+  uint16_t expert[kMaxPairs], start[kMaxPairs + 2];  // of an active expert; its pairs are [start[i], start[i + 1])
+  uint16_t token[kMaxPairs];  // of a pair
+  uint16_t place[kMaxPairs];  // of a token's slot: its pair, or kNone
   float weight[kMaxPairs];
 };
+constexpr uint32_t kNone = 0xFFFF;
 
 struct ExpertsArgs {
   const void *x, *router;
@@ -49,11 +55,14 @@ struct ExpertsArgs {
   int64_t ldo;
   int32_t* ids;
   float* weights;
-  uint32_t tokens, experts, top, normalize, dtype;
+  uint32_t tokens, experts, top, normalize;
   uint32_t width, inner, width_chunks, inner_chunks;
-  float* scores;   // tokens x experts
+  int32_t* chosen;        // tokens x top: the caller's, or the choice where there are many pairs
+  float* chosen_weights;
+  float* scores;      // tokens x experts
   uint16_t* x_parts;  // [part][token][256 width_chunks]
   uint16_t* h_parts;  // [part][pair][256 inner_chunks]
+  float* y;           // [pair][16 ceil(width / 16)]; many pairs
   Routing* routing;
 };
 
@@ -75,41 +84,108 @@ __device__ __forceinline__ void split(float v, uint16_t (&part)[kParts]) {
 }
 
 // ---- stage ---------------------------------------------------------------------------------
-constexpr int kScoreTokens = 8;
+// The sum over a wave's lanes, in every lane.
+template <int kCtrl>
+__device__ __forceinline__ double add_moved(double x) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = dpp_move<kCtrl>(static_cast<uint32_t>(bits)), hi = dpp_move<kCtrl>(static_cast<uint32_t>(bits >> 32));
+  return x + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  x = add_moved<kRowRotate + 8>(x);
+  x = add_moved<kRowRotate + 4>(x);
+  x = add_moved<kRowRotate + 2>(x);
+  x = add_moved<kRowRotate + 1>(x);
+  auto swapped = [&](auto swap) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const auto lo = swap(static_cast<uint32_t>(bits)), hi = swap(static_cast<uint32_t>(bits >> 32));
+    x = __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) +
+        __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+  };
+  swapped([](uint32_t v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false); });
+  swapped([](uint32_t v) { return __builtin_amdgcn_permlane32_swap(v, v, false, false); });
+  return x;
+}
 
-template <typename T, int kParts>
+// Eight elements from column c on of a row of at least eight, zeros past its end.
+template <typename T>
+__device__ __forceinline__ Packed8<T> load_cut(const T* row, int32_t c, int32_t width) {
+  Packed8<T> q;
+  const int32_t at = min(c, width - 8);
+  __builtin_memcpy(q.q, row + at, sizeof(q.q));
+  if (c + 8 > width) {
+    if (c < width)
+      q.drop(static_cast<uint32_t>(c - at));
+    else
+      q.fill(static_cast<T>(0.0f));
+  }
+  return q;
+}
+
+// A workgroup takes the scores of kExperts experts and kTokens tokens, or 2048 values of
+// a token of x.
+template <typename T, int kParts, int kExperts, int kTokens>
 __global__ __launch_bounds__(256) void experts_stage_kernel(ExpertsArgs a, uint32_t score_blocks) {
+  __shared__ double sums[4][kExperts * kTokens];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (blockIdx.x < score_blocks) {
-    const uint32_t per = (a.experts + 3) / 4;
-    const uint32_t e = 4 * (blockIdx.x % per) + wave, t0 = kScoreTokens * (blockIdx.x / per);
-    if (e >= a.experts) return;
-    const T* const r = static_cast<const T*>(a.router) + e * a.ldrouter;
-    const T* const x = static_cast<const T*>(a.x) + t0 * a.ldx;
-    const uint32_t count = min(a.tokens - t0, static_cast<uint32_t>(kScoreTokens));
-    double sum[kScoreTokens] = {};
-    for (uint32_t c = 8 * lane; c < a.width; c += 512) {
-      float w[8];
-      load_upto8(r + c, a.width - c, w, 0.0f);
+    const uint32_t per = (a.experts + kExperts - 1) / kExperts;
+    const uint32_t e0 = kExperts * (blockIdx.x % per), t0 = kTokens * (blockIdx.x / per);
+    // (rows past the last read it again; their scores are not stored)
+    const T *r[kExperts], *x[kTokens];
 #pragma unroll
-      for (uint32_t t = 0; t < kScoreTokens; ++t) {
-        if (t >= count) break;
-        float v[8];
-        load_upto8(x + t * a.ldx + c, a.width - c, v, 0.0f);
+    for (uint32_t e = 0; e < kExperts; ++e) r[e] = static_cast<const T*>(a.router) + min(e0 + e, a.experts - 1) * a.ldrouter;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[t] = fma(static_cast<double>(v[i]), static_cast<double>(w[i]), sum[t]);
+    for (uint32_t t = 0; t < kTokens; ++t) x[t] = static_cast<const T*>(a.x) + min(t0 + t, a.tokens - 1) * a.ldx;
+    const int32_t width = static_cast<int32_t>(a.width);
+    double sum[kExperts][kTokens] = {};
+    constexpr int U = kTokens == 1 ? 2 : 1;  // loads in flight together
+    for (int32_t c = 8 * threadIdx.x; c < width && width >= 8; c += 2048 * U) {
+      Packed8<T> w[U][kExperts], v[U][kTokens];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+#pragma unroll
+        for (int e = 0; e < kExperts; ++e) w[i][e] = load_cut(r[e], c + 2048 * i, width);
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) v[i][t] = load_cut(x[t], c + 2048 * i, width);
       }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          double we[kExperts];
+#pragma unroll
+          for (int e = 0; e < kExperts; ++e) we[e] = static_cast<double>(w[i][e].at(k));
+#pragma unroll
+          for (int t = 0; t < kTokens; ++t) {
+            const double vt = static_cast<double>(v[i][t].at(k));
+#pragma unroll
+            for (int e = 0; e < kExperts; ++e) sum[e][t] = fma(we[e], vt, sum[e][t]);
+          }
+        }
+    }
+    if (width < 8 && static_cast<int32_t>(threadIdx.x) < width) {
+#pragma unroll
+      for (int e = 0; e < kExperts; ++e)
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t)
+          sum[e][t] = static_cast<double>(static_cast<float>(r[e][threadIdx.x])) * static_cast<double>(static_cast<float>(x[t][threadIdx.x]));
     }
 #pragma unroll
-    for (uint32_t t = 0; t < kScoreTokens; ++t) {
-      if (t >= count) break;
+    for (int e = 0; e < kExperts; ++e)
 #pragma unroll
-      for (int step = 32; step >= 1; step /= 2) sum[t] += __shfl_xor(sum[t], step);
-      if (lane == 0) a.scores[(t0 + t) * a.experts + e] = static_cast<float>(sum[t]);
+      for (int t = 0; t < kTokens; ++t) {
+        const double all = wave_sum(sum[e][t]);
+        if (lane == 0) sums[wave][e * kTokens + t] = all;
+      }
+    __syncthreads();
+    if (threadIdx.x < kExperts * kTokens) {
+      const uint32_t i = threadIdx.x, e = e0 + i / kTokens, t = t0 + i % kTokens;
+      if (e < a.experts && t < a.tokens)
+        a.scores[t * a.experts + e] = static_cast<float>((sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]));
     }
     return;
   }
-  // x: 256 threads take eight values of a token each
   const uint32_t padded = 256 * a.width_chunks, per = (padded + 2047) / 2048;
   const uint32_t b = blockIdx.x - score_blocks, t = b / per, c = 2048 * (b % per) + 8 * threadIdx.x;
   if (t >= a.tokens || c >= padded) return;
@@ -127,8 +203,16 @@ __global__ __launch_bounds__(256) void experts_stage_kernel(ExpertsArgs a, uint3
   }
 }
 
-// ---- route -------------------------------------------------------------------------------------
-constexpr int kRouteThreads = 512;
+// ---- choice of experts --------------------------------------------------------------------------
+constexpr int kRouteThreads = 512, kRouteWaves = kRouteThreads / 64;
+
+struct RouteScratch {
+  uint16_t id[kMaxPairs];  // of a token's slot, or kNone
+  float weight[kMaxPairs];
+  uint32_t tokens[2][kMaxExperts];  // an expert's tokens, a bit each
+  uint16_t start[kMaxExperts];
+  uint32_t totals[kRouteWaves];
+};
 
 // Ordered as the scores are, NaN first.
 __device__ __forceinline__ uint32_t score_key(float v) {
@@ -137,124 +221,184 @@ __device__ __forceinline__ uint32_t score_key(float v) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kRouteThreads) void experts_route_kernel(ExpertsArgs a) {
-  __shared__ uint32_t key[kMaxPairs];   // expert << 16 | pair, or ~0
-  __shared__ float weight[kMaxPairs];
-  __shared__ uint32_t sorted[kMaxPairs];
-  __shared__ uint32_t firsts[kMaxPairs / 64 + 1];
+// A wave's choice for one token of at most 64 kPer experts, the largest left `top` times:
+// put(slot, expert, weight) by the lanes that hold them.
+template <int kPer, typename Put>
+__device__ __forceinline__ void choose_of(const ExpertsArgs& a, uint32_t t, int lane, Put&& put) {
+  const float* const scores = a.scores + t * a.experts;
+  float score[kPer];
+  uint32_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t e = 64u * i + lane;
+    score[i] = e < a.experts ? scores[e] : 0.0f;
+    key[i] = e < a.experts ? score_key(score[i]) : 0u;
+  }
+  float largest = 0.0f, chosen = 0.0f;
+  uint32_t id = 0;
+  for (uint32_t n = 0; n < a.top; ++n) {
+    uint32_t best = 0, at = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = 64u * i + lane;
+      }
+    const uint32_t top = wave_reduce(best, MaxU{});
+    const uint32_t e = ~wave_reduce(best == top ? ~at : 0u, MaxU{});
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (64u * i + lane == e) {
+        key[i] = 0;
+        mine = score[i];
+      }
+    const float value = as_float(__builtin_amdgcn_readlane(as_uint(mine), __builtin_amdgcn_readfirstlane(e & 63u)));
+    if (n == 0) largest = value;
+    if (lane == static_cast<int>(n)) {
+      id = e;
+      chosen = value;
+    }
+  }
+  const bool holds = static_cast<uint32_t>(lane) < a.top;
+  const float p = holds ? expf(chosen - largest) : 0.0f;
+  float total = p;
+  if (!a.normalize) {
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (64u * i + lane < a.experts) total += expf(score[i] - largest);
+  }
+  total = as_float(wave_reduce(as_uint(total), AddF{}));
+  if (holds) put(static_cast<uint32_t>(lane), id, p / total);
+}
+template <typename Put>
+__device__ __forceinline__ void choose(const ExpertsArgs& a, uint32_t t, int lane, Put&& put) {
+  if (a.experts <= 128)
+    choose_of<2>(a, t, lane, put);
+  else if (a.experts <= 256)
+    choose_of<4>(a, t, lane, put);
+  else
+    choose_of<kMaxExperts / 64>(a, t, lane, put);
+}
+
+// The choice alone, a token to a workgroup: where there are many, each workgroup of the
+// next kernel would choose for eight tokens to a wave (64 tokens, 8 of 128: 27 us).
+__global__ __launch_bounds__(64) void experts_choose_kernel(ExpertsArgs a) {
+  const uint32_t t = blockIdx.x;
+  choose(a, t, threadIdx.x, [&](uint32_t slot, uint32_t id, float weight) {
+    const uint32_t pair = t * a.top + slot;
+    a.chosen[pair] = static_cast<int32_t>(id);
+    a.chosen_weights[pair] = weight;
+    if (a.ids) a.ids[pair] = static_cast<int32_t>(id);
+    if (a.weights) a.weights[pair] = weight;
+  });
+}
+
+// The lists, in LDS; all kRouteThreads threads. writes: this workgroup gives the
+// next kernels the lists, and the caller its experts and weights where they are chosen
+// here (kChooses).
+template <bool kChooses>
+__device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteScratch& s, Routing& r) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t pairs = a.tokens * a.top;
-  // each token's experts and weights
-  if (a.router) {
-    for (uint32_t t = wave; t < a.tokens; t += kRouteThreads / 64) {
-      constexpr int kPer = kMaxExperts / 64;
-      const float* const scores = a.scores + t * a.experts;
-      uint32_t mine[kPer];
-      float largest = 0.0f, total = 0.0f, chosen = 0.0f;
-      uint32_t id = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) mine[i] = 64u * i + lane < a.experts ? score_key(scores[64 * i + lane]) : 0u;
-      for (uint32_t s = 0; s < a.top; ++s) {
-        uint32_t best = 0, at = 0xFFFFFFFFu;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (mine[i] > best) {
-            best = mine[i];
-            at = 64u * i + lane;
-          }
-        const uint32_t top = wave_reduce(best, MaxU{});
-        const uint32_t e = ~wave_reduce(best == top ? ~at : 0u, MaxU{});
-        const float score = scores[e];
-        if (s == 0) largest = score;
-        if (lane == static_cast<int>(s)) {
-          id = e;
-          chosen = score;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (64u * i + lane == e) mine[i] = 0;
-      }
-      const float p = static_cast<uint32_t>(lane) < a.top ? expf(chosen - largest) : 0.0f;
-      if (a.normalize) {
-        total = p;
-      } else {
-        for (uint32_t e = lane; e < a.experts; e += 64) total += expf(scores[e] - largest);
-      }
-      total = as_float(wave_reduce(as_uint(total), AddF{}));
-      if (static_cast<uint32_t>(lane) < a.top) {
-        const uint32_t pair = t * a.top + lane;
-        key[pair] = id << 16 | pair;
-        weight[pair] = p / total;
-        if (a.ids) a.ids[pair] = static_cast<int32_t>(id);
-        if (a.weights) a.weights[pair] = p / total;
-      }
-    }
+  const uint32_t pairs = a.tokens * a.top, tid = threadIdx.x;
+  for (uint32_t e = tid; e < a.experts; e += kRouteThreads) s.tokens[0][e] = s.tokens[1][e] = 0;
+  if (kChooses && a.router) {
+    for (uint32_t t = wave; t < a.tokens; t += kRouteWaves)
+      choose(a, t, lane, [&](uint32_t slot, uint32_t id, float weight) {
+        const uint32_t pair = t * a.top + slot;
+        s.id[pair] = static_cast<uint16_t>(id);
+        s.weight[pair] = weight;
+        if (writes && a.ids) a.ids[pair] = static_cast<int32_t>(id);
+        if (writes && a.weights) a.weights[pair] = weight;
+      });
   } else {
-    for (uint32_t pair = threadIdx.x; pair < pairs; pair += kRouteThreads) {
-      const int32_t id = a.ids[pair];
-      const uint32_t first = pair - pair % a.top;
-      bool counts = id >= 0 && id < static_cast<int32_t>(a.experts);
-      float w = a.weights[pair];
-      // an expert that the token has twice is one pair, the first
-      for (uint32_t q = first; q < first + a.top; ++q) {
-        if (q == pair || a.ids[q] != id) continue;
-        counts = counts && q > pair;
-        w += q > pair ? a.weights[q] : 0.0f;
-      }
-      key[pair] = counts ? static_cast<uint32_t>(id) << 16 | pair : 0xFFFFFFFFu;
-      weight[pair] = w;
+    for (uint32_t pair = tid; pair < pairs; pair += kRouteThreads) {
+      const int32_t id = a.chosen[pair];
+      s.id[pair] = id >= 0 && id < static_cast<int32_t>(a.experts) ? static_cast<uint16_t>(id) : static_cast<uint16_t>(kNone);
+      s.weight[pair] = a.chosen_weights[pair];
+    }
+    if (!a.router) {
+      // an expert that a token has twice is one pair, the first, with both weights
+      __syncthreads();
+      for (uint32_t t = tid; t < a.tokens; t += kRouteThreads)
+        for (uint32_t n = t * a.top; n < (t + 1) * a.top; ++n)
+          for (uint32_t q = t * a.top; q < n; ++q)
+            if (s.id[q] == s.id[n] && s.id[n] != kNone) {
+              s.weight[q] += s.weight[n];
+              s.id[n] = static_cast<uint16_t>(kNone);
+            }
     }
   }
   __syncthreads();
-  // sorted by counting the smaller keys
-  for (uint32_t pair = threadIdx.x; pair < pairs; pair += kRouteThreads) {
-    const uint32_t mine = key[pair];
-    uint32_t rank = 0;
-    for (uint32_t q = 0; q < pairs; ++q) rank += key[q] < mine || (key[q] == mine && q < pair);
-    sorted[rank] = mine;
-    if (mine != 0xFFFFFFFFu) {
-      a.routing->token[rank] = static_cast<uint16_t>(pair / a.top);
-      a.routing->weight[rank] = weight[pair];
-    }
+  for (uint32_t pair = tid; pair < pairs; pair += kRouteThreads) {
+    const uint32_t t = pair / a.top;
+    if (s.id[pair] != kNone) atomicOr(&s.tokens[t >> 5][s.id[pair]], 1u << (t & 31));
   }
   __syncthreads();
-  // where experts begin
-  const uint32_t rounds = (pairs + kRouteThreads - 1) / kRouteThreads;
-  auto begins = [&](uint32_t r) {
-    return r < pairs && sorted[r] != 0xFFFFFFFFu && (r == 0 || sorted[r - 1] >> 16 != sorted[r] >> 16);
-  };
-  for (uint32_t i = 0; i < rounds; ++i) {
-    const uint32_t r = i * kRouteThreads + threadIdx.x;
-    const uint64_t mask = __ballot(begins(r));
-    if (lane == 0 && r / 64 < kMaxPairs / 64) firsts[r / 64] = static_cast<uint32_t>(__popcll(mask));
+  // pairs (low half) and experts (high half) before each expert: two experts to a thread
+  static_assert(kMaxExperts == 2 * kRouteThreads, "two experts to a thread");
+  uint32_t mine[2];
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t e = 2 * tid + i;
+    const uint32_t n = e < a.experts ? __popc(s.tokens[0][e]) + __popc(s.tokens[1][e]) : 0u;
+    mine[i] = n ? n | 0x10000u : 0u;
+  }
+  uint32_t sum = mine[0] + mine[1];
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) {
+    const uint32_t below = __shfl_up(sum, step);
+    if (lane >= step) sum += below;
+  }
+  if (lane == 63) s.totals[wave] = sum;
+  __syncthreads();
+  uint32_t before = sum - mine[0] - mine[1], total = 0;
+#pragma unroll
+  for (int w = 0; w < kRouteWaves; ++w) {
+    if (w < wave) before += s.totals[w];
+    total += s.totals[w];
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    if (!mine[i]) continue;
+    const uint32_t at = i ? before + mine[0] : before;
+    s.start[2 * tid + i] = static_cast<uint16_t>(at);
+    r.expert[at >> 16] = static_cast<uint16_t>(2 * tid + i);
+    r.start[at >> 16] = static_cast<uint16_t>(at);
+  }
+  if (tid == 0) {
+    r.active = total >> 16;
+    r.start[total >> 16] = static_cast<uint16_t>(total);
   }
   __syncthreads();
-  for (uint32_t i = 0; i < rounds; ++i) {
-    const uint32_t r = i * kRouteThreads + threadIdx.x;
-    const uint64_t mask = __ballot(begins(r));
-    uint32_t index = static_cast<uint32_t>(__popcll(mask & ((uint64_t{1} << lane) - 1)));
-    for (uint32_t q = 0; q < r / 64; ++q) index += firsts[q];
-    if (begins(r)) {
-      a.routing->expert[index] = static_cast<uint16_t>(sorted[r] >> 16);
-      a.routing->start[index] = static_cast<uint16_t>(r);
+  for (uint32_t pair = tid; pair < pairs; pair += kRouteThreads) {
+    const uint32_t t = pair / a.top, id = s.id[pair];
+    uint32_t at = kNone;
+    if (id != kNone) {
+      const uint32_t lower = (1u << (t & 31)) - 1;
+      at = s.start[id] + (t < 32 ? __popc(s.tokens[0][id] & lower)
+                                 : __popc(s.tokens[0][id]) + __popc(s.tokens[1][id] & lower));
+      r.token[at] = static_cast<uint16_t>(t);
+      r.weight[at] = s.weight[pair];
     }
+    r.place[pair] = static_cast<uint16_t>(at);
   }
-  if (threadIdx.x == 0) {
-    uint32_t active = 0, count = 0;
-    for (uint32_t q = 0; q < (pairs + 63) / 64; ++q) active += firsts[q];
-    for (uint32_t q = 0; q < pairs; ++q) count += sorted[q] != 0xFFFFFFFFu;
-    a.routing->active = active;
-    a.routing->start[active] = static_cast<uint16_t>(count);
-  }
+  __syncthreads();
+  if (writes)
+    for (uint32_t i = tid; i < sizeof(Routing) / 4; i += kRouteThreads)
+      reinterpret_cast<uint32_t*>(a.routing)[i] = reinterpret_cast<const uint32_t*>(&r)[i];
 }
 
 // ---- products -----------------------------------------------------------------------------------
 // A fragment's 32 codes of a lane's block as bf16: four operands of eight.
-__device__ __forceinline__ void widen(i32x4 codes, uint32_t scale, bf16x8 (&w)[4]) {
-  const float s = as_float(scale ? scale << 23 : 0x00400000u);
+template <int kFragment>
+__device__ __forceinline__ void widen(const Mx4Unit& unit, bf16x8 (&w)[4]) {
+  // the scale's byte as a float's exponent (2^-127 is below the normal floats)
+  const float s = as_float(max(unit.scales << (23 - 8 * kFragment) & 0x7F800000u, 0x00400000u));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t word = static_cast<uint32_t>(codes[i]);
+    const uint32_t word = static_cast<uint32_t>(unit.codes[kFragment][i]);
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 0);
     const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 1);
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, s, 2);
@@ -266,184 +410,363 @@ __device__ __forceinline__ void widen(i32x4 codes, uint32_t scale, bf16x8 (&w)[4
 struct Quad {
   bf16x8 v[4];
 };
-// 32 values of a row of parts; zeros where there is no row.
-__device__ __forceinline__ Quad load_quad(const uint16_t* p, bool there) {
-  Quad q = {};
-  if (there) {
+// 32 values of a row of parts: `row` is the same in every lane, `offset` (in bytes) a
+// lane's own. Lanes past an expert's last token read that token's again: a column of
+// the product that is not stored may hold anything.
+__device__ __forceinline__ Quad load_quad(const uint16_t* row, uint32_t offset) {
+  Quad q;
+  const char* const p = reinterpret_cast<const char*>(row) + offset;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q.v[i] = *reinterpret_cast<const bf16x8*>(p + 8 * i);
-  }
+  for (int i = 0; i < 4; ++i) q.v[i] = *reinterpret_cast<const bf16x8*>(p + 16 * i);
   return q;
 }
+__device__ __forceinline__ f32x4 multiply(const bf16x8 (&w)[4], const Quad& q, f32x4 acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], q.v[i], acc, 0, 0, 0);
+  return acc;
+}
+// f(integral constant) for both fragments of a unit.
+template <typename F>
+__device__ __forceinline__ void both_fragments(F&& f) {
+  f(std::integral_constant<int, 0>{});
+  f(std::integral_constant<int, 1>{});
+}
 
-constexpr int kHiddenWaves = 8, kHiddenThreads = 64 * kHiddenWaves;
+constexpr int kHiddenWaves = kRouteWaves, kHiddenThreads = kRouteThreads;
+constexpr uint32_t kLdsX = 32768;    // few tokens: values of x's parts that a workgroup holds
+constexpr uint32_t kLdsH = 49152;    // and of the hidden values'
+constexpr uint32_t kFewTokens = 16;  // that the down kernel's tables hold
+constexpr uint32_t kLdsRows = 65536;  // many: bytes of an expert's tokens
 
+// Four hidden values of a pair, rounded to parts.
+template <int kHiddenParts>
+__device__ __forceinline__ void store_hidden(uint16_t* to, int64_t part, const float (&v)[4]) {
+  uint16_t parts[4][kHiddenParts];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split<kHiddenParts>(v[i], parts[i]);
+#pragma unroll
+  for (int p = 0; p < kHiddenParts; ++p) {
+    const uint16_t four[4] = {parts[0][p], parts[1][p], parts[2][p], parts[3][p]};
+    __builtin_memcpy(to + p * part, four, 8);
+  }
+}
+
+// silu(g) u weight.
+__device__ __forceinline__ void gated(const f32x4& g, const f32x4& u, float weight, float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = g[i] / (1.0f + expf(-g[i])) * u[i] * weight;
+}
+
+// ---- hidden, few pairs: eight waves to 16 rows, the tokens' parts in LDS ------------------------
 template <int kParts, int kHiddenParts>
-__global__ __launch_bounds__(kHiddenThreads) void experts_hidden_kernel(ExpertsArgs a) {
-  __shared__ __attribute__((aligned(16))) f32x4 sums[kHiddenWaves][2][kMaxFrags][64];
+__global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(ExpertsArgs a) {
+  constexpr int U = 2;  // chunks whose weights are in flight together
+  __shared__ __attribute__((aligned(16))) union {
+    RouteScratch route;
+    f32x4 sums[kHiddenWaves][2][64];
+  } scratch;
+  __shared__ Routing lists;
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds_x[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t chunks = a.width_chunks, x_row = 256 * chunks, x_part = a.tokens * x_row;
+  for (uint32_t i = 8 * threadIdx.x; i < kParts * x_part; i += 8 * kHiddenThreads)
+    *reinterpret_cast<u32x4*>(lds_x + i) = *reinterpret_cast<const u32x4*>(a.x_parts + i);
+  route<true>(a, blockIdx.x == 0, scratch.route, lists);
+  __syncthreads();
   const uint32_t groups = 16 * a.inner_chunks, real = (a.inner + 15) / 16;  // the last are zeros
-  const uint32_t chunks = a.width_chunks, stride = chunks * kMx4Unit;
+  const uint32_t stride = chunks * kMx4Unit;
   const uint32_t first = chunks * wave / kHiddenWaves, last = chunks * (wave + 1) / kHiddenWaves;
-  const int64_t x_part = static_cast<int64_t>(a.tokens) * 256 * chunks;
   const int64_t h_row = 256 * static_cast<int64_t>(a.inner_chunks), h_part = static_cast<int64_t>(a.tokens) * a.top * h_row;
-  const uint32_t items = a.routing->active * groups;
+  const uint32_t items = lists.active * groups;
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint32_t slot = item / groups, group = item - slot * groups;
-    const uint32_t e = a.routing->expert[slot], start = a.routing->start[slot];
-    const uint32_t count = a.routing->start[slot + 1] - start, frags = (count + 15) / 16;
-    if (group < real) {
-      const uint8_t* const gate = a.gate + (static_cast<uint64_t>(e) * real + group) * stride;
-      const uint8_t* const up = a.up + (static_cast<uint64_t>(e) * real + group) * stride;
-      const uint16_t* row[kMaxFrags];
-      bool there[kMaxFrags];
+    const uint32_t e = lists.expert[slot], start = lists.start[slot], count = lists.start[slot + 1] - start;
+    const uint8_t* const gate = a.gate + (static_cast<uint64_t>(e) * real + group) * stride;
+    const uint8_t* const up = a.up + (static_cast<uint64_t>(e) * real + group) * stride;
+    const uint32_t r = lane & 15;
+    const uint32_t row = 2 * (lists.token[start + min(r, count - 1)] * x_row + 32 * (lane >> 4));
+    f32x4 acc[2] = {};
+    for (uint32_t c = first; c < (group < real ? last : first); c += U) {
+      Mx4Unit g[U], u[U];
 #pragma unroll
-      for (int f = 0; f < kMaxFrags; ++f) {
-        const uint32_t r = 16 * f + (lane & 15);
-        there[f] = r < count;
-        row[f] = a.x_parts + static_cast<int64_t>(there[f] ? a.routing->token[start + r] : 0) * 256 * chunks;
+      for (int i = 0; i < U; ++i) {
+        // (past the last it is read again and not used)
+        const uint32_t at = min(c + i, last - 1) * kMx4Unit;
+        g[i] = stream_unit(gate + at, lane);
+        u[i] = stream_unit(up + at, lane);
       }
-      f32x4 acc[2][kMaxFrags] = {};
-      Mx4Unit g = {}, u = {};
-      if (first < last) {
-        g = load_unit(gate + first * kMx4Unit, lane);
-        u = load_unit(up + first * kMx4Unit, lane);
-      }
-      for (uint32_t c = first; c < last; ++c) {
-        const uint32_t ahead = min(c + 1, last - 1) * kMx4Unit;
-        const Mx4Unit next_g = load_unit(gate + ahead, lane), next_u = load_unit(up + ahead, lane);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+      for (int i = 0; i < U; ++i) {
+        if (c + i >= last) break;
+        both_fragments([&](auto half) __attribute__((always_inline)) {
+          constexpr int h = decltype(half)::value;
           bf16x8 wg[4], wu[4];
-          widen(g.codes[h], g.scales >> (8 * h) & 0xFFu, wg);
-          widen(u.codes[h], u.scales >> (8 * h) & 0xFFu, wu);
-          const uint32_t k = 256 * c + 128 * h + 32 * (lane >> 4);
+          widen<h>(g[i], wg);
+          widen<h>(u[i], wu);
 #pragma unroll
-          for (int f = 0; f < kMaxFrags; ++f) {
-            if (f >= static_cast<int>(frags)) break;
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-              const Quad q = load_quad(row[f] + p * x_part + k, there[f]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                acc[0][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wg[i], q.v[i], acc[0][f], 0, 0, 0);
-                acc[1][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wu[i], q.v[i], acc[1][f], 0, 0, 0);
-              }
-            }
+          for (int p = 0; p < kParts; ++p) {
+            const Quad q = load_quad(lds_x + p * x_part + 256 * (c + i) + 128 * h, row);
+            acc[0] = multiply(wg, q, acc[0]);
+            acc[1] = multiply(wu, q, acc[1]);
           }
-        }
-        g = next_g;
-        u = next_u;
-      }
-#pragma unroll
-      for (int f = 0; f < kMaxFrags; ++f) {
-        if (f >= static_cast<int>(frags)) break;
-        sums[wave][0][f][lane] = acc[0][f];
-        sums[wave][1][f][lane] = acc[1][f];
+        });
       }
     }
+    scratch.sums[wave][0][lane] = acc[0];
+    scratch.sums[wave][1][lane] = acc[1];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 64 * frags; i += kHiddenThreads) {
-      const uint32_t f = i / 64, l = i % 64, r = 16 * f + l % 16;
-      if (r >= count) continue;
-      f32x4 hidden = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (group < real) {
-        f32x4 gv = sums[0][0][f][l], uv = sums[0][1][f][l];
+    if (wave == 0 && r < count) {
 #pragma unroll
-        for (int w = 1; w < kHiddenWaves; ++w) {
-          gv += sums[w][0][f][l];
-          uv += sums[w][1][f][l];
-        }
-        const float weight = a.routing->weight[start + r];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) hidden[v] = gv[v] / (1.0f + expf(-gv[v])) * uv[v] * weight;
+      for (int w = 1; w < kHiddenWaves; ++w) {
+        acc[0] += scratch.sums[w][0][lane];
+        acc[1] += scratch.sums[w][1][lane];
       }
-      uint16_t parts[4][kHiddenParts];
-#pragma unroll
-      for (int v = 0; v < 4; ++v) split<kHiddenParts>(hidden[v], parts[v]);
-      uint16_t* const out = a.h_parts + (start + r) * h_row + 16 * group + 4 * (l / 16);
-#pragma unroll
-      for (int p = 0; p < kHiddenParts; ++p) {
-        const uint16_t four[4] = {parts[0][p], parts[1][p], parts[2][p], parts[3][p]};
-        __builtin_memcpy(out + p * h_part, four, 8);
-      }
+      float v[4] = {};
+      if (group < real) gated(acc[0], acc[1], lists.weight[start + r], v);
+      store_hidden<kHiddenParts>(a.h_parts + (start + r) * h_row + 16 * group + 4 * (lane >> 4), h_part, v);
     }
     __syncthreads();
   }
 }
 
+// ---- many pairs: a wave takes 32 rows of one expert's weights -----------------------------------
+// (gate and up of 16 hidden values, or 32 channels of down.) The rows of all experts
+// that have tokens are cut evenly over the workgroups, in blocks of eight, a wave each; an expert's tokens, as many as fit, lie in LDS while its rows stream by, three
+// units' loads ahead. A further batch of tokens reads the weights again.
+template <bool kDown, int kParts, int kHiddenParts>
+__global__ __launch_bounds__(kHiddenThreads, 4) void experts_many_kernel(ExpertsArgs a) {
+  constexpr int D = 3;
+  __shared__ __attribute__((aligned(16))) union {
+    RouteScratch route;
+    uint8_t rows[kLdsRows];
+  } lds;
+  __shared__ Routing lists;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (kDown) {
+    for (uint32_t i = threadIdx.x; i < sizeof(Routing) / 4; i += kHiddenThreads)
+      reinterpret_cast<uint32_t*>(&lists)[i] = reinterpret_cast<const uint32_t*>(a.routing)[i];
+  } else {
+    route<false>(a, blockIdx.x == 0, lds.route, lists);
+  }
+  __syncthreads();
+  const uint32_t chunks = kDown ? a.inner_chunks : a.width_chunks, stride = chunks * kMx4Unit;
+  const uint32_t groups = ((kDown ? a.width : a.inner) + 15) / 16;  // of 16 rows of a matrix
+  const uint32_t per = kDown ? (groups + 1) / 2 : groups;           // a wave's turns to an expert
+  const uint32_t in_row = 256 * chunks;
+  const uint16_t* const in = kDown ? a.h_parts : a.x_parts;
+  const int64_t in_part = static_cast<int64_t>(a.tokens) * (kDown ? a.top : 1) * in_row;
+  const uint32_t out_row = kDown ? 16 * groups : 256 * a.inner_chunks;
+  const int64_t h_part = static_cast<int64_t>(a.tokens) * a.top * out_row;
+  // what LDS holds: `batch` tokens' values of `held` chunks, 16 bytes after each row (so
+  // that sixteen rows' reads meet no bank twice)
+  const uint32_t held = min(chunks, (kLdsRows / kParts - 16) / 512);
+  const uint32_t lds_row = 512 * held + 16;
+  const uint32_t batch = min(16u, kLdsRows / (kParts * lds_row));
+  const uint32_t lds_part = batch * lds_row;
+
+  // an item is eight turns of one expert
+  const uint32_t blocks = (per + kHiddenWaves - 1) / kHiddenWaves;
+  const uint64_t items = static_cast<uint64_t>(lists.active) * blocks;
+  const uint32_t begin = static_cast<uint32_t>(items * blockIdx.x / gridDim.x);
+  const uint32_t end = static_cast<uint32_t>(items * (blockIdx.x + 1) / gridDim.x);
+  for (uint32_t item = begin; item < end;) {
+    const uint32_t slot = item / blocks, block = item - slot * blocks, rounds = min(blocks - block, end - item);
+    item += rounds;
+    const uint32_t from = block * kHiddenWaves, to = min(per, from + rounds * kHiddenWaves), steps = rounds * chunks;
+    const uint32_t e = lists.expert[slot], start = lists.start[slot], count = lists.start[slot + 1] - start;
+    for (uint32_t r0 = 0; r0 < count; r0 += batch) {
+      const uint32_t tokens = min(batch, count - r0), r = lane & 15;
+      const uint32_t row = min(r, tokens - 1) * lds_row + 64 * (lane >> 4);
+      // Loads run three steps ahead, over rounds as well (past the last turn or step the
+      // last row again), and have no branches: a wait in the loop then counts them.
+      const uint64_t matrix = static_cast<uint64_t>(groups) * stride;
+      const uint8_t* const base0 = (kDown ? a.down : a.gate) + e * matrix;
+      const uint8_t* const base1 = (kDown ? a.down : a.up) + e * matrix;
+      uint32_t ahead_chunk = 0, ahead_turn = from + wave;
+      auto load = [&](Mx4Unit (&u)[2]) __attribute__((always_inline)) {
+        const uint32_t t = min(ahead_turn, to - 1);
+        // (an odd last group is read twice, its second results are not stored)
+        const uint32_t g0 = kDown ? 2 * t : t, g1 = kDown ? min(2 * t + 1, groups - 1) : t;
+        u[0] = stream_unit(base0 + static_cast<uint64_t>(g0) * stride + ahead_chunk * kMx4Unit, lane);
+        u[1] = stream_unit(base1 + static_cast<uint64_t>(g1) * stride + ahead_chunk * kMx4Unit, lane);
+        const bool wraps = ahead_chunk + 1 == chunks;
+        ahead_turn += wraps ? kHiddenWaves : 0;
+        ahead_chunk = wraps ? 0 : ahead_chunk + 1;
+      };
+      Mx4Unit w[D][2];
+#pragma unroll
+      for (int i = 0; i < D; ++i) load(w[i]);
+      f32x4 acc[2] = {};
+      uint32_t c = 0, held_at = 0, mine = from + wave;
+      bool staged = false;
+      for (uint32_t step = 0; step < steps; step += D) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+          if (step + i < steps) {
+            if (!staged || c - held_at >= held) {
+              held_at = c;
+              staged = true;
+              const uint32_t now = min(held, chunks - c), vectors = 32 * now;
+              __syncthreads();
+              for (uint32_t v = threadIdx.x; v < kParts * tokens * vectors; v += kHiddenThreads) {
+                const uint32_t line = v / vectors, at = v - line * vectors, p = line / tokens, t = line - p * tokens;
+                const uint32_t source = kDown ? start + r0 + t : lists.token[start + r0 + t];
+                *reinterpret_cast<u32x4*>(lds.rows + p * lds_part + t * lds_row + 16 * at) =
+                    *reinterpret_cast<const u32x4*>(in + p * in_part + static_cast<int64_t>(source) * in_row + 256 * c + 8 * at);
+              }
+              __syncthreads();
+            }
+            both_fragments([&](auto half) __attribute__((always_inline)) {
+              constexpr int h = decltype(half)::value;
+              bf16x8 w0[4], w1[4];
+              widen<h>(w[i][0], w0);
+              widen<h>(w[i][1], w1);
+#pragma unroll
+              for (int p = 0; p < kParts; ++p) {
+                const Quad q = load_quad(reinterpret_cast<const uint16_t*>(lds.rows + p * lds_part) + 256 * (c - held_at) + 128 * h, row);
+                acc[0] = multiply(w0, q, acc[0]);
+                acc[1] = multiply(w1, q, acc[1]);
+              }
+            });
+            if (++c == chunks) {
+              const uint32_t pair = start + r0 + r;
+              if (mine < to && r < tokens) {
+                if constexpr (kDown) {
+#pragma unroll
+                  for (uint32_t j = 0; j < 2; ++j)
+                    if (2 * mine + j < groups)
+                      *reinterpret_cast<f32x4*>(a.y + static_cast<int64_t>(pair) * out_row + 16 * (2 * mine + j) + 4 * (lane >> 4)) = acc[j];
+                } else {
+                  float v[4];
+                  gated(acc[0], acc[1], lists.weight[pair], v);
+                  uint16_t* const out = a.h_parts + static_cast<int64_t>(pair) * out_row + 4 * (lane >> 4);
+                  store_hidden<kHiddenParts>(out + 16 * mine, h_part, v);
+                  // the zeros after the last
+                  const float zeros[4] = {};
+                  if (mine + 1 == groups)
+                    for (uint32_t g = groups; g < 16 * a.inner_chunks; ++g) store_hidden<kHiddenParts>(out + 16 * g, h_part, zeros);
+                }
+              }
+              acc[0] = acc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+              c = 0;
+              mine += kHiddenWaves;
+              if (held < chunks) staged = false;
+            }
+          }
+          load(w[i]);
+        }
+      }
+    }
+  }
+}
+
+// ---- down, few pairs ------------------------------------------------------------------------------
 constexpr int kDownWaves = 16, kDownThreads = 64 * kDownWaves;
 
 template <int kHiddenParts, typename T>
-__global__ __launch_bounds__(kDownThreads) void experts_down_kernel(ExpertsArgs a) {
-  // [wave][token][16 channels]
-  extern __shared__ __attribute__((aligned(16))) float table[];
+__global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsArgs a) {
+  constexpr int U = 3;  // units in flight together
+  __shared__ __attribute__((aligned(16))) float table[kDownWaves][kFewTokens][16];
+  __shared__ __attribute__((aligned(16))) uint16_t lds_h[kLdsH];
+  __shared__ Routing lists;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t chunks = a.inner_chunks, stride = chunks * kMx4Unit, groups = (a.width + 15) / 16;
-  const uint32_t group = blockIdx.x, row = 16 * a.tokens;
-  const int64_t h_row = 256 * static_cast<int64_t>(chunks), h_part = static_cast<int64_t>(a.tokens) * a.top * h_row;
-  for (uint32_t i = threadIdx.x; i < kDownWaves * row; i += kDownThreads) table[i] = 0.0f;
+  const uint32_t chunks = a.inner_chunks, stride = chunks * kMx4Unit, groups = (a.width + 15) / 16, group = blockIdx.x;
+  const uint32_t h_row = 256 * chunks, pairs = a.tokens * a.top, h_part = pairs * h_row;
+  for (uint32_t i = threadIdx.x; i < sizeof(Routing) / 4; i += kDownThreads)
+    reinterpret_cast<uint32_t*>(&lists)[i] = reinterpret_cast<const uint32_t*>(a.routing)[i];
+  for (uint32_t i = threadIdx.x; i < kDownWaves * kFewTokens * 16; i += kDownThreads) (&table[0][0][0])[i] = 0.0f;
   __syncthreads();
-  const uint32_t units = a.routing->active * chunks;
+  const uint32_t units = lists.active * chunks;
   const uint32_t first = units * wave / kDownWaves, last = units * (wave + 1) / kDownWaves;
   auto unit_at = [&](uint32_t q) {
     const uint32_t slot = q / chunks, c = q - slot * chunks;
-    return load_unit(a.down + (static_cast<uint64_t>(a.routing->expert[slot]) * groups + group) * stride + c * kMx4Unit, lane);
+    return stream_unit(a.down + (static_cast<uint64_t>(lists.expert[slot]) * groups + group) * stride + c * kMx4Unit, lane);
   };
-  f32x4 acc[kMaxFrags] = {};
-  Mx4Unit now = {};
-  if (first < last) now = unit_at(first);
-  for (uint32_t q = first; q < last; ++q) {
-    const Mx4Unit next = unit_at(min(q + 1, last - 1));
+  Mx4Unit w[U] = {};
+  if (first < last) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) w[i] = unit_at(min(first + i, last - 1));
+  }
+  // (only pairs that there are have been written)
+  const uint32_t used = lists.start[lists.active] * h_row;
+  for (int p = 0; p < kHiddenParts; ++p)
+    for (uint32_t i = 8 * threadIdx.x; i < used; i += 8 * kDownThreads)
+      *reinterpret_cast<u32x4*>(lds_h + p * h_part + i) = *reinterpret_cast<const u32x4*>(a.h_parts + p * h_part + i);
+  __syncthreads();
+  f32x4 acc = {};
+  auto multiply_unit = [&](uint32_t q, const Mx4Unit& unit) __attribute__((always_inline)) {
     const uint32_t slot = q / chunks, c = q - slot * chunks;
-    const uint32_t start = a.routing->start[slot], count = a.routing->start[slot + 1] - start, frags = (count + 15) / 16;
+    const uint32_t start = lists.start[slot], count = lists.start[slot + 1] - start, r = lane & 15;
+    const uint32_t row = 2 * ((start + min(r, count - 1)) * h_row + 32 * (lane >> 4));
+    both_fragments([&](auto half) __attribute__((always_inline)) {
+      constexpr int h = decltype(half)::value;
+      bf16x8 wide[4];
+      widen<h>(unit, wide);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8 w[4];
-      widen(now.codes[h], now.scales >> (8 * h) & 0xFFu, w);
-      const uint32_t k = 256 * c + 128 * h + 32 * (lane >> 4);
-#pragma unroll
-      for (int f = 0; f < kMaxFrags; ++f) {
-        if (f >= static_cast<int>(frags)) break;
-        const uint32_t r = 16 * f + (lane & 15);
-#pragma unroll
-        for (int p = 0; p < kHiddenParts; ++p) {
-          const Quad v = load_quad(a.h_parts + p * h_part + (start + min(r, count - 1)) * h_row + k, r < count);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], v.v[i], acc[f], 0, 0, 0);
-        }
-      }
-    }
+      for (int p = 0; p < kHiddenParts; ++p) acc = multiply(wide, load_quad(lds_h + p * h_part + 256 * c + 128 * h, row), acc);
+    });
     if (c + 1 == chunks || q + 1 == last) {
       // the expert's share of its tokens (no token is twice in the list)
-#pragma unroll
-      for (int f = 0; f < kMaxFrags; ++f) {
-        if (f >= static_cast<int>(frags)) break;
-        const uint32_t r = 16 * f + (lane & 15);
-        if (r < count) {
-          f32x4* const at = reinterpret_cast<f32x4*>(table + wave * row + 16 * a.routing->token[start + r] + 4 * (lane >> 4));
-          *at += acc[f];
-        }
-        acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < count) {
+        f32x4* const sum = reinterpret_cast<f32x4*>(&table[wave][lists.token[start + r]][4 * (lane >> 4)]);
+        *sum += acc;
       }
+      acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    now = next;
-  }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < row / 4; i += kDownThreads) {
-    const uint32_t t = i / 4, channel = 16 * group + 4 * (i % 4);
-    f32x4 sum = *reinterpret_cast<const f32x4*>(table + 4 * i);
+  };
+  uint32_t base = first;
+  for (; base + U < last; base += U) {
 #pragma unroll
-    for (int w = 1; w < kDownWaves; ++w) sum += *reinterpret_cast<const f32x4*>(table + w * row + 4 * i);
-    const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-    if (channel < a.width) store4(static_cast<T*>(a.out) + t * a.ldo + channel, static_cast<int64_t>(a.width) - channel, v);
+    for (int i = 0; i < U; ++i) {
+      multiply_unit(base + i, w[i]);
+      w[i] = unit_at(min(base + U + i, last - 1));
+    }
   }
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+    if (base + i < last) multiply_unit(base + i, w[i]);
+  __syncthreads();
+  const uint32_t i = threadIdx.x;
+  if (i < 4 * a.tokens) {
+    const uint32_t t = i / 4, channel = 16 * group + 4 * (i % 4);
+    f32x4 sum = *reinterpret_cast<const f32x4*>(&table[0][t][4 * (i % 4)]);
+#pragma unroll
+    for (int v = 1; v < kDownWaves; ++v) sum += *reinterpret_cast<const f32x4*>(&table[v][t][4 * (i % 4)]);
+    const float out[4] = {sum[0], sum[1], sum[2], sum[3]};
+    if (channel < a.width) store4(static_cast<T*>(a.out) + t * a.ldo + channel, static_cast<int64_t>(a.width) - channel, out);
+  }
+}
+
+// Each token's pairs, by its slots: four channels to a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void experts_combine_kernel(ExpertsArgs a) {
+  const uint32_t row = (a.width + 15) / 16 * 16, quads = (a.width + 3) / 4;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.tokens * quads) return;
+  const uint32_t t = i / quads, channel = 4 * (i - t * quads);
+  f32x4 v[kMaxExpertTop], sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (uint32_t n = 0; n < kMaxExpertTop; ++n) {
+    v[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t place = n < a.top ? a.routing->place[t * a.top + n] : kNone;
+    if (place != kNone) v[n] = *reinterpret_cast<const f32x4*>(a.y + static_cast<int64_t>(place) * row + channel);
+  }
+#pragma unroll
+  for (uint32_t n = 0; n < kMaxExpertTop; ++n) sum += v[n];
+  const float out[4] = {sum[0], sum[1], sum[2], sum[3]};
+  store4(static_cast<T*>(a.out) + t * a.ldo + channel, static_cast<int64_t>(a.width) - channel, out);
 }
 
 int parts_of(uint32_t dtype) { return dtype == RNS8_MI355X_F32 ? 3 : dtype == RNS8_MI355X_F16 ? 2 : 1; }
 int hidden_parts_of(uint32_t dtype) { return dtype == RNS8_MI355X_F32 ? 3 : 2; }
 
-// The workspace: scores, the parts of x and of the hidden values, the lists.
+// Whether x and the hidden values fit a workgroup's LDS, and the tokens its tables.
+bool few(const rns8_mi355x_experts_mx4_args& a) {
+  return a.tokens <= kFewTokens && parts_of(a.dtype) * a.tokens * mx4_chunks(a.width) * 256 <= kLdsX &&
+         hidden_parts_of(a.dtype) * a.tokens * a.top * mx4_chunks(a.inner) * 256 <= kLdsH;
+}
+
+// The workspace: scores, the parts of x and of the hidden values, pairs' results, the lists.
 uint64_t lay_out(const rns8_mi355x_experts_mx4_args& a, ExpertsArgs& e) {
   uint8_t* const at = static_cast<uint8_t*>(a.workspace);
   uint64_t bytes = 0;
@@ -452,27 +775,49 @@ uint64_t lay_out(const rns8_mi355x_experts_mx4_args& a, ExpertsArgs& e) {
     bytes += round_up(size, 256);
     return got;
   };
-  const uint64_t tokens = static_cast<uint64_t>(a.tokens);
+  const uint64_t tokens = static_cast<uint64_t>(a.tokens), pairs = tokens * a.top;
   e.scores = reinterpret_cast<float*>(take(a.router ? tokens * static_cast<uint64_t>(a.experts) * sizeof(float) : 0));
   e.x_parts = reinterpret_cast<uint16_t*>(
       take(static_cast<uint64_t>(parts_of(a.dtype)) * tokens * static_cast<uint64_t>(mx4_chunks(a.width)) * 512));
   e.h_parts = reinterpret_cast<uint16_t*>(
-      take(static_cast<uint64_t>(hidden_parts_of(a.dtype)) * tokens * a.top * static_cast<uint64_t>(mx4_chunks(a.inner)) * 512));
+      take(static_cast<uint64_t>(hidden_parts_of(a.dtype)) * pairs * static_cast<uint64_t>(mx4_chunks(a.inner)) * 512));
+  e.chosen = a.ids;
+  e.chosen_weights = a.weights;
+  if (a.router && !few(a)) {
+    e.chosen = reinterpret_cast<int32_t*>(take(pairs * sizeof(int32_t)));
+    e.chosen_weights = reinterpret_cast<float*>(take(pairs * sizeof(float)));
+  }
+  e.y = reinterpret_cast<float*>(take(few(a) ? 0 : pairs * static_cast<uint64_t>(mx4_groups(a.width)) * 64));
   e.routing = reinterpret_cast<Routing*>(take(sizeof(Routing)));
   return bytes;
 }
 
 template <typename T, int kParts, int kHiddenParts>
-hipError_t launch_typed(const ExpertsArgs& e, hipStream_t stream) {
-  const uint32_t score_blocks = e.router ? (e.experts + 3) / 4 * ((e.tokens + kScoreTokens - 1) / kScoreTokens) : 0;
+hipError_t launch_typed(const ExpertsArgs& e, bool is_few, hipStream_t stream) {
   const uint32_t x_blocks = e.tokens * ((256 * e.width_chunks + 2047) / 2048);
-  hipLaunchKernelGGL((experts_stage_kernel<T, kParts>), dim3(score_blocks + x_blocks), dim3(256), 0, stream, e, score_blocks);
-  hipLaunchKernelGGL(experts_route_kernel, dim3(1), dim3(kRouteThreads), 0, stream, e);
-  const uint32_t most = std::min(e.experts, e.tokens * e.top) * 16 * e.inner_chunks;
-  hipLaunchKernelGGL((experts_hidden_kernel<kParts, kHiddenParts>), dim3(std::min(most, 256u * 8)), dim3(kHiddenThreads), 0,
-                     stream, e);
-  hipLaunchKernelGGL((experts_down_kernel<kHiddenParts, T>), dim3((e.width + 15) / 16), dim3(kDownThreads),
-                     kDownWaves * 16 * e.tokens * sizeof(float), stream, e);
+  auto stage = [&](auto experts, auto tokens) {
+    constexpr uint32_t kExperts = decltype(experts)::value, kTokens = decltype(tokens)::value;
+    const uint32_t blocks = e.router ? (e.experts + kExperts - 1) / kExperts * ((e.tokens + kTokens - 1) / kTokens) : 0;
+    hipLaunchKernelGGL((experts_stage_kernel<T, kParts, kExperts, kTokens>), dim3(blocks + x_blocks), dim3(256), 0, stream, e, blocks);
+  };
+  if (e.tokens <= 2)
+    stage(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  else
+    stage(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
+  const uint32_t active = std::min(e.experts, e.tokens * e.top), groups = (e.width + 15) / 16;
+  const dim3 threads(kHiddenThreads);
+  if (is_few) {
+    hipLaunchKernelGGL((experts_hidden_few_kernel<kParts, kHiddenParts>), dim3(std::min(active * 16 * e.inner_chunks, 512u)), threads,
+                       kParts * e.tokens * e.width_chunks * 512, stream, e);
+    hipLaunchKernelGGL((experts_down_few_kernel<kHiddenParts, T>), dim3(groups), dim3(kDownThreads), 0, stream, e);
+    return hipGetLastError();
+  }
+  if (e.router) hipLaunchKernelGGL(experts_choose_kernel, dim3(e.tokens), dim3(64), 0, stream, e);
+  // two workgroups to a CU
+  auto grid = [&](uint32_t turns) { return dim3(std::min(active * ((turns + kHiddenWaves - 1) / kHiddenWaves), 512u)); };
+  hipLaunchKernelGGL((experts_many_kernel<false, kParts, kHiddenParts>), grid((e.inner + 15) / 16), threads, 0, stream, e);
+  hipLaunchKernelGGL((experts_many_kernel<true, kHiddenParts, kHiddenParts>), grid((groups + 1) / 2), threads, 0, stream, e);
+  hipLaunchKernelGGL(experts_combine_kernel<T>, dim3((e.tokens * ((e.width + 3) / 4) + 255) / 256), dim3(256), 0, stream, e);
   return hipGetLastError();
 }
 
@@ -508,15 +853,14 @@ hipError_t launch_experts_mx4(const rns8_mi355x_experts_mx4_args& a, hipStream_t
   e.experts = static_cast<uint32_t>(a.experts);
   e.top = a.top;
   e.normalize = a.flags & RNS8_MI355X_EXPERTS_NORMALIZE;
-  e.dtype = a.dtype;
   e.width = static_cast<uint32_t>(a.width);
   e.inner = static_cast<uint32_t>(a.inner);
   e.width_chunks = static_cast<uint32_t>(mx4_chunks(a.width));
   e.inner_chunks = static_cast<uint32_t>(mx4_chunks(a.inner));
   lay_out(a, e);
-  if (a.dtype == RNS8_MI355X_F32) return launch_typed<float, 3, 3>(e, stream);
-  if (a.dtype == RNS8_MI355X_F16) return launch_typed<f16, 2, 2>(e, stream);
-  return launch_typed<bf16, 1, 2>(e, stream);
+  if (a.dtype == RNS8_MI355X_F32) return launch_typed<float, 3, 3>(e, few(a), stream);
+  if (a.dtype == RNS8_MI355X_F16) return launch_typed<f16, 2, 2>(e, few(a), stream);
+  return launch_typed<bf16, 1, 2>(e, few(a), stream);
 }
 
 }  // namespace rns8x

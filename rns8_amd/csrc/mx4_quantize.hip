@@ -2,14 +2,16 @@
 // read once and leaves as 0.53 bytes for each form.
 //
 //   * A lane holds 16 bytes (V = 4 or 8 columns) of each of its rows as loaded;
-//     sixteen lanes a row's 64 or 128 columns, so loads are whole lines.
+//     sixteen lanes a row's 64 or 128 columns, so loads are whole lines. A vector that
+//     the row's end cuts is the row's last 16 bytes, moved down: no lane waits for single
+//     elements (which took 15 us for a matrix of 1000 x 1101).
 //   * q (blocks along a row): a block is 4 or 8 neighbouring lanes, its largest
 //     magnitude two or three lane moves after the lane's own (as integers: two
 //     16-bit values at a time); v_cvt_scalef32_pk_fp4_* divides by the power of two
 //     and rounds two values, half to even, 6 at most.
 //   * q_t (blocks along a column): a lane's 32 rows are a block of each of its V
-//     columns, so both forms come from one read and without LDS.
-//   * Scales are gathered in LDS and leave as whole lines with the unit's.
+//     columns, so both forms come from one read.
+//   * Codes and scales are gathered in LDS as units and leave in whole lines.
 //   * Sums of columns (a bias' gradient) in 32 bits for each 128 rows, in a fixed
 //     order; a second kernel adds those.
 #include <algorithm>
@@ -18,14 +20,18 @@
 #include "mx4.hpp"
 #include "operators.hpp"
 #include "row_shape.hpp"
+#include "tables.hpp"
 
 namespace rns8x {
 namespace {
 
 struct Jobs {
   Mx4Quantize job[2];
-  int64_t blocks[2];  // workgroups' tiles
+  uint32_t tiles[2];
+  DivU31 chunks[2];  // of a row
 };
+
+__device__ __forceinline__ uint32_t div_u31(uint32_t n, DivU31 v) { return __umulhi(n << 1, v.mul) >> v.shift; }
 
 constexpr int kQuadSwap1 = 0xB1, kQuadSwap2 = 0x4E, kHalfMirror = 0x141;  // DPP controls
 
@@ -41,46 +47,74 @@ struct Shape {
   static constexpr int kHigh = 4 * kRows * kDown;
 };
 
+// A unit in LDS: its fragments with room after every block of 16 rows, then the
+// scales, and room again, so that neither form's writes meet in a bank.
+constexpr int kLdsFragment = 16 * 17 * 4, kLdsScales = 2 * kLdsFragment, kLdsUnit = kLdsScales + 128 + 32;
+__device__ __forceinline__ int lds_place(int fragment, int block, int row) {
+  return kLdsFragment * fragment + 16 * (17 * block + row);
+}
+
+// `count` units from LDS, `stride` bytes apart in memory.
+template <int kThreads>
+__device__ __forceinline__ void store_units(const uint8_t* lds, int64_t count, uint8_t* to, int64_t stride) {
+  for (uint32_t i = threadIdx.x; i < 136 * count; i += kThreads) {
+    const uint32_t unit = i / 136, v = i - 136 * unit;
+    const uint32_t at = v < 128 ? lds_place(v / 64, v % 64 / 16, v % 16) : kLdsScales + 16 * (v - 128);
+    *reinterpret_cast<u32x4*>(to + unit * stride + 16 * v) = *reinterpret_cast<const u32x4*>(lds + kLdsUnit * unit + at);
+  }
+}
+
 template <typename T, bool kTransposed>
 __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx4_kernel(Jobs jobs) {
   using S = Shape<T, kTransposed>;
   constexpr int V = S::V, R = S::kRows;
-  __shared__ __attribute__((aligned(16))) uint8_t row_scales[S::kHigh / 16 * 128];
-  __shared__ __attribute__((aligned(16))) uint8_t column_scales[kTransposed ? 2048 : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t row_units[S::kHigh / 16 * kLdsUnit];
+  __shared__ __attribute__((aligned(16))) uint8_t column_units[kTransposed ? 16 * kLdsUnit : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cl = lane & 15, g = lane >> 4;
   const int across = wave % S::kAcross, down = wave / S::kAcross;
-  for (int64_t tile = blockIdx.x; tile < jobs.blocks[0] + jobs.blocks[1]; tile += gridDim.x) {
-    const bool second = tile >= jobs.blocks[0];
+  for (uint32_t tile = blockIdx.x; tile < jobs.tiles[0] + jobs.tiles[1]; tile += gridDim.x) {
+    const bool second = tile >= jobs.tiles[0];
     const Mx4Quantize& job = jobs.job[second ? 1 : 0];
-    const int64_t at = second ? tile - jobs.blocks[0] : tile;
-    const int64_t chunks = mx4_chunks(job.cols), rows = job.rows, cols = job.cols;
-    const int64_t tile_row = at / chunks, chunk = at - tile_row * chunks;
-    const int64_t wave_r0 = tile_row * S::kHigh + down * (4 * R), wave_c0 = chunk * 256 + across * (16 * V);
-    const int64_t r0 = wave_r0 + g * R, c0 = wave_c0 + V * cl;
+    const DivU31 chunks_of = jobs.chunks[second ? 1 : 0];
+    const uint32_t at = second ? tile - jobs.tiles[0] : tile;
+    const uint32_t tile_row = div_u31(at, chunks_of), chunk = at - tile_row * chunks_of.d;
+    const int64_t chunks = chunks_of.d, rows = job.rows, cols = job.cols;
+    const int wave_row = down * (4 * R), wave_col = across * (16 * V);
+    const int64_t tile_r0 = static_cast<int64_t>(tile_row) * S::kHigh, wave_r0 = tile_r0 + wave_row;
+    const int64_t wave_c0 = static_cast<int64_t>(chunk) * 256 + wave_col, c0 = wave_c0 + V * cl;
+    // row i of this lane is row_of(i) of the tile: 32 neighbours, or every fourth row (a
+    // wave's four are then 64 bytes of a fragment)
+    constexpr int kRowStep = kTransposed ? 1 : 4;
+    auto row_of = [&](int i) { return wave_row + (kTransposed ? g * R : g) + kRowStep * i; };
     const T* const x = static_cast<const T*>(job.x);
+    const int64_t step = kRowStep * job.ldx;
     u32x4 raw[R];
     if (wave_r0 + 4 * R <= rows && wave_c0 + 16 * V <= cols) {
+      const T* p = x + (tile_r0 + row_of(0)) * job.ldx + c0;
 #pragma unroll
-      for (int i = 0; i < R; ++i) __builtin_memcpy(&raw[i], x + (r0 + i) * job.ldx + c0, 16);
+      for (int i = 0; i < R; ++i, p += step) __builtin_memcpy(&raw[i], p, 16);
+    } else if (wave_r0 >= rows || wave_c0 >= cols) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) raw[i] = u32x4{0, 0, 0, 0};
     } else {
+      // rows past the last read it again
+      const int64_t from = c0 + V <= cols ? c0 : cols - V;
+      const uint32_t drop = static_cast<uint32_t>(min<int64_t>(c0 - from, V) * sizeof(T));
+      const T* p = x + min(tile_r0 + row_of(0), rows - 1) * job.ldx + from;
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        raw[i] = u32x4{0, 0, 0, 0};
-        const T* const p = x + (r0 + i) * job.ldx + c0;
-        if (r0 + i < rows && c0 + V <= cols) {
-          __builtin_memcpy(&raw[i], p, 16);
-        } else if (r0 + i < rows && c0 < cols) {
-          T t[V] = {};
+        __builtin_memcpy(&raw[i], p, 16);
+        if (tile_r0 + row_of(i + 1) < rows) p += step;
+      }
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (c0 + e < cols) t[e] = p[e];
-          __builtin_memcpy(&raw[i], t, 16);
-        }
+      for (int i = 0; i < R; ++i) {
+        const u32x4 cut = drop_bytes(raw[i], drop);
+        raw[i] = drop < 16 && tile_r0 + row_of(i) < rows ? cut : u32x4{0, 0, 0, 0};
       }
     }
     // this lane's place in a unit of q: fragment, block of it, bytes of the block
-    const int in_chunk = across * 16 * V + V * cl;
+    const int in_chunk = wave_col + V * cl;
     const int fragment = in_chunk / 128, block = in_chunk % 128 / 32;
     if (job.q) {
 #pragma unroll
@@ -104,27 +138,19 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
           codes = mx4_codes<3, T>(codes, raw[i][3], s.scale);
         }
         if (s.code == 255u) codes = 0;
-        const int64_t row = r0 + i;
-        const int place = static_cast<int>(row & 15) + 16 * block;
-        uint8_t* const unit = job.q + (row >> 4) * chunks * kMx4Unit + chunk * kMx4Unit;
-        if constexpr (sizeof(T) == 4) {
-          codes |= dpp_move<kQuadSwap1>(codes) << 16;  // two lanes' codes, of which the even one writes both
-          if (row < mx4_groups(rows) * 16 && !(lane & 1))
-            *reinterpret_cast<uint32_t*>(unit + 1024 * fragment + 16 * place + 2 * (cl & 7)) = codes;
-        } else {
-          if (row < mx4_groups(rows) * 16)
-            *reinterpret_cast<uint32_t*>(unit + 1024 * fragment + 16 * place + 4 * (cl & 3)) = codes;
-        }
-        if (in_chunk % 32 == 0) {
-          const int local = static_cast<int>(row - tile_row * S::kHigh) >> 4;
-          row_scales[128 * local + 2 * place + fragment] = static_cast<uint8_t>(s.code);
-        }
+        const int row = row_of(i) & 15;
+        uint8_t* const unit = row_units + kLdsUnit * (row_of(i) >> 4);
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<uint16_t*>(unit + lds_place(fragment, block, row) + 2 * (cl & 7)) = static_cast<uint16_t>(codes);
+        else
+          *reinterpret_cast<uint32_t*>(unit + lds_place(fragment, block, row) + 4 * (cl & 3)) = codes;
+        if (in_chunk % 32 == 0) unit[kLdsScales + 2 * (row + 16 * block) + fragment] = static_cast<uint8_t>(s.code);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (all rows at once do not fit the registers)
       }
     }
     if constexpr (kTransposed) {
       if (job.q_t || job.sums) {
-        const int64_t t_stride = mx4_stride(rows);
-        const int64_t t_chunk = tile_row;  // 256 rows are a chunk of q_t, `down` its fragment
+        // 256 rows are a chunk of q_t, `down` its fragment, g the block of it
         uint32_t largest[4] = {};
 #pragma unroll
         for (int i = 0; i < R; ++i)
@@ -154,11 +180,11 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
             pair(std::integral_constant<int, 3>{});
             out[k] = s.code == 255u ? 0u : codes;
           }
-          const int64_t column = c0 + v;
-          const int place = static_cast<int>(column & 15) + 16 * g;
-          if (job.q_t && column < mx4_groups(cols) * 16)
-            *reinterpret_cast<u32x4*>(job.q_t + (column >> 4) * t_stride + t_chunk * kMx4Unit + 1024 * down + 16 * place) = out;
-          column_scales[128 * ((in_chunk + v) >> 4) + 2 * place + down] = static_cast<uint8_t>(s.code);
+          const int row = (in_chunk + v) & 15;
+          uint8_t* const unit = column_units + kLdsUnit * ((in_chunk + v) >> 4);
+          *reinterpret_cast<u32x4*>(unit + lds_place(down, g, row)) = out;
+          unit[kLdsScales + 2 * (row + 16 * g) + down] = static_cast<uint8_t>(s.code);
+          __builtin_amdgcn_sched_barrier(0);
           if (job.sums) {
             float sum = 0.0f;
 #pragma unroll
@@ -174,28 +200,78 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
             sum = as_float(a[0]) + as_float(a[1]);
             const auto b = __builtin_amdgcn_permlane32_swap(as_uint(sum), as_uint(sum), false, false);
             sum = as_float(b[0]) + as_float(b[1]);
-            if (g == 0 && column < cols && wave_r0 < rows) job.sums[(wave_r0 >> 7) * cols + column] = sum;
+            if (g == 0 && c0 + v < cols && wave_r0 < rows) job.sums[(wave_r0 >> 7) * cols + c0 + v] = sum;
           }
         }
       }
     }
     __syncthreads();
-    const int t = threadIdx.x;
-    if (job.q && t < S::kHigh / 16 * 8) {
-      const int64_t group = tile_row * (S::kHigh / 16) + t / 8;
-      if (group < mx4_groups(rows))
-        *reinterpret_cast<u32x4*>(job.q + (group * chunks + chunk) * kMx4Unit + kMx4Scales + t % 8 * 16) =
-            *reinterpret_cast<const u32x4*>(row_scales + 16 * t);
+    if (job.q) {
+      const int64_t group = static_cast<int64_t>(tile_row) * (S::kHigh / 16);
+      store_units<S::kThreads>(row_units, min<int64_t>(S::kHigh / 16, mx4_groups(rows) - group),
+                               job.q + (group * chunks + chunk) * kMx4Unit, chunks * kMx4Unit);
     }
     if constexpr (kTransposed) {
-      if (job.q_t && t < 128) {
-        const int64_t group = chunk * 16 + t / 8;
-        if (group < mx4_groups(cols))
-          *reinterpret_cast<u32x4*>(job.q_t + group * mx4_stride(rows) + tile_row * kMx4Unit + kMx4Scales + t % 8 * 16) =
-              *reinterpret_cast<const u32x4*>(column_scales + 16 * t);
+      if (job.q_t) {
+          const int64_t group = static_cast<int64_t>(chunk) * 16, t_stride = mx4_stride(rows);
+        store_units<S::kThreads>(column_units, min<int64_t>(16, mx4_groups(cols) - group),
+                                 job.q_t + group * t_stride + static_cast<int64_t>(tile_row) * kMx4Unit, t_stride);
       }
     }
     __syncthreads();
+  }
+}
+
+// Rows shorter than a vector: a thread takes a block of 32 values and loads them one
+// by one. kTransposed: the matrix is x's transpose.
+template <typename T, bool kTransposed>
+__global__ __launch_bounds__(64) void quantize_narrow_kernel(Mx4Quantize job) {
+  const int64_t rows = kTransposed ? job.cols : job.rows, cols = kTransposed ? job.rows : job.cols;
+  const int64_t chunks = mx4_chunks(cols), units = mx4_groups(rows) * chunks;
+  const int lane = threadIdx.x;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t group = u / chunks, chunk = u - group * chunks, r = group * 16 + (lane & 15);
+    uint8_t* const unit = (kTransposed ? job.q_t : job.q) + u * kMx4Unit;
+    uint32_t scales = 0;
+    for (int f = 0; f < 2; ++f) {
+      const int64_t c = chunk * 256 + 128 * f + 32 * (lane >> 4);
+      float v[32];
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int64_t at = kTransposed ? (c + e) * job.ldx + r : r * job.ldx + c + e;
+        v[e] = r < rows && c + e < cols ? static_cast<float>(static_cast<const T*>(job.x)[at]) : 0.0f;
+        bits = larger<float>(bits, magnitude_bits(v[e]));
+      }
+      const Mx4Scale s = mx4_scale(bits);
+      scales |= s.code << (8 * f);
+      u32x4 out;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t codes = mx4_codes<0>(0u, v[8 * q], v[8 * q + 1], s.scale);
+        codes = mx4_codes<1>(codes, v[8 * q + 2], v[8 * q + 3], s.scale);
+        codes = mx4_codes<2>(codes, v[8 * q + 4], v[8 * q + 5], s.scale);
+        codes = mx4_codes<3>(codes, v[8 * q + 6], v[8 * q + 7], s.scale);
+        out[q] = s.code == 255u ? 0u : codes;
+      }
+      *reinterpret_cast<u32x4*>(unit + 1024 * f + 16 * lane) = out;
+    }
+    *reinterpret_cast<uint16_t*>(unit + kMx4Scales + 2 * lane) = static_cast<uint16_t>(scales);
+  }
+}
+
+// Sums of 128 rows of a column to a thread.
+template <typename T>
+__global__ __launch_bounds__(64) void sum_narrow_kernel(Mx4Quantize job) {
+  const int64_t parts = (job.rows + 127) / 128;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x; i < parts * job.cols;
+       i += static_cast<int64_t>(gridDim.x) * 64) {
+    const int64_t part = i / job.cols, c = i - part * job.cols;
+    float sum = 0.0f;
+#pragma unroll 16
+    for (int64_t r = 128 * part; r < min(128 * part + 128, job.rows); ++r)
+      sum += static_cast<float>(static_cast<const T*>(job.x)[r * job.ldx + c]);
+    job.sums[i] = sum;
   }
 }
 
@@ -206,8 +282,16 @@ __global__ __launch_bounds__(256) void sum_partials_kernel(const float* partials
     __shared__ float part[4][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     float sum = 0.0f;
-    if (c < cols)
-      for (int64_t i = wave; i < count; i += 4) sum += partials[i * cols + c];
+    if (c < cols) {
+      for (int64_t i = wave; i < count; i += 32) {
+        // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = partials[min(i + 4 * j, count - 1) * cols + c];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += i + 4 * j < count ? v[j] : 0.0f;
+      }
+    }
     part[wave][lane] = sum;
     __syncthreads();
     if (wave == 0 && c < cols) sums[c] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
@@ -299,23 +383,49 @@ template <typename T, bool kTransposed>
 hipError_t launch_jobs(const Mx4Quantize* jobs, int count, hipStream_t stream) {
   using S = Shape<T, kTransposed>;
   Jobs j{};
+  int64_t tiles = 0;
   for (int i = 0; i < count; ++i) {
+    const int64_t chunks = mx4_chunks(jobs[i].cols), mine = (jobs[i].rows + S::kHigh - 1) / S::kHigh * chunks;
+    tiles += mine;
+    if (tiles > 0x3FFFFFFF) return hipErrorInvalidValue;
     j.job[i] = jobs[i];
-    // (of q_t, whole chunks of rows; of q alone, whole units)
-    j.blocks[i] = (jobs[i].rows + S::kHigh - 1) / S::kHigh * mx4_chunks(jobs[i].cols);
+    j.tiles[i] = static_cast<uint32_t>(mine);
+    j.chunks[i] = make_div_u31(static_cast<uint32_t>(chunks));
   }
-  const int64_t blocks = j.blocks[0] + j.blocks[1];
-  if (blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL((quantize_mx4_kernel<T, kTransposed>), dim3(static_cast<unsigned>(std::min(blocks, kMaxBlocks))),
+  if (tiles == 0) return hipSuccess;
+  hipLaunchKernelGGL((quantize_mx4_kernel<T, kTransposed>), dim3(static_cast<unsigned>(std::min(tiles, kMaxBlocks))),
                      dim3(S::kThreads), 0, stream, j);
   return hipGetLastError();
 }
 
 template <typename T>
+hipError_t launch_narrow(const Mx4Quantize& job, hipStream_t stream) {
+  auto grid = [](int64_t blocks) { return dim3(static_cast<unsigned>(std::min(blocks, kMaxBlocks))); };
+  if (job.rows == 0) return hipSuccess;
+  if (job.q)
+    hipLaunchKernelGGL((quantize_narrow_kernel<T, false>), grid(mx4_groups(job.rows)), dim3(64), 0, stream, job);
+  if (job.q_t)
+    hipLaunchKernelGGL((quantize_narrow_kernel<T, true>), grid(mx4_chunks(job.rows)), dim3(64), 0, stream, job);
+  if (job.sums)
+    hipLaunchKernelGGL(sum_narrow_kernel<T>, grid((job.rows + 127) / 128), dim3(64), 0, stream, job);
+  return hipGetLastError();
+}
+
+template <typename T>
 hipError_t launch_typed(const Mx4Quantize* jobs, int count, hipStream_t stream) {
+  Mx4Quantize wide[2];
+  int n = 0;
   bool transposed = false;
-  for (int i = 0; i < count; ++i) transposed = transposed || jobs[i].q_t || jobs[i].sums;
-  return transposed ? launch_jobs<T, true>(jobs, count, stream) : launch_jobs<T, false>(jobs, count, stream);
+  for (int i = 0; i < count; ++i) {
+    if (jobs[i].cols < 16 / static_cast<int64_t>(sizeof(T))) {
+      const hipError_t e = launch_narrow<T>(jobs[i], stream);
+      if (e != hipSuccess) return e;
+      continue;
+    }
+    wide[n++] = jobs[i];
+    transposed = transposed || jobs[i].q_t || jobs[i].sums;
+  }
+  return transposed ? launch_jobs<T, true>(wide, n, stream) : launch_jobs<T, false>(wide, n, stream);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

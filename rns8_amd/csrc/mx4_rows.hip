@@ -33,11 +33,22 @@ struct RowsArgs {
   uint32_t dtype;
 };
 
+// As many chunks as a wave has of 8192 columns, where the registers of two waves to a
+// SIMD hold them.
+template <int MB, int RB, typename T>
+constexpr int ring_depth() {
+  if constexpr (std::is_void_v<T>)
+    return MB + RB <= 4 ? 4 : MB + RB <= 5 ? 3 : 2;
+  else
+    return sizeof(T) == 4 ? 2 : RB == 2 ? 3 : 4;
+}
+
 // T: the rows' type, or void where they are an MX4 matrix.
 template <int kTokens16, int kChannels16, typename T>
 __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a) {
-  constexpr int MB = kTokens16, RB = kChannels16, U = 2;
+  constexpr int MB = kTokens16, RB = kChannels16;
   constexpr bool kFused = !std::is_void_v<T>;
+  constexpr int D = ring_depth<MB, RB, T>();  // chunks in flight
   __shared__ __attribute__((aligned(16))) f32x4 sums[kWaves][MB * RB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (16 * RB), m0 = static_cast<int64_t>(blockIdx.y) * (16 * MB);
@@ -52,55 +63,67 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a) {
 #pragma unroll
   for (int i = 0; i < MB; ++i) arow[i] = kFused ? nullptr : a.a + min(m0 / 16 + i, mx4_groups(a.m) - 1) * stride;
 
+  using X = std::conditional_t<kFused, T, float>;
   struct Group {
-    Mx4Unit w[U][RB], t[U][MB];
+    Mx4Unit w[RB], t[MB];
+    RawBlock<X> x[kFused ? 2 : 1];
   };
-  auto load = [&](uint32_t c, Group& f) {
+  // a lane's row of floating x, its block of each fragment
+  const int64_t mine = m0 + (lane & 15);
+  const bool live = mine < a.m;
+  const X* const row = static_cast<const X*>(a.x) + (live ? mine : 0) * a.ldx;
+  auto load = [&](uint32_t c, Group& f) __attribute__((always_inline)) {
+    // (past the wave's last chunk it is read again and not used)
+    const uint32_t chunk = min(c, last - 1);
+    const int64_t at = static_cast<int64_t>(chunk) * kMx4Unit;
+    if constexpr (kFused) {
+      // the rows first: loads return in order, and rounding them takes time
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (groups past the wave's last chunk read it again and are not used)
-      const int64_t at = static_cast<int64_t>(min(c + u, last - 1)) * kMx4Unit;
+      for (int h = 0; h < 2; ++h) load_block(row, 256 * chunk + 128 * h + 32 * (lane >> 4), a.k, f.x[h]);
+    }
 #pragma unroll
-      for (int j = 0; j < RB; ++j) f.w[u][j] = load_unit(wrow[j] + at, lane);
-      if constexpr (!kFused) {
+    for (int j = 0; j < RB; ++j) f.w[j] = stream_unit(wrow[j] + at, lane);
+    if constexpr (!kFused) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) f.t[u][i] = load_unit(arow[i] + at, lane);
-      }
+      for (int i = 0; i < MB; ++i) f.t[i] = load_unit(arow[i] + at, lane);
     }
   };
   f32x4 acc[MB][RB] = {};
-  auto multiply = [&](uint32_t c, Group& f) {
+  auto multiply = [&](uint32_t c, Group& f) __attribute__((always_inline)) {
+    if constexpr (kFused) {
+      f.t[0].scales = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c + u >= last) break;  // the same in every lane
-      if constexpr (kFused) {
-        static_assert(MB == 1, "one fragment of floating rows");
-        const int64_t token = m0 + (lane & 15);
-        const uint32_t k0 = 256 * (c + u) + 32 * (lane >> 4);
-        const T* const row = static_cast<const T*>(a.x) + (token < a.m ? token : 0) * a.ldx;
-        f.t[u][0].scales = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Mx4Block b = round_block(row, token < a.m ? k0 + 128 * h : a.k, a.k);
-          f.t[u][0].codes[h] = b.codes;
-          f.t[u][0].scales |= b.scale << (8 * h);
-        }
+      for (int h = 0; h < 2; ++h) {
+        cut_block(row, 256 * c + 128 * h + 32 * (lane >> 4), live ? a.k : 0, f.x[h]);
+        const Mx4Block b = round_block(f.x[h]);
+        f.t[0].codes[h] = b.codes;
+        f.t[0].scales |= b.scale << (8 * h);
       }
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
-          acc[i][j] = mx4_mfma<0>(f.w[u][j].codes[0], f.t[u][i].codes[0], acc[i][j], f.w[u][j].scales, f.t[u][i].scales);
-          acc[i][j] = mx4_mfma<1>(f.w[u][j].codes[1], f.t[u][i].codes[1], acc[i][j], f.w[u][j].scales, f.t[u][i].scales);
-        }
     }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        acc[i][j] = mx4_mfma<0>(f.w[j].codes[0], f.t[i].codes[0], acc[i][j], f.w[j].scales, f.t[i].scales);
+        acc[i][j] = mx4_mfma<1>(f.w[j].codes[1], f.t[i].codes[1], acc[i][j], f.w[j].scales, f.t[i].scales);
+      }
   };
-  Group now, next;
-  if (first < last) load(first, now);
-  for (uint32_t c = first; c < last; c += U) {
-    if (c + U < last) load(c + U, next);
-    multiply(c, now);
-    now = next;
+  // a ring of D chunks' loads, without branches about them: a wait then counts them
+  if (first < last) {
+    Group ring[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(first + d, ring[d]);
+    uint32_t c = first;
+    for (; c + D < last; c += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        multiply(c + d, ring[d]);
+        load(c + D + d, ring[d]);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (c + d < last) multiply(c + d, ring[d]);
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i)
