@@ -58,22 +58,25 @@ struct RawBlock {
   uint32_t raw[kWords];
 };
 
-// Columns [c, c + 32) of a row of k values. Where the row ends before their end its
-// first 32 are loaded instead, and cut_block takes what there is one by one.
+// Columns [c, c + 32) of a row of k values: all there, or zeros past its end.
 template <typename T>
-__device__ __forceinline__ void load_block(const T* row, uint32_t c, uint32_t k, RawBlock<T>& b) {
-  if (k >= 32) __builtin_memcpy(b.raw, row + (c + 32 <= k ? c : 0), sizeof(b.raw));
+__device__ __forceinline__ void load_block(const T* row, uint32_t c, RawBlock<T>& b) {
+  __builtin_memcpy(b.raw, row + c, sizeof(b.raw));
 }
 template <typename T>
-__device__ __forceinline__ void cut_block(const T* row, uint32_t c, uint32_t k, RawBlock<T>& b) {
-  if (c + 32 <= k) return;
-  T t[32] = {};
-  if (c < k) {
+__device__ __forceinline__ void load_cut_block(const T* row, uint32_t c, uint32_t k, RawBlock<T>& b) {
 #pragma unroll
-    for (uint32_t e = 0; e < 32; ++e)
-      if (c + e < k) t[e] = row[c + e];
+  for (uint32_t i = 0; i < 32; i += 8) {
+    T t[8] = {};
+    if (c + i + 8 <= k) {
+      __builtin_memcpy(t, row + c + i, sizeof(t));
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e)
+        if (c + i + e < k) t[e] = row[c + i + e];
+    }
+    __builtin_memcpy(b.raw + i * sizeof(T) / 4, t, sizeof(t));
   }
-  __builtin_memcpy(b.raw, t, sizeof(b.raw));
 }
 
 template <typename T>
