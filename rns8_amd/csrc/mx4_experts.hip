@@ -221,6 +221,10 @@ __device__ __forceinline__ uint32_t score_key(float v) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return as_float(key == 0xFFFFFFFFu ? 0x7FC00000u : key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+}
+
 // A wave's choice for one token of at most 64 kPer experts, the largest left `top` times:
 // put(slot, expert, weight) by the lanes that hold them.
 template <int kPer, typename Put>
@@ -237,23 +241,22 @@ __device__ __forceinline__ void choose_of(const ExpertsArgs& a, uint32_t t, int 
   float largest = 0.0f, chosen = 0.0f;
   uint32_t id = 0;
   for (uint32_t n = 0; n < a.top; ++n) {
-    uint32_t best = 0, at = 0;
+    uint32_t best = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = 64u * i + lane;
-      }
+    for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
     const uint32_t top = wave_reduce(best, MaxU{});
-    const uint32_t e = ~wave_reduce(best == top ? ~at : 0u, MaxU{});
-    float mine = 0.0f;
+    // the first of those that have it
+    uint32_t e = 0;
+    bool found = false;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (64u * i + lane == e) {
-        key[i] = 0;
-        mine = score[i];
-      }
-    const float value = as_float(__builtin_amdgcn_readlane(as_uint(mine), __builtin_amdgcn_readfirstlane(e & 63u)));
+    for (int i = 0; i < kPer; ++i) {
+      const uint64_t has = __ballot(key[i] == top);
+      const bool here = !found && has != 0;
+      e = here ? 64u * i + static_cast<uint32_t>(__builtin_ctzll(has)) : e;
+      if (here && static_cast<uint32_t>(lane) == (e & 63u)) key[i] = 0;
+      found = found || here;
+    }
+    const float value = score_of(top);
     if (n == 0) largest = value;
     if (lane == static_cast<int>(n)) {
       id = e;
@@ -295,6 +298,50 @@ __global__ __launch_bounds__(64) void experts_choose_kernel(ExpertsArgs a) {
   });
 }
 
+// The lists of at most 64 pairs, in LDS: one wave's work, a pair to a lane.
+__device__ __forceinline__ void list_few(const ExpertsArgs& a, int lane, uint32_t id, float weight, Routing& r) {
+  const uint32_t pairs = a.tokens * a.top, token = lane / a.top;
+  const bool live = static_cast<uint32_t>(lane) < pairs;
+  auto pair_id = [&](uint32_t q) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(id), static_cast<int>(q))); };
+  // an expert that a token has twice is one pair, the first, with both weights
+  bool counts = live && id != kNone;
+  if (!a.router) {
+    const uint32_t first = token * a.top, end = first + a.top;
+    for (uint32_t q = 0; q < pairs; ++q) {
+      const bool same = counts && pair_id(q) == id && q >= first && q < end;
+      const float other = as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(as_uint(weight)), static_cast<int>(q))));
+      if (same && q > static_cast<uint32_t>(lane)) weight += other;
+      if (same && q < static_cast<uint32_t>(lane)) counts = false;
+    }
+  }
+  const uint64_t counted = __ballot(counts);
+  const uint32_t key = counts ? id << 6 | lane : 0xFFFFFFFFu;  // (1024 experts, 64 pairs)
+  uint32_t rank = 0, same_before = 0;
+  for (uint32_t q = 0; q < pairs; ++q) {
+    const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), static_cast<int>(q)));
+    rank += other < key;
+    same_before += other < key && other >> 6 == id;
+  }
+  const uint64_t firsts = __ballot(counts && same_before == 0);
+  // the experts before: the first pairs with a smaller key, whose ids are smaller then
+  uint32_t index = 0;
+  for (uint64_t left = firsts; left; left &= left - 1)
+    index += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), __builtin_ctzll(left))) < key;
+  if (counts) {
+    r.token[rank] = static_cast<uint16_t>(token);
+    r.weight[rank] = weight;
+    if (same_before == 0) {
+      r.expert[index] = static_cast<uint16_t>(id);
+      r.start[index] = static_cast<uint16_t>(rank);
+    }
+  }
+  if (live) r.place[lane] = static_cast<uint16_t>(counts ? rank : kNone);
+  if (lane == 0) {
+    r.active = static_cast<uint32_t>(__popcll(firsts));
+    r.start[__popcll(firsts)] = static_cast<uint16_t>(__popcll(counted));
+  }
+}
+
 // The lists, in LDS; all kRouteThreads threads. writes: this workgroup gives the
 // next kernels the lists, and the caller its experts and weights where they are chosen
 // here (kChooses).
@@ -302,6 +349,42 @@ template <bool kChooses>
 __device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteScratch& s, Routing& r) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t pairs = a.tokens * a.top, tid = threadIdx.x;
+  auto give = [&]() {
+    if (writes)
+      for (uint32_t i = tid; i < sizeof(Routing) / 4; i += kRouteThreads)
+        reinterpret_cast<uint32_t*>(a.routing)[i] = reinterpret_cast<const uint32_t*>(&r)[i];
+  };
+  if (kChooses && pairs <= 64) {
+    if (a.router) {
+      for (uint32_t t = wave; t < a.tokens; t += kRouteWaves)
+        choose(a, t, lane, [&](uint32_t slot, uint32_t id, float weight) {
+          const uint32_t pair = t * a.top + slot;
+          s.id[pair] = static_cast<uint16_t>(id);
+          s.weight[pair] = weight;
+          if (writes && a.ids) a.ids[pair] = static_cast<int32_t>(id);
+          if (writes && a.weights) a.weights[pair] = weight;
+        });
+      if (a.tokens > 1) __syncthreads();
+    }
+    if (wave == 0) {
+      uint32_t id = kNone;
+      float weight = 0.0f;
+      if (static_cast<uint32_t>(lane) < pairs) {
+        if (a.router) {
+          id = s.id[lane];
+          weight = s.weight[lane];
+        } else {
+          const int32_t given = a.chosen[lane];
+          id = given >= 0 && given < static_cast<int32_t>(a.experts) ? static_cast<uint32_t>(given) : kNone;
+          weight = a.chosen_weights[lane];
+        }
+      }
+      list_few(a, lane, id, weight, r);
+    }
+    __syncthreads();
+    give();
+    return;
+  }
   for (uint32_t e = tid; e < a.experts; e += kRouteThreads) s.tokens[0][e] = s.tokens[1][e] = 0;
   if (kChooses && a.router) {
     for (uint32_t t = wave; t < a.tokens; t += kRouteWaves)
@@ -385,9 +468,7 @@ __device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteSc
     r.place[pair] = static_cast<uint16_t>(at);
   }
   __syncthreads();
-  if (writes)
-    for (uint32_t i = tid; i < sizeof(Routing) / 4; i += kRouteThreads)
-      reinterpret_cast<uint32_t*>(a.routing)[i] = reinterpret_cast<const uint32_t*>(&r)[i];
+  give();
 }
 
 // ---- products -----------------------------------------------------------------------------------
@@ -469,9 +550,13 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(E
   extern __shared__ __attribute__((aligned(16))) uint16_t lds_x[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t chunks = a.width_chunks, x_row = 256 * chunks, x_part = a.tokens * x_row;
-  for (uint32_t i = 8 * threadIdx.x; i < kParts * x_part; i += 8 * kHiddenThreads)
-    *reinterpret_cast<u32x4*>(lds_x + i) = *reinterpret_cast<const u32x4*>(a.x_parts + i);
+  // (x's first values are on their way while the experts are chosen)
+  const uint32_t mine = 8 * threadIdx.x;
+  const u32x4 early = *reinterpret_cast<const u32x4*>(a.x_parts + min(mine, kParts * x_part - 8));
   route<true>(a, blockIdx.x == 0, scratch.route, lists);
+  if (mine < kParts * x_part) *reinterpret_cast<u32x4*>(lds_x + mine) = early;
+  for (uint32_t i = mine + 8 * kHiddenThreads; i < kParts * x_part; i += 8 * kHiddenThreads)
+    *reinterpret_cast<u32x4*>(lds_x + i) = *reinterpret_cast<const u32x4*>(a.x_parts + i);
   __syncthreads();
   const uint32_t groups = 16 * a.inner_chunks, real = (a.inner + 15) / 16;  // the last are zeros
   const uint32_t stride = chunks * kMx4Unit;
@@ -674,6 +759,13 @@ __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsA
   const uint32_t h_row = 256 * chunks, pairs = a.tokens * a.top, h_part = pairs * h_row;
   for (uint32_t i = threadIdx.x; i < sizeof(Routing) / 4; i += kDownThreads)
     reinterpret_cast<uint32_t*>(&lists)[i] = reinterpret_cast<const uint32_t*>(a.routing)[i];
+  // The hidden values are asked for before the weights: loads return in order. (Pairs that
+  // there are not hold anything, and meet no weights.)
+  constexpr int kVectors = kLdsH / (8 * kDownThreads);
+  u32x4 early[kVectors];
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+    early[i] = *reinterpret_cast<const u32x4*>(a.h_parts + min(8 * (threadIdx.x + i * kDownThreads), kHiddenParts * h_part - 8));
   for (uint32_t i = threadIdx.x; i < kDownWaves * kFewTokens * 16; i += kDownThreads) (&table[0][0][0])[i] = 0.0f;
   __syncthreads();
   const uint32_t units = lists.active * chunks;
@@ -687,11 +779,11 @@ __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsA
 #pragma unroll
     for (int i = 0; i < U; ++i) w[i] = unit_at(min(first + i, last - 1));
   }
-  // (only pairs that there are have been written)
-  const uint32_t used = lists.start[lists.active] * h_row;
-  for (int p = 0; p < kHiddenParts; ++p)
-    for (uint32_t i = 8 * threadIdx.x; i < used; i += 8 * kDownThreads)
-      *reinterpret_cast<u32x4*>(lds_h + p * h_part + i) = *reinterpret_cast<const u32x4*>(a.h_parts + p * h_part + i);
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const uint32_t at = 8 * (threadIdx.x + i * kDownThreads);
+    if (at < kHiddenParts * h_part) *reinterpret_cast<u32x4*>(lds_h + at) = early[i];
+  }
   __syncthreads();
   f32x4 acc = {};
   auto multiply_unit = [&](uint32_t q, const Mx4Unit& unit) __attribute__((always_inline)) {
