@@ -34,13 +34,15 @@ inline uint64_t mx4_bytes(int64_t rows, int64_t cols) {
 struct Mx4Scale {
   uint32_t code;  // the scale's byte
   float scale;    // the same as a float, as the conversions take it
+  bool bad;       // the block has no finite scale: its codes are zeros
 };
-// Of a block whose largest magnitude has these bits (as a float).
+// Of a block whose largest magnitude has these bits (as a float): its exponent less
+// two, at least 2^-127, which is below the normal floats.
 __device__ __forceinline__ Mx4Scale mx4_scale(uint32_t amax_bits) {
-  const uint32_t exponent = amax_bits >> 23;
-  const uint32_t code = exponent < 2 ? 0u : exponent - 2;
-  // (2^-127 is below the normal floats)
-  return {exponent == 255u ? 255u : code, as_float(code ? code << 23 : 0x00400000u)};
+  const uint32_t exponent = amax_bits & 0x7F800000u;
+  const int32_t scale = max(static_cast<int32_t>(exponent) - 0x01000000, 0x00400000);
+  const bool bad = exponent == 0x7F800000u;
+  return {bad ? 255u : static_cast<uint32_t>(scale) >> 23, as_float(static_cast<uint32_t>(scale)), bad};
 }
 
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));

@@ -104,7 +104,7 @@ __device__ __forceinline__ Mx4Block round_block(const RawBlock<T>& b) {
     pair(std::integral_constant<int, 1>{});
     pair(std::integral_constant<int, 2>{});
     pair(std::integral_constant<int, 3>{});
-    out.codes[q] = s.code == 255u ? 0 : static_cast<int>(codes);
+    out.codes[q] = s.bad ? 0 : static_cast<int>(codes);
   }
   return out;
 }

@@ -36,13 +36,13 @@ __device__ __forceinline__ uint32_t div_u31(uint32_t n, DivU31 v) { return __umu
 constexpr int kQuadSwap1 = 0xB1, kQuadSwap2 = 0x4E, kHalfMirror = 0x141;  // DPP controls
 
 // A workgroup's tile is 256 columns wide; kRows rows to a lane, of which a wave has
-// four times as many. kTransposed: the tile is 256 rows high and q_t may be wanted.
+// four times as many. kTransposed: the tile is 128 rows high, a fragment of q_t's units.
 template <typename T, bool kTransposed>
 struct Shape {
   static constexpr int V = 16 / sizeof(T);
   static constexpr int kAcross = 16 / V;
   static constexpr int kRows = kTransposed ? 32 : 8;
-  static constexpr int kDown = kTransposed ? 2 : 4 / kAcross;
+  static constexpr int kDown = kTransposed ? 1 : 4 / kAcross;
   static constexpr int kThreads = 64 * kAcross * kDown;
   static constexpr int kHigh = 4 * kRows * kDown;
 };
@@ -64,12 +64,24 @@ __device__ __forceinline__ void store_units(const uint8_t* lds, int64_t count, u
   }
 }
 
+// Fragment `fragment` of 16 units of q_t: the codes, then the scales, every other byte.
+constexpr int kLdsColumns = kLdsFragment + 64 + 16;
+template <int kThreads>
+__device__ __forceinline__ void store_fragments(const uint8_t* lds, int64_t count, int fragment, uint8_t* to, int64_t stride) {
+  for (uint32_t i = threadIdx.x; i < 64 * count; i += kThreads) {
+    const uint32_t unit = i / 64, place = i % 64;
+    *reinterpret_cast<u32x4*>(to + unit * stride + 1024 * fragment + 16 * place) =
+        *reinterpret_cast<const u32x4*>(lds + kLdsColumns * unit + lds_place(0, place / 16, place % 16));
+    to[unit * stride + kMx4Scales + 2 * place + fragment] = lds[kLdsColumns * unit + kLdsFragment + place];
+  }
+}
+
 template <typename T, bool kTransposed>
 __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx4_kernel(Jobs jobs) {
   using S = Shape<T, kTransposed>;
   constexpr int V = S::V, R = S::kRows;
   __shared__ __attribute__((aligned(16))) uint8_t row_units[S::kHigh / 16 * kLdsUnit];
-  __shared__ __attribute__((aligned(16))) uint8_t column_units[kTransposed ? 16 * kLdsUnit : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t column_units[kTransposed ? 16 * kLdsColumns : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cl = lane & 15, g = lane >> 4;
   const int across = wave % S::kAcross, down = wave / S::kAcross;
@@ -137,7 +149,7 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
           codes = mx4_codes<2, T>(codes, raw[i][2], s.scale);
           codes = mx4_codes<3, T>(codes, raw[i][3], s.scale);
         }
-        if (s.code == 255u) codes = 0;
+        if (s.bad) codes = 0;
         const int row = row_of(i) & 15;
         uint8_t* const unit = row_units + kLdsUnit * (row_of(i) >> 4);
         if constexpr (sizeof(T) == 4)
@@ -150,7 +162,7 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
     }
     if constexpr (kTransposed) {
       if (job.q_t || job.sums) {
-        // 256 rows are a chunk of q_t, `down` its fragment, g the block of it
+        // 256 rows are a chunk of q_t, this tile one of its fragments, g the block of it
         uint32_t largest[4] = {};
 #pragma unroll
         for (int i = 0; i < R; ++i)
@@ -178,12 +190,12 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
             pair(std::integral_constant<int, 1>{});
             pair(std::integral_constant<int, 2>{});
             pair(std::integral_constant<int, 3>{});
-            out[k] = s.code == 255u ? 0u : codes;
+            out[k] = s.bad ? 0u : codes;
           }
           const int row = (in_chunk + v) & 15;
-          uint8_t* const unit = column_units + kLdsUnit * ((in_chunk + v) >> 4);
-          *reinterpret_cast<u32x4*>(unit + lds_place(down, g, row)) = out;
-          unit[kLdsScales + 2 * (row + 16 * g) + down] = static_cast<uint8_t>(s.code);
+          uint8_t* const unit = column_units + kLdsColumns * ((in_chunk + v) >> 4);
+          *reinterpret_cast<u32x4*>(unit + lds_place(0, g, row)) = out;
+          unit[kLdsFragment + row + 16 * g] = static_cast<uint8_t>(s.code);
           __builtin_amdgcn_sched_barrier(0);
           if (job.sums) {
             float sum = 0.0f;
@@ -214,8 +226,8 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
     if constexpr (kTransposed) {
       if (job.q_t) {
           const int64_t group = static_cast<int64_t>(chunk) * 16, t_stride = mx4_stride(rows);
-        store_units<S::kThreads>(column_units, min<int64_t>(16, mx4_groups(cols) - group),
-                                 job.q_t + group * t_stride + static_cast<int64_t>(tile_row) * kMx4Unit, t_stride);
+        store_fragments<S::kThreads>(column_units, min<int64_t>(16, mx4_groups(cols) - group), tile_row & 1,
+                                     job.q_t + group * t_stride + static_cast<int64_t>(tile_row / 2) * kMx4Unit, t_stride);
       }
     }
     __syncthreads();
@@ -252,7 +264,7 @@ __global__ __launch_bounds__(64) void quantize_narrow_kernel(Mx4Quantize job) {
         codes = mx4_codes<1>(codes, v[8 * q + 2], v[8 * q + 3], s.scale);
         codes = mx4_codes<2>(codes, v[8 * q + 4], v[8 * q + 5], s.scale);
         codes = mx4_codes<3>(codes, v[8 * q + 6], v[8 * q + 7], s.scale);
-        out[q] = s.code == 255u ? 0u : codes;
+        out[q] = s.bad ? 0u : codes;
       }
       *reinterpret_cast<u32x4*>(unit + 1024 * f + 16 * lane) = out;
     }
@@ -385,7 +397,9 @@ hipError_t launch_jobs(const Mx4Quantize* jobs, int count, hipStream_t stream) {
   Jobs j{};
   int64_t tiles = 0;
   for (int i = 0; i < count; ++i) {
-    const int64_t chunks = mx4_chunks(jobs[i].cols), mine = (jobs[i].rows + S::kHigh - 1) / S::kHigh * chunks;
+    // (of q_t whole units, which are two tiles high)
+    const int64_t chunks = mx4_chunks(jobs[i].cols);
+    const int64_t mine = (kTransposed ? 2 * mx4_chunks(jobs[i].rows) : (jobs[i].rows + S::kHigh - 1) / S::kHigh) * chunks;
     tiles += mine;
     if (tiles > 0x3FFFFFFF) return hipErrorInvalidValue;
     j.job[i] = jobs[i];
