@@ -29,6 +29,9 @@ struct Jobs {
   Mx4Quantize job[2];
   uint32_t tiles[2];
   DivU31 chunks[2];  // of a row
+  // both forms of a tile by workgroups of their own, which read it twice: where a SIMD
+  // would have one wave or none (1024 x 1024 in bf16 9.2 us together, 6.2 apart)
+  uint32_t apart;
 };
 
 __device__ __forceinline__ uint32_t div_u31(uint32_t n, DivU31 v) { return __umulhi(n << 1, v.mul) >> v.shift; }
@@ -85,7 +88,9 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cl = lane & 15, g = lane >> 4;
   const int across = wave % S::kAcross, down = wave / S::kAcross;
-  for (uint32_t tile = blockIdx.x; tile < jobs.tiles[0] + jobs.tiles[1]; tile += gridDim.x) {
+  for (uint32_t turn = blockIdx.x; turn < (jobs.tiles[0] + jobs.tiles[1]) << jobs.apart; turn += gridDim.x) {
+    const uint32_t tile = turn >> jobs.apart;
+    const bool rows_here = !jobs.apart || (turn & 1) == 0, columns_here = !jobs.apart || (turn & 1) == 1;
     const bool second = tile >= jobs.tiles[0];
     const Mx4Quantize& job = jobs.job[second ? 1 : 0];
     const DivU31 chunks_of = jobs.chunks[second ? 1 : 0];
@@ -128,7 +133,8 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
     // this lane's place in a unit of q: fragment, block of it, bytes of the block
     const int in_chunk = wave_col + V * cl;
     const int fragment = in_chunk / 128, block = in_chunk % 128 / 32;
-    if (job.q) {
+    const bool makes_q = job.q && rows_here;
+    if (makes_q) {
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         uint32_t m = 0;
@@ -161,7 +167,7 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
       }
     }
     if constexpr (kTransposed) {
-      if (job.q_t || job.sums) {
+      if (columns_here && (job.q_t || job.sums)) {
         // 256 rows are a chunk of q_t, this tile one of its fragments, g the block of it
         uint32_t largest[4] = {};
 #pragma unroll
@@ -218,14 +224,14 @@ __global__ __launch_bounds__((Shape<T, kTransposed>::kThreads)) void quantize_mx
       }
     }
     __syncthreads();
-    if (job.q) {
+    if (makes_q) {
       const int64_t group = static_cast<int64_t>(tile_row) * (S::kHigh / 16);
       store_units<S::kThreads>(row_units, min<int64_t>(S::kHigh / 16, mx4_groups(rows) - group),
                                job.q + (group * chunks + chunk) * kMx4Unit, chunks * kMx4Unit);
     }
     if constexpr (kTransposed) {
-      if (job.q_t) {
-          const int64_t group = static_cast<int64_t>(chunk) * 16, t_stride = mx4_stride(rows);
+      if (job.q_t && columns_here) {
+        const int64_t group = static_cast<int64_t>(chunk) * 16, t_stride = mx4_stride(rows);
         store_fragments<S::kThreads>(column_units, min<int64_t>(16, mx4_groups(cols) - group), tile_row & 1,
                                      job.q_t + group * t_stride + static_cast<int64_t>(tile_row / 2) * kMx4Unit, t_stride);
       }
@@ -407,6 +413,10 @@ hipError_t launch_jobs(const Mx4Quantize* jobs, int count, hipStream_t stream) {
     j.chunks[i] = make_div_u31(static_cast<uint32_t>(chunks));
   }
   if (tiles == 0) return hipSuccess;
+  bool both = false;
+  for (int i = 0; i < count; ++i) both = both || (jobs[i].q && (jobs[i].q_t || jobs[i].sums));
+  j.apart = both && tiles * (S::kThreads / 64) <= 1024;
+  tiles <<= j.apart;
   hipLaunchKernelGGL((quantize_mx4_kernel<T, kTransposed>), dim3(static_cast<unsigned>(std::min(tiles, kMaxBlocks))),
                      dim3(S::kThreads), 0, stream, j);
   return hipGetLastError();
