@@ -118,28 +118,35 @@ rns8_status check_linear_backward(const rns8_mi355x_linear_mx4_backward_args& a)
 }
 
 struct BackwardParts {
-  uint8_t *dy = nullptr, *dy_t = nullptr, *x_t = nullptr, *dx = nullptr, *dw = nullptr;
-  float* sums = nullptr;
+  uint8_t *dy = nullptr, *dy_t = nullptr, *x_t = nullptr;
+  Mx4Sums sums{};
+  Mx4Gemm products[2] = {};  // dx and dw, empty where not wanted
+  void* workspaces[2] = {};
   uint64_t bytes = 0;
 };
-int64_t sum_parts(int64_t m) { return (m + 127) / 128; }
 
 BackwardParts backward_parts(const rns8_mi355x_linear_mx4_backward_args& a, void* workspace) {
   BackwardParts p;
-  if (a.m == 0) return p;
   Parts parts{static_cast<uint8_t*>(workspace)};
   if (a.dx) {
     p.dy = parts.take(mx4_bytes(a.m, a.n));
-    p.dx = parts.take(gemm_mx4_bytes(a.m, a.k, a.n));
+    p.products[0] = gemm_of(a.m, a.k, a.n, p.dy, a.w_t, nullptr, a.dx, a.lddx, a.dtype);
   }
   if (a.dw) {
     p.dy_t = parts.take(mx4_bytes(a.n, a.m));
     p.x_t = parts.take(mx4_bytes(a.k, a.m));
-    p.dw = parts.take(gemm_mx4_bytes(a.n, a.k, a.m));
+    p.products[1] = gemm_of(a.n, a.k, a.m, p.dy_t, p.x_t, nullptr, a.dw, a.lddw, RNS8_MI355X_F32);
   }
-  if (a.dbias)
-    p.sums = reinterpret_cast<float*>(
-        parts.take(static_cast<uint64_t>(sum_parts(a.m)) * static_cast<uint64_t>(a.n) * sizeof(float)));
+  if (a.dbias) {
+    p.sums.count = (a.m + 127) / 128;
+    p.sums.cols = a.n;
+    p.sums.out = a.dbias;
+    p.sums.partials = reinterpret_cast<const float*>(
+        parts.take(static_cast<uint64_t>(p.sums.count) * static_cast<uint64_t>(a.n) * sizeof(float)));
+  }
+  uint64_t bytes[2];
+  gemm_mx4_pair_bytes(p.products, bytes);
+  for (int i = 0; i < 2; ++i) p.workspaces[i] = parts.take(bytes[i]);
   p.bytes = parts.bytes;
   return p;
 }
@@ -147,17 +154,13 @@ uint64_t backward_bytes(const rns8_mi355x_linear_mx4_backward_args& a) { return 
 
 hipError_t enqueue_backward(const rns8_mi355x_linear_mx4_backward_args& a, hipStream_t s) {
   const BackwardParts p = backward_parts(a, a.workspace);
-  hipError_t e = hipSuccess;
   if (a.m > 0) {
-    const Mx4Quantize jobs[2] = {{a.dy, a.m, a.n, a.lddy, p.dy, p.dy_t, p.sums}, {a.x, a.m, a.k, a.ldx, nullptr, p.x_t, nullptr}};
-    e = launch_quantize_mx4(jobs, a.dw ? 2 : 1, a.dtype, s);
+    const Mx4Quantize jobs[2] = {{a.dy, a.m, a.n, a.lddy, p.dy, p.dy_t, const_cast<float*>(p.sums.partials)},
+                                 {a.x, a.m, a.k, a.ldx, nullptr, p.x_t, nullptr}};
+    const hipError_t e = launch_quantize_mx4(jobs, a.dw ? 2 : 1, a.dtype, s);
+    if (e != hipSuccess) return e;
   }
-  if (e == hipSuccess && a.dbias) e = launch_sum_partials(p.sums, sum_parts(a.m), a.n, a.dbias, s);
-  if (e == hipSuccess && a.dx)
-    e = launch_gemm_mx4(gemm_of(a.m, a.k, a.n, p.dy, a.w_t, nullptr, a.dx, a.lddx, a.dtype), p.dx, s);
-  if (e == hipSuccess && a.dw)
-    e = launch_gemm_mx4(gemm_of(a.n, a.k, a.m, p.dy_t, p.x_t, nullptr, a.dw, a.lddw, RNS8_MI355X_F32), p.dw, s);
-  return e;
+  return launch_gemm_mx4_pair(p.products, p.workspaces, p.sums, s);
 }
 
 // ---- experts ---------------------------------------------------------------------------------

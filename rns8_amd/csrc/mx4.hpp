@@ -99,11 +99,17 @@ struct Mx4Quantize {
 };
 // Up to two quantizations of one type in one launch.
 hipError_t launch_quantize_mx4(const Mx4Quantize* jobs, int count, uint32_t dtype, hipStream_t stream);
-hipError_t launch_sum_partials(const float* partials, int64_t count, int64_t cols, float* sums, hipStream_t stream);
+// Partial sums [count][cols], added in a fixed order.
+struct Mx4Sums {
+  const float* partials;
+  int64_t count, cols;
+  float* out;  // or NULL: nothing to add
+};
+hipError_t launch_sum_partials(const Mx4Sums& s, hipStream_t stream);
 hipError_t launch_dequantize_mx4(const rns8_mi355x_mx4_args& a, hipStream_t stream);
 hipError_t launch_pack_mx4(const rns8_mi355x_pack_mx4_args& a, hipStream_t stream);
 
-// Products (mx4_gemm.hip chooses between mx4_tiles.hip and mx4_rows.hip).
+// Products (mx4_tiles.hip, which chooses between its tiles and mx4_rows.hip).
 struct Mx4Gemm {
   int64_t m, n, k;
   const uint8_t *a, *b;
@@ -118,6 +124,12 @@ struct Mx4Gemm {
 uint64_t gemm_mx4_bytes(int64_t m, int64_t n, int64_t k);
 hipError_t launch_gemm_mx4(const Mx4Gemm& g, void* workspace, hipStream_t stream);
 
+// Two products (empty ones among them) and partial sums to add up: in one launch where
+// that is faster. Their workspaces are apart.
+void gemm_mx4_pair_bytes(const Mx4Gemm (&g)[2], uint64_t (&bytes)[2]);
+hipError_t launch_gemm_mx4_pair(const Mx4Gemm (&g)[2], void* const (&workspaces)[2], const Mx4Sums& sums, hipStream_t stream);
+
+// How the tile kernel cuts a product.
 struct Mx4Tiles {
   uint32_t bm, bn, slices;
   int64_t slice_chunks;
@@ -126,7 +138,6 @@ struct Mx4Tiles {
   double cost;  // predicted us
 };
 Mx4Tiles choose_mx4_tiles(int64_t m, int64_t n, int64_t k);
-hipError_t launch_mx4_tiles(const Mx4Gemm& g, const Mx4Tiles& t, float* partials, hipStream_t stream);
 
 // Few rows: m <= 64 (MX4), or m <= kMx4FusedRows of floating rows.
 constexpr int64_t kMx4Rows = 64, kMx4FusedRows = 16;

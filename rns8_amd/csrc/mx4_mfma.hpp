@@ -1,6 +1,8 @@
-// The scaled MFMA on MX4 fragments, and the rounding of a lane's own block.
+// The scaled MFMA on MX4 fragments, the rounding of a lane's own block, and the sum of
+// partial sums.
 #pragma once
 
+#include "elements.hpp"
 #include "mx4.hpp"
 
 namespace rns8x {
@@ -34,16 +36,43 @@ __device__ __forceinline__ Mx4Unit stream_unit(const uint8_t* unit, int lane) {
   return u;
 }
 
-// acc[row of b][row of a] += sum over 128 columns; kFragment: which byte of the
-// scales is this fragment's. Lane L then has rows 4 (L / 16) + e of b and row L % 16
+// acc[row of b][row of a] += sum over 128 columns; kByteB, kByteA: which bytes of the
+// scales are this fragment's. Lane L then has rows 4 (L / 16) + e of b and row L % 16
 // of a.
-template <int kFragment>
+template <int kByteB, int kByteA>
 __device__ __forceinline__ f32x4 mx4_mfma(i32x4 b, i32x4 a, f32x4 acc, uint32_t b_scales, uint32_t a_scales) {
   const i32x8 b8 = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
   const i32x8 a8 = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
   constexpr int kFp4 = 4;
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b8, a8, acc, kFp4, kFp4, kFragment, static_cast<int>(b_scales),
-                                                          kFragment, static_cast<int>(a_scales));
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b8, a8, acc, kFp4, kFp4, kByteB, static_cast<int>(b_scales),
+                                                          kByteA, static_cast<int>(a_scales));
+}
+// Both fragments of a unit.
+__device__ __forceinline__ f32x4 mx4_mfma(const Mx4Unit& b, const Mx4Unit& a, f32x4 acc) {
+  acc = mx4_mfma<0, 0>(b.codes[0], a.codes[0], acc, b.scales, a.scales);
+  return mx4_mfma<1, 1>(b.codes[1], a.codes[1], acc, b.scales, a.scales);
+}
+
+// Adds up partial sums: sixteen columns to a wave, a quarter of the partials to each
+// sixteen lanes; their order is the same whatever the grid.
+__device__ __forceinline__ void add_partials(const Mx4Sums& s, uint32_t wave, uint32_t waves, int lane) {
+  const int g = lane >> 4;
+  for (int64_t c0 = static_cast<int64_t>(wave) * 16; c0 < s.cols; c0 += static_cast<int64_t>(waves) * 16) {
+    const int64_t c = min(c0 + (lane & 15), s.cols - 1);
+    float sum = 0.0f;
+    for (int64_t i = g; i < s.count; i += 32) {
+      float v[8];  // eight loads in flight
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = s.partials[min(i + 4 * j, s.count - 1) * s.cols + c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += i + 4 * j < s.count ? v[j] : 0.0f;
+    }
+    const auto a = __builtin_amdgcn_permlane16_swap(as_uint(sum), as_uint(sum), false, false);
+    sum = as_float(a[0]) + as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(as_uint(sum), as_uint(sum), false, false);
+    sum = as_float(b[0]) + as_float(b[1]);
+    if (lane < 16 && c0 + lane < s.cols) s.out[c0 + lane] = sum;
+  }
 }
 
 struct Mx4Block {

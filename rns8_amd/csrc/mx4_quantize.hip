@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "mx4.hpp"
+#include "mx4_mfma.hpp"
 #include "operators.hpp"
 #include "row_shape.hpp"
 #include "tables.hpp"
@@ -293,28 +294,8 @@ __global__ __launch_bounds__(64) void sum_narrow_kernel(Mx4Quantize job) {
   }
 }
 
-__global__ __launch_bounds__(256) void sum_partials_kernel(const float* partials, int64_t count, int64_t cols, float* sums) {
-  for (int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63); c - (threadIdx.x & 63) < cols;
-       c += static_cast<int64_t>(gridDim.x) * 64) {
-    // four waves share the partials of 64 columns
-    __shared__ float part[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    float sum = 0.0f;
-    if (c < cols) {
-      for (int64_t i = wave; i < count; i += 32) {
-        // eight loads in flight
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = partials[min(i + 4 * j, count - 1) * cols + c];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += i + 4 * j < count ? v[j] : 0.0f;
-      }
-    }
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave == 0 && c < cols) sums[c] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-    __syncthreads();
-  }
+__global__ __launch_bounds__(256) void sum_partials_kernel(Mx4Sums s) {
+  add_partials(s, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4, threadIdx.x & 63);
 }
 
 // ---- back ------------------------------------------------------------------------------
@@ -474,10 +455,10 @@ hipError_t launch_quantize_mx4(const Mx4Quantize* jobs, int count, uint32_t dtyp
   return hipErrorInvalidValue;
 }
 
-hipError_t launch_sum_partials(const float* partials, int64_t count, int64_t cols, float* sums, hipStream_t stream) {
-  if (cols < 1) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(sum_partials_kernel, dim3(static_cast<unsigned>(std::min((cols + 63) / 64, kMaxBlocks))), dim3(256), 0,
-                     stream, partials, count, cols, sums);
+hipError_t launch_sum_partials(const Mx4Sums& s, hipStream_t stream) {
+  if (s.cols < 1) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(sum_partials_kernel, dim3(static_cast<unsigned>(std::min((s.cols + 63) / 64, kMaxBlocks))), dim3(256), 0,
+                     stream, s);
   return hipGetLastError();
 }
 

@@ -90,10 +90,7 @@ __global__ __launch_bounds__(kThreads) void mx4_rows_kernel(RowsArgs a) {
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        acc[i][j] = mx4_mfma<0>(f.w[j].codes[0], f.t[i].codes[0], acc[i][j], f.w[j].scales, f.t[i].scales);
-        acc[i][j] = mx4_mfma<1>(f.w[j].codes[1], f.t[i].codes[1], acc[i][j], f.w[j].scales, f.t[i].scales);
-      }
+      for (int j = 0; j < RB; ++j) acc[i][j] = mx4_mfma(f.w[j], f.t[i], acc[i][j]);
   };
   // a ring of D chunks' loads, without branches about them: a wait then counts them
   if (first < last) {
@@ -176,10 +173,7 @@ __global__ __launch_bounds__(kThreads) void mx4_linear_rows_kernel(RowsArgs a) {
     t.codes[1] = *reinterpret_cast<const i32x4*>(unit + 1024 + 16 * lane);
     t.scales = *reinterpret_cast<const uint16_t*>(unit + kMx4Scales + 2 * lane);
 #pragma unroll
-    for (int j = 0; j < RB; ++j) {
-      acc[j] = mx4_mfma<0>(w[j].codes[0], t.codes[0], acc[j], w[j].scales, t.scales);
-      acc[j] = mx4_mfma<1>(w[j].codes[1], t.codes[1], acc[j], w[j].scales, t.scales);
-    }
+    for (int j = 0; j < RB; ++j) acc[j] = mx4_mfma(w[j], t, acc[j]);
   };
   if (first < end) {
     // Rows before weights: loads return in order. No branches about them: a wait then

@@ -18,6 +18,15 @@
 //   * The next step's fragments are read beside a step's MFMAs.
 //   * Few tiles: K is cut into slices of whole units, whose 32-bit sums go to the
 //     workspace; a second kernel adds them in order.
+//   * Both gradients of a linear layer are one launch where their tiles are on the chip
+//     at once (the second product's after the first's), and the gradient of the bias,
+//     partial sums of rows, is added up by waves that have asked for their first tiles:
+//     7.5 us where two products and the sum are 14.3 (f32, m = 500, n = 701, k = 611). Larger
+//     ones gain nothing from it (4096^3: 105 us in one launch, 86 in two).
+// Measured on rounded normal values, bf16 outputs: 8192^3 257 us, 4.3 PFLOP/s; 4096^3
+// 43 us, 3.2. Bare scaled MFMAs at one wave to a SIMD run at 5.3 PFLOP/s on random codes
+// (6.8 on zeros: the clock gives way); eight waves of 128 x 64, two to a SIMD, issue them
+// closer but read fragments more often: 8192^3 275 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -75,23 +84,35 @@ __device__ __forceinline__ void sched_slots() {
   }
 }
 
-template <typename C>
-__global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void mx4_tiles_kernel(TileArgs args) {
+// One product, or two: the second's units come after the first's.
+struct OneProduct {
+  TileArgs product[1];
+};
+struct TwoProducts {
+  TileArgs product[2];
+  uint32_t units;
+  Mx4Sums sums;
+};
+
+template <typename C, typename Products>
+__global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void mx4_tiles_kernel(Products p) {
+  constexpr bool kTwo = std::is_same<Products, TwoProducts>::value;
   constexpr int TM = C::TM, TN = C::TN, BM = C::BM, BN = C::BN;
   __shared__ __attribute__((aligned(16))) int8_t lds[C::kLds];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave_m = wave / C::WN, wave_n = wave % C::WN;
 
-  uint32_t u_first, u_step, u_end;
+  uint32_t units = p.product[0].units, u_first, u_step, u_end;
+  if constexpr (kTwo) units = p.units;
   if ((gridDim.x & 7u) == 0u) {
     const uint32_t xcd = blockIdx.x & 7u;
-    u_first = static_cast<uint32_t>((static_cast<uint64_t>(xcd) * args.units) / 8) + (blockIdx.x >> 3);
-    u_end = static_cast<uint32_t>((static_cast<uint64_t>(xcd + 1) * args.units) / 8);
+    u_first = static_cast<uint32_t>((static_cast<uint64_t>(xcd) * units) / 8) + (blockIdx.x >> 3);
+    u_end = static_cast<uint32_t>((static_cast<uint64_t>(xcd + 1) * units) / 8);
     u_step = gridDim.x >> 3;
   } else {
     u_first = blockIdx.x;
-    u_end = args.units;
+    u_end = units;
     u_step = gridDim.x;
   }
   u_first = __builtin_amdgcn_readfirstlane(u_first);
@@ -99,10 +120,13 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   if (u_first >= u_end) return;
 
   struct Unit {
-    uint32_t slice, m0, n0, first, count;  // chunks
+    uint32_t product, slice, m0, n0, first, count;  // chunks
   };
   auto decode = [&](uint32_t u) {
     Unit U;
+    U.product = kTwo && u >= p.product[0].units ? 1 : 0;
+    const TileArgs& args = p.product[U.product];
+    if (U.product) u -= p.product[0].units;
     U.slice = div_u31(u, args.tiles);
     const uint32_t pid = u - U.slice * args.tiles.d;
     const uint32_t group = div_u31(pid, args.group);
@@ -123,13 +147,15 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   struct Cursor {
     const uint8_t *a, *b;
     int32_t a_n, b_n;  // bytes from there to the end of the tile's last 16 rows
-    uint32_t left, u;
+    uint32_t left, u, stride;
   };
   auto cursor_of = [&](uint32_t u) {
     const bool live = u < u_end;
     const Unit U = decode(live ? u : u_end - 1);
+    const TileArgs& args = p.product[U.product];
     const uint32_t skip = U.first * kMx4Unit;
     Cursor c;
+    c.stride = args.stride;
     c.a = args.a + static_cast<uint64_t>(U.m0 / 16) * args.stride + skip;
     c.b = args.b + static_cast<uint64_t>(U.n0 / 16) * args.stride + skip;
     const uint32_t ga = min(static_cast<uint32_t>(BM / 16), args.groups_m - U.m0 / 16);
@@ -141,9 +167,24 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
     return c;
   };
   Cursor cur = cursor_of(u_first);
+  // (what is past the buffer's bytes reads as zero: offsets stay below 2^31)
+  uint32_t a_voff[C::kDmaA], b_voff[C::kDmaB], as_voff, bs_voff;
+  auto set_offsets = [&]() {
+#pragma unroll
+    for (int i = 0; i < C::kDmaA; ++i) a_voff[i] = static_cast<uint32_t>(wave * C::kDmaA + i) * cur.stride + 16 * lane;
+#pragma unroll
+    for (int i = 0; i < C::kDmaB; ++i) b_voff[i] = static_cast<uint32_t>(wave * C::kDmaB + i) * cur.stride + 16 * lane;
+    // a wave's share of the scales: eight lanes to the 128 bytes of 16 rows
+    const uint32_t row = lane >> 3, at = kMx4Scales + 16 * (lane & 7);
+    as_voff = lane < 8 * C::kDmaA ? (wave * C::kDmaA + row) * cur.stride + at : 0x80000000u;
+    bs_voff = lane < 8 * C::kDmaB ? (wave * C::kDmaB + row) * cur.stride + at : 0x80000000u;
+  };
+  set_offsets();
   auto advance = [&]() {
     if (--cur.left == 0) {
+      const uint32_t stride = cur.stride;
       cur = cursor_of(cur.u + u_step);
+      if (kTwo && cur.stride != stride) set_offsets();
       return;
     }
     const int32_t step = cur.a_n ? kMx4Unit : 0;
@@ -152,19 +193,6 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
     cur.a_n -= step;
     cur.b_n -= step;
   };
-  // (what is past the buffer's bytes reads as zero: offsets stay below 2^31)
-  uint32_t a_voff[C::kDmaA], b_voff[C::kDmaB];
-#pragma unroll
-  for (int i = 0; i < C::kDmaA; ++i) a_voff[i] = static_cast<uint32_t>(wave * C::kDmaA + i) * args.stride + 16 * lane;
-#pragma unroll
-  for (int i = 0; i < C::kDmaB; ++i) b_voff[i] = static_cast<uint32_t>(wave * C::kDmaB + i) * args.stride + 16 * lane;
-  // a wave's share of the scales: eight lanes to the 128 bytes of 16 rows
-  const uint32_t as_voff = lane < 8 * C::kDmaA ? static_cast<uint32_t>(wave * C::kDmaA + (lane >> 3)) * args.stride + kMx4Scales +
-                                                     16 * (lane & 7)
-                                               : 0x80000000u;
-  const uint32_t bs_voff = lane < 8 * C::kDmaB ? static_cast<uint32_t>(wave * C::kDmaB + (lane >> 3)) * args.stride + kMx4Scales +
-                                                     16 * (lane & 7)
-                                               : 0x80000000u;
   const uint32_t lds0 = lds_address(lds);
   const uint32_t lds_a = lds0 + static_cast<uint32_t>(wave * C::kDmaA * 1024);
   const uint32_t lds_b = lds0 + static_cast<uint32_t>(C::kStageA + wave * C::kDmaB * 1024);
@@ -186,7 +214,7 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
     i32x4 a[TM];
     i32x4 b[TN];
   };
-  struct Scales {
+  struct Scales {  // both fragments' bytes
     uint32_t a[TM];
     uint32_t b[TN];
   };
@@ -212,7 +240,7 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
       for (int jj = 0; jj < TN; ++jj) {
         const int i = i0 + ii, j = (ii & 1) ? TN - 1 - jj : jj;
         const f32x4 start = {0.0f, 0.0f, 0.0f, 0.0f};
-        acc[i][j] = mx4_mfma<half>(f.b[j], f.a[i], decltype(first)::value ? start : acc[i][j], s.b[j], s.a[i]);
+        acc[i][j] = mx4_mfma<half, half>(f.b[j], f.a[i], decltype(first)::value ? start : acc[i][j], s.b[j], s.a[i]);
       }
   };
   constexpr int kMfma = TM / 2 * TN;
@@ -238,6 +266,7 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
     return f32x4{as_float(v.v[0]), as_float(v.v[1]), as_float(v.v[2]), as_float(v.v[3])};
   };
   auto epilogue = [&](const Unit& U) {
+    const TileArgs& args = p.product[U.product];
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");  // the reads below are asm: MFMA results settle first
     const int64_t row0 = static_cast<int64_t>(U.m0) + wave_m * (16 * TM) + frag_row;
     const int64_t col0 = static_cast<int64_t>(U.n0) + wave_n * (16 * TN);
@@ -342,6 +371,9 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
       for (int i = 0; i < C::kDmaB; ++i) dma_b(sb, (2 * c + half) * C::kStage, half, i);
     }
     advance();
+  }
+  if constexpr (kTwo) {
+    if (p.sums.out) add_partials(p.sums, blockIdx.x * C::kWaves + wave, gridDim.x * C::kWaves, lane);
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(2 * kDmaStep + 2));  // chunk 0 landed
   __syncthreads();
@@ -465,36 +497,43 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(JoinArgs a) {
 }
 
 template <int TM, int TN, int WN, int kResident>
-hipError_t launch_cfg(TileArgs a, uint32_t slices, hipStream_t stream) {
+hipError_t launch_cfg(TwoProducts p, const uint32_t* slices, int count, hipStream_t stream) {
   using Cf = Cfg<TM, TN, WN, kResident>;
-  const uint32_t tiles_m = (a.m + Cf::BM - 1) / Cf::BM, tiles_n = (a.n + Cf::BN - 1) / Cf::BN;
-  const uint64_t tiles = static_cast<uint64_t>(tiles_m) * tiles_n, units = tiles * slices;
-  if (units == 0 || units > 0x7FFFFFFFull) return hipErrorInvalidValue;
-  a.units = static_cast<uint32_t>(units);
-  a.tiles_m = tiles_m;
-  a.tiles = make_div_u31(static_cast<uint32_t>(tiles));
-  a.group = make_div_u31(static_cast<uint32_t>(Cf::kGroupM) * tiles_n);
-  a.rows = make_div_u31(Cf::kGroupM);
-  a.tail = make_div_u31(tiles_m - (tiles_m - 1) / Cf::kGroupM * Cf::kGroupM);
-  const uint32_t grid =
-      static_cast<uint32_t>(persistent_grid(units, static_cast<uint64_t>(device_cu_count()) * kResident));
-  hipLaunchKernelGGL((mx4_tiles_kernel<Cf>), dim3(grid), dim3(Cf::kThreads), 0, stream, a);
+  uint64_t all = 0;
+  for (int i = 0; i < count; ++i) {
+    TileArgs& a = p.product[i];
+    const uint32_t tiles_m = (a.m + Cf::BM - 1) / Cf::BM, tiles_n = (a.n + Cf::BN - 1) / Cf::BN;
+    const uint64_t tiles = static_cast<uint64_t>(tiles_m) * tiles_n, units = tiles * slices[i];
+    all += units;
+    if (units == 0 || all > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    a.units = static_cast<uint32_t>(units);
+    a.tiles_m = tiles_m;
+    a.tiles = make_div_u31(static_cast<uint32_t>(tiles));
+    a.group = make_div_u31(static_cast<uint32_t>(Cf::kGroupM) * tiles_n);
+    a.rows = make_div_u31(Cf::kGroupM);
+    a.tail = make_div_u31(tiles_m - (tiles_m - 1) / Cf::kGroupM * Cf::kGroupM);
+  }
+  p.units = static_cast<uint32_t>(all);
+  const uint32_t grid = static_cast<uint32_t>(persistent_grid(all, static_cast<uint64_t>(device_cu_count()) * kResident));
+  if (count == 1)
+    hipLaunchKernelGGL((mx4_tiles_kernel<Cf, OneProduct>), dim3(grid), dim3(Cf::kThreads), 0, stream, OneProduct{{p.product[0]}});
+  else
+    hipLaunchKernelGGL((mx4_tiles_kernel<Cf, TwoProducts>), dim3(grid), dim3(Cf::kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
-// A tile's costs in us: a start (launch, first loads, epilogue) and one chunk of 256
-// columns on a CU that holds one workgroup, where few CUs do (`alone`) and where all do
-// (`full`: clock and memory are shared), and per workgroup where it holds more
-// (`shared`).
+// A tile's costs in us, fitted to launches of 16 shapes from 100^3 to 8192^3 (bf16
+// outputs, 1 to 32 slices each; the choices are within 0.4% of the best of them): a
+// start (launch, first loads, epilogue) and one chunk of 256 columns on a CU that holds
+// one workgroup, where few CUs do (`alone`) and where all do (`full`: clock and memory
+// are shared), and per workgroup where it holds more (`shared`).
 struct TileCost {
   uint32_t bm, bn, resident;
   double start, alone, full, shared;
 };
-constexpr TileCost kTileCosts[] = {{256, 256, 1, 10.8, 1.05, 1.60, 1.60},
-                                   {256, 128, 1, 6.6, 0.67, 1.10, 1.10},
-                                   {128, 256, 1, 6.6, 0.71, 1.15, 1.15},
-                                   {128, 128, 2, 5.8, 0.42, 0.50, 0.61},
-                                   {64, 64, 4, 3.6, 0.35, 0.35, 0.25}};
+constexpr TileCost kTileCosts[] = {{256, 256, 1, 10.8, 1.05, 1.92, 1.92},
+                                   {128, 128, 2, 5.18, 0.47, 0.53, 0.58},
+                                   {64, 64, 4, 4.16, 0.28, 0.31, 0.21}};
 
 double tile_cost(const TileCost& c, int64_t m, int64_t n, int64_t k, double units, int64_t slice_chunks) {
   const double per_cu = std::ceil(units / 256);
@@ -504,47 +543,75 @@ double tile_cost(const TileCost& c, int64_t m, int64_t n, int64_t k, double unit
   return c.start + std::max(static_cast<double>(slice_chunks) * chunk, operands);
 }
 
-}  // namespace
-
-Mx4Tiles choose_mx4_tiles(int64_t m, int64_t n, int64_t k) {
-  Mx4Tiles best{};
+// The best cut of a product into this kind of tile, if it beats `best`.
+void choose_slices(const TileCost& c, int64_t m, int64_t n, int64_t k, Mx4Tiles& best) {
   const int64_t chunks = mx4_chunks(k);
-  for (const TileCost& c : kTileCosts) {
-    const double tiles = static_cast<double>((m + c.bm - 1) / c.bm) * static_cast<double>((n + c.bn - 1) / c.bn);
-    for (const int64_t wanted : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (wanted > 1 && chunks < 2 * wanted) continue;  // slices of two chunks at least
-      const int64_t slice_chunks = (chunks + wanted - 1) / wanted, s = (chunks + slice_chunks - 1) / slice_chunks;
-      const double units = tiles * static_cast<double>(s);
-      if (units > 0x7FFFFFFF) continue;
-      double cost = tile_cost(c, m, n, k, units, slice_chunks);
-      // the join: a launch, and the partial sums written and read
-      if (s > 1)
-        cost += 2.2 + 0.03 * static_cast<double>(s) +
-                static_cast<double>(s) * static_cast<double>(m) * static_cast<double>(n) * 8 / 4e6;
-      if (best.cost != 0 && cost >= best.cost) continue;
-      best.cost = cost;
-      best.bm = c.bm;
-      best.bn = c.bn;
-      best.slices = static_cast<uint32_t>(s);
-      best.slice_chunks = slice_chunks;
-    }
+  const double tiles = static_cast<double>((m + c.bm - 1) / c.bm) * static_cast<double>((n + c.bn - 1) / c.bn);
+  for (const int64_t wanted : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (wanted > 1 && chunks < 2 * wanted) continue;  // slices of two chunks at least
+    const int64_t slice_chunks = (chunks + wanted - 1) / wanted, s = (chunks + slice_chunks - 1) / slice_chunks;
+    const double units = tiles * static_cast<double>(s);
+    if (units > 0x3FFFFFFF) continue;
+    double cost = tile_cost(c, m, n, k, units, slice_chunks);
+    // the join: a launch, and the partial sums written and read
+    if (s > 1)
+      cost += 2.2 + 0.03 * static_cast<double>(s) +
+              static_cast<double>(s) * static_cast<double>(m) * static_cast<double>(n) * 8 / 4e6;
+    if (best.cost != 0 && cost >= best.cost) continue;
+    best.cost = cost;
+    best.bm = c.bm;
+    best.bn = c.bn;
+    best.slices = static_cast<uint32_t>(s);
+    best.slice_chunks = slice_chunks;
   }
   best.ldp = (n + 3) / 4 * 4;
   best.bytes = best.slices > 1 ? static_cast<uint64_t>(best.slices) * static_cast<uint64_t>(m) *
                                      static_cast<uint64_t>(best.ldp) * sizeof(float)
                                : 0u;
+}
+
+}  // namespace
+
+Mx4Tiles choose_mx4_tiles(int64_t m, int64_t n, int64_t k) {
+  Mx4Tiles best{};
+  for (const TileCost& c : kTileCosts) choose_slices(c, m, n, k, best);
   return best;
 }
 
-hipError_t launch_mx4_tiles(const Mx4Gemm& g, const Mx4Tiles& t, float* partials, hipStream_t stream) {
+namespace {
+
+// Tiles for two products in one launch, where both fit on the chip at once and that is
+// predicted to take less than one after the other.
+bool choose_pair(const Mx4Gemm (&g)[2], Mx4Tiles (&tiles)[2]) {
+  double least = 0;
+  for (const Mx4Gemm& one : g) least += choose_mx4_tiles(one.m, one.n, one.k).cost;
+  bool pair = false;
+  for (const TileCost& c : kTileCosts) {
+    Mx4Tiles t[2]{};
+    double units = 0;
+    for (int i = 0; i < 2; ++i) {
+      choose_slices(c, g[i].m, g[i].n, g[i].k, t[i]);
+      units += static_cast<double>((g[i].m + c.bm - 1) / c.bm) * static_cast<double>((g[i].n + c.bn - 1) / c.bn) * t[i].slices;
+    }
+    const double together = std::max(t[0].cost, t[1].cost);
+    if (t[0].cost == 0 || t[1].cost == 0 || units > 256.0 * c.resident || together >= least) continue;
+    least = together;
+    pair = true;
+    tiles[0] = t[0];
+    tiles[1] = t[1];
+  }
+  return pair;
+}
+
+// The kernel's arguments, if it can take the product.
+bool tile_args(const Mx4Gemm& g, const Mx4Tiles& t, float* partials, TileArgs& a) {
   if (g.m < 1 || g.n < 1 || g.k < 1 || g.m > kMaxMx4Size || g.n > kMaxMx4Size || g.k > kMaxMx4Sum ||
       g.dtype > RNS8_MI355X_BF16 || reinterpret_cast<uintptr_t>(g.a) % 16 || reinterpret_cast<uintptr_t>(g.b) % 16 ||
       t.slices < 1 || t.slice_chunks < 1 || (t.slices > 1 && !partials))
-    return hipErrorInvalidValue;
+    return false;
   const int64_t chunks = mx4_chunks(g.k);
   // (every slice has a chunk)
-  if (t.slice_chunks * (t.slices - 1) >= chunks || t.slice_chunks * t.slices < chunks) return hipErrorInvalidValue;
-  TileArgs a{};
+  if (t.slice_chunks * (t.slices - 1) >= chunks || t.slice_chunks * t.slices < chunks) return false;
   a.a = g.a;
   a.b = g.b;
   a.bias = g.bias;
@@ -560,23 +627,43 @@ hipError_t launch_mx4_tiles(const Mx4Gemm& g, const Mx4Tiles& t, float* partials
   a.stride = static_cast<uint32_t>(mx4_stride(g.k));
   a.dtype = g.dtype;
   a.slice_chunks = static_cast<uint32_t>(t.slice_chunks);
-  hipError_t e = hipErrorInvalidValue;
-  if (t.bm == 256 && t.bn == 256) e = launch_cfg<8, 8, 2, 1>(a, t.slices, stream);
-  if (t.bm == 256 && t.bn == 128) e = launch_cfg<8, 4, 2, 1>(a, t.slices, stream);
-  if (t.bm == 128 && t.bn == 256) e = launch_cfg<4, 8, 2, 1>(a, t.slices, stream);
-  if (t.bm == 128 && t.bn == 128) e = launch_cfg<4, 4, 2, 2>(a, t.slices, stream);
-  if (t.bm == 64 && t.bn == 64) e = launch_cfg<2, 4, 1, 4>(a, t.slices, stream);
-  if (e != hipSuccess || t.slices == 1) return e;
-  const JoinArgs j{partials, t.slices, g.m, g.n, t.ldp, g.ldo, g.bias, g.out, g.dtype};
-  hipLaunchKernelGGL(mx4_join_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((g.m * (t.ldp / 4) + 255) / 256, 1 << 20))),
-                     dim3(256), 0, stream, j);
-  return hipGetLastError();
+  return true;
 }
 
-namespace {
+// Products of one kind of tile in one launch, then the joins of those cut into slices.
+hipError_t launch_tiles(const Mx4Gemm* g, const Mx4Tiles* t, float* const* partials, int count, const Mx4Sums& sums,
+                        hipStream_t stream) {
+  TwoProducts p{};
+  p.sums = sums;
+  uint32_t slices[2] = {};
+  for (int i = 0; i < count; ++i) {
+    if (t[i].bm != t[0].bm || t[i].bn != t[0].bn || !tile_args(g[i], t[i], partials[i], p.product[i])) return hipErrorInvalidValue;
+    slices[i] = t[i].slices;
+  }
+  hipError_t e = hipErrorInvalidValue;
+  if (t[0].bm == 256) e = launch_cfg<8, 8, 2, 1>(p, slices, count, stream);
+  if (t[0].bm == 128) e = launch_cfg<4, 4, 2, 2>(p, slices, count, stream);
+  if (t[0].bm == 64) e = launch_cfg<2, 4, 1, 4>(p, slices, count, stream);
+  for (int i = 0; i < count && e == hipSuccess; ++i) {
+    if (slices[i] == 1) continue;
+    const JoinArgs j{partials[i], slices[i], g[i].m, g[i].n, t[i].ldp, g[i].ldo, g[i].bias, g[i].out, g[i].dtype};
+    const int64_t blocks = std::min<int64_t>((g[i].m * (t[i].ldp / 4) + 255) / 256, 1 << 20);
+    hipLaunchKernelGGL(mx4_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, j);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
 // Few rows read b once however many waves share it; an empty sum has no tiles.
 constexpr int64_t kMaxRowsChannels = int64_t{1} << 26;
 bool rows_take(int64_t m, int64_t n, int64_t k) { return k == 0 || (m <= kMx4Rows && n <= kMaxRowsChannels); }
+bool tiles_take(const Mx4Gemm& g) { return g.m > 0 && g.n > 0 && !g.x && !rows_take(g.m, g.n, g.k); }
+
+// Whether one launch takes both, and their tiles.
+bool as_pair(const Mx4Gemm (&g)[2], Mx4Tiles (&tiles)[2]) {
+  return tiles_take(g[0]) && tiles_take(g[1]) && choose_pair(g, tiles);
+}
+
 }  // namespace
 
 bool linear_mx4_in_one_kernel(int64_t m, int64_t n) { return m <= kMx4FusedRows && n <= kMaxRowsChannels; }
@@ -587,8 +674,27 @@ uint64_t gemm_mx4_bytes(int64_t m, int64_t n, int64_t k) {
 
 hipError_t launch_gemm_mx4(const Mx4Gemm& g, void* workspace, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return hipSuccess;
-  if (g.x || rows_take(g.m, g.n, g.k)) return launch_mx4_rows(g, stream);
-  return launch_mx4_tiles(g, choose_mx4_tiles(g.m, g.n, g.k), static_cast<float*>(workspace), stream);
+  if (!tiles_take(g)) return launch_mx4_rows(g, stream);
+  const Mx4Tiles t = choose_mx4_tiles(g.m, g.n, g.k);
+  float* const partials = static_cast<float*>(workspace);
+  return launch_tiles(&g, &t, &partials, 1, Mx4Sums{}, stream);
+}
+
+void gemm_mx4_pair_bytes(const Mx4Gemm (&g)[2], uint64_t (&bytes)[2]) {
+  Mx4Tiles t[2];
+  const bool pair = as_pair(g, t);
+  for (int i = 0; i < 2; ++i) bytes[i] = pair ? t[i].bytes : gemm_mx4_bytes(g[i].m, g[i].n, g[i].k);
+}
+
+hipError_t launch_gemm_mx4_pair(const Mx4Gemm (&g)[2], void* const (&workspaces)[2], const Mx4Sums& sums, hipStream_t stream) {
+  Mx4Tiles t[2];
+  if (as_pair(g, t)) {
+    float* const partials[2] = {static_cast<float*>(workspaces[0]), static_cast<float*>(workspaces[1])};
+    return launch_tiles(g, t, partials, 2, sums, stream);
+  }
+  hipError_t e = sums.out ? launch_sum_partials(sums, stream) : hipSuccess;
+  for (int i = 0; i < 2 && e == hipSuccess; ++i) e = launch_gemm_mx4(g[i], workspaces[i], stream);
+  return e;
 }
 
 }  // namespace rns8x
