@@ -229,7 +229,7 @@ bool wide(int64_t n) { return n >= 256 * 32; }
 template <int MB>
 hipError_t launch_shape(const RowsArgs& a, hipStream_t stream) {
   const int64_t tokens = (a.m + 16 * MB - 1) / (16 * MB), blocks = (a.n + (wide(a.n) ? 31 : 15)) / (wide(a.n) ? 32 : 16);
-  if (tokens > 65535 || blocks * tokens > 0x7FFFFF) return hipErrorInvalidValue;
+  if (blocks > 0x7FFFFF) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(tokens));
   if (wide(a.n))
     hipLaunchKernelGGL((mx4_rows_kernel<MB, 2>), grid, dim3(kThreads), 0, stream, a);
@@ -258,7 +258,7 @@ hipError_t launch_typed(const RowsArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_mx4_rows(const Mx4Gemm& g, hipStream_t stream) {
-  if (g.m < 1 || g.n < 1 || g.k < 0 || g.k > kMaxMx4Sum || g.dtype > RNS8_MI355X_BF16) return hipErrorInvalidValue;
+  if (g.m < 1 || g.n < 1 || g.k < 1 || g.k > kMaxMx4Sum || g.dtype > RNS8_MI355X_BF16) return hipErrorInvalidValue;
   RowsArgs a{};
   a.a = g.a;
   a.b = g.b;

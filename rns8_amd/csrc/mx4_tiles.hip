@@ -117,7 +117,16 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   }
   u_first = __builtin_amdgcn_readfirstlane(u_first);
   u_end = __builtin_amdgcn_readfirstlane(u_end);
-  if (u_first >= u_end) return;
+  // (a grid is whole multiples of eight: a workgroup may have no unit, but has its sums)
+  auto add_sums = [&]() {
+    if constexpr (kTwo) {
+      if (p.sums.out) add_partials(p.sums, blockIdx.x * C::kWaves + wave, gridDim.x * C::kWaves, lane);
+    }
+  };
+  if (u_first >= u_end) {
+    add_sums();
+    return;
+  }
 
   struct Unit {
     uint32_t product, slice, m0, n0, first, count;  // chunks
@@ -372,9 +381,7 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
     }
     advance();
   }
-  if constexpr (kTwo) {
-    if (p.sums.out) add_partials(p.sums, blockIdx.x * C::kWaves + wave, gridDim.x * C::kWaves, lane);
-  }
+  add_sums();
   __builtin_amdgcn_s_waitcnt(wait_vm(2 * kDmaStep + 2));  // chunk 0 landed
   __syncthreads();
 #pragma unroll
@@ -630,6 +637,14 @@ bool tile_args(const Mx4Gemm& g, const Mx4Tiles& t, float* partials, TileArgs& a
   return true;
 }
 
+// (no slices: the bias alone)
+hipError_t launch_join(const Mx4Gemm& g, const float* partials, uint32_t slices, int64_t ldp, hipStream_t stream) {
+  const JoinArgs j{partials, slices, g.m, g.n, ldp, g.ldo, g.bias, g.out, g.dtype};
+  const int64_t blocks = std::min<int64_t>((g.m * (ldp / 4) + 255) / 256, 1 << 20);
+  hipLaunchKernelGGL(mx4_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, j);
+  return hipGetLastError();
+}
+
 // Products of one kind of tile in one launch, then the joins of those cut into slices.
 hipError_t launch_tiles(const Mx4Gemm* g, const Mx4Tiles* t, float* const* partials, int count, const Mx4Sums& sums,
                         hipStream_t stream) {
@@ -644,20 +659,15 @@ hipError_t launch_tiles(const Mx4Gemm* g, const Mx4Tiles* t, float* const* parti
   if (t[0].bm == 256) e = launch_cfg<8, 8, 2, 1>(p, slices, count, stream);
   if (t[0].bm == 128) e = launch_cfg<4, 4, 2, 2>(p, slices, count, stream);
   if (t[0].bm == 64) e = launch_cfg<2, 4, 1, 4>(p, slices, count, stream);
-  for (int i = 0; i < count && e == hipSuccess; ++i) {
-    if (slices[i] == 1) continue;
-    const JoinArgs j{partials[i], slices[i], g[i].m, g[i].n, t[i].ldp, g[i].ldo, g[i].bias, g[i].out, g[i].dtype};
-    const int64_t blocks = std::min<int64_t>((g[i].m * (t[i].ldp / 4) + 255) / 256, 1 << 20);
-    hipLaunchKernelGGL(mx4_join_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, j);
-    e = hipGetLastError();
-  }
+  for (int i = 0; i < count && e == hipSuccess; ++i)
+    if (slices[i] > 1) e = launch_join(g[i], partials[i], slices[i], t[i].ldp, stream);
   return e;
 }
 
-// Few rows read b once however many waves share it; an empty sum has no tiles.
+// Few rows read b once however many waves share it.
 constexpr int64_t kMaxRowsChannels = int64_t{1} << 26;
-bool rows_take(int64_t m, int64_t n, int64_t k) { return k == 0 || (m <= kMx4Rows && n <= kMaxRowsChannels); }
-bool tiles_take(const Mx4Gemm& g) { return g.m > 0 && g.n > 0 && !g.x && !rows_take(g.m, g.n, g.k); }
+bool rows_take(int64_t m, int64_t n) { return m <= kMx4Rows && n <= kMaxRowsChannels; }
+bool tiles_take(const Mx4Gemm& g) { return g.m > 0 && g.n > 0 && g.k > 0 && !g.x && !rows_take(g.m, g.n); }
 
 // Whether one launch takes both, and their tiles.
 bool as_pair(const Mx4Gemm (&g)[2], Mx4Tiles (&tiles)[2]) {
@@ -669,11 +679,12 @@ bool as_pair(const Mx4Gemm (&g)[2], Mx4Tiles (&tiles)[2]) {
 bool linear_mx4_in_one_kernel(int64_t m, int64_t n) { return m <= kMx4FusedRows && n <= kMaxRowsChannels; }
 
 uint64_t gemm_mx4_bytes(int64_t m, int64_t n, int64_t k) {
-  return m == 0 || n == 0 || rows_take(m, n, k) ? 0u : choose_mx4_tiles(m, n, k).bytes;
+  return m == 0 || n == 0 || k == 0 || rows_take(m, n) ? 0u : choose_mx4_tiles(m, n, k).bytes;
 }
 
 hipError_t launch_gemm_mx4(const Mx4Gemm& g, void* workspace, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return hipSuccess;
+  if (g.k == 0) return launch_join(g, nullptr, 0, (g.n + 3) / 4 * 4, stream);
   if (!tiles_take(g)) return launch_mx4_rows(g, stream);
   const Mx4Tiles t = choose_mx4_tiles(g.m, g.n, g.k);
   float* const partials = static_cast<float*>(workspace);
