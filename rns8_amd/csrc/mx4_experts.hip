@@ -47,6 +47,13 @@ struct Routing {
 };
 constexpr uint32_t kNone = 0xFFFF;
 
+// Many pairs: what LDS holds of an expert's tokens, `tokens` rows of `chunks` chunks (16
+// bytes after each, so that sixteen rows' reads meet no bank twice), and how many
+// workgroups share them.
+struct Batches {
+  uint32_t chunks, row, tokens, spread;
+};
+
 struct ExpertsArgs {
   const void *x, *router;
   int64_t ldx, ldrouter;
@@ -64,6 +71,7 @@ struct ExpertsArgs {
   uint16_t* h_parts;  // [part][pair][256 inner_chunks]
   float* y;           // [pair][16 ceil(width / 16)]; many pairs
   Routing* routing;
+  Batches batches[2];  // hidden, down; many pairs
 };
 
 // v as bf16 parts whose sum is v to 8 kParts bits: its leading bits, then the leading
@@ -513,6 +521,10 @@ __device__ __forceinline__ void both_fragments(F&& f) {
   f(std::integral_constant<int, 1>{});
 }
 
+// What is the same in every lane, told so (LDS gives it to each): addresses from it are
+// scalars.
+__device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
 constexpr int kHiddenWaves = kRouteWaves, kHiddenThreads = kRouteThreads;
 constexpr uint32_t kLdsX = 32768;    // few tokens: values of x's parts that a workgroup holds
 constexpr uint32_t kLdsH = 49152;    // and of the hidden values'
@@ -562,10 +574,10 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(E
   const uint32_t stride = chunks * kMx4Unit;
   const uint32_t first = chunks * wave / kHiddenWaves, last = chunks * (wave + 1) / kHiddenWaves;
   const int64_t h_row = 256 * static_cast<int64_t>(a.inner_chunks), h_part = static_cast<int64_t>(a.tokens) * a.top * h_row;
-  const uint32_t items = lists.active * groups;
+  const uint32_t items = same(lists.active) * groups;
   for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
     const uint32_t slot = item / groups, group = item - slot * groups;
-    const uint32_t e = lists.expert[slot], start = lists.start[slot], count = lists.start[slot + 1] - start;
+    const uint32_t e = same(lists.expert[slot]), start = same(lists.start[slot]), count = same(lists.start[slot + 1]) - start;
     const uint8_t* const gate = a.gate + (static_cast<uint64_t>(e) * real + group) * stride;
     const uint8_t* const up = a.up + (static_cast<uint64_t>(e) * real + group) * stride;
     const uint32_t r = lane & 15;
@@ -616,11 +628,16 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(E
 
 // ---- many pairs: a wave takes 32 rows of one expert's weights -----------------------------------
 // (gate and up of 16 hidden values, or 32 channels of down.) The rows of all experts
-// that have tokens are cut evenly over the workgroups, in blocks of eight, a wave each; an expert's tokens, as many as fit, lie in LDS while its rows stream by, three
-// units' loads ahead. A further batch of tokens reads the weights again.
+// that have tokens are cut evenly over the workgroups, in blocks of eight, a wave each; an
+// expert's tokens, as many as fit, lie in LDS while its rows stream by, two or three
+// units' loads ahead. A further batch of tokens reads the weights again, in a workgroup of its own where
+// the blocks alone are fewer than the CUs: 64 tokens, 4 of 4 experts, 4096 -> 2048, f32,
+// whole layer 228 us instead of 926; 4 of 16 experts, 2048 -> 1024, bf16, 40 instead of 59.
+// Measured (64 tokens, 8 of 128 experts, 4096 -> 1536, bf16): hidden 172 us, 5.0 TB/s of
+// weights; down 80 us, 5.3 TB/s.
 template <bool kDown, int kParts, int kHiddenParts>
 __global__ __launch_bounds__(kHiddenThreads, 4) void experts_many_kernel(ExpertsArgs a) {
-  constexpr int D = 3;
+  constexpr int D = kParts == 1 ? 3 : 2;  // (three with more parts spill: down of the above 92 us)
   __shared__ __attribute__((aligned(16))) union {
     RouteScratch route;
     uint8_t rows[kLdsRows];
@@ -642,27 +659,25 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_many_kernel(Experts
   const int64_t in_part = static_cast<int64_t>(a.tokens) * (kDown ? a.top : 1) * in_row;
   const uint32_t out_row = kDown ? 16 * groups : 256 * a.inner_chunks;
   const int64_t h_part = static_cast<int64_t>(a.tokens) * a.top * out_row;
-  // what LDS holds: `batch` tokens' values of `held` chunks, 16 bytes after each row (so
-  // that sixteen rows' reads meet no bank twice)
-  const uint32_t held = min(chunks, (kLdsRows / kParts - 16) / 512);
-  const uint32_t lds_row = 512 * held + 16;
-  const uint32_t batch = min(16u, kLdsRows / (kParts * lds_row));
+  const Batches& room = a.batches[kDown ? 1 : 0];
+  const uint32_t held = room.chunks, lds_row = room.row, batch = room.tokens, spread = room.spread;
   const uint32_t lds_part = batch * lds_row;
 
-  // an item is eight turns of one expert
+  // an item is eight turns of one expert, and where they are spread one batch of its tokens
   const uint32_t blocks = (per + kHiddenWaves - 1) / kHiddenWaves;
-  const uint64_t items = static_cast<uint64_t>(lists.active) * blocks;
+  const uint64_t items = static_cast<uint64_t>(same(lists.active)) * spread * blocks;
   const uint32_t begin = static_cast<uint32_t>(items * blockIdx.x / gridDim.x);
   const uint32_t end = static_cast<uint32_t>(items * (blockIdx.x + 1) / gridDim.x);
   for (uint32_t item = begin; item < end;) {
-    const uint32_t slot = item / blocks, block = item - slot * blocks, rounds = min(blocks - block, end - item);
+    const uint32_t share = item / blocks, block = item - share * blocks, rounds = min(blocks - block, end - item);
+    const uint32_t slot = share / spread;
     item += rounds;
     const uint32_t from = block * kHiddenWaves, to = min(per, from + rounds * kHiddenWaves), steps = rounds * chunks;
-    const uint32_t e = lists.expert[slot], start = lists.start[slot], count = lists.start[slot + 1] - start;
-    for (uint32_t r0 = 0; r0 < count; r0 += batch) {
+    const uint32_t e = same(lists.expert[slot]), start = same(lists.start[slot]), count = same(lists.start[slot + 1]) - start;
+    for (uint32_t r0 = (share - slot * spread) * batch; r0 < count; r0 += batch * spread) {
       const uint32_t tokens = min(batch, count - r0), r = lane & 15;
       const uint32_t row = min(r, tokens - 1) * lds_row + 64 * (lane >> 4);
-      // Loads run three steps ahead, over rounds as well (past the last turn or step the
+      // Loads run D steps ahead, over rounds as well (past the last turn or step the
       // last row again), and have no branches: a wait in the loop then counts them.
       const uint64_t matrix = static_cast<uint64_t>(groups) * stride;
       const uint8_t* const base0 = (kDown ? a.down : a.gate) + e * matrix;
@@ -768,11 +783,11 @@ __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsA
     early[i] = *reinterpret_cast<const u32x4*>(a.h_parts + min(8 * (threadIdx.x + i * kDownThreads), kHiddenParts * h_part - 8));
   for (uint32_t i = threadIdx.x; i < kDownWaves * kFewTokens * 16; i += kDownThreads) (&table[0][0][0])[i] = 0.0f;
   __syncthreads();
-  const uint32_t units = lists.active * chunks;
+  const uint32_t units = same(lists.active) * chunks;
   const uint32_t first = units * wave / kDownWaves, last = units * (wave + 1) / kDownWaves;
   auto unit_at = [&](uint32_t q) {
     const uint32_t slot = q / chunks, c = q - slot * chunks;
-    return stream_unit(a.down + (static_cast<uint64_t>(lists.expert[slot]) * groups + group) * stride + c * kMx4Unit, lane);
+    return stream_unit(a.down + (static_cast<uint64_t>(same(lists.expert[slot])) * groups + group) * stride + c * kMx4Unit, lane);
   };
   Mx4Unit w[U] = {};
   if (first < last) {
@@ -788,7 +803,7 @@ __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsA
   f32x4 acc = {};
   auto multiply_unit = [&](uint32_t q, const Mx4Unit& unit) __attribute__((always_inline)) {
     const uint32_t slot = q / chunks, c = q - slot * chunks;
-    const uint32_t start = lists.start[slot], count = lists.start[slot + 1] - start, r = lane & 15;
+    const uint32_t start = same(lists.start[slot]), count = same(lists.start[slot + 1]) - start, r = lane & 15;
     const uint32_t row = 2 * ((start + min(r, count - 1)) * h_row + 32 * (lane >> 4));
     both_fragments([&](auto half) __attribute__((always_inline)) {
       constexpr int h = decltype(half)::value;
@@ -885,7 +900,7 @@ uint64_t lay_out(const rns8_mi355x_experts_mx4_args& a, ExpertsArgs& e) {
 }
 
 template <typename T, int kParts, int kHiddenParts>
-hipError_t launch_typed(const ExpertsArgs& e, bool is_few, hipStream_t stream) {
+hipError_t launch_typed(ExpertsArgs e, bool is_few, hipStream_t stream) {
   const uint32_t x_blocks = e.tokens * ((256 * e.width_chunks + 2047) / 2048);
   auto stage = [&](auto experts, auto tokens) {
     constexpr uint32_t kExperts = decltype(experts)::value, kTokens = decltype(tokens)::value;
@@ -905,10 +920,20 @@ hipError_t launch_typed(const ExpertsArgs& e, bool is_few, hipStream_t stream) {
     return hipGetLastError();
   }
   if (e.router) hipLaunchKernelGGL(experts_choose_kernel, dim3(e.tokens), dim3(64), 0, stream, e);
-  // two workgroups to a CU
-  auto grid = [&](uint32_t turns) { return dim3(std::min(active * ((turns + kHiddenWaves - 1) / kHiddenWaves), 512u)); };
-  hipLaunchKernelGGL((experts_many_kernel<false, kParts, kHiddenParts>), grid((e.inner + 15) / 16), threads, 0, stream, e);
-  hipLaunchKernelGGL((experts_many_kernel<true, kHiddenParts, kHiddenParts>), grid((groups + 1) / 2), threads, 0, stream, e);
+  uint32_t grid[2];
+  for (int down = 0; down < 2; ++down) {
+    const uint32_t turns = down ? (groups + 1) / 2 : (e.inner + 15) / 16, parts = down ? kHiddenParts : kParts;
+    const uint32_t blocks = active * ((turns + kHiddenWaves - 1) / kHiddenWaves);
+    Batches& b = e.batches[down];
+    b.chunks = std::min(down ? e.inner_chunks : e.width_chunks, (kLdsRows / parts - 16) / 512);
+    b.row = 512 * b.chunks + 16;
+    b.tokens = std::min(kLdsRows / (parts * b.row), 16u);
+    // an expert's batches if tokens are even; a batch more comes second in its workgroup
+    b.spread = blocks < 256 ? (e.tokens * e.top + active * b.tokens - 1) / (active * b.tokens) : 1;
+    grid[down] = std::min(blocks * b.spread, 512u);  // two workgroups to a CU
+  }
+  hipLaunchKernelGGL((experts_many_kernel<false, kParts, kHiddenParts>), dim3(grid[0]), threads, 0, stream, e);
+  hipLaunchKernelGGL((experts_many_kernel<true, kHiddenParts, kHiddenParts>), dim3(grid[1]), threads, 0, stream, e);
   hipLaunchKernelGGL(experts_combine_kernel<T>, dim3((e.tokens * ((e.width + 3) / 4) + 255) / 256), dim3(256), 0, stream, e);
   return hipGetLastError();
 }
