@@ -783,9 +783,11 @@ RNS8_API rns8_status rns8_mi355x_linear_mx4_backward_workspace(
  * slot that adds nothing (its expert is elsewhere), and an expert that a token has
  * twice counts twice. With one they are outputs, and each may be NULL. gate and
  * up hold one inner x width matrix for each expert, down one width x inner, one
- * after the other. A score that is not finite, or a value of a token, makes that
- * token's row alone NaN (or infinite). tokens at most 64, experts at most 1024,
- * top at most 16 and at most `experts`, width and inner at most 65536. */
+ * after the other. A score that is NaN or +infinity, or a value of a
+ * token that is not finite, makes that token's row alone NaN (or infinite); an
+ * expert whose score is -infinity beside a finite one has weight 0. tokens at most
+ * 64, experts at most 1024, top at most 16 and at most `experts`, width and inner
+ * at most 65536. */
 #define RNS8_MI355X_EXPERTS_NORMALIZE 1u
 typedef struct rns8_mi355x_experts_mx4_args {
   uint64_t struct_size;

@@ -14,6 +14,8 @@
 //   * Codes and scales are gathered in LDS as units and leave in whole lines.
 //   * Sums of columns (a bias' gradient) in 32 bits for each 128 rows, in a fixed
 //     order; a second kernel adds those.
+// Measured at 8192 x 8192 in bf16: rows alone 33 us (5.1 TB/s), both forms 54 (3.8 TB/s),
+// back to bf16 29 (5.9 TB/s).
 #include <algorithm>
 #include <type_traits>
 

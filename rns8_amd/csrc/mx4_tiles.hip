@@ -18,11 +18,13 @@
 //   * The next step's fragments are read beside a step's MFMAs.
 //   * Few tiles: K is cut into slices of whole units, whose 32-bit sums go to the
 //     workspace; a second kernel adds them in order.
-//   * Both gradients of a linear layer are one launch where their tiles are on the chip
-//     at once (the second product's after the first's), and the gradient of the bias,
-//     partial sums of rows, is added up by waves that have asked for their first tiles:
-//     7.5 us where two products and the sum are 14.3 (f32, m = 500, n = 701, k = 611). Larger
-//     ones gain nothing from it (4096^3: 105 us in one launch, 86 in two).
+//   * Both gradients of a linear layer are one launch where their tiles fit on the chip
+//     at once: an eighth of each product to every XCD, the longer sums first. The gradient of
+//     the bias, partial sums of rows, is added up there too, by waves that have asked for
+//     their first tile. All gradients, with their roundings: 500 x 701 x 611 in f32 15.2
+//     us instead of 23.8 (three launches), 2048^3 in bf16 31.7 instead of 38.6, 4096 x 1024
+//     x 1024 30.0 instead of 32.2. Tiles that follow one another gain nothing (4096^3 in
+//     one walk over both: 105 us, 86 apart).
 // Measured on rounded normal values, bf16 outputs: 8192^3 257 us, 4.3 PFLOP/s; 4096^3
 // 43 us, 3.2. Bare scaled MFMAs at one wave to a SIMD run at 5.3 PFLOP/s on random codes
 // (6.8 on zeros: the clock gives way); eight waves of 128 x 64, two to a SIMD, issue them
@@ -84,13 +86,12 @@ __device__ __forceinline__ void sched_slots() {
   }
 }
 
-// One product, or two: the second's units come after the first's.
+// One product, or two, of each an eighth to every XCD and a unit to a workgroup.
 struct OneProduct {
   TileArgs product[1];
 };
 struct TwoProducts {
   TileArgs product[2];
-  uint32_t units;
   Mx4Sums sums;
 };
 
@@ -103,24 +104,32 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave_m = wave / C::WN, wave_n = wave % C::WN;
 
-  uint32_t units = p.product[0].units, u_first, u_step, u_end;
-  if constexpr (kTwo) units = p.units;
-  if ((gridDim.x & 7u) == 0u) {
-    const uint32_t xcd = blockIdx.x & 7u;
-    u_first = static_cast<uint32_t>((static_cast<uint64_t>(xcd) * units) / 8) + (blockIdx.x >> 3);
-    u_end = static_cast<uint32_t>((static_cast<uint64_t>(xcd + 1) * units) / 8);
+  uint32_t which = 0, u_first, u_step = 1, u_end;
+  const uint32_t xcd = blockIdx.x & 7u, place = blockIdx.x >> 3;
+  auto share = [&](uint32_t units, uint32_t x) { return static_cast<uint32_t>((static_cast<uint64_t>(x) * units) / 8); };
+  if constexpr (kTwo) {
+    const uint32_t first = share(p.product[0].units, xcd + 1) - share(p.product[0].units, xcd);
+    which = place >= first ? 1 : 0;
+    const uint32_t units = p.product[which].units;
+    u_first = share(units, xcd) + place - (which ? first : 0);
+    u_end = min(u_first + 1, share(units, xcd + 1));
+  } else if ((gridDim.x & 7u) == 0u) {
+    u_first = share(p.product[0].units, xcd) + place;
+    u_end = share(p.product[0].units, xcd + 1);
     u_step = gridDim.x >> 3;
   } else {
     u_first = blockIdx.x;
-    u_end = units;
+    u_end = p.product[0].units;
     u_step = gridDim.x;
   }
+  const TileArgs& args = p.product[which];
   u_first = __builtin_amdgcn_readfirstlane(u_first);
   u_end = __builtin_amdgcn_readfirstlane(u_end);
-  // (a grid is whole multiples of eight: a workgroup may have no unit, but has its sums)
+  // (a grid is whole multiples of eight: a workgroup may have no unit, but has its sums;
+  // the last ones begin)
   auto add_sums = [&]() {
     if constexpr (kTwo) {
-      if (p.sums.out) add_partials(p.sums, blockIdx.x * C::kWaves + wave, gridDim.x * C::kWaves, lane);
+      if (p.sums.out) add_partials(p.sums, (gridDim.x - 1 - blockIdx.x) * C::kWaves + wave, gridDim.x * C::kWaves, lane);
     }
   };
   if (u_first >= u_end) {
@@ -129,13 +138,10 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   }
 
   struct Unit {
-    uint32_t product, slice, m0, n0, first, count;  // chunks
+    uint32_t slice, m0, n0, first, count;  // chunks
   };
   auto decode = [&](uint32_t u) {
     Unit U;
-    U.product = kTwo && u >= p.product[0].units ? 1 : 0;
-    const TileArgs& args = p.product[U.product];
-    if (U.product) u -= p.product[0].units;
     U.slice = div_u31(u, args.tiles);
     const uint32_t pid = u - U.slice * args.tiles.d;
     const uint32_t group = div_u31(pid, args.group);
@@ -156,15 +162,13 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   struct Cursor {
     const uint8_t *a, *b;
     int32_t a_n, b_n;  // bytes from there to the end of the tile's last 16 rows
-    uint32_t left, u, stride;
+    uint32_t left, u;
   };
   auto cursor_of = [&](uint32_t u) {
     const bool live = u < u_end;
     const Unit U = decode(live ? u : u_end - 1);
-    const TileArgs& args = p.product[U.product];
     const uint32_t skip = U.first * kMx4Unit;
     Cursor c;
-    c.stride = args.stride;
     c.a = args.a + static_cast<uint64_t>(U.m0 / 16) * args.stride + skip;
     c.b = args.b + static_cast<uint64_t>(U.n0 / 16) * args.stride + skip;
     const uint32_t ga = min(static_cast<uint32_t>(BM / 16), args.groups_m - U.m0 / 16);
@@ -177,23 +181,18 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
   };
   Cursor cur = cursor_of(u_first);
   // (what is past the buffer's bytes reads as zero: offsets stay below 2^31)
-  uint32_t a_voff[C::kDmaA], b_voff[C::kDmaB], as_voff, bs_voff;
-  auto set_offsets = [&]() {
+  uint32_t a_voff[C::kDmaA], b_voff[C::kDmaB];
 #pragma unroll
-    for (int i = 0; i < C::kDmaA; ++i) a_voff[i] = static_cast<uint32_t>(wave * C::kDmaA + i) * cur.stride + 16 * lane;
+  for (int i = 0; i < C::kDmaA; ++i) a_voff[i] = static_cast<uint32_t>(wave * C::kDmaA + i) * args.stride + 16 * lane;
 #pragma unroll
-    for (int i = 0; i < C::kDmaB; ++i) b_voff[i] = static_cast<uint32_t>(wave * C::kDmaB + i) * cur.stride + 16 * lane;
-    // a wave's share of the scales: eight lanes to the 128 bytes of 16 rows
-    const uint32_t row = lane >> 3, at = kMx4Scales + 16 * (lane & 7);
-    as_voff = lane < 8 * C::kDmaA ? (wave * C::kDmaA + row) * cur.stride + at : 0x80000000u;
-    bs_voff = lane < 8 * C::kDmaB ? (wave * C::kDmaB + row) * cur.stride + at : 0x80000000u;
-  };
-  set_offsets();
+  for (int i = 0; i < C::kDmaB; ++i) b_voff[i] = static_cast<uint32_t>(wave * C::kDmaB + i) * args.stride + 16 * lane;
+  // a wave's share of the scales: eight lanes to the 128 bytes of 16 rows
+  const uint32_t row = lane >> 3, at = kMx4Scales + 16 * (lane & 7);
+  const uint32_t as_voff = lane < 8 * C::kDmaA ? (wave * C::kDmaA + row) * args.stride + at : 0x80000000u;
+  const uint32_t bs_voff = lane < 8 * C::kDmaB ? (wave * C::kDmaB + row) * args.stride + at : 0x80000000u;
   auto advance = [&]() {
     if (--cur.left == 0) {
-      const uint32_t stride = cur.stride;
       cur = cursor_of(cur.u + u_step);
-      if (kTwo && cur.stride != stride) set_offsets();
       return;
     }
     const int32_t step = cur.a_n ? kMx4Unit : 0;
@@ -275,7 +274,6 @@ __global__ __launch_bounds__(C::kThreads, (C::kResident * C::kWaves / 4)) void m
     return f32x4{as_float(v.v[0]), as_float(v.v[1]), as_float(v.v[2]), as_float(v.v[3])};
   };
   auto epilogue = [&](const Unit& U) {
-    const TileArgs& args = p.product[U.product];
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");  // the reads below are asm: MFMA results settle first
     const int64_t row0 = static_cast<int64_t>(U.m0) + wave_m * (16 * TM) + frag_row;
     const int64_t col0 = static_cast<int64_t>(U.n0) + wave_n * (16 * TN);
@@ -520,12 +518,12 @@ hipError_t launch_cfg(TwoProducts p, const uint32_t* slices, int count, hipStrea
     a.rows = make_div_u31(Cf::kGroupM);
     a.tail = make_div_u31(tiles_m - (tiles_m - 1) / Cf::kGroupM * Cf::kGroupM);
   }
-  p.units = static_cast<uint32_t>(all);
   const uint32_t grid = static_cast<uint32_t>(persistent_grid(all, static_cast<uint64_t>(device_cu_count()) * kResident));
   if (count == 1)
     hipLaunchKernelGGL((mx4_tiles_kernel<Cf, OneProduct>), dim3(grid), dim3(Cf::kThreads), 0, stream, OneProduct{{p.product[0]}});
-  else
-    hipLaunchKernelGGL((mx4_tiles_kernel<Cf, TwoProducts>), dim3(grid), dim3(Cf::kThreads), 0, stream, p);
+  else if constexpr (kResident > 1)
+    hipLaunchKernelGGL((mx4_tiles_kernel<Cf, TwoProducts>),
+                       dim3((p.product[0].units + 7) / 8 * 8 + (p.product[1].units + 7) / 8 * 8), dim3(Cf::kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -601,7 +599,8 @@ bool choose_pair(const Mx4Gemm (&g)[2], Mx4Tiles (&tiles)[2]) {
       units += static_cast<double>((g[i].m + c.bm - 1) / c.bm) * static_cast<double>((g[i].n + c.bn - 1) / c.bn) * t[i].slices;
     }
     const double together = std::max(t[0].cost, t[1].cost);
-    if (t[0].cost == 0 || t[1].cost == 0 || units > 256.0 * c.resident || together >= least) continue;
+    // (not the largest tile, whose workgroups fill a CU: 3000 x 2500 x 2500 65 us with it, 60 apart)
+    if (t[0].cost == 0 || t[1].cost == 0 || c.resident < 2 || units > 256.0 * c.resident || together >= least) continue;
     least = together;
     pair = true;
     tiles[0] = t[0];
@@ -656,7 +655,7 @@ hipError_t launch_tiles(const Mx4Gemm* g, const Mx4Tiles* t, float* const* parti
     slices[i] = t[i].slices;
   }
   hipError_t e = hipErrorInvalidValue;
-  if (t[0].bm == 256) e = launch_cfg<8, 8, 2, 1>(p, slices, count, stream);
+  if (t[0].bm == 256 && count == 1) e = launch_cfg<8, 8, 2, 1>(p, slices, count, stream);
   if (t[0].bm == 128) e = launch_cfg<4, 4, 2, 2>(p, slices, count, stream);
   if (t[0].bm == 64) e = launch_cfg<2, 4, 1, 4>(p, slices, count, stream);
   for (int i = 0; i < count && e == hipSuccess; ++i)
@@ -700,8 +699,12 @@ void gemm_mx4_pair_bytes(const Mx4Gemm (&g)[2], uint64_t (&bytes)[2]) {
 hipError_t launch_gemm_mx4_pair(const Mx4Gemm (&g)[2], void* const (&workspaces)[2], const Mx4Sums& sums, hipStream_t stream) {
   Mx4Tiles t[2];
   if (as_pair(g, t)) {
-    float* const partials[2] = {static_cast<float*>(workspaces[0]), static_cast<float*>(workspaces[1])};
-    return launch_tiles(g, t, partials, 2, sums, stream);
+    // the longer sums first: as the last units of the grid they would start last
+    const int first = t[1].slice_chunks > t[0].slice_chunks ? 1 : 0;
+    const Mx4Gemm products[2] = {g[first], g[1 - first]};
+    const Mx4Tiles tiles[2] = {t[first], t[1 - first]};
+    float* const partials[2] = {static_cast<float*>(workspaces[first]), static_cast<float*>(workspaces[1 - first])};
+    return launch_tiles(products, tiles, partials, 2, sums, stream);
   }
   hipError_t e = sums.out ? launch_sum_partials(sums, stream) : hipSuccess;
   for (int i = 0; i < 2 && e == hipSuccess; ++i) e = launch_gemm_mx4(g[i], workspaces[i], stream);

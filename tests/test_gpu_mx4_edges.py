@@ -10,7 +10,8 @@ from test_gpu_mx4 import normal, product_limit, ready
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("m,n,k", [(300, 300, 100), (65, 65, 65), (129, 700, 64), (128, 2000, 700), (1000, 130, 1025)])
+@pytest.mark.parametrize("m,n,k", [(300, 300, 100), (65, 65, 65), (129, 700, 64), (128, 2000, 700), (1000, 130, 1025), (9000, 100, 90),
+                                   (100, 9000, 90), (4096, 1024, 1024)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gradients_in_one_launch(gpu_ctx, dtype, m, n, k):
     """Tiles of both products that are no multiple of the grid's eighths; each gradient as it is by itself."""
