@@ -777,17 +777,17 @@ RNS8_API rns8_status rns8_mi355x_linear_mx4_backward_workspace(
  *     RNS8_MI355X_EXPERTS_NORMALIZE the sum over the chosen experts alone,
  *   out[t] = sum_s weights[t][s] down[e] (silu(gate[e] x[t]) * (up[e] x[t])),  e = ids[t][s],
  *   silu(v) = v / (1 + exp(-v)).
- * x is not rounded: few tokens wait for the weights alone. Sums are 32-bit; a
- * hidden value is kept in 16 bits of precision (24 where dtype is float). Without a
- * router, ids and weights are inputs: an id below 0 or not below `experts` is a
- * slot that adds nothing (its expert is elsewhere), and an expert that a token has
- * twice counts twice. With one they are outputs, and each may be NULL. gate and
- * up hold one inner x width matrix for each expert, down one width x inner, one
- * after the other. A score that is NaN or +infinity, or a value of a
- * token that is not finite, makes that token's row alone NaN (or infinite); an
- * expert whose score is -infinity beside a finite one has weight 0. tokens at most
- * 64, experts at most 1024, top at most 16 and at most `experts`, width and inner
- * at most 65536. */
+ * x is not rounded: few tokens wait for the weights alone. Sums are 32-bit; x and the
+ * hidden values keep their bits (up to 24, of those worth 2^-133 and more), and a
+ * weight past float's range is infinite. Without a router, ids and weights are inputs:
+ * an id below 0 or not below `experts` is a slot that adds nothing (its expert is
+ * elsewhere), and an expert that a token has twice counts twice. With one they are
+ * outputs, and each may be NULL. gate and up hold one inner x width matrix for each
+ * expert, down one width x inner, one after the other. A score that is NaN or
+ * +infinity, or a value of a token that is not finite, makes that token's row alone NaN
+ * (or infinite); an expert whose score is -infinity beside a finite one has weight 0.
+ * tokens at most 64, experts at most 1024, top at most 16 and at most `experts`, width
+ * and inner at most 65536. */
 #define RNS8_MI355X_EXPERTS_NORMALIZE 1u
 typedef struct rns8_mi355x_experts_mx4_args {
   uint64_t struct_size;

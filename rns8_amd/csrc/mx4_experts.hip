@@ -8,7 +8,7 @@
 //     a launch), experts with a token first to last, each one's tokens in order; of few
 //     tokens it also chooses the experts. Then 16 rows of one expert's gate and up at a
 //     time; silu(gate) up times the token's weight goes to the workspace, again as bf16
-//     parts (two: 16 bits; float three).
+//     parts: three, the 24 bits of the 32-bit value.
 //   * down, few pairs: 16 channels to a workgroup, its waves a share of all experts' rows,
 //     the hidden values in LDS; a wave adds an expert's result to its own table of
 //     tokens, the tables are added in order. Three launches.
@@ -23,8 +23,9 @@
 // waits for tokens from memory has waited for all weights asked for before: tokens lie
 // in LDS, so that a wave always has the next units' weights in flight.
 // Measured (1 token, 8 of 128 experts, 4096 -> 1536, bf16): stage 2.5 us, hidden 14.0
-// (3.8 TB/s; some 4 of them before the first weights: lists and tokens), down 9.9 (2.7).
+// (3.8 TB/s; some 4 of them before the first weights: lists and tokens), down 10.5 (2.5).
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "mx4.hpp"
@@ -41,7 +42,8 @@ constexpr int kMaxPairs = kMaxExpertTokens * kMaxExpertTop;
 
 // Who computes what: pairs sorted by expert, then token.
 struct Routing {
-  uint32_t active;  // experts with a token
+  uint32_t active;      // experts with a token
+  uint32_t batches[2];  // of all experts' tokens (hidden, down); many pairs
   uint16_t expert[kMaxPairs], start[kMaxPairs + 2];  // of an active expert; its pairs are [start[i], start[i + 1])
   uint16_t token[kMaxPairs];  // of a pair
   uint16_t place[kMaxPairs];  // of a token's slot: its pair, or kNone
@@ -50,11 +52,16 @@ struct Routing {
 constexpr uint32_t kNone = 0xFFFF;
 
 // Many pairs: what LDS holds of an expert's tokens, `tokens` rows of `chunks` chunks (16
-// bytes after each, so that sixteen rows' reads meet no bank twice), and how many
-// workgroups share them.
+// bytes after each, so that sixteen rows' reads meet no bank twice). inverse: 2^16 /
+// tokens and one.
 struct Batches {
-  uint32_t chunks, row, tokens, spread;
+  uint32_t chunks, row, tokens, inverse;
 };
+// Whose a batch is: an index among the active experts and, in the low bits, its number
+// among that one's.
+constexpr uint32_t kBatchBits = 6;
+static_assert(kMaxExpertTokens <= 1 << kBatchBits && kMaxExperts << kBatchBits <= 1 << 16, "an owner in 16 bits");
+
 
 struct ExpertsArgs {
   const void *x, *router;
@@ -73,6 +80,7 @@ struct ExpertsArgs {
   uint16_t* h_parts;  // [part][pair][256 inner_chunks]
   float* y;           // [pair][16 ceil(width / 16)]; many pairs
   Routing* routing;
+  uint16_t* down_owner;  // of each of down's batches; many pairs
   Batches batches[2];  // hidden, down; many pairs
 };
 
@@ -221,7 +229,7 @@ struct RouteScratch {
   float weight[kMaxPairs];
   uint32_t tokens[2][kMaxExperts];  // an expert's tokens, a bit each
   uint16_t start[kMaxExperts];
-  uint32_t totals[kRouteWaves];
+  uint32_t totals[kRouteWaves], batches[kRouteWaves];
 };
 
 // Ordered as the scores are, NaN first.
@@ -354,9 +362,9 @@ __device__ __forceinline__ void list_few(const ExpertsArgs& a, int lane, uint32_
 
 // The lists, in LDS; all kRouteThreads threads. writes: this workgroup gives the
 // next kernels the lists, and the caller its experts and weights where they are chosen
-// here (kChooses).
+// here (kChooses: few pairs; otherwise `owner` receives the owners of hidden's batches).
 template <bool kChooses>
-__device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteScratch& s, Routing& r) {
+__device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteScratch& s, Routing& r, uint16_t* owner) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t pairs = a.tokens * a.top, tid = threadIdx.x;
   auto give = [&]() {
@@ -438,19 +446,38 @@ __device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteSc
     const uint32_t n = e < a.experts ? __popc(s.tokens[0][e]) + __popc(s.tokens[1][e]) : 0u;
     mine[i] = n ? n | 0x10000u : 0u;
   }
-  uint32_t sum = mine[0] + mine[1];
+  // batches of hidden (low half) and of down (high half)
+  uint32_t cut[2] = {};
+  if constexpr (!kChooses) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i)
+      for (uint32_t down = 0; down < 2; ++down)
+        cut[i] |= ((mine[i] & 0xFFFFu) + a.batches[down].tokens - 1) * a.batches[down].inverse >> 16 << (16 * down);
+  }
+  uint32_t sum = mine[0] + mine[1], cuts = cut[0] + cut[1];
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) {
     const uint32_t below = __shfl_up(sum, step);
     if (lane >= step) sum += below;
+    if constexpr (!kChooses) {
+      const uint32_t cuts_below = __shfl_up(cuts, step);
+      if (lane >= step) cuts += cuts_below;
+    }
   }
-  if (lane == 63) s.totals[wave] = sum;
+  if (lane == 63) {
+    s.totals[wave] = sum;
+    s.batches[wave] = cuts;
+  }
   __syncthreads();
-  uint32_t before = sum - mine[0] - mine[1], total = 0;
+  uint32_t before = sum - mine[0] - mine[1], total = 0, cuts_before = cuts - cut[0] - cut[1], all_cuts = 0;
 #pragma unroll
   for (int w = 0; w < kRouteWaves; ++w) {
-    if (w < wave) before += s.totals[w];
+    if (w < wave) {
+      before += s.totals[w];
+      cuts_before += s.batches[w];
+    }
     total += s.totals[w];
+    all_cuts += s.batches[w];
   }
 #pragma unroll
   for (uint32_t i = 0; i < 2; ++i) {
@@ -459,8 +486,15 @@ __device__ __forceinline__ void route(const ExpertsArgs& a, bool writes, RouteSc
     s.start[2 * tid + i] = static_cast<uint16_t>(at);
     r.expert[at >> 16] = static_cast<uint16_t>(2 * tid + i);
     r.start[at >> 16] = static_cast<uint16_t>(at);
+    if constexpr (!kChooses) {
+      const uint32_t first = i ? cuts_before + cut[0] : cuts_before, id = at >> 16 << kBatchBits;
+      for (uint32_t n = 0; n < (cut[i] & 0xFFFFu); ++n) owner[(first & 0xFFFFu) + n] = static_cast<uint16_t>(id + n);
+      for (uint32_t n = 0; writes && n < cut[i] >> 16; ++n) a.down_owner[(first >> 16) + n] = static_cast<uint16_t>(id + n);
+    }
   }
   if (tid == 0) {
+    r.batches[0] = all_cuts & 0xFFFFu;
+    r.batches[1] = all_cuts >> 16;
     r.active = total >> 16;
     r.start[total >> 16] = static_cast<uint16_t>(total);
   }
@@ -523,14 +557,14 @@ __device__ __forceinline__ void both_fragments(F&& f) {
   f(std::integral_constant<int, 1>{});
 }
 
+constexpr int kHiddenParts = 3;  // of a hidden value, whatever the type of x
 constexpr int kHiddenWaves = kRouteWaves, kHiddenThreads = kRouteThreads;
 constexpr uint32_t kLdsX = 32768;    // few tokens: values of x's parts that a workgroup holds
-constexpr uint32_t kLdsH = 49152;    // and of the hidden values'
+constexpr uint32_t kLdsH = 65536;    // and of the hidden values' (beside tables and lists all that LDS has)
 constexpr uint32_t kFewTokens = 16;  // that the down kernel's tables hold
 constexpr uint32_t kLdsRows = 65536;  // many: bytes of an expert's tokens
 
-// Four hidden values of a pair, rounded to parts.
-template <int kHiddenParts>
+// Four hidden values of a pair as parts.
 __device__ __forceinline__ void store_hidden(uint16_t* to, int64_t part, const float (&v)[4]) {
   uint16_t parts[4][kHiddenParts];
 #pragma unroll
@@ -549,7 +583,7 @@ __device__ __forceinline__ void gated(const f32x4& g, const f32x4& u, float weig
 }
 
 // ---- hidden, few pairs: eight waves to 16 rows, the tokens' parts in LDS ------------------------
-template <int kParts, int kHiddenParts>
+template <int kParts>
 __global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(ExpertsArgs a) {
   constexpr int U = 2;  // chunks whose weights are in flight together
   __shared__ __attribute__((aligned(16))) union {
@@ -563,7 +597,7 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(E
   // (x's first values are on their way while the experts are chosen)
   const uint32_t mine = 8 * threadIdx.x;
   const u32x4 early = *reinterpret_cast<const u32x4*>(a.x_parts + min(mine, kParts * x_part - 8));
-  route<true>(a, blockIdx.x == 0, scratch.route, lists);
+  route<true>(a, blockIdx.x == 0, scratch.route, lists, nullptr);
   if (mine < kParts * x_part) *reinterpret_cast<u32x4*>(lds_x + mine) = early;
   for (uint32_t i = mine + 8 * kHiddenThreads; i < kParts * x_part; i += 8 * kHiddenThreads)
     *reinterpret_cast<u32x4*>(lds_x + i) = *reinterpret_cast<const u32x4*>(a.x_parts + i);
@@ -618,7 +652,7 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_hidden_few_kernel(E
       }
       float v[4] = {};
       if (group < real) gated(acc[0], acc[1], lists.weight[start + r], v);
-      store_hidden<kHiddenParts>(a.h_parts + (start + r) * h_row + 16 * group + 4 * (lane >> 4), h_part, v);
+      store_hidden(a.h_parts + (start + r) * h_row + 16 * group + 4 * (lane >> 4), h_part, v);
     }
     __syncthreads();
   }
@@ -632,25 +666,59 @@ __device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_r
 // (gate and up of 16 hidden values, or 32 channels of down.) The rows of all experts
 // that have tokens are cut evenly over the workgroups, in blocks of eight, a wave each; an
 // expert's tokens, as many as fit, lie in LDS while its rows stream by, two or three
-// units' loads ahead. A further batch of tokens reads the weights again, in a workgroup of
-// its own where the blocks alone are fewer than the CUs: 64 tokens, 4 of 4 experts, 4096 -> 2048, f32,
-// whole layer 228 us instead of 926; 4 of 16 experts, 2048 -> 1024, bf16, 40 instead of 59.
-// Measured (64 tokens, 8 of 128 experts, 4096 -> 1536, bf16): hidden 172 us, 5.0 TB/s of
-// weights; down 80 us, 5.3 TB/s.
-template <bool kDown, int kParts, int kHiddenParts>
+// units' loads ahead. A further batch of tokens reads the weights again, as work of its
+// own: behind the first in its workgroup it would be what the launch ends with (64 tokens,
+// 8 of 128 experts, 4096 -> 1536, f32, whole layer 416 us, 569 that way; the most tokens of
+// an expert were 10).
+// Measured (the same in bf16): hidden 164 us, 5.2 TB/s of weights; down 88 us, 4.9 TB/s.
+
+// A batch's lines, part by part and in each its tokens, are the columns of one or two
+// MFMAs (three parts of up to five tokens are one's: down of the above 106 us with an MFMA
+// for each part); here a token's are added, in the column of its number.
+template <int kParts>
+constexpr uint32_t kColumnGroups = kParts == 1 ? 1 : 2;
+template <int kParts>
+__device__ __forceinline__ void add_lines(f32x4 (&acc)[kColumnGroups<kParts>][2], uint32_t tokens, int lane) {
+  f32x4 sum[2] = {acc[0][0], acc[0][1]};
+#pragma unroll
+  for (uint32_t p = 1; p < kParts; ++p) {
+    const uint32_t line = p * tokens + (lane & 15);
+    const int from = static_cast<int>((lane & 48) + (line & 15));
+#pragma unroll
+    for (uint32_t g = 0; g < kColumnGroups<kParts>; ++g) {
+      if (g > 0 && kParts * tokens <= 16) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = __shfl(acc[g][j][e], from);
+          sum[j][e] += line >> 4 == g ? v : 0.0f;
+        }
+    }
+  }
+  acc[0][0] = sum[0];
+  acc[0][1] = sum[1];
+}
+
+template <bool kDown, int kParts>
 __global__ __launch_bounds__(kHiddenThreads, 4) void experts_many_kernel(ExpertsArgs a) {
-  constexpr int D = kParts == 1 ? 3 : 2;  // (three with more parts spill: down of the above 92 us)
+  constexpr uint32_t G = kColumnGroups<kParts>;
+  constexpr int D = kParts == 1 ? 3 : 2;  // (three with more parts spill)
   __shared__ __attribute__((aligned(16))) union {
     RouteScratch route;
     uint8_t rows[kLdsRows];
   } lds;
   __shared__ Routing lists;
+  __shared__ __attribute__((aligned(16))) uint16_t owner[kMaxPairs];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if constexpr (kDown) {
-    for (uint32_t i = threadIdx.x; i < sizeof(Routing) / 4; i += kHiddenThreads)
+    // (of the lists what comes before the tokens)
+    for (uint32_t i = threadIdx.x; i < offsetof(Routing, token) / 4; i += kHiddenThreads)
       reinterpret_cast<uint32_t*>(&lists)[i] = reinterpret_cast<const uint32_t*>(a.routing)[i];
+    for (uint32_t i = threadIdx.x; i < sizeof(owner) / 4; i += kHiddenThreads)
+      reinterpret_cast<uint32_t*>(owner)[i] = reinterpret_cast<const uint32_t*>(a.down_owner)[i];
   } else {
-    route<false>(a, blockIdx.x == 0, lds.route, lists);
+    route<false>(a, blockIdx.x == 0, lds.route, lists, owner);
   }
   __syncthreads();
   const uint32_t chunks = kDown ? a.inner_chunks : a.width_chunks, stride = chunks * kMx4Unit;
@@ -662,101 +730,106 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_many_kernel(Experts
   const uint32_t out_row = kDown ? 16 * groups : 256 * a.inner_chunks;
   const int64_t h_part = static_cast<int64_t>(a.tokens) * a.top * out_row;
   const Batches& room = a.batches[kDown ? 1 : 0];
-  const uint32_t held = room.chunks, lds_row = room.row, batch = room.tokens, spread = room.spread;
-  const uint32_t lds_part = batch * lds_row;
+  const uint32_t held = room.chunks, lds_row = room.row, batch = room.tokens;
 
-  // an item is eight turns of one expert, and where they are spread one batch of its tokens
+  // an item is eight turns of one expert for one batch of its tokens
   const uint32_t blocks = (per + kHiddenWaves - 1) / kHiddenWaves;
-  const uint64_t items = static_cast<uint64_t>(same(lists.active)) * spread * blocks;
-  const uint32_t begin = static_cast<uint32_t>(items * blockIdx.x / gridDim.x);
-  const uint32_t end = static_cast<uint32_t>(items * (blockIdx.x + 1) / gridDim.x);
+  const uint64_t items = static_cast<uint64_t>(same(lists.batches[kDown ? 1 : 0])) * blocks;
+  // (where there are fewer than workgroups, an expert's batches meet in one XCD's L2 if its
+  // blocks are a multiple of eight: 64 tokens, 4 of 16 experts, 2048 -> 1024, bf16, hidden 18.1 us, cut evenly 18.7)
+  const uint64_t cut = max(items, static_cast<uint64_t>(gridDim.x));
+  const uint32_t begin = static_cast<uint32_t>(min(cut * blockIdx.x / gridDim.x, items));
+  const uint32_t end = static_cast<uint32_t>(min(cut * (blockIdx.x + 1) / gridDim.x, items));
   for (uint32_t item = begin; item < end;) {
     const uint32_t share = item / blocks, block = item - share * blocks, rounds = min(blocks - block, end - item);
-    const uint32_t slot = share / spread;
+    const uint32_t own = same(owner[share]), slot = own >> kBatchBits, r0 = (own & ((1u << kBatchBits) - 1)) * batch;
     item += rounds;
     const uint32_t from = block * kHiddenWaves, to = min(per, from + rounds * kHiddenWaves), steps = rounds * chunks;
     const uint32_t e = same(lists.expert[slot]), start = same(lists.start[slot]), count = same(lists.start[slot + 1]) - start;
-    for (uint32_t r0 = (share - slot * spread) * batch; r0 < count; r0 += batch * spread) {
-      const uint32_t tokens = min(batch, count - r0), r = lane & 15;
-      const uint32_t row = min(r, tokens - 1) * lds_row + 64 * (lane >> 4);
-      // Loads run D steps ahead, over rounds as well (past the last turn or step the
-      // last row again), and have no branches: a wait in the loop then counts them.
-      const uint64_t matrix = static_cast<uint64_t>(groups) * stride;
-      const uint8_t* const base0 = (kDown ? a.down : a.gate) + e * matrix;
-      const uint8_t* const base1 = (kDown ? a.down : a.up) + e * matrix;
-      uint32_t ahead_chunk = 0, ahead_turn = from + wave;
-      auto load = [&](Mx4Unit (&u)[2]) __attribute__((always_inline)) {
-        const uint32_t t = min(ahead_turn, to - 1);
-        // (an odd last group is read twice, its second results are not stored)
-        const uint32_t g0 = kDown ? 2 * t : t, g1 = kDown ? min(2 * t + 1, groups - 1) : t;
-        u[0] = stream_unit(base0 + static_cast<uint64_t>(g0) * stride + ahead_chunk * kMx4Unit, lane);
-        u[1] = stream_unit(base1 + static_cast<uint64_t>(g1) * stride + ahead_chunk * kMx4Unit, lane);
-        const bool wraps = ahead_chunk + 1 == chunks;
-        ahead_turn += wraps ? kHiddenWaves : 0;
-        ahead_chunk = wraps ? 0 : ahead_chunk + 1;
-      };
-      Mx4Unit w[D][2];
+    const uint32_t tokens = min(batch, count - r0), r = lane & 15, lines = kParts * tokens;
+    uint32_t row[G];
 #pragma unroll
-      for (int i = 0; i < D; ++i) load(w[i]);
-      f32x4 acc[2] = {};
-      uint32_t c = 0, held_at = 0, mine = from + wave;
-      bool staged = false;
-      for (uint32_t step = 0; step < steps; step += D) {
+    for (uint32_t g = 0; g < G; ++g) row[g] = min(16 * g + r, lines - 1) * lds_row + 64 * (lane >> 4);
+    // Loads run D steps ahead, over rounds as well (past the last turn or step the
+    // last row again), and have no branches: a wait in the loop then counts them.
+    const uint64_t matrix = static_cast<uint64_t>(groups) * stride;
+    const uint8_t* const base0 = (kDown ? a.down : a.gate) + e * matrix;
+    const uint8_t* const base1 = (kDown ? a.down : a.up) + e * matrix;
+    uint32_t ahead_chunk = 0, ahead_turn = from + wave;
+    auto load = [&](Mx4Unit (&u)[2]) __attribute__((always_inline)) {
+      const uint32_t t = min(ahead_turn, to - 1);
+      // (an odd last group is read twice, its second results are not stored)
+      const uint32_t g0 = kDown ? 2 * t : t, g1 = kDown ? min(2 * t + 1, groups - 1) : t;
+      u[0] = stream_unit(base0 + static_cast<uint64_t>(g0) * stride + ahead_chunk * kMx4Unit, lane);
+      u[1] = stream_unit(base1 + static_cast<uint64_t>(g1) * stride + ahead_chunk * kMx4Unit, lane);
+      const bool wraps = ahead_chunk + 1 == chunks;
+      ahead_turn += wraps ? kHiddenWaves : 0;
+      ahead_chunk = wraps ? 0 : ahead_chunk + 1;
+    };
+    Mx4Unit w[D][2];
 #pragma unroll
-        for (int i = 0; i < D; ++i) {
-          if (step + i < steps) {
-            if (!staged || c - held_at >= held) {
-              held_at = c;
-              staged = true;
-              const uint32_t now = min(held, chunks - c), vectors = 32 * now;
-              __syncthreads();
-              for (uint32_t v = threadIdx.x; v < kParts * tokens * vectors; v += kHiddenThreads) {
-                const uint32_t line = v / vectors, at = v - line * vectors, p = line / tokens, t = line - p * tokens;
-                const uint32_t source = kDown ? start + r0 + t : lists.token[start + r0 + t];
-                *reinterpret_cast<u32x4*>(lds.rows + p * lds_part + t * lds_row + 16 * at) =
-                    *reinterpret_cast<const u32x4*>(in + p * in_part + static_cast<int64_t>(source) * in_row + 256 * c + 8 * at);
-              }
-              __syncthreads();
+    for (int i = 0; i < D; ++i) load(w[i]);
+    f32x4 acc[G][2] = {};
+    uint32_t c = 0, held_at = 0, mine = from + wave;
+    bool staged = false;
+    for (uint32_t step = 0; step < steps; step += D) {
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        if (step + i < steps) {
+          if (!staged || c - held_at >= held) {
+            held_at = c;
+            staged = true;
+            const uint32_t now = min(held, chunks - c), vectors = 32 * now;
+            __syncthreads();
+            for (uint32_t v = threadIdx.x; v < lines * vectors; v += kHiddenThreads) {
+              const uint32_t line = v / vectors, at = v - line * vectors, p = line / tokens, t = line - p * tokens;
+              const uint32_t source = kDown ? start + r0 + t : lists.token[start + r0 + t];
+              *reinterpret_cast<u32x4*>(lds.rows + line * lds_row + 16 * at) =
+                  *reinterpret_cast<const u32x4*>(in + p * in_part + static_cast<int64_t>(source) * in_row + 256 * c + 8 * at);
             }
-            both_fragments([&](auto half) __attribute__((always_inline)) {
-              constexpr int h = decltype(half)::value;
-              bf16x8 w0[4], w1[4];
-              widen<h>(w[i][0], w0);
-              widen<h>(w[i][1], w1);
-#pragma unroll
-              for (int p = 0; p < kParts; ++p) {
-                const Quad q = load_quad(reinterpret_cast<const uint16_t*>(lds.rows + p * lds_part) + 256 * (c - held_at) + 128 * h, row);
-                acc[0] = multiply(w0, q, acc[0]);
-                acc[1] = multiply(w1, q, acc[1]);
-              }
-            });
-            if (++c == chunks) {
-              const uint32_t pair = start + r0 + r;
-              if (mine < to && r < tokens) {
-                if constexpr (kDown) {
-#pragma unroll
-                  for (uint32_t j = 0; j < 2; ++j)
-                    if (2 * mine + j < groups)
-                      *reinterpret_cast<f32x4*>(a.y + static_cast<int64_t>(pair) * out_row + 16 * (2 * mine + j) + 4 * (lane >> 4)) = acc[j];
-                } else {
-                  float v[4];
-                  gated(acc[0], acc[1], lists.weight[pair], v);
-                  uint16_t* const out = a.h_parts + static_cast<int64_t>(pair) * out_row + 4 * (lane >> 4);
-                  store_hidden<kHiddenParts>(out + 16 * mine, h_part, v);
-                  // the zeros after the last
-                  const float zeros[4] = {};
-                  if (mine + 1 == groups)
-                    for (uint32_t g = groups; g < 16 * a.inner_chunks; ++g) store_hidden<kHiddenParts>(out + 16 * g, h_part, zeros);
-                }
-              }
-              acc[0] = acc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-              c = 0;
-              mine += kHiddenWaves;
-              if (held < chunks) staged = false;
-            }
+            __syncthreads();
           }
-          load(w[i]);
+          both_fragments([&](auto half) __attribute__((always_inline)) {
+            constexpr int h = decltype(half)::value;
+            bf16x8 w0[4], w1[4];
+            widen<h>(w[i][0], w0);
+            widen<h>(w[i][1], w1);
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) {
+              if (g > 0 && lines <= 16) break;
+              const Quad q = load_quad(reinterpret_cast<const uint16_t*>(lds.rows) + 256 * (c - held_at) + 128 * h, row[g]);
+              acc[g][0] = multiply(w0, q, acc[g][0]);
+              acc[g][1] = multiply(w1, q, acc[g][1]);
+            }
+          });
+          if (++c == chunks) {
+            add_lines<kParts>(acc, tokens, lane);
+            const uint32_t pair = start + r0 + r;
+            if (mine < to && r < tokens) {
+              if constexpr (kDown) {
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j)
+                  if (2 * mine + j < groups)
+                    *reinterpret_cast<f32x4*>(a.y + static_cast<int64_t>(pair) * out_row + 16 * (2 * mine + j) + 4 * (lane >> 4)) = acc[0][j];
+              } else {
+                float v[4];
+                gated(acc[0][0], acc[0][1], lists.weight[pair], v);
+                uint16_t* const out = a.h_parts + static_cast<int64_t>(pair) * out_row + 4 * (lane >> 4);
+                store_hidden(out + 16 * mine, h_part, v);
+                // the zeros after the last
+                const float zeros[4] = {};
+                if (mine + 1 == groups)
+                  for (uint32_t g = groups; g < 16 * a.inner_chunks; ++g) store_hidden(out + 16 * g, h_part, zeros);
+              }
+            }
+#pragma unroll
+            for (auto& group : acc) group[0] = group[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            c = 0;
+            mine += kHiddenWaves;
+            if (held < chunks) staged = false;
+          }
         }
+        load(w[i]);
       }
     }
   }
@@ -765,7 +838,7 @@ __global__ __launch_bounds__(kHiddenThreads, 4) void experts_many_kernel(Experts
 // ---- down, few pairs ------------------------------------------------------------------------------
 constexpr int kDownWaves = 16, kDownThreads = 64 * kDownWaves;
 
-template <int kHiddenParts, typename T>
+template <typename T>
 __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsArgs a) {
   constexpr int U = 3;  // units in flight together
   __shared__ __attribute__((aligned(16))) float table[kDownWaves][kFewTokens][16];
@@ -774,7 +847,7 @@ __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsA
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t chunks = a.inner_chunks, stride = chunks * kMx4Unit, groups = (a.width + 15) / 16, group = blockIdx.x;
   const uint32_t h_row = 256 * chunks, pairs = a.tokens * a.top, h_part = pairs * h_row;
-  for (uint32_t i = threadIdx.x; i < sizeof(Routing) / 4; i += kDownThreads)
+  for (uint32_t i = threadIdx.x; i < offsetof(Routing, place) / 4; i += kDownThreads)
     reinterpret_cast<uint32_t*>(&lists)[i] = reinterpret_cast<const uint32_t*>(a.routing)[i];
   // The hidden values are asked for before the weights: loads return in order. (Pairs that
   // there are not hold anything, and meet no weights.)
@@ -782,7 +855,8 @@ __global__ __launch_bounds__(kDownThreads) void experts_down_few_kernel(ExpertsA
   u32x4 early[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i)
-    early[i] = *reinterpret_cast<const u32x4*>(a.h_parts + min(8 * (threadIdx.x + i * kDownThreads), kHiddenParts * h_part - 8));
+    if (8u * kDownThreads * i < kHiddenParts * h_part)
+      early[i] = *reinterpret_cast<const u32x4*>(a.h_parts + min(8 * (threadIdx.x + i * kDownThreads), kHiddenParts * h_part - 8));
   for (uint32_t i = threadIdx.x; i < kDownWaves * kFewTokens * 16; i += kDownThreads) (&table[0][0][0])[i] = 0.0f;
   __syncthreads();
   const uint32_t units = lists.active * chunks;
@@ -867,12 +941,11 @@ __global__ __launch_bounds__(256) void experts_combine_kernel(ExpertsArgs a) {
 }
 
 int parts_of(uint32_t dtype) { return dtype == RNS8_MI355X_F32 ? 3 : dtype == RNS8_MI355X_F16 ? 2 : 1; }
-int hidden_parts_of(uint32_t dtype) { return dtype == RNS8_MI355X_F32 ? 3 : 2; }
 
 // Whether x and the hidden values fit a workgroup's LDS, and the tokens its tables.
 bool few(const rns8_mi355x_experts_mx4_args& a) {
   return a.tokens <= kFewTokens && parts_of(a.dtype) * a.tokens * mx4_chunks(a.width) * 256 <= kLdsX &&
-         hidden_parts_of(a.dtype) * a.tokens * a.top * mx4_chunks(a.inner) * 256 <= kLdsH;
+         kHiddenParts * a.tokens * a.top * mx4_chunks(a.inner) * 256 <= kLdsH;
 }
 
 // The workspace: scores, the parts of x and of the hidden values, pairs' results, the lists.
@@ -889,7 +962,7 @@ uint64_t lay_out(const rns8_mi355x_experts_mx4_args& a, ExpertsArgs& e) {
   e.x_parts = reinterpret_cast<uint16_t*>(
       take(static_cast<uint64_t>(parts_of(a.dtype)) * tokens * static_cast<uint64_t>(mx4_chunks(a.width)) * 512));
   e.h_parts = reinterpret_cast<uint16_t*>(
-      take(static_cast<uint64_t>(hidden_parts_of(a.dtype)) * pairs * static_cast<uint64_t>(mx4_chunks(a.inner)) * 512));
+      take(static_cast<uint64_t>(kHiddenParts) * pairs * static_cast<uint64_t>(mx4_chunks(a.inner)) * 512));
   e.chosen = a.ids;
   e.chosen_weights = a.weights;
   if (a.router && !few(a)) {
@@ -898,10 +971,11 @@ uint64_t lay_out(const rns8_mi355x_experts_mx4_args& a, ExpertsArgs& e) {
   }
   e.y = reinterpret_cast<float*>(take(few(a) ? 0 : pairs * static_cast<uint64_t>(mx4_groups(a.width)) * 64));
   e.routing = reinterpret_cast<Routing*>(take(sizeof(Routing)));
+  e.down_owner = reinterpret_cast<uint16_t*>(take(few(a) ? 0 : kMaxPairs * sizeof(uint16_t)));
   return bytes;
 }
 
-template <typename T, int kParts, int kHiddenParts>
+template <typename T, int kParts>
 hipError_t launch_typed(ExpertsArgs e, bool is_few, hipStream_t stream) {
   const uint32_t x_blocks = e.tokens * ((256 * e.width_chunks + 2047) / 2048);
   auto stage = [&](auto experts, auto tokens) {
@@ -916,26 +990,26 @@ hipError_t launch_typed(ExpertsArgs e, bool is_few, hipStream_t stream) {
   const uint32_t active = std::min(e.experts, e.tokens * e.top), groups = (e.width + 15) / 16;
   const dim3 threads(kHiddenThreads);
   if (is_few) {
-    hipLaunchKernelGGL((experts_hidden_few_kernel<kParts, kHiddenParts>), dim3(std::min(active * 16 * e.inner_chunks, 512u)), threads,
+    hipLaunchKernelGGL(experts_hidden_few_kernel<kParts>, dim3(std::min(active * 16 * e.inner_chunks, 512u)), threads,
                        kParts * e.tokens * e.width_chunks * 512, stream, e);
-    hipLaunchKernelGGL((experts_down_few_kernel<kHiddenParts, T>), dim3(groups), dim3(kDownThreads), 0, stream, e);
+    hipLaunchKernelGGL(experts_down_few_kernel<T>, dim3(groups), dim3(kDownThreads), 0, stream, e);
     return hipGetLastError();
   }
   if (e.router) hipLaunchKernelGGL(experts_choose_kernel, dim3(e.tokens), dim3(64), 0, stream, e);
   uint32_t grid[2];
   for (int down = 0; down < 2; ++down) {
     const uint32_t turns = down ? (groups + 1) / 2 : (e.inner + 15) / 16, parts = down ? kHiddenParts : kParts;
-    const uint32_t blocks = active * ((turns + kHiddenWaves - 1) / kHiddenWaves);
+    const uint32_t blocks = (turns + kHiddenWaves - 1) / kHiddenWaves;
     Batches& b = e.batches[down];
     b.chunks = std::min(down ? e.inner_chunks : e.width_chunks, (kLdsRows / parts - 16) / 512);
     b.row = 512 * b.chunks + 16;
-    b.tokens = std::min(kLdsRows / (parts * b.row), 16u);
-    // an expert's batches if tokens are even; a batch more comes second in its workgroup
-    b.spread = blocks < 256 ? (e.tokens * e.top + active * b.tokens - 1) / (active * b.tokens) : 1;
-    grid[down] = std::min(blocks * b.spread, 512u);  // two workgroups to a CU
+    b.tokens = std::min(kLdsRows / (parts * b.row), parts == 3 ? 10u : 16u);  // two MFMAs' columns
+    b.inverse = 65536 / b.tokens + 1;  // (right for what it divides, below 80)
+    const uint32_t batches = active + (e.tokens * e.top - active) / b.tokens;  // at most
+    grid[down] = std::min(batches * blocks, 512u);  // two workgroups to a CU
   }
-  hipLaunchKernelGGL((experts_many_kernel<false, kParts, kHiddenParts>), dim3(grid[0]), threads, 0, stream, e);
-  hipLaunchKernelGGL((experts_many_kernel<true, kHiddenParts, kHiddenParts>), dim3(grid[1]), threads, 0, stream, e);
+  hipLaunchKernelGGL((experts_many_kernel<false, kParts>), dim3(grid[0]), threads, 0, stream, e);
+  hipLaunchKernelGGL((experts_many_kernel<true, kHiddenParts>), dim3(grid[1]), threads, 0, stream, e);
   hipLaunchKernelGGL(experts_combine_kernel<T>, dim3((e.tokens * ((e.width + 3) / 4) + 255) / 256), dim3(256), 0, stream, e);
   return hipGetLastError();
 }
@@ -977,9 +1051,9 @@ hipError_t launch_experts_mx4(const rns8_mi355x_experts_mx4_args& a, hipStream_t
   e.width_chunks = static_cast<uint32_t>(mx4_chunks(a.width));
   e.inner_chunks = static_cast<uint32_t>(mx4_chunks(a.inner));
   lay_out(a, e);
-  if (a.dtype == RNS8_MI355X_F32) return launch_typed<float, 3, 3>(e, few(a), stream);
-  if (a.dtype == RNS8_MI355X_F16) return launch_typed<f16, 2, 2>(e, few(a), stream);
-  return launch_typed<bf16, 1, 2>(e, few(a), stream);
+  if (a.dtype == RNS8_MI355X_F32) return launch_typed<float, 3>(e, few(a), stream);
+  if (a.dtype == RNS8_MI355X_F16) return launch_typed<f16, 2>(e, few(a), stream);
+  return launch_typed<bf16, 1>(e, few(a), stream);
 }
 
 }  // namespace rns8x
