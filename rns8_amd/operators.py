@@ -464,7 +464,8 @@ class LinearMx4Backward(_Call):
         self.args.m, self.args.n, self.args.k = m, n, k
         o.matrix("dy", "lddy", dy, m, n)
         o.matrix("x", "ldx", x, m, k)
-        o.mx4("w_t", w_t, k, n)
+        if dx is not None:  # (its rows say k)
+            o.mx4("w_t", w_t, k, n)
         o.matrix("dx", "lddx", dx, m, k)
         o.matrix("dw", "lddw", dw, n, k, "float32")
         o.vector("dbias", dbias, n)
