@@ -640,7 +640,8 @@ RNS8_API rns8_status rns8_mi355x_token_logprobs_backward(
  * where c is even) of byte 1024 (c / 128) + 16 L + (c % 32) / 2 and its scale in
  * byte 2048 + 2 L + c / 128, L = r % 16 + 16 ((c % 128) / 32). What lies past the
  * matrix in its units is zeros. 16 rows at a multiple of 16 are themselves an MX4
- * matrix.
+ * matrix, and matrices of as many rows, a multiple of 16, one after the other are one of
+ * all their rows: one call packs, rounds or reads them.
  *
  * The rules of the operators above hold here too. rows and cols of an MX4 matrix
  * are below 2^31 - 256 and those that a product sums over at most 2^23. */

@@ -402,7 +402,9 @@ class DequantizeMx4(_Call):
 
 
 class PackMx4(_Call):
-    """Rows of codes, two to a byte, and of scales as an MX4 matrix (rns8_mi355x_pack_mx4)."""
+    """Rows of codes, two to a byte, and of scales as an MX4 matrix (rns8_mi355x_pack_mx4).
+
+    Matrices of a multiple of 16 rows that follow one another are one: a stack of experts is one call."""
 
     _entry, _args = "rns8_mi355x_pack_mx4", abi.PackMx4Args
 
