@@ -22,8 +22,10 @@
 // otherwise eight waves', each with a share of the sum. Loads return in order, and who
 // waits for tokens from memory has waited for all weights asked for before: tokens lie
 // in LDS, so that a wave always has the next units' weights in flight.
-// Measured (1 token, 8 of 128 experts, 4096 -> 1536, bf16): stage 2.5 us, hidden 14.0
-// (3.8 TB/s; some 4 of them before the first weights: lists and tokens), down 10.5 (2.5).
+// Measured (1 token, 8 of 128 experts, 4096 -> 1536, bf16): stage 2.7 us, hidden 14.0
+// (3.8 TB/s; some 4 of them before the first weights: lists and tokens), down 10.5 (2.5),
+// on the same 80 MB again and again; hidden 14.8 and down 11.1 where other experts are chosen each
+// time and their weights come from HBM.
 #include <algorithm>
 #include <cstddef>
 #include <type_traits>
@@ -670,7 +672,7 @@ __device__ __forceinline__ uint32_t same(uint32_t v) { return __builtin_amdgcn_r
 // own: behind the first in its workgroup it would be what the launch ends with (64 tokens,
 // 8 of 128 experts, 4096 -> 1536, f32, whole layer 416 us, 569 that way; the most tokens of
 // an expert were 10).
-// Measured (the same in bf16): hidden 164 us, 5.2 TB/s of weights; down 88 us, 4.9 TB/s.
+// Measured (the same in bf16): hidden 166 us, 5.1 TB/s of weights; down 90 us, 4.8 TB/s.
 
 // A batch's lines, part by part and in each its tokens, are the columns of one or two
 // MFMAs (three parts of up to five tokens are one's: down of the above 106 us with an MFMA

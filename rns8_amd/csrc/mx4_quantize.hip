@@ -11,7 +11,9 @@
 //     and rounds two values, half to even, 6 at most.
 //   * q_t (blocks along a column): a lane's 32 rows are a block of each of its V
 //     columns, so both forms come from one read.
-//   * Codes and scales are gathered in LDS as units and leave in whole lines.
+//   * Codes and scales are gathered in LDS as units and leave in whole lines. (A tile of
+//     both forms has one fragment of q_t's units: its scales are every other byte of
+//     lines that two workgroups share, and leave as bytes.)
 //   * Sums of columns (a bias' gradient) in 32 bits for each 128 rows, in a fixed
 //     order; a second kernel adds those.
 // Measured at 8192 x 8192 in bf16: rows alone 33 us (5.1 TB/s), both forms 54 (3.8 TB/s),
